@@ -1,0 +1,118 @@
+"""ctypes binding of include/tenmo_hip_transformer.h, and what its operators share: results and workspaces in torch's allocator, and
+their order with the caller's stream.
+
+The library enqueues on one stream (``tenmo_hip_get_stream``).  An operator called under another current torch stream joins the two: the
+library's stream waits for the current one before the launch, the current one for the library's behind it.  Under
+``torch.cuda.graph`` that makes the launches part of the captured graph.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import TenmoHipError, check
+from .ndbuffer import NDBuffer
+
+_vp, _ptr, _i64, _i32, _f32 = C.POINTER(_lib.CView), C.c_void_p, C.c_int64, C.c_int32, C.c_float
+
+# name -> (restype, argtypes); every function include/tenmo_hip_transformer.h declares
+SIGNATURES = {
+    "tenmo_hip_layer_norm_forward_f32": (C.c_int, [_vp, _ptr, _ptr, _f32, _ptr, _ptr, _ptr, _i32]),
+    "tenmo_hip_layer_norm_backward_workspace_bytes": (_i64, [_i64, _i64]),
+    "tenmo_hip_layer_norm_backward_f32": (C.c_int, [_vp, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i32, _ptr, _i64, _i32]),
+    "tenmo_hip_attention_forward_workspace_bytes": (_i64, [_i64] * 6),
+    "tenmo_hip_attention_forward_f32": (C.c_int, [_vp, _vp, _vp, _f32, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i32]),
+    "tenmo_hip_attention_backward_workspace_bytes": (_i64, [_i64] * 6),
+    "tenmo_hip_attention_backward_f32": (C.c_int, [_vp, _vp, _vp, _f32, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _vp, _vp, _vp, _i32, _ptr, _i64, _i32]),
+    "tenmo_hip_vocabulary_loss_forward_workspace_bytes": (_i64, [_i64] * 3),
+    "tenmo_hip_vocabulary_loss_forward_f32": (C.c_int, [_vp, _vp, _ptr, _ptr, _i32, _i64, _f32, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i32]),
+    "tenmo_hip_vocabulary_loss_backward_workspace_bytes": (_i64, [_i64] * 3),
+    "tenmo_hip_vocabulary_loss_backward_f32": (C.c_int, [_vp, _vp, _ptr, _ptr, _i32, _i64, _f32, _ptr, _ptr, _i32, _ptr, _ptr, _vp, _ptr, _i32, _ptr, _i64, _i32]),
+}
+
+_bound = None
+
+
+def load() -> C.CDLL:
+    """The library with these functions bound (raises if one is missing)."""
+    global _bound
+    L = _lib.load()
+    if _bound is not L:
+        for name, (res, args) in SIGNATURES.items():
+            fn = getattr(L, name)
+            fn.restype, fn.argtypes = res, args
+        L.hipStreamGetFlags.argtypes = [_ptr, C.POINTER(C.c_uint)]
+        _bound = L
+    return L
+
+
+class Launch:
+    """``with Launch(buffer, ...) as L:`` — the library initialised, every operand on its device, its stream joined with the current one."""
+
+    __slots__ = ("_join",)
+
+    def __init__(self, *operands: Optional[NDBuffer]):
+        _lib.init()
+        for b in operands:
+            if b is not None and b.storage.get_device() != 0:  # _lib.init's device
+                raise TenmoHipError(-3, f"operand on {b.storage.device}: the library runs on device 0")
+
+    def __enter__(self) -> C.CDLL:
+        L = load()
+        current, own = torch.cuda.current_stream(0), L.tenmo_hip_get_stream() or 0
+        self._join = None
+        if current.cuda_stream != own and not (current.cuda_stream == 0 and self._follows_default(L, own)):
+            library = torch.cuda.ExternalStream(own, device=0)
+            library.wait_stream(current)
+            self._join = (current, library)
+        return L
+
+    @staticmethod
+    def _follows_default(L: C.CDLL, stream: int) -> bool:
+        """Whether the stream is ordered with the default stream by itself (it was not created as a non-blocking one)."""
+        flags = C.c_uint(1)
+        return L.hipStreamGetFlags(stream, C.byref(flags)) == 0 and flags.value == 0
+
+    def __exit__(self, *exc) -> None:
+        if self._join is not None:
+            current, library = self._join
+            current.wait_stream(library)
+
+
+def empty(like: NDBuffer, *shape: int) -> NDBuffer:
+    n = 1
+    for s in shape:
+        n *= s
+    return NDBuffer(torch.empty(max(n, 1), dtype=torch.float32, device=like.storage.device), shape)
+
+
+def workspace(like: NDBuffer, nbytes: int):
+    """(tensor that owns it, address, bytes); torch's allocator aligns to 512 bytes and, under capture, keeps it for the graph."""
+    check(nbytes)
+    if nbytes == 0:
+        return None, None, 0
+    t = torch.empty(nbytes, dtype=torch.uint8, device=like.storage.device)
+    return t, t.data_ptr(), nbytes
+
+
+def address(b: Optional[NDBuffer]) -> Optional[int]:
+    """Of a dense buffer's first element."""
+    return None if b is None else b.storage.data_ptr() + 4 * b.offset
+
+
+def dense(b: Optional[NDBuffer], shape, what: str) -> Optional[NDBuffer]:
+    if b is not None and (tuple(b.shape) != tuple(shape) or not b.is_contiguous()):
+        raise TenmoHipError(-2, f"{what} must be dense with shape {tuple(shape)}, got shape {b.shape} with strides {b.strides}")
+    return b
+
+
+def device_ints(t: Optional[torch.Tensor], n: int, what: str, dtypes=(torch.int32,)) -> Optional[int]:
+    """Address of a dense device tensor of n whole numbers."""
+    if t is None:
+        return None
+    if t.dtype not in dtypes or t.numel() != n or not t.is_contiguous() or not t.is_cuda or t.get_device() != 0:
+        raise TenmoHipError(-3, f"{what}: needs {n} dense {' or '.join(str(d) for d in dtypes)} values on the library's device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()

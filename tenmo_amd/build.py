@@ -18,6 +18,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
+KERNELS = os.path.join(HERE, "kernels")  # the operators of include/tenmo_hip_transformer.h
 # TENMO_HIP_BUILD_OUT: another output path (a variant library to compare against; load it with TENMO_HIP_LIBRARY)
 LIB = os.environ.get("TENMO_HIP_BUILD_OUT") or os.path.join(HERE, "libtenmo_hip.so")
 
@@ -47,8 +48,11 @@ def _run(cmd):
     return err
 
 
-def _headers_mtime() -> float:
+def _headers_mtime(source: str) -> float:
+    """The newest header that a unit may include: those of kernels/ are its own."""
     paths = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hpp")] + [os.path.join(ROOT, "include", "tenmo_hip.h")]
+    if os.path.dirname(source) == KERNELS:
+        paths += [os.path.join(KERNELS, f) for f in os.listdir(KERNELS) if f.endswith(".hpp")] + [os.path.join(ROOT, "include", "tenmo_hip_transformer.h")]
     return max(os.path.getmtime(p) for p in paths)
 
 
@@ -69,15 +73,16 @@ def build(verbose: bool = False) -> str:
         units.append(([os.path.join(CSRC, "gemm_smallk.hip")], os.path.join(tmp, "gemm_smallk.o")))
         units.append(([os.path.join(CSRC, "gemm_panel.hip")], os.path.join(tmp, "gemm_panel.o")))
         units.append(([os.path.join(CSRC, "gemm_resident.hip")], os.path.join(tmp, "gemm_resident.o")))
+        for name in sorted(f for f in os.listdir(KERNELS) if f.endswith(".hip")):
+            units.append(([os.path.join(KERNELS, name)], os.path.join(tmp, name[:-4] + ".o")))
         stamp = " ".join(FLAGS)
         stamp_file = os.path.join(tmp, "flags.txt")
         same_flags = keep and os.path.exists(stamp_file) and open(stamp_file).read() == stamp
-        newest_header = _headers_mtime()
 
         def stale(src, obj):
             if not (same_flags and os.path.exists(obj)):
                 return True
-            return os.path.getmtime(obj) < max(newest_header, os.path.getmtime(src[-1]))
+            return os.path.getmtime(obj) < max(_headers_mtime(src[-1]), os.path.getmtime(src[-1]))
 
         cmds = [[HIPCC] + FLAGS + ["-c"] + src + ["-o", obj] for src, obj in units if stale(src, obj)]
         if verbose:

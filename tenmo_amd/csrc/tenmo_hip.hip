@@ -27,6 +27,7 @@
 #include "gemm_launch.hpp"
 #include "elementwise.hpp"
 #include "gemv.hpp"
+#include "library_state.hpp"
 
 using namespace tenmo;
 
@@ -1002,6 +1003,14 @@ void launch_ce_forward(const CeForwardArgs& a, bool int64_target, bool vec) {
 }
 
 } // namespace
+
+int tenmo::library_state(LibraryState* out) {
+    if (int rc = ensure_ready()) return rc;
+    *out = LibraryState{S.stream, S.device, S.cus};
+    return 0;
+}
+
+int tenmo::library_error(int code, const char* message) { return fail(code, "%s", message); }
 
 // ================================================================================================
 // C ABI

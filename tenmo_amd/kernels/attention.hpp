@@ -1,0 +1,78 @@
+// What the kernels of attention share: the operands, and which keys a query may use.
+#ifndef TENMO_KERNELS_ATTENTION_HPP
+#define TENMO_KERNELS_ATTENTION_HPP
+#include "entry.hpp"
+
+namespace tenmo {
+
+struct AttnOperand { // element (b, s, h, d)
+    float* p;
+    int64_t b, s, h, d;
+};
+
+struct AttnShape {
+    int batch, queries, keys, heads, kv_heads, dim;
+    int group;   // heads / kv_heads
+    int causal;
+    float scale;
+    const int32_t *key_lengths, *query_starts;
+};
+
+// keys of sequence b
+__device__ __forceinline__ int attn_length(const AttnShape& a, int b) {
+    const int n = a.key_lengths ? a.key_lengths[b] : a.keys;
+    return n < 0 ? 0 : n > a.keys ? a.keys : n;
+}
+// position of the first query of sequence b, limited to where it makes a difference (so that sums with an index stay in 32 bits)
+__device__ __forceinline__ int attn_start(const AttnShape& a, int b) {
+    if (!a.causal) return a.keys;
+    const int s = a.query_starts ? a.query_starts[b] : a.keys - a.queries;
+    return s < -a.queries ? -a.queries : s > a.keys ? a.keys : s;
+}
+// query i may use the keys 0 .. attn_limit - 1 (i >= 0)
+__device__ __forceinline__ int attn_limit(int length, int start, int i) {
+    const int64_t n = (int64_t)start + i + 1;
+    return n < 0 ? 0 : n < length ? (int)n : length;
+}
+
+constexpr float kNone = -__builtin_inff(); // the maximum and the logarithm of the sum of no scores
+
+// exp(a - m) for a running maximum m >= a, which is -inf while nothing was seen.  The hardware's 2^x after one multiplication: x below the
+// maximum by t comes out with a relative error of (t + 2) 2^-24, where its weight is exp(-t).
+__device__ __forceinline__ float below(float a, float m) { return __expf(a - (m == kNone ? 0.f : m)); }
+
+// Four values of d, of which the first is 4 * part, from p (that value's place): 16 bytes where they are there and adjacent, else one by one, zero behind the last.
+template <bool UNIT>
+__device__ __forceinline__ f32x4 attn_load4(const float* p, int64_t ds, int part, int D) {
+    if (UNIT && 4 * part + 3 < D) return *(const f32x4_u*)p;
+    f32x4 x{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (4 * part + e < D) x[e] = p[e * ds];
+    return x;
+}
+__device__ __forceinline__ float dot4(f32x4 a, f32x4 b) { return (a[0] * b[0] + a[1] * b[1]) + (a[2] * b[2] + a[3] * b[3]); }
+// the sum over the L lanes that hold one key or row
+template <int L>
+__device__ __forceinline__ float lanes_sum(float x) {
+#pragma unroll
+    for (int d = L / 2; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
+    return x;
+}
+
+struct AttnBackward {
+    AttnShape s;
+    AttnOperand q, k, v;           // q.p .. never written
+    AttnOperand grad_q, grad_k, grad_v; // p NULL: not wanted
+    const float *out, *lse, *dout;
+    int accumulate;
+};
+
+// ---- attention_rows.hip ----
+void attn_rows_forward(const AttnShape&, const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, float* out, float* lse,
+                       Workspace& ws, int cus, hipStream_t stream, bool launch);
+
+void attn_rows_backward(const AttnBackward&, Workspace& ws, hipStream_t stream, bool launch);
+
+} // namespace tenmo
+#endif

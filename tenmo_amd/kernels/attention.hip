@@ -57,11 +57,19 @@ __global__ __launch_bounds__(256) void attn_zero_kernel(AttnOperand g, int64_t n
     }
 }
 
+// Rows or tiles: a tile is 32 queries against 32 keys, and its operands take two launches first.
+bool forward_by_rows(const AttnShape& s) { return s.queries <= 16; }
+bool backward_by_rows(const AttnShape& s) { return s.queries <= 48 || s.keys <= 48; }
+
 void forward_plan(const AttnShape& s, const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, float* out, float* lse, Workspace& ws, const LibraryState& lib, bool launch) {
-    attn_rows_forward(s, q, k, v, out, lse, ws, lib.cus, lib.stream, launch);
+    if (forward_by_rows(s)) attn_rows_forward(s, q, k, v, out, lse, ws, lib.cus, lib.stream, launch);
+    else attn_tiles_forward(s, q, k, v, out, lse, ws, lib.cus, lib.stream, launch);
 }
 
-void backward_plan(const AttnBackward& b, Workspace& ws, const LibraryState& lib, bool launch) { attn_rows_backward(b, ws, lib.stream, launch); }
+void backward_plan(const AttnBackward& b, Workspace& ws, const LibraryState& lib, bool launch) {
+    if (backward_by_rows(b.s)) attn_rows_backward(b, ws, lib.stream, launch);
+    else attn_tiles_backward(b, ws, lib.stream, launch);
+}
 
 } // namespace
 } // namespace tenmo

@@ -135,22 +135,22 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const RowsArgs a) {
 }
 
 // The runs of one row joined: a thread a value of d.
-__global__ __launch_bounds__(128) void attn_rows_join_kernel(const RowsArgs a) {
-    const int D = a.s.dim, d = threadIdx.x;
-    const int64_t row = blockIdx.x, all = (int64_t)a.s.batch * a.s.heads * a.s.queries;
-    const float* __restrict p = a.part + row * (D + 2);
+__global__ __launch_bounds__(128) void attn_join_kernel(const AttnShape s, const float* __restrict part, int splits, float* __restrict out, float* __restrict lse) {
+    const int D = s.dim, d = threadIdx.x;
+    const int64_t row = blockIdx.x, all = (int64_t)s.batch * s.heads * s.queries;
+    const float* __restrict p = part + row * (D + 2);
     float top = kNone, sum = 0.f, o = 0.f;
-    for (int t = 0; t < a.splits; ++t) top = fmaxf(top, p[t * all * (D + 2) + D]);
-    for (int t = 0; t < a.splits; ++t) {
+    for (int t = 0; t < splits; ++t) top = fmaxf(top, p[t * all * (D + 2) + D]);
+    for (int t = 0; t < splits; ++t) {
         const float* __restrict x = p + t * all * (D + 2);
         const float keep = below(x[D], top);
         sum += keep * x[D + 1];
         if (d < D) o += keep * x[d];
     }
-    const int i = (int)(row % a.s.queries), h = (int)(row / a.s.queries % a.s.heads);
-    const int64_t b = row / a.s.queries / a.s.heads;
-    if (d < D) a.out[((b * a.s.queries + i) * a.s.heads + h) * D + d] = sum == 0.f ? 0.f : o / sum;
-    if (d == 0 && a.lse) a.lse[row] = sum == 0.f ? kNone : top + logf(sum);
+    const int i = (int)(row % s.queries), h = (int)(row / s.queries % s.heads);
+    const int64_t b = row / s.queries / s.heads;
+    if (d < D) out[((b * s.queries + i) * s.heads + h) * D + d] = sum == 0.f ? 0.f : o / sum;
+    if (d == 0 && lse) lse[row] = sum == 0.f ? kNone : top + logf(sum);
 }
 
 template <int L, int R>
@@ -300,7 +300,11 @@ void attn_rows_forward(const AttnShape& s, const AttnOperand& q, const AttnOpera
     if (s.dim <= 32) launch_rows<8>(a, r, unit, grid, stream);
     else if (s.dim <= 64) launch_rows<16>(a, r, unit, grid, stream);
     else launch_rows<32>(a, r, unit, grid, stream);
-    if (a.splits > 1) hipLaunchKernelGGL(attn_rows_join_kernel, dim3((unsigned)((int64_t)s.batch * s.heads * s.queries)), dim3(128), 0, stream, a);
+    if (a.splits > 1) attn_join(s, a.part, a.splits, out, lse, stream);
+}
+
+void attn_join(const AttnShape& s, const float* part, int splits, float* out, float* lse, hipStream_t stream) {
+    hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)((int64_t)s.batch * s.heads * s.queries)), dim3(128), 0, stream, s, part, splits, out, lse);
 }
 
 } // namespace tenmo

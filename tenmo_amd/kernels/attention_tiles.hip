@@ -1,0 +1,707 @@
+// Attention for many query rows, forward and backward, on the fp16 matrix units (the split products of split_gemm.hpp).
+//
+// Forward, a wavefront for 32 queries, 32 keys at a time:
+//   S^T = K Q^T (keys x queries), p = 2^(S c - m + 7) with c = scale log2(e), O^T += V^T P^T, l += sum p.
+// S^T comes out of the matrix units with a query in each lane (twice: the halves hold the keys 8 a + 0..3 and 8 a + 4..7), so the softmax needs one
+// exchange between lanes, and its registers are the operand of the second product as they are: the order in which that product takes the keys is free, and V is
+// fetched in the same one.  The running maximum m is renewed when a score passes it by 2^8 (p and the sums keep to the range of their types below that).
+//
+// Backward, the probabilities again, without atomics and so without an order:
+//   keys:    a wavefront for 32 keys, over the queries that see them (of all heads that share the key's): S = Q K^T, dP = dO V^T,
+//            P = 2^(S c - lse), dS = P (dP - delta); dV^T += dO^T P, dK^T += Q^T dS.
+//   queries: a wavefront for 32 queries, over their keys: S^T, dP^T, dS^T; dQ^T += K^T dS^T.
+// Seven products for the five that one pass with atomics would need.
+//
+// Two launches bring the operands into split form first: the largest magnitude of each head (of the rows that count), then the halves, head by head,
+// rows padded to 128 and D to DP = 32, 64, 96 or 128 with zeros; rows that no allowed pair touches are zeros too, whatever the operand holds there.
+// dS has |dS| <= 2 max |dO_i| max |V_j| (norms of rows), which gives its scale before it is known.
+//
+// LDS tile: 32 rows of DP / 4 chunks of 16 bytes, chunk c = 2 * (d / 8) + kind at slot c ^ swizzle(row); read by rows (16 bytes a lane: 16 rows in 16 different slots of the
+// banks) and by columns (the transposing read: 4 rows x 4 chunks in 16 different slots).
+#include "attention.hpp"
+#include "split_gemm.hpp"
+
+#include <algorithm>
+
+namespace tenmo {
+namespace {
+
+constexpr int kRowPad = 128;        // rows of a head are padded to the rows of a workgroup
+constexpr int kHeadParts = 32;      // partial maxima of a head
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kPBits = 7.f;       // p is held as p 2^7
+constexpr float kRenew = 8.f;
+
+__host__ __device__ constexpr int row_pad(int n) { return (n + kRowPad - 1) / kRowPad * kRowPad; }
+
+enum { kQ, kK, kV, kDO };
+
+struct TileArgs {
+    AttnShape s;
+    AttnOperand src[4]; // q, k, v, dout
+    int jobs;           // 3 or 4 of them
+    int parts;
+    float* split[4];    // [batch][heads][rows padded][DP]
+    uint32_t* amax[4];  // [batch * heads][parts]
+    float* norm[4];     // the same of the rows' norms: of v and dout, for the backward call
+    const float *out, *lse;
+    float *lse2, *delta; // [batch][heads][queries padded]: lse log2(e) (+inf where there is none: no probability), and dO . O
+    // forward
+    float *to, *to_lse, *part;
+    int splits;
+    // backward
+    AttnOperand grad_q, grad_k, grad_v;
+    int accumulate;
+};
+
+// first query row with a key, and the number of keys that some query may use
+__device__ __forceinline__ int first_query(const AttnShape& s, int length, int start) { return length == 0 ? s.queries : start < 0 ? -start : 0; }
+__device__ __forceinline__ int used_keys(const AttnShape& s, int length, int start) { return attn_limit(length, start, s.queries - 1); }
+
+struct HeadJob {
+    int job, heads, bh, b, h, rows, pad;
+    AttnOperand src;
+    float *split, *norm;
+    uint32_t* amax;
+};
+// (the operand is picked by comparisons: an index into the arguments that is not known to the compiler would put them into scratch memory)
+__device__ __forceinline__ HeadJob head_job(const TileArgs& a, int y) {
+    HeadJob j;
+    const int q = a.s.batch * a.s.heads, k = a.s.batch * a.s.kv_heads;
+    j.job = y < q ? kQ : y < q + k ? kK : y < q + 2 * k ? kV : kDO;
+    const bool key = j.job == kK || j.job == kV;
+    j.bh = j.job == kQ ? y : j.job == kK ? y - q : j.job == kV ? y - q - k : y - q - 2 * k;
+    j.heads = key ? a.s.kv_heads : a.s.heads;
+    j.b = j.bh / j.heads;
+    j.h = j.bh - j.b * j.heads;
+    j.rows = key ? a.s.keys : a.s.queries;
+    j.pad = row_pad(j.rows);
+#define TENMO_PICK(x) (j.job == kQ ? a.x[kQ] : j.job == kK ? a.x[kK] : j.job == kV ? a.x[kV] : a.x[kDO])
+    j.src.p = TENMO_PICK(src).p;
+    j.src.b = TENMO_PICK(src).b;
+    j.src.s = TENMO_PICK(src).s;
+    j.src.h = TENMO_PICK(src).h;
+    j.src.d = TENMO_PICK(src).d;
+    j.split = TENMO_PICK(split);
+    j.norm = TENMO_PICK(norm);
+    j.amax = TENMO_PICK(amax);
+#undef TENMO_PICK
+    return j;
+}
+
+// largest magnitude (and norm) of the rows that count, delta and the base-2 lse: a run of a head's rows each workgroup, L lanes a row
+template <int L>
+__global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
+    constexpr int SLOTS = 64 / L;
+    __shared__ uint32_t top_of[4];
+    __shared__ float norm_of[4];
+    const HeadJob j = head_job(a, blockIdx.y);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = lane % L, D = a.s.dim;
+    const int length = attn_length(a.s, j.b), start = attn_start(a.s, j.b);
+    const bool query = j.job == kQ || j.job == kDO;
+    const int lo = query ? first_query(a.s, length, start) : 0, hi = query ? a.s.queries : used_keys(a.s, length, start);
+    const AttnOperand& src = j.src;
+    const float* p = src.p + j.b * src.b + j.h * src.h + 4 * part * src.d;
+    const int all = j.job == kDO ? j.pad : j.rows, per = (all + a.parts - 1) / a.parts;
+    const int first = blockIdx.x * per, last = first + per < all ? first + per : all;
+    uint32_t top = 0;
+    float norm = 0.f;
+    for (int r = first + wave * SLOTS + lane / L; __any(r < last); r += 4 * SLOTS) {
+        const bool in = r < last && r >= lo && r < hi;
+        f32x4 x{0.f, 0.f, 0.f, 0.f};
+        if (in) x = src.d == 1 ? attn_load4<true>(p + r * src.s, 1, part, D) : attn_load4<false>(p + r * src.s, src.d, part, D);
+        uint32_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mine = max(mine, finite_magnitude(x[e]));
+        top = max(top, mine);
+        if (j.norm) {
+            float sq = lanes_sum<L>(dot4(x, x));
+            if (!(sq < 1e37f && sq > 1e-30f)) { // out of range: the largest magnitude times sqrt(D) instead
+#pragma unroll
+                for (int d = L / 2; d > 0; d >>= 1) mine = max(mine, (uint32_t)__shfl_xor((int)mine, d, 64));
+                norm = fmaxf(norm, fminf(__uint_as_float(mine) * sqrtf((float)D), 1e38f));
+            } else norm = fmaxf(norm, sqrtf(sq));
+        }
+        if (j.job == kDO) {
+            f32x4 o{0.f, 0.f, 0.f, 0.f};
+            if (in) o = attn_load4<true>(a.out + (((int64_t)j.b * a.s.queries + r) * a.s.heads + j.h) * D + 4 * part, 1, part, D);
+            const float delta = lanes_sum<L>(dot4(x, o));
+            if (part == 0 && r < last) {
+                a.delta[(int64_t)j.bh * j.pad + r] = in ? delta : 0.f;
+                a.lse2[(int64_t)j.bh * j.pad + r] = in ? a.lse[(int64_t)j.bh * a.s.queries + r] * kLog2e : __builtin_inff();
+            }
+        }
+    }
+    top = wave_max_bits(top);
+    norm = wave_max(norm);
+    if (lane == 0) top_of[wave] = top, norm_of[wave] = norm;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        j.amax[(int64_t)j.bh * a.parts + blockIdx.x] = max(max(top_of[0], top_of[1]), max(top_of[2], top_of[3]));
+        if (j.norm) j.norm[(int64_t)j.bh * a.parts + blockIdx.x] = fmaxf(fmaxf(norm_of[0], norm_of[1]), fmaxf(norm_of[2], norm_of[3]));
+    }
+}
+
+// the scale of a head of an operand, and its largest row norm, in every lane
+__device__ __forceinline__ float head_scale(const uint32_t* __restrict amax, int parts, int64_t bh) {
+    const int lane = threadIdx.x & 63;
+    return split_scale(wave_max_bits(lane < parts ? amax[bh * parts + lane] : 0u));
+}
+__device__ __forceinline__ float head_scale(const TileArgs& a, int job, int64_t bh) { return head_scale(a.amax[job], a.parts, bh); } // job: a constant
+__device__ __forceinline__ float head_norm(const TileArgs& a, int job, int64_t bh) {
+    const int lane = threadIdx.x & 63;
+    return wave_max(lane < a.parts ? a.norm[job][bh * a.parts + lane] : 0.f);
+}
+
+// the halves: 8 values a thread
+template <int DP>
+__global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
+    constexpr int GROUPS = DP / 8, ROWS = 64;
+    const HeadJob j = head_job(a, blockIdx.y);
+    const int length = attn_length(a.s, j.b), start = attn_start(a.s, j.b);
+    const bool query = j.job == kQ || j.job == kDO;
+    const int lo = query ? first_query(a.s, length, start) : 0, hi = query ? a.s.queries : used_keys(a.s, length, start);
+    if ((int)blockIdx.x * ROWS >= j.pad) return;
+    const float scale = head_scale(j.amax, a.parts, j.bh);
+    const AttnOperand& src = j.src;
+    const float* p = src.p + j.b * src.b + j.h * src.h;
+    for (int x = threadIdx.x; x < ROWS * GROUPS; x += 256) {
+        const int r = blockIdx.x * ROWS + x / GROUPS, d = x % GROUPS * 8;
+        f16x8 h, l;
+        f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        if (r >= lo && r < hi) {
+            const float* q = p + r * src.s + d * src.d;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                v[i] = src.d == 1 ? attn_load4<true>(q + 4 * i, 1, d / 4 + i, a.s.dim) : attn_load4<false>(q + 4 * i * src.d, src.d, d / 4 + i, a.s.dim);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            _Float16 hi16, lo16;
+            split_value(v[e >> 2][e & 3] * scale, hi16, lo16);
+            h[e] = hi16;
+            l[e] = lo16;
+        }
+        float* to = j.split + ((int64_t)j.bh * j.pad + r) * DP + d;
+        *(f16x8*)to = h;
+        *(f16x8*)(to + 4) = l;
+    }
+}
+
+// ---- tiles in LDS ------------------------------------------------------------------------------------------------------------------
+
+template <int DP>
+struct Tile {
+    static constexpr int CH = DP / 4, KD = DP / 16, ND = DP / 32, BYTES = 32 * CH * 16, BLOCKS = BYTES / 1024;
+    static constexpr bool WIDE = DP % 64 == 0;
+
+    static __device__ __forceinline__ int swizzle(int row) { return WIDE ? (row & 1) | ((row >> 1) & 6) | ((row & 2) << 2) : (row >> 1) & 7; }
+
+    // this lane's byte offsets for the 1 KiB blocks wave, wave + 4, .. of N tiles that lie one behind the other
+    template <int N>
+    static __device__ __forceinline__ void offsets(uint32_t (&off)[N * BLOCKS / 4], int wave, int lane) {
+#pragma unroll
+        for (int i = 0; i < N * BLOCKS / 4; ++i) {
+            const int x = (i * 4 + wave) % BLOCKS * 64 + lane, row = x / CH, slot = x % CH;
+            off[i] = (uint32_t)(row * CH + (slot ^ swizzle(row))) * 16u;
+        }
+    }
+    // N tiles from src[0 ..] (the same rows of N operands) into LDS
+    template <int N>
+    static __device__ __forceinline__ void load(float* lds, uint32_t at, const float* const (&src)[N], const uint32_t (&off)[N * BLOCKS / 4], int wave) {
+#pragma unroll
+        for (int i = 0; i < N * BLOCKS / 4; ++i) {
+            const int block = i * 4 + wave; // blocks of a tile come in fours: the tile does not depend on the wavefront
+            direct_load_16B(lds, at + (uint32_t)block * 1024u, off[i], src[i * 4 / BLOCKS]);
+        }
+    }
+    // row operand: lane % 32 is the row, lane / 32 the half of 16 values of d
+    static __device__ __forceinline__ uint32_t row_offset(int lane, int kind) {
+        const int r = lane & 31;
+        return (uint32_t)(r * CH + ((2 * (lane >> 5) + kind) ^ swizzle(r))) * 16u;
+    }
+    static __device__ __forceinline__ f16x8 row_read(const char* tile, uint32_t off, int ks) {
+        constexpr int XM = WIDE ? 3 : 1;
+        return *(const f16x8*)(tile + (off ^ ((ks & XM) * 64)) + (ks & ~XM) * 64);
+    }
+    // column operand: lane % 32 is the value of d (of 32), the 8 values rows 16 t + 4 (lane / 32) + {0..3, 8..11}
+    static __device__ __forceinline__ uint32_t column_offset(int lane, int kind) {
+        const int p = lane & 15, sub = (lane >> 4) & 1, row = 4 * (lane >> 5) + (p >> 2);
+        return (uint32_t)(row * CH + ((4 * sub + 2 * ((p & 3) >> 1) + kind) ^ swizzle(row))) * 16u + 8u * (p & 1);
+    }
+    static __device__ __forceinline__ f16x8 column_read(const char* tile, uint32_t off, int t, int db) {
+        typedef __attribute__((address_space(3))) i16x4* lds_p;
+        union { i16x4 s[2]; f16x8 v; } x;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint32_t at = WIDE ? (off ^ (u * 64) ^ ((db & 1) * 128)) + (db >> 1) * 256 : (off ^ (u * 64)) + db * 128;
+            x.s[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + at + (16 * t + 8 * u) * CH * 16));
+        }
+        return x.v;
+    }
+};
+
+// c += a b of 32 x 32 x 16 with both operands as halves
+__device__ __forceinline__ void split_mfma(f32x16& c, f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z[e] = 0.f;
+    return z;
+}
+// registers 8 t .. 8 t + 7 of a product as an operand
+__device__ __forceinline__ void halves(const f32x16& x, int t, f16x8& h, f16x8& l) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const _Float16 hi = (_Float16)x[8 * t + e];
+        h[e] = hi;
+        l[e] = (_Float16)(x[8 * t + e] - (float)hi);
+    }
+}
+// row operand of the wavefront's own 32 rows, straight from memory
+template <int DP>
+__device__ __forceinline__ void own_rows(f16x8 (&h)[DP / 16], f16x8 (&l)[DP / 16], const float* rows, int lane) {
+    const float* p = rows + (lane & 31) * DP + 8 * (lane >> 5);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+        h[ks] = *(const f16x8*)(p + 16 * ks);
+        l[ks] = *(const f16x8*)(p + 16 * ks + 4);
+    }
+}
+// register e of a product is row 8 (e / 4) + 4 (lane / 32) + e % 4
+__device__ __forceinline__ int reg_row(int e) { return 8 * (e >> 2) + (e & 3); }
+
+// a workgroup's head and block of rows: heads are dealt to the XCDs, so that one head's rows meet in one L2; blocks of a head in descending order (the long ones of a causal mask first)
+__device__ __forceinline__ void head_and_block(int id, int heads, int blocks, bool descending, int* bh, int* block) {
+    int t = id;
+    if (heads % 8 == 0) {
+        t = id / 8;
+        *bh = __builtin_amdgcn_readfirstlane(id % 8 + 8 * (t / blocks));
+    } else *bh = __builtin_amdgcn_readfirstlane(t / blocks);
+    t %= blocks;
+    *block = __builtin_amdgcn_readfirstlane(descending ? blocks - 1 - t : t);
+}
+
+// ---- forward -------------------------------------------------------------------------------------------------------------------------
+
+template <int DP>
+__global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArgs a) {
+    using T = Tile<DP>;
+    constexpr int STAGES = DP <= 64 ? 3 : 2, LOADS = 2 * T::BLOCKS / 4;
+    __shared__ __align__(1024) float lds[STAGES * 2 * T::BYTES / 4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, D = a.s.dim;
+    const int pad_q = row_pad(a.s.queries), pad_k = row_pad(a.s.keys), q_blocks = pad_q / kRowPad;
+    int bh, block;
+    const int split = blockIdx.x % a.splits;
+    head_and_block(blockIdx.x / a.splits, a.s.batch * a.s.heads, q_blocks, true, &bh, &block);
+    const int b = bh / a.s.heads, h = bh % a.s.heads, bk = b * a.s.kv_heads + h / a.s.group;
+    const int length = attn_length(a.s, b), start = attn_start(a.s, b);
+    const int q0 = block * kRowPad + wave * 32, i = q0 + (lane & 31);
+    const int limit = i < a.s.queries ? attn_limit(length, start, i) : 0;
+    const int wave_last = q0 + 31 < a.s.queries ? q0 + 31 : a.s.queries - 1, block_last = (block + 1) * kRowPad < a.s.queries ? (block + 1) * kRowPad - 1 : a.s.queries - 1;
+    const int wave_most = q0 < a.s.queries ? attn_limit(length, start, wave_last) : 0, wave_least = wave_last == q0 + 31 ? attn_limit(length, start, q0) : 0;
+    const int tiles = (attn_limit(length, start, block_last) + 31) / 32, per = (tiles + a.splits - 1) / a.splits;
+    const int t0 = split * per < tiles ? split * per : tiles, t1 = t0 + per < tiles ? t0 + per : tiles;
+
+    f16x8 qh[T::KD], ql[T::KD];
+    own_rows<DP>(qh, ql, a.split[kQ] + ((int64_t)bh * pad_q + q0) * DP, lane);
+    const float inv_v = 1.f / head_scale(a, kV, bk);
+    const float c = a.s.scale * kLog2e / head_scale(a, kQ, bh) / head_scale(a, kK, bk);
+    const float* const base[2] = {a.split[kK] + (int64_t)bk * pad_k * DP, a.split[kV] + (int64_t)bk * pad_k * DP};
+    uint32_t off[LOADS];
+    T::template offsets<2>(off, wave, lane);
+    auto load = [&](int t, int stage) {
+        const float* const src[2] = {base[0] + (int64_t)t * 32 * DP, base[1] + (int64_t)t * 32 * DP};
+        T::template load<2>(lds, stage * 2 * T::BYTES, src, off, wave);
+    };
+    const uint32_t row_off[2] = {T::row_offset(lane, 0), T::row_offset(lane, 1)}, col_off[2] = {T::column_offset(lane, 0), T::column_offset(lane, 1)};
+
+    f32x16 o[T::ND];
+#pragma unroll
+    for (int d = 0; d < T::ND; ++d) o[d] = zero16();
+    float m = kNone, l = 0.f;
+    if (t0 < t1) load(t0, 0);
+    if (STAGES == 3 && t0 + 1 < t1) load(t0 + 1, 1);
+    int stage = 0;
+    for (int t = t0; t < t1; ++t) {
+        if (STAGES == 3 && t + 1 < t1) stage_barrier<LOADS>();
+        else stage_barrier<0>();
+        if (t + STAGES - 1 < t1) load(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+        const char* ks_tile = (const char*)lds + stage * 2 * T::BYTES;
+        const char* vs_tile = ks_tile + T::BYTES;
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
+        if (t * 32 >= wave_most) continue; // nothing here for these 32 queries (every wavefront meets at the next barrier)
+        f32x16 s = zero16();
+#pragma unroll
+        for (int ks = 0; ks < T::KD; ++ks) split_mfma(s, T::row_read(ks_tile, row_off[0], ks), T::row_read(ks_tile, row_off[1], ks), qh[ks], ql[ks]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] *= c;
+        if (t * 32 + 32 > wave_least) {
+            const int left = limit - t * 32 - 4 * half;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = reg_row(e) < left ? s[e] : kNone;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (__any(top > m + kRenew)) { // (an m of -inf is passed by any score)
+            const float now = top > m + kRenew ? top : m, keep = m == kNone ? 0.f : __builtin_amdgcn_exp2f(m - now);
+            m = now;
+            l *= keep;
+#pragma unroll
+            for (int d = 0; d < T::ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[d][e] *= keep;
+        }
+        const float shift = kPBits - (m == kNone ? 0.f : m);
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            s[e] = __builtin_amdgcn_exp2f(s[e] + shift);
+            sum += s[e];
+        }
+        l += sum;
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+            f16x8 ph, pl;
+            halves(s, t2, ph, pl);
+#pragma unroll
+            for (int d = 0; d < T::ND; ++d) split_mfma(o[d], T::column_read(vs_tile, col_off[0], t2, d), T::column_read(vs_tile, col_off[1], t2, d), ph, pl);
+        }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (i >= a.s.queries) return;
+    const int64_t row = (int64_t)bh * a.s.queries + i;
+    float* to;
+    float factor;
+    if (a.part) {
+        to = a.part + ((int64_t)split * a.s.batch * a.s.heads * a.s.queries + row) * (D + 2);
+        factor = inv_v * (1.f / 128.f);
+        if (half == 0) to[D] = m * kLn2, to[D + 1] = l * (1.f / 128.f);
+    } else {
+        to = a.to + (((int64_t)b * a.s.queries + i) * a.s.heads + h) * D;
+        factor = l == 0.f ? 0.f : inv_v / l;
+        if (half == 0 && a.to_lse) a.to_lse[row] = l == 0.f ? kNone : (m + __builtin_amdgcn_logf(l) - kPBits) * kLn2;
+    }
+#pragma unroll
+    for (int d = 0; d < T::ND; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int at = 32 * d + 8 * q + 4 * half;
+            const f32x4 x{o[d][4 * q] * factor, o[d][4 * q + 1] * factor, o[d][4 * q + 2] * factor, o[d][4 * q + 3] * factor};
+            if (at + 3 < D) *(f32x4_u*)(to + at) = x;
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (at + e < D) to[at + e] = x[e];
+        }
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------------------------
+
+// 2^15 over the largest that |dS| can be, as a power of two
+__device__ __forceinline__ float ds_scale(const TileArgs& a, int64_t bh, int64_t bk) {
+    const float bound = 2.f * head_norm(a, kDO, bh) * head_norm(a, kV, bk);
+    const int e = (int)(__float_as_uint(fminf(bound, 1e38f)) >> 23) - 127 + 1; // bound < 2^e
+    const int up = 15 - e;
+    return __uint_as_float((uint32_t)((up > 126 ? 126 : up) + 127) << 23);
+}
+
+__device__ __forceinline__ void store_gradient(const AttnOperand& g, int64_t at, int d, int D, f32x4 x, int accumulate) {
+    float* to = g.p + at + d * g.d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (d + e < D) to[e * g.d] = accumulate ? to[e * g.d] + x[e] : x[e];
+}
+
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(const TileArgs a) {
+    using T = Tile<DP>;
+    constexpr int STAGES = DP <= 64 ? 3 : 2, LOADS = 2 * T::BLOCKS / 4;
+    __shared__ __align__(1024) float lds[STAGES * 2 * T::BYTES / 4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, D = a.s.dim;
+    const int pad_q = row_pad(a.s.queries), pad_k = row_pad(a.s.keys), k_blocks = pad_k / kRowPad;
+    int bk, block;
+    head_and_block(blockIdx.x, a.s.batch * a.s.kv_heads, k_blocks, false, &bk, &block);
+    const int b = bk / a.s.kv_heads, hk = bk % a.s.kv_heads;
+    const int length = attn_length(a.s, b), start = attn_start(a.s, b), keys = used_keys(a.s, length, start);
+    const int j0 = block * kRowPad + wave * 32, j = j0 + (lane & 31);
+    // query i sees key j when i >= j - start and j < length
+    const int see = a.s.causal ? j - start : 0;
+    const int wave_first = a.s.causal && j0 - start > 0 ? j0 - start : 0, block_first = a.s.causal && block * kRowPad - start > 0 ? block * kRowPad - start : 0;
+    const int tile0 = block_first / 32, tile1 = block * kRowPad < keys ? (a.s.queries + 31) / 32 : 0, tiles = tile1 > tile0 ? tile1 - tile0 : 0;
+
+    f16x8 kh[T::KD], kl[T::KD], vh[T::KD], vl[T::KD];
+    own_rows<DP>(kh, kl, a.split[kK] + ((int64_t)bk * pad_k + j0) * DP, lane);
+    own_rows<DP>(vh, vl, a.split[kV] + ((int64_t)bk * pad_k + j0) * DP, lane);
+    const float scale_k = head_scale(a, kK, bk), scale_v = head_scale(a, kV, bk);
+    uint32_t off[LOADS];
+    T::template offsets<2>(off, wave, lane);
+    const uint32_t row_off[2] = {T::row_offset(lane, 0), T::row_offset(lane, 1)}, col_off[2] = {T::column_offset(lane, 0), T::column_offset(lane, 1)};
+
+    f32x16 dk_all[T::ND], dv_all[T::ND]; // over the heads of the group
+    float inv_dk = 0.f, inv_dv = 0.f;
+#pragma unroll
+    for (int d = 0; d < T::ND; ++d) dk_all[d] = dv_all[d] = zero16();
+    const int total = tiles * a.s.group;
+    auto load = [&](int t, int stage) {
+        const int64_t at = ((int64_t)(b * a.s.heads + hk * a.s.group + t / tiles) * pad_q + (tile0 + t % tiles) * 32) * DP;
+        const float* const src[2] = {a.split[kQ] + at, a.split[kDO] + at};
+        T::template load<2>(lds, stage * 2 * T::BYTES, src, off, wave);
+    };
+    if (total > 0) load(0, 0);
+    if (STAGES == 3 && total > 1) load(1, 1);
+    int stage = 0;
+    float c = 0.f, inv_dp = 0.f, ds_up = 0.f, p_up = 0.f;
+    for (int t = 0; t < total; ++t) {
+        if (STAGES == 3 && t + 1 < total) stage_barrier<LOADS>();
+        else stage_barrier<0>();
+        if (t + STAGES - 1 < total) load(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+        const char* q_tile = (const char*)lds + stage * 2 * T::BYTES;
+        const char* g_tile = q_tile + T::BYTES;
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
+        const int64_t bh = b * a.s.heads + hk * a.s.group + t / tiles;
+        if (t % tiles == 0) { // the next head of the group.  The sums are kept in the largest head's units (powers of two): nothing overflows that the result holds
+            const float scale_q = head_scale(a, kQ, bh), scale_g = head_scale(a, kDO, bh);
+            c = a.s.scale * kLog2e / scale_q / scale_k;
+            inv_dp = 1.f / scale_g / scale_v;
+            ds_up = ds_scale(a, bh, bk);
+            p_up = 16384.f;
+            const float next_dk = 1.f / ds_up / scale_q, next_dv = 1.f / p_up / scale_g;
+            float fk = 1.f, fv = 1.f;
+            if (t == 0 || next_dk > inv_dk) fk = inv_dk / next_dk, inv_dk = next_dk;
+            else if (next_dk < inv_dk) ds_up *= next_dk / inv_dk;
+            if (t == 0 || next_dv > inv_dv) fv = inv_dv / next_dv, inv_dv = next_dv;
+            else if (next_dv < inv_dv) p_up *= next_dv / inv_dv;
+            if (t > 0 && (fk != 1.f || fv != 1.f))
+#pragma unroll
+                for (int d = 0; d < T::ND; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) dk_all[d][e] *= fk, dv_all[d][e] *= fv;
+        }
+        const int i0 = (tile0 + t % tiles) * 32;
+        if (i0 + 31 < wave_first || j0 >= keys) continue;
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int ks = 0; ks < T::KD; ++ks) {
+            split_mfma(s, T::row_read(q_tile, row_off[0], ks), T::row_read(q_tile, row_off[1], ks), kh[ks], kl[ks]);
+            split_mfma(dp, T::row_read(g_tile, row_off[0], ks), T::row_read(g_tile, row_off[1], ks), vh[ks], vl[ks]);
+        }
+        const bool edge = i0 < j0 + 31 - start || j0 + 32 > length;
+        const float* lse2 = a.lse2 + bh * pad_q + i0 + 4 * half;
+        const float* delta = a.delta + bh * pad_q + i0 + 4 * half;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 lse4 = *(const f32x4*)(lse2 + 8 * q), delta4 = *(const f32x4*)(delta + 8 * q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = 4 * q + e;
+                float p = __builtin_amdgcn_exp2f(s[r] * c - lse4[e]);
+                float ds = p * (dp[r] * inv_dp - delta4[e]);
+                if (edge) {
+                    const bool ok = i0 + 4 * half + 8 * q + e >= see && j < length;
+                    p = ok ? p : 0.f;
+                    ds = ok ? ds : 0.f;
+                }
+                s[r] = p * p_up;
+                dp[r] = ds * ds_up;
+            }
+        }
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+            f16x8 ph, pl, sh, sl;
+            halves(s, t2, ph, pl);
+            halves(dp, t2, sh, sl);
+#pragma unroll
+            for (int d = 0; d < T::ND; ++d) {
+                split_mfma(dv_all[d], T::column_read(g_tile, col_off[0], t2, d), T::column_read(g_tile, col_off[1], t2, d), ph, pl);
+                split_mfma(dk_all[d], T::column_read(q_tile, col_off[0], t2, d), T::column_read(q_tile, col_off[1], t2, d), sh, sl);
+            }
+        }
+    }
+    if (j >= a.s.keys) return;
+    inv_dk *= a.s.scale;
+    const int64_t at_k = b * a.grad_k.b + hk * a.grad_k.h + j * a.grad_k.s, at_v = b * a.grad_v.b + hk * a.grad_v.h + j * a.grad_v.s;
+#pragma unroll
+    for (int d = 0; d < T::ND; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int at = 32 * d + 8 * q + 4 * half;
+            f32x4 x, y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = dk_all[d][4 * q + e] * inv_dk, y[e] = dv_all[d][4 * q + e] * inv_dv;
+            if (a.grad_k.p) store_gradient(a.grad_k, at_k, at, D, x, a.accumulate);
+            if (a.grad_v.p) store_gradient(a.grad_v, at_v, at, D, y, a.accumulate);
+        }
+}
+
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(const TileArgs a) {
+    using T = Tile<DP>;
+    constexpr int STAGES = DP <= 64 ? 3 : 2, LOADS = 2 * T::BLOCKS / 4;
+    __shared__ __align__(1024) float lds[STAGES * 2 * T::BYTES / 4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, D = a.s.dim;
+    const int pad_q = row_pad(a.s.queries), pad_k = row_pad(a.s.keys), q_blocks = pad_q / kRowPad;
+    int bh, block;
+    head_and_block(blockIdx.x, a.s.batch * a.s.heads, q_blocks, true, &bh, &block);
+    const int b = bh / a.s.heads, h = bh % a.s.heads, bk = b * a.s.kv_heads + h / a.s.group;
+    const int length = attn_length(a.s, b), start = attn_start(a.s, b);
+    const int q0 = block * kRowPad + wave * 32, i = q0 + (lane & 31);
+    const int limit = i < a.s.queries ? attn_limit(length, start, i) : 0;
+    const int wave_last = q0 + 31 < a.s.queries ? q0 + 31 : a.s.queries - 1, block_last = (block + 1) * kRowPad < a.s.queries ? (block + 1) * kRowPad - 1 : a.s.queries - 1;
+    const int wave_most = q0 < a.s.queries ? attn_limit(length, start, wave_last) : 0, wave_least = wave_last == q0 + 31 ? attn_limit(length, start, q0) : 0;
+    const int tiles = (attn_limit(length, start, block_last) + 31) / 32;
+
+    f16x8 qh[T::KD], ql[T::KD], gh[T::KD], gl[T::KD];
+    own_rows<DP>(qh, ql, a.split[kQ] + ((int64_t)bh * pad_q + q0) * DP, lane);
+    own_rows<DP>(gh, gl, a.split[kDO] + ((int64_t)bh * pad_q + q0) * DP, lane);
+    const float scale_k = head_scale(a, kK, bk), ds_up = ds_scale(a, bh, bk);
+    const float c = a.s.scale * kLog2e / head_scale(a, kQ, bh) / scale_k, inv_dp = 1.f / head_scale(a, kDO, bh) / head_scale(a, kV, bk);
+    const float lse2 = a.lse2[(int64_t)bh * pad_q + i], delta = a.delta[(int64_t)bh * pad_q + i];
+    const float* const base[2] = {a.split[kK] + (int64_t)bk * pad_k * DP, a.split[kV] + (int64_t)bk * pad_k * DP};
+    uint32_t off[LOADS];
+    T::template offsets<2>(off, wave, lane);
+    auto load = [&](int t, int stage) {
+        const float* const src[2] = {base[0] + (int64_t)t * 32 * DP, base[1] + (int64_t)t * 32 * DP};
+        T::template load<2>(lds, stage * 2 * T::BYTES, src, off, wave);
+    };
+    const uint32_t row_off[2] = {T::row_offset(lane, 0), T::row_offset(lane, 1)}, col_off[2] = {T::column_offset(lane, 0), T::column_offset(lane, 1)};
+
+    f32x16 dq[T::ND];
+#pragma unroll
+    for (int d = 0; d < T::ND; ++d) dq[d] = zero16();
+    if (tiles > 0) load(0, 0);
+    if (STAGES == 3 && tiles > 1) load(1, 1);
+    int stage = 0;
+    for (int t = 0; t < tiles; ++t) {
+        if (STAGES == 3 && t + 1 < tiles) stage_barrier<LOADS>();
+        else stage_barrier<0>();
+        if (t + STAGES - 1 < tiles) load(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+        const char* k_tile = (const char*)lds + stage * 2 * T::BYTES;
+        const char* v_tile = k_tile + T::BYTES;
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
+        if (t * 32 >= wave_most) continue;
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int ks = 0; ks < T::KD; ++ks) {
+            split_mfma(s, T::row_read(k_tile, row_off[0], ks), T::row_read(k_tile, row_off[1], ks), qh[ks], ql[ks]);
+            split_mfma(dp, T::row_read(v_tile, row_off[0], ks), T::row_read(v_tile, row_off[1], ks), gh[ks], gl[ks]);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] = __builtin_amdgcn_exp2f(s[e] * c - lse2) * (dp[e] * inv_dp - delta) * ds_up;
+        if (t * 32 + 32 > wave_least) {
+            const int left = limit - t * 32 - 4 * half;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dp[e] = reg_row(e) < left ? dp[e] : 0.f;
+        }
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+            f16x8 sh, sl;
+            halves(dp, t2, sh, sl);
+#pragma unroll
+            for (int d = 0; d < T::ND; ++d) split_mfma(dq[d], T::column_read(k_tile, col_off[0], t2, d), T::column_read(k_tile, col_off[1], t2, d), sh, sl);
+        }
+    }
+    if (i >= a.s.queries) return;
+    const float factor = a.s.scale / ds_up / scale_k;
+    const int64_t at_q = b * a.grad_q.b + h * a.grad_q.h + i * a.grad_q.s;
+#pragma unroll
+    for (int d = 0; d < T::ND; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            f32x4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = dq[d][4 * q + e] * factor;
+            store_gradient(a.grad_q, at_q, 32 * d + 8 * q + 4 * half, D, x, a.accumulate);
+        }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------------
+
+int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
+
+void plan_operands(TileArgs& a, Workspace& ws, int jobs) {
+    const AttnShape& s = a.s;
+    a.jobs = jobs;
+    a.parts = std::max(1, std::min(kHeadParts, (std::max(s.queries, s.keys) + 63) / 64));
+    for (int j = 0; j < jobs; ++j) {
+        const bool key = j == kK || j == kV;
+        const int64_t heads = (int64_t)s.batch * (key ? s.kv_heads : s.heads);
+        a.split[j] = ws.take<float>(heads * row_pad(key ? s.keys : s.queries) * padded_dim(s.dim));
+        a.amax[j] = ws.take<uint32_t>(heads * a.parts);
+        if (jobs == 4 && (j == kV || j == kDO)) a.norm[j] = ws.take<float>(heads * a.parts);
+    }
+}
+
+template <int DP, int L>
+void launch_operands(const TileArgs& a, hipStream_t stream) {
+    const AttnShape& s = a.s;
+    const unsigned heads = (unsigned)(s.batch * (s.heads * (a.jobs - 2) + s.kv_heads * 2));
+    hipLaunchKernelGGL(attn_amax_kernel<L>, dim3(a.parts, heads), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(attn_split_kernel<DP>, dim3((unsigned)(std::max(row_pad(s.queries), row_pad(s.keys)) / 64), heads), dim3(256), 0, stream, a);
+}
+
+template <int DP, int L>
+void launch_forward(const TileArgs& a, hipStream_t stream) {
+    launch_operands<DP, L>(a, stream);
+    const AttnShape& s = a.s;
+    hipLaunchKernelGGL(attn_tile_forward_kernel<DP>, dim3((unsigned)(s.batch * s.heads * (row_pad(s.queries) / kRowPad) * a.splits)), dim3(256), 0, stream, a);
+}
+
+template <int DP, int L>
+void launch_backward(const TileArgs& a, hipStream_t stream) {
+    launch_operands<DP, L>(a, stream);
+    const AttnShape& s = a.s;
+    if (a.grad_k.p || a.grad_v.p)
+        hipLaunchKernelGGL(attn_tile_dkv_kernel<DP>, dim3((unsigned)(s.batch * s.kv_heads * (row_pad(s.keys) / kRowPad))), dim3(256), 0, stream, a);
+    if (a.grad_q.p) hipLaunchKernelGGL(attn_tile_dq_kernel<DP>, dim3((unsigned)(s.batch * s.heads * (row_pad(s.queries) / kRowPad))), dim3(256), 0, stream, a);
+}
+
+} // namespace
+
+void attn_tiles_forward(const AttnShape& s, const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, float* out, float* lse,
+                        Workspace& ws, int cus, hipStream_t stream, bool launch) {
+    TileArgs a{};
+    a.s = s;
+    a.src[kQ] = q; a.src[kK] = k; a.src[kV] = v;
+    a.to = out; a.to_lse = lse;
+    plan_operands(a, ws, 3);
+    // two workgroups a CU fill it; a run of fewer than 256 keys is not worth its part of the join
+    const int64_t groups = (int64_t)s.batch * s.heads * (row_pad(s.queries) / kRowPad);
+    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(2LL * cus / groups, s.keys / 256));
+    if (a.splits > 1) a.part = ws.take<float>((int64_t)a.splits * s.batch * s.heads * s.queries * (s.dim + 2));
+    if (!launch) return;
+    switch (padded_dim(s.dim)) {
+        case 32: launch_forward<32, 8>(a, stream); break;
+        case 64: launch_forward<64, 16>(a, stream); break;
+        case 96: launch_forward<96, 32>(a, stream); break;
+        default: launch_forward<128, 32>(a, stream);
+    }
+    if (a.splits > 1) attn_join(s, a.part, a.splits, out, lse, stream);
+}
+
+void attn_tiles_backward(const AttnBackward& b, Workspace& ws, hipStream_t stream, bool launch) {
+    TileArgs a{};
+    a.s = b.s;
+    a.src[kQ] = b.q; a.src[kK] = b.k; a.src[kV] = b.v;
+    a.src[kDO] = AttnOperand{const_cast<float*>(b.dout), (int64_t)b.s.queries * b.s.heads * b.s.dim, (int64_t)b.s.heads * b.s.dim, b.s.dim, 1};
+    a.out = b.out; a.lse = b.lse;
+    a.grad_q = b.grad_q; a.grad_k = b.grad_k; a.grad_v = b.grad_v; a.accumulate = b.accumulate;
+    plan_operands(a, ws, 4);
+    a.lse2 = ws.take<float>((int64_t)b.s.batch * b.s.heads * row_pad(b.s.queries));
+    a.delta = ws.take<float>((int64_t)b.s.batch * b.s.heads * row_pad(b.s.queries));
+    if (!launch) return;
+    switch (padded_dim(b.s.dim)) {
+        case 32: launch_backward<32, 8>(a, stream); break;
+        case 64: launch_backward<64, 16>(a, stream); break;
+        case 96: launch_backward<96, 32>(a, stream); break;
+        default: launch_backward<128, 32>(a, stream);
+    }
+}
+
+} // namespace tenmo

@@ -7,7 +7,7 @@
 // fetched in the same one.  The running maximum m is renewed when a score passes it by 2^8 (p and the sums keep to the range of their types below that).
 //
 // Backward, the probabilities again, without atomics and so without an order:
-//   keys:    a wavefront for 32 keys, over the queries that see them (of all heads that share the key's): S = Q K^T, dP = dO V^T,
+//   keys:    a wavefront for 32 keys of a query head, over the queries that see them: S = Q K^T, dP = dO V^T,
 //            P = 2^(S c - lse), dS = P (dP - delta); dV^T += dO^T P, dK^T += Q^T dS.
 //   queries: a wavefront for 32 queries, over their keys: S^T, dP^T, dS^T; dQ^T += K^T dS^T.
 // Seven products for the five that one pass with atomics would need.
@@ -45,13 +45,14 @@ struct TileArgs {
     uint32_t* amax[4];  // [batch * heads][parts]
     float* norm[4];     // the same of the rows' norms: of v and dout, for the backward call
     const float *out, *lse;
-    float *lse2, *delta; // [batch][heads][queries padded]: lse log2(e) (+inf where there is none: no probability), and dO . O
+    f32x2* stats;        // [batch][heads][queries padded] (and 128 behind the last): lse log2(e) (+inf where there is none: no probability), and dO . O
     // forward
     float *to, *to_lse, *part;
     int splits;
     // backward
     AttnOperand grad_q, grad_k, grad_v;
     int accumulate;
+    float *part_k, *part_v; // [batch][heads][keys][dim]: each query head's part where heads share a key head
 };
 
 // first query row with a key, and the number of keys that some query may use
@@ -126,10 +127,8 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
             f32x4 o{0.f, 0.f, 0.f, 0.f};
             if (in) o = attn_load4<true>(a.out + (((int64_t)j.b * a.s.queries + r) * a.s.heads + j.h) * D + 4 * part, 1, part, D);
             const float delta = lanes_sum<L>(dot4(x, o));
-            if (part == 0 && r < last) {
-                a.delta[(int64_t)j.bh * j.pad + r] = in ? delta : 0.f;
-                a.lse2[(int64_t)j.bh * j.pad + r] = in ? a.lse[(int64_t)j.bh * a.s.queries + r] * kLog2e : __builtin_inff();
-            }
+            if (part == 0 && r < last)
+                a.stats[(int64_t)j.bh * j.pad + r] = in ? f32x2{a.lse[(int64_t)j.bh * a.s.queries + r] * kLog2e, delta} : f32x2{__builtin_inff(), 0.f};
         }
     }
     top = wave_max_bits(top);
@@ -253,14 +252,20 @@ __device__ __forceinline__ f32x16 zero16() {
     for (int e = 0; e < 16; ++e) z[e] = 0.f;
     return z;
 }
+// a 1 that the compiler takes for a variable: x * one - h, rounded to fp16, is one mixed-precision instruction, x - h converts twice
+__device__ __forceinline__ float variable_one() {
+    float one = 1.f;
+    asm volatile("" : "+v"(one));
+    return one;
+}
 // registers 8 t .. 8 t + 7 of a product as an operand
-__device__ __forceinline__ void halves(const f32x16& x, int t, f16x8& h, f16x8& l) {
+__device__ __forceinline__ void halves(const f32x16& x, int t, float one, f16x8& h, f16x8& l) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const _Float16 hi = (_Float16)x[8 * t + e];
-        h[e] = hi;
-        l[e] = (_Float16)(x[8 * t + e] - (float)hi);
-    }
+    for (int e = 0; e < 8; ++e) h[e] = (_Float16)x[8 * t + e];
+    // one h for both uses: left alone, the compiler may round a product that ends in x to fp16 by two ways that differ where x lies between two halves
+    asm("" : "+v"(h));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) l[e] = (_Float16)__builtin_fmaf(x[8 * t + e], one, -(float)h[e]);
 }
 // row operand of the wavefront's own 32 rows, straight from memory
 template <int DP>
@@ -320,6 +325,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
     };
     const uint32_t row_off[2] = {T::row_offset(lane, 0), T::row_offset(lane, 1)}, col_off[2] = {T::column_offset(lane, 0), T::column_offset(lane, 1)};
 
+    const float one = variable_one();
     f32x16 o[T::ND];
 #pragma unroll
     for (int d = 0; d < T::ND; ++d) o[d] = zero16();
@@ -369,7 +375,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
             f16x8 ph, pl;
-            halves(s, t2, ph, pl);
+            halves(s, t2, one, ph, pl);
 #pragma unroll
             for (int d = 0; d < T::ND; ++d) split_mfma(o[d], T::column_read(vs_tile, col_off[0], t2, d), T::column_read(vs_tile, col_off[1], t2, d), ph, pl);
         }
@@ -419,72 +425,64 @@ __device__ __forceinline__ void store_gradient(const AttnOperand& g, int64_t at,
         if (d + e < D) to[e * g.d] = accumulate ? to[e * g.d] + x[e] : x[e];
 }
 
+__device__ __forceinline__ void store_part(float* to, int d, int D, f32x4 x) {
+    if (d + 3 < D) *(f32x4_u*)(to + d) = x;
+    else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < D) to[d + e] = x[e];
+}
+
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(const TileArgs a) {
     using T = Tile<DP>;
-    constexpr int STAGES = DP <= 64 ? 3 : 2, LOADS = 2 * T::BLOCKS / 4;
-    __shared__ __align__(1024) float lds[STAGES * 2 * T::BYTES / 4];
+    constexpr int STAGES = DP <= 64 ? 3 : 2, LOADS = 2 * T::BLOCKS / 4 + 1, STAGE = 2 * T::BYTES + 1024;
+    __shared__ __align__(1024) float lds[STAGES * STAGE / 4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, D = a.s.dim;
     const int pad_q = row_pad(a.s.queries), pad_k = row_pad(a.s.keys), k_blocks = pad_k / kRowPad;
-    int bk, block;
-    head_and_block(blockIdx.x, a.s.batch * a.s.kv_heads, k_blocks, false, &bk, &block);
-    const int b = bk / a.s.kv_heads, hk = bk % a.s.kv_heads;
+    int bh, block;
+    head_and_block(blockIdx.x, a.s.batch * a.s.heads, k_blocks, false, &bh, &block);
+    const int b = bh / a.s.heads, h = bh % a.s.heads, hk = h / a.s.group, bk = b * a.s.kv_heads + hk;
     const int length = attn_length(a.s, b), start = attn_start(a.s, b), keys = used_keys(a.s, length, start);
     const int j0 = block * kRowPad + wave * 32, j = j0 + (lane & 31);
     // query i sees key j when i >= j - start and j < length
     const int see = a.s.causal ? j - start : 0;
     const int wave_first = a.s.causal && j0 - start > 0 ? j0 - start : 0, block_first = a.s.causal && block * kRowPad - start > 0 ? block * kRowPad - start : 0;
-    const int tile0 = block_first / 32, tile1 = block * kRowPad < keys ? (a.s.queries + 31) / 32 : 0, tiles = tile1 > tile0 ? tile1 - tile0 : 0;
+    const int t0 = block_first / 32, t1 = block * kRowPad < keys ? (a.s.queries + 31) / 32 : 0;
 
     f16x8 kh[T::KD], kl[T::KD], vh[T::KD], vl[T::KD];
     own_rows<DP>(kh, kl, a.split[kK] + ((int64_t)bk * pad_k + j0) * DP, lane);
     own_rows<DP>(vh, vl, a.split[kV] + ((int64_t)bk * pad_k + j0) * DP, lane);
-    const float scale_k = head_scale(a, kK, bk), scale_v = head_scale(a, kV, bk);
-    uint32_t off[LOADS];
+    const float scale_q = head_scale(a, kQ, bh), scale_g = head_scale(a, kDO, bh), ds_up = ds_scale(a, bh, bk);
+    const float c = a.s.scale * kLog2e / scale_q / head_scale(a, kK, bk), inv_dp = 1.f / scale_g / head_scale(a, kV, bk);
+    const float* const base[2] = {a.split[kQ] + (int64_t)bh * pad_q * DP, a.split[kDO] + (int64_t)bh * pad_q * DP};
+    const float* const stats = (const float*)(a.stats + (int64_t)bh * pad_q);
+    uint32_t off[LOADS - 1];
     T::template offsets<2>(off, wave, lane);
+    auto load = [&](int t, int stage) {
+        const float* const src[2] = {base[0] + (int64_t)t * 32 * DP, base[1] + (int64_t)t * 32 * DP};
+        T::template load<2>(lds, stage * STAGE, src, off, wave);
+        // the tile's 32 lse and delta, and 96 rows behind them that are not used: every wavefront brings the same
+        direct_load_16B(lds, stage * STAGE + 2 * T::BYTES, lane * 16, stats + (int64_t)t * 64);
+    };
     const uint32_t row_off[2] = {T::row_offset(lane, 0), T::row_offset(lane, 1)}, col_off[2] = {T::column_offset(lane, 0), T::column_offset(lane, 1)};
 
-    f32x16 dk_all[T::ND], dv_all[T::ND]; // over the heads of the group
-    float inv_dk = 0.f, inv_dv = 0.f;
+    const float one = variable_one();
+    f32x16 dk[T::ND], dv[T::ND];
 #pragma unroll
-    for (int d = 0; d < T::ND; ++d) dk_all[d] = dv_all[d] = zero16();
-    const int total = tiles * a.s.group;
-    auto load = [&](int t, int stage) {
-        const int64_t at = ((int64_t)(b * a.s.heads + hk * a.s.group + t / tiles) * pad_q + (tile0 + t % tiles) * 32) * DP;
-        const float* const src[2] = {a.split[kQ] + at, a.split[kDO] + at};
-        T::template load<2>(lds, stage * 2 * T::BYTES, src, off, wave);
-    };
-    if (total > 0) load(0, 0);
-    if (STAGES == 3 && total > 1) load(1, 1);
+    for (int d = 0; d < T::ND; ++d) dk[d] = dv[d] = zero16();
+    if (t0 < t1) load(t0, 0);
+    if (STAGES == 3 && t0 + 1 < t1) load(t0 + 1, 1);
     int stage = 0;
-    float c = 0.f, inv_dp = 0.f, ds_up = 0.f, p_up = 0.f;
-    for (int t = 0; t < total; ++t) {
-        if (STAGES == 3 && t + 1 < total) stage_barrier<LOADS>();
+    for (int t = t0; t < t1; ++t) {
+        if (STAGES == 3 && t + 1 < t1) stage_barrier<LOADS>();
         else stage_barrier<0>();
-        if (t + STAGES - 1 < total) load(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-        const char* q_tile = (const char*)lds + stage * 2 * T::BYTES;
+        if (t + STAGES - 1 < t1) load(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+        const char* q_tile = (const char*)lds + stage * STAGE;
         const char* g_tile = q_tile + T::BYTES;
+        const f32x4* st = (const f32x4*)(g_tile + T::BYTES) + 2 * half; // two rows each
         stage = stage == STAGES - 1 ? 0 : stage + 1;
-        const int64_t bh = b * a.s.heads + hk * a.s.group + t / tiles;
-        if (t % tiles == 0) { // the next head of the group.  The sums are kept in the largest head's units (powers of two): nothing overflows that the result holds
-            const float scale_q = head_scale(a, kQ, bh), scale_g = head_scale(a, kDO, bh);
-            c = a.s.scale * kLog2e / scale_q / scale_k;
-            inv_dp = 1.f / scale_g / scale_v;
-            ds_up = ds_scale(a, bh, bk);
-            p_up = 16384.f;
-            const float next_dk = 1.f / ds_up / scale_q, next_dv = 1.f / p_up / scale_g;
-            float fk = 1.f, fv = 1.f;
-            if (t == 0 || next_dk > inv_dk) fk = inv_dk / next_dk, inv_dk = next_dk;
-            else if (next_dk < inv_dk) ds_up *= next_dk / inv_dk;
-            if (t == 0 || next_dv > inv_dv) fv = inv_dv / next_dv, inv_dv = next_dv;
-            else if (next_dv < inv_dv) p_up *= next_dv / inv_dv;
-            if (t > 0 && (fk != 1.f || fv != 1.f))
-#pragma unroll
-                for (int d = 0; d < T::ND; ++d)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) dk_all[d][e] *= fk, dv_all[d][e] *= fv;
-        }
-        const int i0 = (tile0 + t % tiles) * 32;
+        const int i0 = t * 32;
         if (i0 + 31 < wave_first || j0 >= keys) continue;
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
@@ -492,41 +490,45 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(co
             split_mfma(s, T::row_read(q_tile, row_off[0], ks), T::row_read(q_tile, row_off[1], ks), kh[ks], kl[ks]);
             split_mfma(dp, T::row_read(g_tile, row_off[0], ks), T::row_read(g_tile, row_off[1], ks), vh[ks], vl[ks]);
         }
-        const bool edge = i0 < j0 + 31 - start || j0 + 32 > length;
-        const float* lse2 = a.lse2 + bh * pad_q + i0 + 4 * half;
-        const float* delta = a.delta + bh * pad_q + i0 + 4 * half;
+        f32x4 rows[8]; // lse and delta of the rows 8 q + 4 half + {0, 1}, {2, 3}
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f32x4 lse4 = *(const f32x4*)(lse2 + 8 * q), delta4 = *(const f32x4*)(delta + 8 * q);
+        for (int q = 0; q < 4; ++q) rows[2 * q] = st[4 * q], rows[2 * q + 1] = st[4 * q + 1];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = 4 * q + e;
-                float p = __builtin_amdgcn_exp2f(s[r] * c - lse4[e]);
-                float ds = p * (dp[r] * inv_dp - delta4[e]);
-                if (edge) {
-                    const bool ok = i0 + 4 * half + 8 * q + e >= see && j < length;
-                    p = ok ? p : 0.f;
-                    ds = ok ? ds : 0.f;
-                }
-                s[r] = p * p_up;
-                dp[r] = ds * ds_up;
+        for (int e = 0; e < 16; ++e) {
+            s[e] = s[e] * c - rows[e >> 1][2 * (e & 1)];
+            dp[e] = dp[e] * inv_dp - rows[e >> 1][2 * (e & 1) + 1];
+        }
+        if (i0 < j0 + 31 - start || j0 + 32 > length) { // some pairs are not allowed: their p is 0, whatever the rest
+            const int from = see - i0 - 4 * half;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const bool ok = reg_row(e) >= from && j < length;
+                s[e] = ok ? s[e] : kNone;
+                dp[e] = ok ? dp[e] : 0.f;
             }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float p = __builtin_amdgcn_exp2f(s[e]);
+            dp[e] *= p * ds_up;
+            s[e] = p * 16384.f;
         }
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
             f16x8 ph, pl, sh, sl;
-            halves(s, t2, ph, pl);
-            halves(dp, t2, sh, sl);
+            halves(s, t2, one, ph, pl);
+            halves(dp, t2, one, sh, sl);
 #pragma unroll
             for (int d = 0; d < T::ND; ++d) {
-                split_mfma(dv_all[d], T::column_read(g_tile, col_off[0], t2, d), T::column_read(g_tile, col_off[1], t2, d), ph, pl);
-                split_mfma(dk_all[d], T::column_read(q_tile, col_off[0], t2, d), T::column_read(q_tile, col_off[1], t2, d), sh, sl);
+                split_mfma(dv[d], T::column_read(g_tile, col_off[0], t2, d), T::column_read(g_tile, col_off[1], t2, d), ph, pl);
+                split_mfma(dk[d], T::column_read(q_tile, col_off[0], t2, d), T::column_read(q_tile, col_off[1], t2, d), sh, sl);
             }
         }
     }
     if (j >= a.s.keys) return;
-    inv_dk *= a.s.scale;
+    const float inv_dk = a.s.scale / ds_up / scale_q, inv_dv = 1.f / 16384.f / scale_g;
     const int64_t at_k = b * a.grad_k.b + hk * a.grad_k.h + j * a.grad_k.s, at_v = b * a.grad_v.b + hk * a.grad_v.h + j * a.grad_v.s;
+    const int64_t at_part = ((int64_t)bh * a.s.keys + j) * D;
 #pragma unroll
     for (int d = 0; d < T::ND; ++d)
 #pragma unroll
@@ -534,10 +536,33 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(co
             const int at = 32 * d + 8 * q + 4 * half;
             f32x4 x, y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = dk_all[d][4 * q + e] * inv_dk, y[e] = dv_all[d][4 * q + e] * inv_dv;
+            for (int e = 0; e < 4; ++e) x[e] = dk[d][4 * q + e] * inv_dk, y[e] = dv[d][4 * q + e] * inv_dv;
+            if (a.part_k) {
+                store_part(a.part_k + at_part, at, D, x);
+                store_part(a.part_v + at_part, at, D, y);
+                continue;
+            }
             if (a.grad_k.p) store_gradient(a.grad_k, at_k, at, D, x, a.accumulate);
             if (a.grad_v.p) store_gradient(a.grad_v, at_v, at, D, y, a.accumulate);
         }
+}
+
+// dK and dV of a key head: the parts of the query heads that share it, in order
+__global__ __launch_bounds__(256) void attn_group_kernel(const TileArgs a) {
+    const int D = a.s.dim, quads = (D + 3) / 4;
+    const AttnOperand g{blockIdx.y ? a.grad_v.p : a.grad_k.p, blockIdx.y ? a.grad_v.b : a.grad_k.b, blockIdx.y ? a.grad_v.s : a.grad_k.s,
+                        blockIdx.y ? a.grad_v.h : a.grad_k.h, blockIdx.y ? a.grad_v.d : a.grad_k.d};
+    if (!g.p) return;
+    const float* __restrict part = blockIdx.y ? a.part_v : a.part_k;
+    const int64_t all = (int64_t)a.s.batch * a.s.kv_heads * a.s.keys * quads;
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.x * 256) {
+        const int d = (int)(x % quads) * 4;
+        const int64_t row = x / quads, bk = row / a.s.keys, j = row - bk * a.s.keys, b = bk / a.s.kv_heads, hk = bk - b * a.s.kv_heads;
+        const float* p = part + (((b * a.s.heads + hk * a.s.group) * a.s.keys) + j) * D + d;
+        f32x4 sum = attn_load4<true>(p, 1, d / 4, D);
+        for (int i = 1; i < a.s.group; ++i) sum += attn_load4<true>(p + (int64_t)i * a.s.keys * D, 1, d / 4, D);
+        store_gradient(g, b * g.b + hk * g.h + j * g.s, d, D, sum, a.accumulate);
+    }
 }
 
 template <int DP>
@@ -562,7 +587,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(con
     own_rows<DP>(gh, gl, a.split[kDO] + ((int64_t)bh * pad_q + q0) * DP, lane);
     const float scale_k = head_scale(a, kK, bk), ds_up = ds_scale(a, bh, bk);
     const float c = a.s.scale * kLog2e / head_scale(a, kQ, bh) / scale_k, inv_dp = 1.f / head_scale(a, kDO, bh) / head_scale(a, kV, bk);
-    const float lse2 = a.lse2[(int64_t)bh * pad_q + i], delta = a.delta[(int64_t)bh * pad_q + i];
+    const f32x2 stats = a.stats[(int64_t)bh * pad_q + i];
+    const float lse2 = stats[0], delta = stats[1];
     const float* const base[2] = {a.split[kK] + (int64_t)bk * pad_k * DP, a.split[kV] + (int64_t)bk * pad_k * DP};
     uint32_t off[LOADS];
     T::template offsets<2>(off, wave, lane);
@@ -572,6 +598,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(con
     };
     const uint32_t row_off[2] = {T::row_offset(lane, 0), T::row_offset(lane, 1)}, col_off[2] = {T::column_offset(lane, 0), T::column_offset(lane, 1)};
 
+    const float one = variable_one();
     f32x16 dq[T::ND];
 #pragma unroll
     for (int d = 0; d < T::ND; ++d) dq[d] = zero16();
@@ -602,7 +629,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(con
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
             f16x8 sh, sl;
-            halves(dp, t2, sh, sl);
+            halves(dp, t2, one, sh, sl);
 #pragma unroll
             for (int d = 0; d < T::ND; ++d) split_mfma(dq[d], T::column_read(k_tile, col_off[0], t2, d), T::column_read(k_tile, col_off[1], t2, d), sh, sl);
         }
@@ -658,7 +685,11 @@ void launch_backward(const TileArgs& a, hipStream_t stream) {
     launch_operands<DP, L>(a, stream);
     const AttnShape& s = a.s;
     if (a.grad_k.p || a.grad_v.p)
-        hipLaunchKernelGGL(attn_tile_dkv_kernel<DP>, dim3((unsigned)(s.batch * s.kv_heads * (row_pad(s.keys) / kRowPad))), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(attn_tile_dkv_kernel<DP>, dim3((unsigned)(s.batch * s.heads * (row_pad(s.keys) / kRowPad))), dim3(256), 0, stream, a);
+    if ((a.grad_k.p || a.grad_v.p) && a.part_k) {
+        const int64_t quads = (int64_t)s.batch * s.kv_heads * s.keys * ((s.dim + 3) / 4);
+        hipLaunchKernelGGL(attn_group_kernel, dim3((unsigned)std::min<int64_t>((quads + 255) / 256, 4096), 2), dim3(256), 0, stream, a);
+    }
     if (a.grad_q.p) hipLaunchKernelGGL(attn_tile_dq_kernel<DP>, dim3((unsigned)(s.batch * s.heads * (row_pad(s.queries) / kRowPad))), dim3(256), 0, stream, a);
 }
 
@@ -693,8 +724,11 @@ void attn_tiles_backward(const AttnBackward& b, Workspace& ws, hipStream_t strea
     a.out = b.out; a.lse = b.lse;
     a.grad_q = b.grad_q; a.grad_k = b.grad_k; a.grad_v = b.grad_v; a.accumulate = b.accumulate;
     plan_operands(a, ws, 4);
-    a.lse2 = ws.take<float>((int64_t)b.s.batch * b.s.heads * row_pad(b.s.queries));
-    a.delta = ws.take<float>((int64_t)b.s.batch * b.s.heads * row_pad(b.s.queries));
+    a.stats = ws.take<f32x2>((int64_t)b.s.batch * b.s.heads * row_pad(b.s.queries) + kRowPad);
+    if (b.s.group > 1) {
+        a.part_k = ws.take<float>((int64_t)b.s.batch * b.s.heads * b.s.keys * b.s.dim);
+        a.part_v = ws.take<float>((int64_t)b.s.batch * b.s.heads * b.s.keys * b.s.dim);
+    }
     if (!launch) return;
     switch (padded_dim(b.s.dim)) {
         case 32: launch_backward<32, 8>(a, stream); break;

@@ -12,6 +12,7 @@
 
 namespace tenmo {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 // 16 bytes at a 4-byte boundary: global memory takes such an access as one instruction
 typedef f32x4 f32x4_u __attribute__((aligned(4)));

@@ -55,17 +55,13 @@ __device__ __forceinline__ float split_scale(uint32_t bits) {
     return __uint_as_float((uint32_t)((e > 126 ? 126 : e) + 127) << 23); // e >= 14 - 127
 }
 
+// (x is the last operation's fp32 result in both uses, or exact: the compiler may otherwise round a product to fp16 by two ways)
 __device__ __forceinline__ void split_value(float x, _Float16& h, _Float16& l) {
+    asm("" : "+v"(x));
     h = (_Float16)x;
     const float r = x - (float)h;
     l = (_Float16)(r - r == 0.f ? r : 0.f); // x not finite: h alone
 }
-// for values known to be finite
-__device__ __forceinline__ void split_finite(float x, _Float16& h, _Float16& l) {
-    h = (_Float16)x;
-    l = (_Float16)(x - (float)h);
-}
-
 // ---- the product ----------------------------------------------------------------------------------------------------------------
 
 // C[m, n] = sum over k of A[m, k] B[k, n] for a tile of BM x BN, wavefronts 2 x 2, K in steps of 16 through a ring of three stages in LDS

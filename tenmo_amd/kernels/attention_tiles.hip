@@ -240,6 +240,11 @@ struct Tile {
     }
 };
 
+// The order of a tile's instructions: the compiler otherwise reads an operand from LDS right before the product that takes it, and one or two wavefronts a SIMD
+// wait for most of these reads.
+#define TENMO_READS(n) __builtin_amdgcn_sched_group_barrier(0x100, n, 0)
+#define TENMO_PRODUCTS(n) __builtin_amdgcn_sched_group_barrier(0x008, n, 0)
+
 // c += a b of 32 x 32 x 16 with both operands as halves
 __device__ __forceinline__ void split_mfma(f32x16& c, f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, c, 0, 0, 0);
@@ -280,15 +285,14 @@ __device__ __forceinline__ void own_rows(f16x8 (&h)[DP / 16], f16x8 (&l)[DP / 16
 // register e of a product is row 8 (e / 4) + 4 (lane / 32) + e % 4
 __device__ __forceinline__ int reg_row(int e) { return 8 * (e >> 2) + (e & 3); }
 
-// a workgroup's head and block of rows: heads are dealt to the XCDs, so that one head's rows meet in one L2; blocks of a head in descending order (the long ones of a causal mask first)
-__device__ __forceinline__ void head_and_block(int id, int heads, int blocks, bool descending, int* bh, int* block) {
-    int t = id;
-    if (heads % 8 == 0) {
-        t = id / 8;
-        *bh = __builtin_amdgcn_readfirstlane(id % 8 + 8 * (t / blocks));
-    } else *bh = __builtin_amdgcn_readfirstlane(t / blocks);
-    t %= blocks;
-    *block = __builtin_amdgcn_readfirstlane(descending ? blocks - 1 - t : t);
+// A workgroup's head and block of rows.  Heads are dealt to the XCDs, so that one head's rows meet in one L2.  With a causal mask the blocks differ in length by the
+// number of blocks: the longest of all heads come first ([8,1024,12,64]: CUs busy for 57 % of the launch when each head's blocks followed each other).
+__device__ __forceinline__ void head_and_block(int id, int heads, int blocks, bool causal, bool last_is_longest, int* bh, int* block) {
+    const bool deal = heads % 8 == 0;
+    const int t = deal ? id / 8 : id, mine = deal ? heads / 8 : heads;
+    const int h = causal ? t % mine : t / blocks, x = causal ? t / mine : t % blocks;
+    *bh = __builtin_amdgcn_readfirstlane(deal ? id % 8 + 8 * h : h);
+    *block = __builtin_amdgcn_readfirstlane(last_is_longest ? blocks - 1 - x : x);
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------------
@@ -302,7 +306,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
     const int pad_q = row_pad(a.s.queries), pad_k = row_pad(a.s.keys), q_blocks = pad_q / kRowPad;
     int bh, block;
     const int split = blockIdx.x % a.splits;
-    head_and_block(blockIdx.x / a.splits, a.s.batch * a.s.heads, q_blocks, true, &bh, &block);
+    head_and_block(blockIdx.x / a.splits, a.s.batch * a.s.heads, q_blocks, a.s.causal, true, &bh, &block);
     const int b = bh / a.s.heads, h = bh % a.s.heads, bk = b * a.s.kv_heads + h / a.s.group;
     const int length = attn_length(a.s, b), start = attn_start(a.s, b);
     const int q0 = block * kRowPad + wave * 32, i = q0 + (lane & 31);
@@ -344,6 +348,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
         f32x16 s = zero16();
 #pragma unroll
         for (int ks = 0; ks < T::KD; ++ks) split_mfma(s, T::row_read(ks_tile, row_off[0], ks), T::row_read(ks_tile, row_off[1], ks), qh[ks], ql[ks]);
+        TENMO_READS(4);
+#pragma unroll
+        for (int ks = 0; ks < T::KD - 2; ++ks) {
+            TENMO_PRODUCTS(3);
+            TENMO_READS(2);
+        }
+        TENMO_PRODUCTS(6);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] *= c;
         if (t * 32 + 32 > wave_least) {
@@ -379,6 +390,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
 #pragma unroll
             for (int d = 0; d < T::ND; ++d) split_mfma(o[d], T::column_read(vs_tile, col_off[0], t2, d), T::column_read(vs_tile, col_off[1], t2, d), ph, pl);
         }
+        TENMO_READS(8);
+#pragma unroll
+        for (int x = 0; x < 2 * T::ND - 2; ++x) {
+            TENMO_PRODUCTS(3);
+            TENMO_READS(4);
+        }
+        TENMO_PRODUCTS(6);
     }
     l += __shfl_xor(l, 32, 64);
     if (i >= a.s.queries) return;
@@ -441,7 +459,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(co
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, D = a.s.dim;
     const int pad_q = row_pad(a.s.queries), pad_k = row_pad(a.s.keys), k_blocks = pad_k / kRowPad;
     int bh, block;
-    head_and_block(blockIdx.x, a.s.batch * a.s.heads, k_blocks, false, &bh, &block);
+    head_and_block(blockIdx.x, a.s.batch * a.s.heads, k_blocks, a.s.causal, false, &bh, &block);
     const int b = bh / a.s.heads, h = bh % a.s.heads, hk = h / a.s.group, bk = b * a.s.kv_heads + hk;
     const int length = attn_length(a.s, b), start = attn_start(a.s, b), keys = used_keys(a.s, length, start);
     const int j0 = block * kRowPad + wave * 32, j = j0 + (lane & 31);
@@ -493,6 +511,15 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(co
         f32x4 rows[8]; // lse and delta of the rows 8 q + 4 half + {0, 1}, {2, 3}
 #pragma unroll
         for (int q = 0; q < 4; ++q) rows[2 * q] = st[4 * q], rows[2 * q + 1] = st[4 * q + 1];
+        TENMO_READS(8);
+#pragma unroll
+        for (int ks = 0; ks < T::KD - 2; ++ks) {
+            TENMO_PRODUCTS(6);
+            TENMO_READS(4);
+        }
+        TENMO_PRODUCTS(6);
+        TENMO_READS(8);
+        TENMO_PRODUCTS(6);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             s[e] = s[e] * c - rows[e >> 1][2 * (e & 1)];
@@ -524,6 +551,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(co
                 split_mfma(dk[d], T::column_read(q_tile, col_off[0], t2, d), T::column_read(q_tile, col_off[1], t2, d), sh, sl);
             }
         }
+        TENMO_READS(16);
+#pragma unroll
+        for (int x = 0; x < 2 * T::ND - 2; ++x) {
+            TENMO_PRODUCTS(6);
+            TENMO_READS(8);
+        }
+        TENMO_PRODUCTS(12);
     }
     if (j >= a.s.keys) return;
     const float inv_dk = a.s.scale / ds_up / scale_q, inv_dv = 1.f / 16384.f / scale_g;
@@ -573,7 +607,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(con
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, D = a.s.dim;
     const int pad_q = row_pad(a.s.queries), pad_k = row_pad(a.s.keys), q_blocks = pad_q / kRowPad;
     int bh, block;
-    head_and_block(blockIdx.x, a.s.batch * a.s.heads, q_blocks, true, &bh, &block);
+    head_and_block(blockIdx.x, a.s.batch * a.s.heads, q_blocks, a.s.causal, true, &bh, &block);
     const int b = bh / a.s.heads, h = bh % a.s.heads, bk = b * a.s.kv_heads + h / a.s.group;
     const int length = attn_length(a.s, b), start = attn_start(a.s, b);
     const int q0 = block * kRowPad + wave * 32, i = q0 + (lane & 31);
@@ -619,6 +653,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(con
             split_mfma(s, T::row_read(k_tile, row_off[0], ks), T::row_read(k_tile, row_off[1], ks), qh[ks], ql[ks]);
             split_mfma(dp, T::row_read(v_tile, row_off[0], ks), T::row_read(v_tile, row_off[1], ks), gh[ks], gl[ks]);
         }
+        TENMO_READS(8);
+#pragma unroll
+        for (int ks = 0; ks < T::KD - 2; ++ks) {
+            TENMO_PRODUCTS(6);
+            TENMO_READS(4);
+        }
+        TENMO_PRODUCTS(12);
 #pragma unroll
         for (int e = 0; e < 16; ++e) dp[e] = __builtin_amdgcn_exp2f(s[e] * c - lse2) * (dp[e] * inv_dp - delta) * ds_up;
         if (t * 32 + 32 > wave_least) {
@@ -633,6 +674,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(con
 #pragma unroll
             for (int d = 0; d < T::ND; ++d) split_mfma(dq[d], T::column_read(k_tile, col_off[0], t2, d), T::column_read(k_tile, col_off[1], t2, d), sh, sl);
         }
+        TENMO_READS(8);
+#pragma unroll
+        for (int x = 0; x < 2 * T::ND - 2; ++x) {
+            TENMO_PRODUCTS(3);
+            TENMO_READS(4);
+        }
+        TENMO_PRODUCTS(6);
     }
     if (i >= a.s.queries) return;
     const float factor = a.s.scale / ds_up / scale_k;

@@ -8,6 +8,7 @@ library's stream waits for the current one before the launch, the current one fo
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
 
 import torch
@@ -61,13 +62,13 @@ class Launch:
                 raise TenmoHipError(-3, f"operand on {b.storage.device}: the library runs on device 0")
 
     def __enter__(self) -> C.CDLL:
-        L = load()
-        current, own = torch.cuda.current_stream(0), L.tenmo_hip_get_stream() or 0
+        L = _bound or load()
+        current, own = torch._C._cuda_getCurrentRawStream(0), L.tenmo_hip_get_stream() or 0
         self._join = None
-        if current.cuda_stream != own and not (current.cuda_stream == 0 and self._follows_default(L, own)):
-            library = torch.cuda.ExternalStream(own, device=0)
-            library.wait_stream(current)
-            self._join = (current, library)
+        if current != own and not (current == 0 and self._follows_default(L, own)):
+            stream, library = torch.cuda.current_stream(0), torch.cuda.ExternalStream(own, device=0)
+            library.wait_stream(stream)
+            self._join = (stream, library)
         return L
 
     @staticmethod
@@ -84,9 +85,27 @@ class Launch:
 
 def empty(like: NDBuffer, *shape: int) -> NDBuffer:
     n = 1
-    for s in shape:
+    strides = []
+    for s in reversed(shape):
+        strides.append(n)
         n *= s
-    return NDBuffer(torch.empty(max(n, 1), dtype=torch.float32, device=like.storage.device), shape)
+    b = NDBuffer.__new__(NDBuffer)  # (what the constructor checks holds here)
+    b.storage = torch.empty(n or 1, dtype=torch.float32, device=like.storage.device)
+    b.shape, b.strides, b.offset = shape, tuple(reversed(strides)), 0
+    return b
+
+
+_VIEW = [struct.Struct(f"@Pqi4x{rank}q{8 * (_lib.MAX_RANK - rank)}x{rank}q{8 * (_lib.MAX_RANK - rank)}x") for rank in range(_lib.MAX_RANK + 1)]
+
+
+def view(b: Optional[NDBuffer]):
+    """Of a buffer, as the library takes it."""
+    if b is None:
+        return None
+    rank = len(b.shape)
+    if rank > _lib.MAX_RANK:
+        raise TenmoHipError(-2, f"rank {rank} exceeds max_rank {_lib.MAX_RANK}")
+    return C.byref(_lib.CView.from_buffer_copy(_VIEW[rank].pack(b.storage.data_ptr(), b.offset, rank, *b.shape, *b.strides)))
 
 
 def workspace(like: NDBuffer, nbytes: int):

@@ -6,7 +6,6 @@ need no copy, and the result reshapes to [batch, queries, heads * dim] for the n
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 from typing import List, Optional, Sequence, Tuple
 
@@ -38,7 +37,7 @@ def attention(q: NDBuffer, k: NDBuffer, v: NDBuffer, scale: Optional[float] = No
         out = _t.empty(q, batch, queries, heads, dim)
         lse = _t.empty(q, batch, heads, queries) if statistics else None
         _, ws, size = _keep = _t.workspace(q, L.tenmo_hip_attention_forward_workspace_bytes(*sizes))
-        check(L.tenmo_hip_attention_forward_f32(C.byref(q.c_view()), C.byref(k.c_view()), C.byref(v.c_view()), 1.0 / math.sqrt(dim) if scale is None else scale,
+        check(L.tenmo_hip_attention_forward_f32(_t.view(q), _t.view(k), _t.view(v), 1.0 / math.sqrt(dim) if scale is None else scale,
                                                 1 if causal else 0, lengths, starts, out.data_ptr(), _t.address(lse), ws, size, 1 if sync else 0))
     return out, lse
 
@@ -59,8 +58,8 @@ def attention_backward(q: NDBuffer, k: NDBuffer, v: NDBuffer, out: NDBuffer, lse
     with _t.Launch(q, k, v, out, lse, dout, *(into or ())) as L:
         grads = tuple(into) if into is not None else tuple(_t.empty(b, *b.shape) if n else None for b, n in zip((q, k, v), need))
         _, ws, size = _keep = _t.workspace(q, L.tenmo_hip_attention_backward_workspace_bytes(*sizes))
-        views = [None if g is None else C.byref(g.c_view()) for g in grads]
-        check(L.tenmo_hip_attention_backward_f32(C.byref(q.c_view()), C.byref(k.c_view()), C.byref(v.c_view()), 1.0 / math.sqrt(dim) if scale is None else scale,
+        views = [_t.view(g) for g in grads]
+        check(L.tenmo_hip_attention_backward_f32(_t.view(q), _t.view(k), _t.view(v), 1.0 / math.sqrt(dim) if scale is None else scale,
                                                  1 if causal else 0, lengths, starts, _t.address(out), _t.address(lse), _t.address(dout), *views,
                                                  0 if into is None else 1, ws, size, 1 if sync else 0))
     return grads

@@ -134,22 +134,37 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const RowsArgs a) {
     }
 }
 
-// The runs of one row joined: a thread a value of d.
-__global__ __launch_bounds__(128) void attn_join_kernel(const AttnShape s, const float* __restrict part, int splits, float* __restrict out, float* __restrict lse) {
-    const int D = s.dim, d = threadIdx.x;
-    const int64_t row = blockIdx.x, all = (int64_t)s.batch * s.heads * s.queries;
+// The runs of one row joined: 4 wavefronts, each with every fourth run, two values of d a lane.
+__global__ __launch_bounds__(256) void attn_join_kernel(const AttnShape s, const float* __restrict part, int splits, float* __restrict out, float* __restrict lse) {
+    __shared__ float keep_of[kMostRuns], sum_of[4], o_of[4][128];
+    const int D = s.dim, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = blockIdx.x, pitch = (int64_t)s.batch * s.heads * s.queries * (D + 2);
     const float* __restrict p = part + row * (D + 2);
-    float top = kNone, sum = 0.f, o = 0.f;
-    for (int t = 0; t < splits; ++t) top = fmaxf(top, p[t * all * (D + 2) + D]);
-    for (int t = 0; t < splits; ++t) {
-        const float* __restrict x = p + t * all * (D + 2);
-        const float keep = below(x[D], top);
-        sum += keep * x[D + 1];
-        if (d < D) o += keep * x[d];
+    float top = kNone;
+    for (int t = threadIdx.x; t < splits; t += 256) top = fmaxf(top, keep_of[t] = p[t * pitch + D]);
+    top = wave_max(top);
+    if (lane == 0) sum_of[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(sum_of[0], sum_of[1]), fmaxf(sum_of[2], sum_of[3]));
+    __syncthreads();
+    float sum = 0.f;
+    for (int t = threadIdx.x; t < splits; t += 256) {
+        const float keep = below(keep_of[t], top);
+        sum += keep * p[t * pitch + D + 1];
+        keep_of[t] = keep;
     }
-    const int i = (int)(row % s.queries), h = (int)(row / s.queries % s.heads);
+    sum = group_sum<4>(sum, sum_of); // (a barrier: keep_of is whole)
+    float o[2] = {0.f, 0.f};
+    for (int t = wave; t < splits; t += 4)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (lane + 64 * e < D) o[e] += keep_of[t] * p[t * pitch + lane + 64 * e];
+    o_of[wave][lane] = o[0];
+    o_of[wave][lane + 64] = o[1];
+    __syncthreads();
+    const int i = (int)(row % s.queries), h = (int)(row / s.queries % s.heads), d = threadIdx.x;
     const int64_t b = row / s.queries / s.heads;
-    if (d < D) out[((b * s.queries + i) * s.heads + h) * D + d] = sum == 0.f ? 0.f : o / sum;
+    if (d < D) out[((b * s.queries + i) * s.heads + h) * D + d] = sum == 0.f ? 0.f : ((o_of[0][d] + o_of[1][d]) + (o_of[2][d] + o_of[3][d])) / sum;
     if (d == 0 && lse) lse[row] = sum == 0.f ? kNone : top + logf(sum);
 }
 
@@ -292,7 +307,7 @@ void attn_rows_forward(const AttnShape& s, const AttnOperand& q, const AttnOpera
     a.row_blocks = (rows + r - 1) / r;
     const int64_t groups = (int64_t)s.batch * s.kv_heads * a.row_blocks;
     // four workgroups a CU fill it (16 wavefronts); a run of fewer than 128 keys is not worth its part of the join
-    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>((4LL * cus + groups - 1) / groups, s.keys / 128));
+    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>((4LL * cus + groups - 1) / groups, std::min(s.keys / 128, kMostRuns)));
     if (a.splits > 1) a.part = ws.take<float>((int64_t)a.splits * s.batch * s.heads * s.queries * (s.dim + 2));
     if (!launch) return;
     const unsigned grid = (unsigned)(groups * a.splits);
@@ -304,7 +319,7 @@ void attn_rows_forward(const AttnShape& s, const AttnOperand& q, const AttnOpera
 }
 
 void attn_join(const AttnShape& s, const float* part, int splits, float* out, float* lse, hipStream_t stream) {
-    hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)((int64_t)s.batch * s.heads * s.queries)), dim3(128), 0, stream, s, part, splits, out, lse);
+    hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)((int64_t)s.batch * s.heads * s.queries)), dim3(256), 0, stream, s, part, splits, out, lse);
 }
 
 } // namespace tenmo

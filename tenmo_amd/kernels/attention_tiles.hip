@@ -752,7 +752,7 @@ void attn_tiles_forward(const AttnShape& s, const AttnOperand& q, const AttnOper
     plan_operands(a, ws, 3);
     // two workgroups a CU fill it; a run of fewer than 256 keys is not worth its part of the join
     const int64_t groups = (int64_t)s.batch * s.heads * (row_pad(s.queries) / kRowPad);
-    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(2LL * cus / groups, s.keys / 256));
+    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(2LL * cus / groups, std::min(s.keys / 256, kMostRuns)));
     if (a.splits > 1) a.part = ws.take<float>((int64_t)a.splits * s.batch * s.heads * s.queries * (s.dim + 2));
     if (!launch) return;
     switch (padded_dim(s.dim)) {

@@ -9,8 +9,8 @@
 //     unit stride, are read again for each pass (from the caches) by norm_*_any_kernel.
 //   * loads and stores are 16 bytes whatever the row's alignment (global memory needs 4): rows of odd length cost split cache lines,
 //     not instructions.
-//   * backward: each wavefront (or workgroup) takes every G-th row and keeps the sums of its columns for dw and db in registers; G rows of
-//     partial sums go to the workspace and are added in a fixed order by a second launch.
+//   * backward: each wavefront (or workgroup) takes every G-th row and keeps the sums of its columns for dw and db in registers; a row of partial sums a workgroup
+//     goes to the workspace, and a second launch adds them in a fixed order.
 #include "entry.hpp"
 
 #include <algorithm>
@@ -146,9 +146,11 @@ struct NormBackward {
     int accumulate;
 };
 
+// A row's x and dy are read while the row before it is worked on, where the registers allow.
 template <int W, int V4>
 __global__ __launch_bounds__(256) void norm_backward_kernel(const NormBackward a) {
     constexpr int T = W * 64, R = 256 / T; // rows a workgroup works on at a time
+    constexpr bool AHEAD = V4 <= 4;
     __shared__ float slots[2][2][4];
     const int t = threadIdx.x % T, n = (int)a.in.n;
     const float inv_n = 1.f / (float)n;
@@ -157,11 +159,23 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(const NormBackward a
     for (int k = 0; k < V4; ++k) w[k] = f32x4{1.f, 1.f, 1.f, 1.f}, sum_w[k] = sum_b[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (a.weight) load_row<T, V4>(w, a.weight, n, t);
     int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / T; row < a.in.rows; row += (int64_t)gridDim.x * R, turn ^= 1) {
+    f32x4 next_x[V4], next_dy[V4];
+    float next_mean = 0.f, next_rstd = 0.f;
+    auto load = [&](int64_t row) {
+        load_row<T, V4>(next_x, norm_row(a.in, row), n, t);
+        load_row<T, V4>(next_dy, a.dy + row * a.in.n, n, t); // zero behind the last column
+        next_mean = a.mean[row];
+        next_rstd = a.rstd[row];
+    };
+    const int64_t first = (int64_t)blockIdx.x * R + threadIdx.x / T, stride = (int64_t)gridDim.x * R;
+    if (AHEAD && first < a.in.rows) load(first);
+    for (int64_t row = first; row < a.in.rows; row += stride, turn ^= 1) {
+        if (!AHEAD) load(row);
         f32x4 x[V4], dy[V4];
-        load_row<T, V4>(x, norm_row(a.in, row), n, t);
-        load_row<T, V4>(dy, a.dy + row * a.in.n, n, t); // zero behind the last column
-        const float mean = a.mean[row], rstd = a.rstd[row];
+#pragma unroll
+        for (int k = 0; k < V4; ++k) x[k] = next_x[k], dy[k] = next_dy[k];
+        const float mean = next_mean, rstd = next_rstd;
+        if (AHEAD && row + stride < a.in.rows) load(row + stride);
         float c1 = 0.f, c2 = 0.f;
 #pragma unroll
         for (int k = 0; k < V4; ++k) {
@@ -192,9 +206,22 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(const NormBackward a
         store_row<T, V4>(g, x, n, t);
     }
     if (!a.partial) return;
-    const int64_t part = (int64_t)blockIdx.x * R + threadIdx.x / T;
-    store_row<T, V4>(a.partial + 2 * part * a.in.n, sum_w, n, t);
-    store_row<T, V4>(a.partial + (2 * part + 1) * a.in.n, sum_b, n, t);
+    float* to = a.partial + 2 * (int64_t)blockIdx.x * a.in.n;
+    if constexpr (W == 4) {
+        store_row<T, V4>(to, sum_w, n, t);
+        store_row<T, V4>(to + a.in.n, sum_b, n, t);
+    } else { // the workgroup's four rows of sums are one
+        __shared__ f32x4 sums[4][2][64 * V4];
+#pragma unroll
+        for (int k = 0; k < V4; ++k) sums[threadIdx.x / T][0][t + T * k] = sum_w[k], sums[threadIdx.x / T][1][t + T * k] = sum_b[k];
+        __syncthreads();
+        for (int c = threadIdx.x; c < 2 * 64 * V4; c += 256) {
+            const int which = c / (64 * V4), g = c - which * 64 * V4;
+            const f32x4 s = (sums[0][which][g] + sums[1][which][g]) + (sums[2][which][g] + sums[3][which][g]);
+            for (int e = 0; e < 4; ++e)
+                if (4 * g + e < n) to[which * a.in.n + 4 * g + e] = s[e];
+        }
+    }
 }
 
 __global__ __launch_bounds__(256) void norm_backward_any_kernel(const NormBackward a) { // grad_x alone
@@ -234,30 +261,28 @@ __global__ __launch_bounds__(256) void norm_columns_any_kernel(const NormBackwar
     a.partial[(2 * (int64_t)blockIdx.y + 1) * n + c] = sb;
 }
 
-// The parts of 64 columns of dw and db added up: each of the 4 wavefronts takes every fourth part, then their sums are added in order.
-__global__ __launch_bounds__(256) void norm_join_kernel(const NormBackward a) {
-    __shared__ float s[4][64];
+// The parts of 64 columns of dw or db added up: each of the 16 wavefronts takes every 16th part, then their sums are added in order.
+__global__ __launch_bounds__(1024) void norm_join_kernel(const NormBackward a) {
+    __shared__ float s[16][64];
     const int64_t n = a.in.n, c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
     const int which = blockIdx.y, wave = threadIdx.x >> 6;
     float* out = which ? a.grad_bias : a.grad_weight;
     if (!out) return; // the same in the whole workgroup
-    float v0 = 0.f, v1 = 0.f, v2 = 0.f, v3 = 0.f;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (c < n) {
         const float* __restrict p = a.partial + which * n + c;
         int64_t i = wave;
-        for (; i + 12 < a.parts; i += 16) { // four loads in flight
-            v0 += p[2 * i * n];
-            v1 += p[2 * (i + 4) * n];
-            v2 += p[2 * (i + 8) * n];
-            v3 += p[2 * (i + 12) * n];
-        }
-        for (; i < a.parts; i += 4) v0 += p[2 * i * n];
+        for (; i + 112 < a.parts; i += 128) // eight loads in flight
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] += p[2 * (i + 16 * u) * n];
+        for (; i < a.parts; i += 16) v[0] += p[2 * i * n];
     }
-    s[wave][threadIdx.x & 63] = (v0 + v1) + (v2 + v3);
+    s[wave][threadIdx.x & 63] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
     __syncthreads();
     if (wave == 0 && c < n) {
-        const float v = (s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]);
-        out[c] = a.accumulate ? out[c] + v : v;
+        float sum = s[0][threadIdx.x];
+        for (int w = 1; w < 16; ++w) sum += s[w][threadIdx.x];
+        out[c] = a.accumulate ? out[c] + sum : sum;
     }
 }
 
@@ -283,24 +308,21 @@ int norm_rows(const tenmo_view* X, const char* who, NormRows* r) {
     return 0;
 }
 
-// Rows of partial sums: enough workgroups to fill the chip twice over (measured at [8192, 768] and [30011, 2049]: 512 workgroups), each with work
-// for at least two turns where there are rows enough.
-constexpr int64_t kNormWorkgroups = 512;
-int64_t norm_parts(int64_t rows, int64_t n) {
-    const int64_t rows_at_a_time = n <= 1024 ? 4 : 1;
-    return std::max<int64_t>(1, std::min<int64_t>((rows + rows_at_a_time - 1) / rows_at_a_time, kNormWorkgroups)) * rows_at_a_time;
-}
+// Rows of partial sums, which is workgroups: enough to fill the chip two or three times over
+constexpr int64_t kNormWorkgroups = 768;
+int64_t norm_rows_at_a_time(int64_t n) { return n <= 1024 ? 4 : 1; }
+int64_t norm_parts(int64_t rows, int64_t n) { return std::max<int64_t>(1, std::min<int64_t>((rows + norm_rows_at_a_time(n) - 1) / norm_rows_at_a_time(n), kNormWorkgroups)); }
 
 template <class Args>
 using NormKernel = void (*)(Args);
 
 NormKernel<const NormForward> norm_forward_for(int64_t n) {
     return n <= 256 ? norm_forward_kernel<1, 1> : n <= 512 ? norm_forward_kernel<1, 2> : n <= 768 ? norm_forward_kernel<1, 3> : n <= 1024 ? norm_forward_kernel<1, 4>
-         : n <= 2048 ? norm_forward_kernel<4, 2> : n <= 4096 ? norm_forward_kernel<4, 4> : norm_forward_kernel<4, 8>;
+         : n <= 2048 ? norm_forward_kernel<4, 2> : n <= 3 * 1024 ? norm_forward_kernel<4, 3> : n <= 4096 ? norm_forward_kernel<4, 4> : n <= 6144 ? norm_forward_kernel<4, 6> : norm_forward_kernel<4, 8>;
 }
 NormKernel<const NormBackward> norm_backward_for(int64_t n) {
     return n <= 256 ? norm_backward_kernel<1, 1> : n <= 512 ? norm_backward_kernel<1, 2> : n <= 768 ? norm_backward_kernel<1, 3> : n <= 1024 ? norm_backward_kernel<1, 4>
-         : n <= 2048 ? norm_backward_kernel<4, 2> : n <= 4096 ? norm_backward_kernel<4, 4> : norm_backward_kernel<4, 8>;
+         : n <= 2048 ? norm_backward_kernel<4, 2> : n <= 3 * 1024 ? norm_backward_kernel<4, 3> : n <= 4096 ? norm_backward_kernel<4, 4> : n <= 6144 ? norm_backward_kernel<4, 6> : norm_backward_kernel<4, 8>;
 }
 
 } // namespace
@@ -322,7 +344,7 @@ int tenmo_hip_layer_norm_forward_f32(const tenmo_view* X, const float* weight, c
     if (a.in.rows == 0) return 0;
     a.weight = weight; a.bias = bias; a.eps = eps; a.out = out; a.mean = mean; a.rstd = rstd;
     if (a.in.n <= 8192 && (a.in.col_stride == 1 || a.in.n == 1)) {
-        const int64_t rows_at_a_time = a.in.n <= 1024 ? 4 : 1;
+        const int64_t rows_at_a_time = norm_rows_at_a_time(a.in.n);
         hipLaunchKernelGGL(norm_forward_for(a.in.n), dim3((unsigned)((a.in.rows + rows_at_a_time - 1) / rows_at_a_time)), dim3(256), 0, call.state.stream, a);
     } else {
         hipLaunchKernelGGL(norm_forward_any_kernel, dim3((unsigned)a.in.rows), dim3(256), 0, call.state.stream, a);
@@ -359,14 +381,13 @@ int tenmo_hip_layer_norm_backward_f32(const tenmo_view* X, const float* weight, 
     }
     if (a.in.rows > 0) {
         if (n <= 8192 && (a.in.col_stride == 1 || n == 1)) {
-            const int64_t blocks = norm_parts(a.in.rows, n) / (n <= 1024 ? 4 : 1);
-            hipLaunchKernelGGL(norm_backward_for(n), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+            hipLaunchKernelGGL(norm_backward_for(n), dim3((unsigned)norm_parts(a.in.rows, n)), dim3(256), 0, stream, a);
         } else {
             if (grad_X) hipLaunchKernelGGL(norm_backward_any_kernel, dim3((unsigned)a.in.rows), dim3(256), 0, stream, a);
             if (a.partial) hipLaunchKernelGGL(norm_columns_any_kernel, dim3((unsigned)((n + 255) / 256), (unsigned)a.parts), dim3(256), 0, stream, a);
         }
     }
-    if (grad_weight || grad_bias) hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)((n + 63) / 64), 2), dim3(256), 0, stream, a);
+    if (grad_weight || grad_bias) hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)((n + 63) / 64), 2), dim3(1024), 0, stream, a);
     return call.finish(sync);
 }
 

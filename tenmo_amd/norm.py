@@ -2,7 +2,6 @@
 The arithmetic is the library's (``tenmo_hip_layer_norm_*``, include/tenmo_hip_transformer.h)."""
 from __future__ import annotations
 
-import ctypes as C
 from typing import List, Optional, Sequence, Tuple
 
 from . import _transformer as _t
@@ -27,7 +26,7 @@ def layer_norm(x: NDBuffer, weight: Optional[NDBuffer] = None, bias: Optional[ND
     with _t.Launch(x, weight, bias) as L:
         out = _t.empty(x, *x.shape)
         mean, rstd = (_t.empty(x, rows), _t.empty(x, rows)) if statistics else (None, None)
-        check(L.tenmo_hip_layer_norm_forward_f32(C.byref(x.c_view()), _t.address(weight), _t.address(bias), eps, out.data_ptr(),
+        check(L.tenmo_hip_layer_norm_forward_f32(_t.view(x), _t.address(weight), _t.address(bias), eps, out.data_ptr(),
                                                  _t.address(mean), _t.address(rstd), 1 if sync else 0))
     return out, mean, rstd
 
@@ -51,7 +50,7 @@ def layer_norm_backward(x: NDBuffer, weight: Optional[NDBuffer], mean: NDBuffer,
         gx, gw, gb = into if into is not None else (_t.empty(x, *x.shape) if need_x else None, _t.empty(x, n) if need_weight else None,
                                                     _t.empty(x, n) if need_bias else None)
         _, ws, size = _keep = _t.workspace(x, L.tenmo_hip_layer_norm_backward_workspace_bytes(rows, n) if gw is not None or gb is not None else 0)
-        check(L.tenmo_hip_layer_norm_backward_f32(C.byref(x.c_view()), _t.address(weight), _t.address(mean), _t.address(rstd), _t.address(dy),
+        check(L.tenmo_hip_layer_norm_backward_f32(_t.view(x), _t.address(weight), _t.address(mean), _t.address(rstd), _t.address(dy),
                                                   _t.address(gx), _t.address(gw), _t.address(gb), 0 if into is None else 1, ws, size, 1 if sync else 0))
     return gx, gw, gb
 

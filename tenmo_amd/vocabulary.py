@@ -5,7 +5,6 @@ h is [tokens, dim], w [dim, vocabulary] (a ``Linear``'s weight, or the transpose
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import List, NamedTuple, Optional, Tuple
 
 import torch
@@ -40,7 +39,7 @@ def vocabulary_loss(h: NDBuffer, w: NDBuffer, bias: Optional[NDBuffer], target: 
     with _t.Launch(h, w, bias) as L:
         loss = Loss(_t.empty(h, m), _t.empty(h, m), _t.empty(h, 1), torch.empty(1, dtype=torch.int32, device=h.storage.device))
         _, ws, size = _keep = _t.workspace(h, L.tenmo_hip_vocabulary_loss_forward_workspace_bytes(*sizes))
-        check(L.tenmo_hip_vocabulary_loss_forward_f32(C.byref(h.c_view()), C.byref(w.c_view()), _t.address(bias), t, 1 if target.dtype == torch.int64 else 0,
+        check(L.tenmo_hip_vocabulary_loss_forward_f32(_t.view(h), _t.view(w), _t.address(bias), t, 1 if target.dtype == torch.int64 else 0,
                                                       ignore_index, label_smoothing, loss.per_sample.data_ptr(), loss.lse.data_ptr(), loss.loss_sum.data_ptr(),
                                                       loss.valid_count.data_ptr(), ws, size, 1 if sync else 0))
     return loss
@@ -71,9 +70,9 @@ def vocabulary_loss_backward(h: NDBuffer, w: NDBuffer, bias: Optional[NDBuffer],
             if need[1]:
                 gw = _t.empty(w, v, d).transpose() if w.strides[0] == 1 and d > 1 else _t.empty(w, d, v)
         _, ws, size = _keep = _t.workspace(h, L.tenmo_hip_vocabulary_loss_backward_workspace_bytes(*sizes))
-        check(L.tenmo_hip_vocabulary_loss_backward_f32(C.byref(h.c_view()), C.byref(w.c_view()), _t.address(bias), t, 1 if target.dtype == torch.int64 else 0,
+        check(L.tenmo_hip_vocabulary_loss_backward_f32(_t.view(h), _t.view(w), _t.address(bias), t, 1 if target.dtype == torch.int64 else 0,
                                                        ignore_index, label_smoothing, loss.lse.data_ptr(), up, REDUCTIONS[reduction], loss.valid_count.data_ptr(),
-                                                       _t.address(gh), None if gw is None else C.byref(gw.c_view()), _t.address(gb), 0 if into is None else 1,
+                                                       _t.address(gh), _t.view(gw), _t.address(gb), 0 if into is None else 1,
                                                        ws, size, 1 if sync else 0))
     return gh, gw, gb
 

@@ -316,14 +316,23 @@ int64_t norm_parts(int64_t rows, int64_t n) { return std::max<int64_t>(1, std::m
 template <class Args>
 using NormKernel = void (*)(Args);
 
-NormKernel<const NormForward> norm_forward_for(int64_t n) {
-    return n <= 256 ? norm_forward_kernel<1, 1> : n <= 512 ? norm_forward_kernel<1, 2> : n <= 768 ? norm_forward_kernel<1, 3> : n <= 1024 ? norm_forward_kernel<1, 4>
-         : n <= 2048 ? norm_forward_kernel<4, 2> : n <= 3 * 1024 ? norm_forward_kernel<4, 3> : n <= 4096 ? norm_forward_kernel<4, 4> : n <= 6144 ? norm_forward_kernel<4, 6> : norm_forward_kernel<4, 8>;
-}
-NormKernel<const NormBackward> norm_backward_for(int64_t n) {
-    return n <= 256 ? norm_backward_kernel<1, 1> : n <= 512 ? norm_backward_kernel<1, 2> : n <= 768 ? norm_backward_kernel<1, 3> : n <= 1024 ? norm_backward_kernel<1, 4>
-         : n <= 2048 ? norm_backward_kernel<4, 2> : n <= 3 * 1024 ? norm_backward_kernel<4, 3> : n <= 4096 ? norm_backward_kernel<4, 4> : n <= 6144 ? norm_backward_kernel<4, 6> : norm_backward_kernel<4, 8>;
-}
+// by the groups of 4 columns that a thread holds: of 64 threads, or of 256
+#define TENMO_NORM_FOR(kernel)                                                                                                                                     \
+    switch (n <= 1024 ? (n + 255) / 256 : 4 + (n + 1023) / 1024) {                                                                                                 \
+        case 1: return kernel<1, 1>;                                                                                                                               \
+        case 2: return kernel<1, 2>;                                                                                                                               \
+        case 3: return kernel<1, 3>;                                                                                                                               \
+        case 4: return kernel<1, 4>;                                                                                                                               \
+        case 6: return kernel<4, 2>;                                                                                                                               \
+        case 7: return kernel<4, 3>;                                                                                                                               \
+        case 8: return kernel<4, 4>;                                                                                                                               \
+        case 9:                                                                                                                                                    \
+        case 10: return kernel<4, 6>;                                                                                                                              \
+        default: return kernel<4, 8>;                                                                                                                              \
+    }
+NormKernel<const NormForward> norm_forward_for(int64_t n) { TENMO_NORM_FOR(norm_forward_kernel) }
+NormKernel<const NormBackward> norm_backward_for(int64_t n) { TENMO_NORM_FOR(norm_backward_kernel) }
+#undef TENMO_NORM_FOR
 
 } // namespace
 } // namespace tenmo

@@ -64,7 +64,7 @@ __device__ __forceinline__ void split_value(float x, _Float16& h, _Float16& l) {
 }
 // ---- the product ----------------------------------------------------------------------------------------------------------------
 
-// C[m, n] = sum over k of A[m, k] B[k, n] for a tile of BM x BN, wavefronts 2 x 2, K in steps of 16 through a ring of three stages in LDS
+// C[m, n] = sum over k of A[m, k] B[k, n] for a tile of 256 x 128 and the K steps k_first .., wavefronts 2 x 2, K in steps of 16 through a ring of three stages in LDS
 // (24 KiB each: two workgroups a CU), filled by direct global -> LDS loads two steps ahead, one barrier a step.
 // An operand is K-major (row m, or n, of the split matrix holds its K values) or MN-major (row k holds the values of all m, or n):
 //   * K-major stage: [row][4 chunks of 16 bytes], chunk c = 2 * (k / 8) + kind (0: h, 1: l) at slot c ^ ((row / 4) & 3): the 16 rows that a quarter of a
@@ -150,7 +150,7 @@ __device__ __forceinline__ void stage_barrier() {
 }
 
 template <bool A_KMAJOR, bool B_KMAJOR>
-__device__ __forceinline__ void split_tile(f32x16 (&acc)[4][2], float* lds, const SplitMatrix& A, int64_t m0, int64_t M, const SplitMatrix& B, int64_t n0, int64_t N, int64_t k_steps) {
+__device__ __forceinline__ void split_tile(f32x16 (&acc)[4][2], float* lds, const SplitMatrix& A, int64_t m0, int64_t M, const SplitMatrix& B, int64_t n0, int64_t N, int64_t k_first, int64_t k_steps) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TileLoader<kTileM, A_KMAJOR> la;
     TileLoader<kTileN, B_KMAJOR> lb;
@@ -168,8 +168,8 @@ __device__ __forceinline__ void split_tile(f32x16 (&acc)[4][2], float* lds, cons
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     constexpr int LOADS = TileLoader<kTileM, A_KMAJOR>::BLOCKS + TileLoader<kTileN, B_KMAJOR>::BLOCKS;
     auto load = [&](int64_t t, uint32_t stage) {
-        la.load(lds, stage * kStageBytes, wave, t);
-        lb.load(lds, stage * kStageBytes + kTileM * kStepK * 4, wave, t);
+        la.load(lds, stage * kStageBytes, wave, k_first + t);
+        lb.load(lds, stage * kStageBytes + kTileM * kStepK * 4, wave, k_first + t);
     };
     if (k_steps > 0) load(0, 0);
     if (k_steps > 1) load(1, 1);

@@ -9,7 +9,7 @@
 //   * forward: tiles of 256 words x 128 tokens; the words of a token lie in the registers of two lanes, so that a tile's maximum and sum of a token take
 //     one exchange, and 8 bytes a token and tile leave the chip instead of 1 KiB of logits.  A second launch joins the tiles of a token in a fixed order.
 //   * backward: a piece of the vocabulary at a time; the tiles of the first launch end as G in split form (|G| <= 1, so its scale is known beforehand: 2^14),
-//     which the second launch multiplies with W and with H.  The piece is as large as 512 MiB of G allow.
+//     which the second launch multiplies with W and with H.  The piece is as large as 1 GiB of G allows.
 #include "split_gemm.hpp"
 
 #include <algorithm>
@@ -18,7 +18,7 @@ namespace tenmo {
 namespace {
 
 constexpr float kGScale = 16384.f;
-constexpr int64_t kPieceValues = 128 << 20; // of G, 4 bytes each
+constexpr int64_t kPieceValues = 256 << 20; // of G, 4 bytes each
 
 struct Source { // an operand in the order in which it is split: rows x cols
     const float* p;
@@ -47,26 +47,53 @@ struct SplitJobs {
     SplitMatrix dst[2];
 };
 
+// (picked by comparisons: an index that the compiler does not know would put the arguments into scratch memory)
+__device__ __forceinline__ Source source_of(const SplitJobs& j) {
+    const bool second = blockIdx.y != 0;
+    Source s;
+    s.p = second ? j.src[1].p : j.src[0].p;
+    s.rows = second ? j.src[1].rows : j.src[0].rows;
+    s.cols = second ? j.src[1].cols : j.src[0].cols;
+    s.rs = second ? j.src[1].rs : j.src[0].rs;
+    s.cs = second ? j.src[1].cs : j.src[0].cs;
+    s.row_scale = second ? j.src[1].row_scale : j.src[0].row_scale;
+    return s;
+}
+
+// four rows of a matrix at a time: four loads in flight a thread
 __global__ __launch_bounds__(256) void vocab_amax_kernel(const SplitJobs j) {
     __shared__ uint32_t slots[4];
-    const Source& s = j.src[blockIdx.y];
+    const Source s = source_of(j);
     uint32_t top = 0;
-    for (int64_t r = blockIdx.x; r < s.rows; r += kAmaxParts) {
-        const float scale = s.row_scale ? s.row_scale[r] : 1.f;
-        const float* p = s.p + r * s.rs;
+    for (int64_t r0 = blockIdx.x; r0 < s.rows; r0 += 4 * kAmaxParts) {
+        const float* p[4];
+        float scale[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) { // (the last row again where there is none)
+            const int64_t r = r0 + u * kAmaxParts < s.rows ? r0 + u * kAmaxParts : s.rows - 1;
+            p[u] = s.p + r * s.rs;
+            scale[u] = s.row_scale ? s.row_scale[r] : 1.f;
+        }
         int64_t c = threadIdx.x * 4;
         if (s.cs == 1)
             for (; c + 3 < s.cols; c += 1024) {
-                const f32x4 x = *(const f32x4_u*)(p + c) * scale;
-                for (int e = 0; e < 4; ++e) top = max(top, finite_magnitude(x[e]));
+                f32x4 x[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[u] = *(const f32x4_u*)(p[u] + c) * scale[u];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = max(top, finite_magnitude(x[u][e]));
             }
         for (; c < s.cols; c += 1024)
-            for (int e = 0; e < 4 && c + e < s.cols; ++e) top = max(top, finite_magnitude(p[(c + e) * s.cs] * scale));
+            for (int e = 0; e < 4 && c + e < s.cols; ++e)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) top = max(top, finite_magnitude(p[u][(c + e) * s.cs] * scale[u]));
     }
     top = wave_max_bits(top);
     if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) j.amax[blockIdx.y][blockIdx.x] = max(max(slots[0], slots[1]), max(slots[2], slots[3]));
+    if (threadIdx.x == 0) (blockIdx.y ? j.amax[1] : j.amax[0])[blockIdx.x] = max(max(slots[0], slots[1]), max(slots[2], slots[3]));
 }
 
 // the scale of a matrix, from its partial maxima, in every thread of a workgroup of 256
@@ -81,9 +108,9 @@ __device__ __forceinline__ float scale_from(const uint32_t* __restrict amax, uin
 
 __global__ __launch_bounds__(256) void vocab_split_kernel(const SplitJobs j) {
     __shared__ uint32_t slots[4];
-    const Source& s = j.src[blockIdx.y];
-    const SplitMatrix& d = j.dst[blockIdx.y];
-    const float scale = scale_from(j.amax[blockIdx.y], slots);
+    const Source s = source_of(j);
+    const SplitMatrix d{blockIdx.y ? j.dst[1].p : j.dst[0].p, blockIdx.y ? j.dst[1].pitch : j.dst[0].pitch, 0};
+    const float scale = scale_from(blockIdx.y ? j.amax[1] : j.amax[0], slots);
     const int64_t groups = d.pitch / 8, all = split_pad(s.rows) * groups;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / groups, c = (i - r * groups) * 8;
@@ -115,6 +142,7 @@ struct ProductArgs {
     const uint32_t *amax_a, *amax_b; // NULL: G, whose scale is kGScale
     int64_t M, N, k_steps;
     int64_t tiles_m, tiles_n;
+    int64_t run_steps, run_stride; // K steps of a run, and floats from one run's result to the next
 };
 
 struct LogitArgs {
@@ -140,7 +168,7 @@ __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs 
     tile_of(blockIdx.x, (uint32_t)p.tiles_m, (uint32_t)p.tiles_n, &tm, &tn);
     const int64_t m0 = tm * kTileM, n0 = tn * kTileN;
     f32x16 acc[4][2];
-    split_tile<A_KMAJOR, true>(acc, lds, p.a, m0, p.M, p.b, n0, p.N, p.k_steps);
+    split_tile<A_KMAJOR, true>(acc, lds, p.a, m0, p.M, p.b, n0, p.N, 0, p.k_steps);
     const float inv = 1.f / scale_from(p.amax_a, slots[0]) / scale_from(p.amax_b, slots[1]);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int64_t v0 = m0 + (wave & 1) * 128 + 4 * half; // of the piece; register e of block i is v0 + 32 i + 8 (e / 4) + e % 4
@@ -247,11 +275,17 @@ __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs 
                         h[e] = hi;
                         l[e] = lo;
                     }
-                    if (store && v < a.g.pitch) { // 8 bytes of the group's h, and of its l: this half's four words
-                        char* group = (char*)(to + (v - 4 * half));
-                        *(f16x4*)(group + 8 * half) = h;
-                        *(f16x4*)(group + 16 + 8 * half) = l;
+                    // The two lanes of a token hold four words each of a group of eight: the lower one takes the eight h, the upper one the eight l
+                    union { f16x4 v[2]; uint32_t u[4]; f32x4 f; } x;
+                    x.v[0] = h;
+                    x.v[1] = l;
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const auto y = __builtin_amdgcn_permlane32_swap(x.u[w], x.u[2 + w], false, false);
+                        x.u[w] = y[0];
+                        x.u[2 + w] = y[1];
                     }
+                    if (store && v < a.g.pitch) *(f32x4*)(to + v) = x.f;
                 }
         }
         if (a.part_db) { // 64 values in each of 32 lanes, summed over the lanes: lane x keeps the sums of values 2 x and 2 x + 1 in bit-reversed order
@@ -279,37 +313,47 @@ __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs 
 struct StoreArgs {
     float* c;
     int64_t rs, cs;
-    const float* row_scale; // of C's rows, or NULL
     int accumulate;
 };
 
 template <bool A_KMAJOR, bool B_KMAJOR>
-__global__ __launch_bounds__(256, 2) void vocab_product_kernel(const ProductArgs p, const StoreArgs s) {
-    __shared__ __align__(1024) float lds[kStages * kStageBytes / 4];
-    __shared__ uint32_t slots[2][4];
+__device__ __forceinline__ void product_tile(const ProductArgs& p, const StoreArgs& s, uint32_t id, float* lds, uint32_t (*slots)[4]) {
     int64_t tm, tn;
-    tile_of(blockIdx.x, (uint32_t)p.tiles_m, (uint32_t)p.tiles_n, &tm, &tn);
+    const uint32_t tiles = (uint32_t)(p.tiles_m * p.tiles_n), run = id / tiles;
+    tile_of(id - run * tiles, (uint32_t)p.tiles_m, (uint32_t)p.tiles_n, &tm, &tn);
     const int64_t m0 = tm * kTileM, n0 = tn * kTileN;
+    const int64_t k0 = __builtin_amdgcn_readfirstlane((uint32_t)(run * p.run_steps));
+    const int64_t steps = p.k_steps - k0 < p.run_steps ? p.k_steps - k0 : p.run_steps;
     f32x16 acc[4][2];
-    split_tile<A_KMAJOR, B_KMAJOR>(acc, lds, p.a, m0, p.M, p.b, n0, p.N, p.k_steps);
+    split_tile<A_KMAJOR, B_KMAJOR>(acc, lds, p.a, m0, p.M, p.b, n0, p.N, k0, steps);
     float inv = 1.f / (p.amax_a ? scale_from(p.amax_a, slots[0]) : kGScale);
     inv /= p.amax_b ? scale_from(p.amax_b, slots[1]) : kGScale;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float* c = s.c + (int64_t)run * p.run_stride;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int64_t m = m0 + (wave & 1) * 128 + 32 * i + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
             if (m >= p.M) continue;
-            const float scale = s.row_scale ? s.row_scale[m] * inv : inv;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int64_t n = n0 + (wave >> 1) * 64 + 32 * j + (lane & 31);
                 if (n >= p.N) continue;
-                float* to = s.c + m * s.rs + n * s.cs;
-                *to = s.accumulate ? *to + acc[i][j][e] * scale : acc[i][j][e] * scale;
+                float* to = c + m * s.rs + n * s.cs;
+                *to = s.accumulate ? *to + acc[i][j][e] * inv : acc[i][j][e] * inv;
             }
         }
+}
+
+// Both products of a piece in one launch, since neither fills the chip evenly by itself: the first `h_tiles` workgroups are G W^T (its reduction over the words cut into runs of about the
+// length of the other's, each into a sum of its own), the others (scale H)^T G, or its transpose.
+template <bool W_KMAJOR>
+__global__ __launch_bounds__(256, 2) void vocab_products_kernel(const ProductArgs h, const StoreArgs sh, uint32_t h_tiles, const ProductArgs w, const StoreArgs sw) {
+    __shared__ __align__(1024) float lds[kStages * kStageBytes / 4];
+    __shared__ uint32_t slots[2][4];
+    if (blockIdx.x < h_tiles) product_tile<true, W_KMAJOR>(h, sh, blockIdx.x, lds, slots);
+    else product_tile<false, false>(w, sw, blockIdx.x - h_tiles, lds, slots);
 }
 
 // ---- rows ------------------------------------------------------------------------------------------------------------------------------
@@ -322,16 +366,16 @@ struct JoinArgs {
     float *loss, *lse;
 };
 
-// 64 tokens a workgroup, the tiles of each dealt to the 4 wavefronts
-__global__ __launch_bounds__(256) void vocab_join_kernel(const JoinArgs a) {
-    __shared__ float s[3][4][64];
+// 64 tokens a workgroup, the tiles of each dealt to the 16 wavefronts
+__global__ __launch_bounds__(1024) void vocab_join_kernel(const JoinArgs a) {
+    __shared__ float s[3][16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t token = (int64_t)blockIdx.x * 64 + lane, M = a.v.M;
     float top = -__builtin_inff(), sum = 0.f, sx = 0.f;
     if (token < M) {
-        for (int64_t t = wave; t < a.tiles; t += 4) top = fmaxf(top, a.part[t * M + token].x);
+        for (int64_t t = wave; t < a.tiles; t += 16) top = fmaxf(top, a.part[t * M + token].x);
         const float base = top == -__builtin_inff() ? 0.f : top;
-        for (int64_t t = wave; t < a.tiles; t += 4) {
+        for (int64_t t = wave; t < a.tiles; t += 16) {
             const float2 p = a.part[t * M + token];
             sum += p.y * __expf(p.x - base);
             if (a.part_x) sx += a.part_x[t * M + token];
@@ -340,10 +384,10 @@ __global__ __launch_bounds__(256) void vocab_join_kernel(const JoinArgs a) {
     s[0][wave][lane] = top; s[1][wave][lane] = sum; s[2][wave][lane] = sx;
     __syncthreads();
     if (wave || token >= M) return;
-    top = fmaxf(fmaxf(s[0][0][lane], s[0][1][lane]), fmaxf(s[0][2][lane], s[0][3][lane]));
+    for (int w = 1; w < 16; ++w) top = fmaxf(top, s[0][w][lane]);
     const float base = top == -__builtin_inff() ? 0.f : top;
     sum = sx = 0.f;
-    for (int w = 0; w < 4; ++w) sum += s[1][w][lane] * __expf(s[0][w][lane] - base), sx += s[2][w][lane];
+    for (int w = 0; w < 16; ++w) sum += s[1][w][lane] * __expf(s[0][w][lane] - base), sx += s[2][w][lane];
     const float lse = base + logf(sum);
     a.lse[token] = lse;
     const int64_t t = target_of(a.v, token);
@@ -390,6 +434,29 @@ __global__ __launch_bounds__(256) void vocab_row_scale_kernel(const VocabArgs v,
     scale[m] = s;
 }
 
+// dH: the runs' sums added in order, times each row's factor
+__global__ __launch_bounds__(256) void vocab_dh_kernel(const float* __restrict part, int64_t runs, int64_t M, int64_t D, const float* __restrict row_scale, float* __restrict dh, int accumulate) {
+    const int64_t all = M * D;
+    for (int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; x < all; x += (int64_t)gridDim.x * 1024) {
+        if (x + 3 < all) {
+            f32x4 s = *(const f32x4*)(part + x);
+            for (int64_t r = 1; r < runs; ++r) s += *(const f32x4_u*)(part + r * all + x);
+            const int64_t m = x / D;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] *= row_scale[x + e < (m + 1) * D ? m : (x + e) / D];
+            if (accumulate) s += *(const f32x4_u*)(dh + x);
+            *(f32x4_u*)(dh + x) = s;
+        } else {
+            for (int64_t y = x; y < all; ++y) {
+                float s = part[y];
+                for (int64_t r = 1; r < runs; ++r) s += part[r * all + y];
+                s *= row_scale[y / D];
+                dh[y] = accumulate ? dh[y] + s : s;
+            }
+        }
+    }
+}
+
 __global__ __launch_bounds__(256) void vocab_db_kernel(const float* __restrict part, int64_t parts, int64_t V, float* db, int accumulate) {
     const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (v >= V) return;
@@ -404,8 +471,9 @@ struct Plan {
     SplitMatrix h, w, hs, g;
     uint32_t *amax_h, *amax_w, *amax_hs;
     float2* part;
-    float *part_x, *target_logit, *row_scale, *part_db;
+    float *part_x, *target_logit, *row_scale, *part_db, *part_h;
     int64_t piece; // words
+    int64_t runs;  // of the words of a piece, in G W^T
 };
 
 int64_t tiles_of(int64_t n, int64_t t) { return (n + t - 1) / t; }
@@ -437,7 +505,13 @@ void plan_backward(Workspace& ws, Plan& p, int64_t M, int64_t D, int64_t V, bool
     p.part_db = ws.take<float>(2 * tiles_of(M, kTileN) * V);
     const int64_t most = std::max<int64_t>(kTileM, kPieceValues / split_pad(M) / kTileM * kTileM);
     p.piece = tiles_of(tiles_of(V, tiles_of(V, most)), kTileM) * kTileM; // pieces of equal size
-    p.g = take_split(ws, M, std::min(p.piece, V));
+    p.piece = std::min(p.piece, split_pad(V));
+    p.g = take_split(ws, M, p.piece);
+    // As many runs as bring their length near the other product's (but not below 2048), or as fill two workgroups a CU where there are fewer
+    // tiles than that, none shorter than 128 words.
+    const int64_t tiles = tiles_of(M, kTileM) * tiles_of(D, kTileN);
+    p.runs = std::max<int64_t>(1, std::max(p.piece / std::max<int64_t>(M, 2048), std::min(p.piece / 128, 512 / tiles)));
+    p.part_h = ws.take<float>(p.runs * M * D);
 }
 
 int check_sizes(int64_t M, int64_t D, int64_t V, const char* who) {
@@ -471,7 +545,7 @@ void launch_split(const SplitJobs& j, int jobs, const LibraryState& lib) {
 }
 
 ProductArgs product(const SplitMatrix& a, const uint32_t* amax_a, const SplitMatrix& b, const uint32_t* amax_b, int64_t M, int64_t N, int64_t K) {
-    return ProductArgs{a, b, amax_a, amax_b, M, N, split_pad(K) / kStepK, tiles_of(M, kTileM), tiles_of(N, kTileN)};
+    return ProductArgs{a, b, amax_a, amax_b, M, N, split_pad(K) / kStepK, tiles_of(M, kTileM), tiles_of(N, kTileN), split_pad(K) / kStepK, 0};
 }
 dim3 grid_of(const ProductArgs& p) { return dim3((unsigned)(p.tiles_m * p.tiles_n)); }
 
@@ -520,7 +594,7 @@ int tenmo_hip_vocabulary_loss_forward_f32(const tenmo_view* H, const tenmo_view*
         if (word_rows) hipLaunchKernelGGL((vocab_logits_kernel<true, false>), grid_of(g), dim3(256), 0, stream, g, a);
         else hipLaunchKernelGGL((vocab_logits_kernel<false, false>), grid_of(g), dim3(256), 0, stream, g, a);
         const JoinArgs jn{v, p.part, a.part_x, p.target_logit, g.tiles_m, per_sample_loss, lse};
-        hipLaunchKernelGGL(vocab_join_kernel, dim3((unsigned)tiles_of(v.M, 64)), dim3(256), 0, stream, jn);
+        hipLaunchKernelGGL(vocab_join_kernel, dim3((unsigned)tiles_of(v.M, 64)), dim3(1024), 0, stream, jn);
     }
     hipLaunchKernelGGL(vocab_total_kernel, dim3(1), dim3(1024), 0, stream, v, per_sample_loss, loss_sum, valid_count);
     return call.finish(sync);
@@ -558,7 +632,6 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
     if (!grad_H && !grad_W && !grad_bias) return 0;
     const hipStream_t stream = call.state.stream;
     const int add = accumulate ? 1 : 0;
-    // dW as [words][D] or [D][words]: the axis with unit stride across the lanes
     float* gw = grad_W ? const_cast<float*>(grad_W->data) + grad_W->offset : nullptr;
     const int64_t gw_d = grad_W ? grad_W->strides[0] : 0, gw_v = grad_W ? grad_W->strides[1] : 0;
     const bool word_rows = rows_of_words(W);
@@ -576,6 +649,7 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
         if (grad_W) launch_split(j, 1, call.state);
     }
     const int64_t piece = v.M > 0 ? p.piece : v.V;
+    int64_t runs = 0;
     for (int64_t first = 0; first < v.V; first += piece) {
         const int64_t words = std::min(piece, v.V - first);
         SplitMatrix G = p.g;
@@ -587,24 +661,36 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
             a.v = v; a.first = first; a.words = words; a.lse = lse; a.row_scale = p.row_scale; a.g = G; a.part_db = grad_bias ? p.part_db : nullptr;
             if (word_rows) hipLaunchKernelGGL((vocab_logits_kernel<true, true>), grid_of(g), dim3(256), 0, stream, g, a);
             else hipLaunchKernelGGL((vocab_logits_kernel<false, true>), grid_of(g), dim3(256), 0, stream, g, a);
-            if (grad_H) {
-                const ProductArgs d = product(G, nullptr, w, p.amax_w, v.M, v.D, words);
-                const StoreArgs s{grad_H, v.D, 1, p.row_scale, first > 0 || add};
-                if (word_rows) hipLaunchKernelGGL((vocab_product_kernel<true, false>), grid_of(d), dim3(256), 0, stream, d, s);
-                else hipLaunchKernelGGL((vocab_product_kernel<true, true>), grid_of(d), dim3(256), 0, stream, d, s);
-            }
         }
-        if (grad_W) {
+        ProductArgs dh{}, dw{};
+        StoreArgs sh{}, sw{};
+        int64_t h_tiles = 0, w_tiles = 0;
+        if (grad_H && v.M > 0) {
+            dh = product(G, nullptr, words_of(p.w, first, word_rows), p.amax_w, v.M, v.D, words);
+            dh.run_steps = tiles_of(tiles_of(p.piece, kStepK), p.runs); // (of the whole piece: a last one that is shorter has as many or fewer runs)
+            dh.run_stride = v.M * v.D;
+            sh = StoreArgs{p.part_h, v.D, 1, first > 0};
+            h_tiles = dh.tiles_m * dh.tiles_n * tiles_of(dh.k_steps, dh.run_steps);
+            runs = std::max(runs, tiles_of(dh.k_steps, dh.run_steps));
+        }
+        if (grad_W) { // as [words][D] or [D][words], whichever puts the axis with unit stride across the lanes
             float* to = gw + first * gw_v;
             if (gw_d == 1 || gw_v != 1) {
-                const ProductArgs d = product(G, nullptr, p.hs, p.amax_hs, words, v.D, v.M);
-                hipLaunchKernelGGL((vocab_product_kernel<false, false>), grid_of(d), dim3(256), 0, stream, d, (StoreArgs{to, gw_v, gw_d, nullptr, add}));
+                dw = product(G, nullptr, p.hs, p.amax_hs, words, v.D, v.M);
+                sw = StoreArgs{to, gw_v, gw_d, add};
             } else {
-                const ProductArgs d = product(p.hs, p.amax_hs, G, nullptr, v.D, words, v.M);
-                hipLaunchKernelGGL((vocab_product_kernel<false, false>), grid_of(d), dim3(256), 0, stream, d, (StoreArgs{to, gw_d, gw_v, nullptr, add}));
+                dw = product(p.hs, p.amax_hs, G, nullptr, v.D, words, v.M);
+                sw = StoreArgs{to, gw_d, gw_v, add};
             }
+            w_tiles = dw.tiles_m * dw.tiles_n;
         }
+        if (h_tiles + w_tiles == 0) continue;
+        const dim3 grid((unsigned)(h_tiles + w_tiles));
+        if (word_rows) hipLaunchKernelGGL(vocab_products_kernel<false>, grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
+        else hipLaunchKernelGGL(vocab_products_kernel<true>, grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
     }
+    if (grad_H && v.M > 0)
+        hipLaunchKernelGGL(vocab_dh_kernel, dim3((unsigned)std::min<int64_t>(tiles_of(v.M * v.D, 1024), 8 * call.state.cus)), dim3(256), 0, stream, p.part_h, runs, v.M, v.D, p.row_scale, grad_H, add);
     if (grad_bias) hipLaunchKernelGGL(vocab_db_kernel, dim3((unsigned)tiles_of(v.V, 256)), dim3(256), 0, stream, p.part_db, v.M > 0 ? 2 * tiles_of(v.M, kTileN) : 0, v.V, grad_bias, add);
     return call.finish(sync);
 }

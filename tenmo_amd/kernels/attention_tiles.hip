@@ -42,8 +42,9 @@ struct TileArgs {
     int jobs;           // 3 or 4 of them
     int parts;
     float* split[4];    // [batch][heads][rows padded][DP]
-    uint32_t* amax[4];  // [batch * heads][parts]
-    float* norm[4];     // the same of the rows' norms: of v and dout, for the backward call
+    f32x4* seen[4];     // [batch * heads][parts]: of a run of rows, the largest finite magnitude, the largest norm of a row, the smallest largest magnitude of a row
+                        // that is not zero, and 1 if there is a value that is not finite
+    f32x4* head[4];     // [batch * heads]: scale, largest norm of a row, 1 if the halves do not hold this head
     const float *out, *lse;
     f32x2* stats;        // [batch][heads][queries padded] (and 128 behind the last): lse log2(e) (+inf where there is none: no probability), and dO . O
     // forward
@@ -61,9 +62,10 @@ __device__ __forceinline__ int used_keys(const AttnShape& s, int length, int sta
 
 struct HeadJob {
     int job, heads, bh, b, h, rows, pad;
+    int lo, hi; // the rows that count
     AttnOperand src;
-    float *split, *norm;
-    uint32_t* amax;
+    float* split;
+    f32x4 *seen, *head;
 };
 // (the operand is picked by comparisons: an index into the arguments that is not known to the compiler would put them into scratch memory)
 __device__ __forceinline__ HeadJob head_job(const TileArgs& a, int y) {
@@ -77,6 +79,9 @@ __device__ __forceinline__ HeadJob head_job(const TileArgs& a, int y) {
     j.h = j.bh - j.b * j.heads;
     j.rows = key ? a.s.keys : a.s.queries;
     j.pad = row_pad(j.rows);
+    const int length = attn_length(a.s, j.b), start = attn_start(a.s, j.b);
+    j.lo = key ? 0 : first_query(a.s, length, start);
+    j.hi = key ? used_keys(a.s, length, start) : a.s.queries;
 #define TENMO_PICK(x) (j.job == kQ ? a.x[kQ] : j.job == kK ? a.x[kK] : j.job == kV ? a.x[kV] : a.x[kDO])
     j.src.p = TENMO_PICK(src).p;
     j.src.b = TENMO_PICK(src).b;
@@ -84,95 +89,96 @@ __device__ __forceinline__ HeadJob head_job(const TileArgs& a, int y) {
     j.src.h = TENMO_PICK(src).h;
     j.src.d = TENMO_PICK(src).d;
     j.split = TENMO_PICK(split);
-    j.norm = TENMO_PICK(norm);
-    j.amax = TENMO_PICK(amax);
+    j.seen = TENMO_PICK(seen);
+    j.head = TENMO_PICK(head);
 #undef TENMO_PICK
     return j;
 }
 
-// largest magnitude (and norm) of the rows that count, delta and the base-2 lse: a run of a head's rows each workgroup, L lanes a row
+// What a run of a head's rows holds, and each row's lse and delta: L lanes a row, U rows in flight
 template <int L>
 __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
-    constexpr int SLOTS = 64 / L;
-    __shared__ uint32_t top_of[4];
-    __shared__ float norm_of[4];
+    constexpr int SLOTS = 64 / L, U = 4;
+    __shared__ f32x4 seen_of[4];
     const HeadJob j = head_job(a, blockIdx.y);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = lane % L, D = a.s.dim;
-    const int length = attn_length(a.s, j.b), start = attn_start(a.s, j.b);
-    const bool query = j.job == kQ || j.job == kDO;
-    const int lo = query ? first_query(a.s, length, start) : 0, hi = query ? a.s.queries : used_keys(a.s, length, start);
-    const AttnOperand& src = j.src;
-    const float* p = src.p + j.b * src.b + j.h * src.h + 4 * part * src.d;
+    const float* p = j.src.p + j.b * j.src.b + j.h * j.src.h + 4 * part * j.src.d;
     const int all = j.job == kDO ? j.pad : j.rows, per = (all + a.parts - 1) / a.parts;
     const int first = blockIdx.x * per, last = first + per < all ? first + per : all;
-    uint32_t top = 0;
-    float norm = 0.f;
-    for (int r = first + wave * SLOTS + lane / L; __any(r < last); r += 4 * SLOTS) {
-        const bool in = r < last && r >= lo && r < hi;
-        f32x4 x{0.f, 0.f, 0.f, 0.f};
-        if (in) x = src.d == 1 ? attn_load4<true>(p + r * src.s, 1, part, D) : attn_load4<false>(p + r * src.s, src.d, part, D);
-        uint32_t mine = 0;
+    float top = 0.f, norm = 0.f, least = __builtin_inff();
+    bool wrong = false;
+    for (int r0 = first + wave * SLOTS + lane / L; __any(r0 < last); r0 += 4 * SLOTS * U) {
+        f32x4 x[U], o[U];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mine = max(mine, finite_magnitude(x[e]));
-        top = max(top, mine);
-        if (j.norm) {
-            float sq = lanes_sum<L>(dot4(x, x));
-            if (!(sq < 1e37f && sq > 1e-30f)) { // out of range: the largest magnitude times sqrt(D) instead
-#pragma unroll
-                for (int d = L / 2; d > 0; d >>= 1) mine = max(mine, (uint32_t)__shfl_xor((int)mine, d, 64));
-                norm = fmaxf(norm, fminf(__uint_as_float(mine) * sqrtf((float)D), 1e38f));
-            } else norm = fmaxf(norm, sqrtf(sq));
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + 4 * SLOTS * u;
+            const bool in = r < last && r >= j.lo && r < j.hi;
+            x[u] = o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (in) x[u] = j.src.d == 1 ? attn_load4<true>(p + r * j.src.s, 1, part, D) : attn_load4<false>(p + r * j.src.s, j.src.d, part, D);
+            if (in && j.job == kDO) o[u] = attn_load4<true>(a.out + (((int64_t)j.b * a.s.queries + r) * a.s.heads + j.h) * D + 4 * part, 1, part, D);
         }
-        if (j.job == kDO) {
-            f32x4 o{0.f, 0.f, 0.f, 0.f};
-            if (in) o = attn_load4<true>(a.out + (((int64_t)j.b * a.s.queries + r) * a.s.heads + j.h) * D + 4 * part, 1, part, D);
-            const float delta = lanes_sum<L>(dot4(x, o));
-            if (part == 0 && r < last)
-                a.stats[(int64_t)j.bh * j.pad + r] = in ? f32x2{a.lse[(int64_t)j.bh * a.s.queries + r] * kLog2e, delta} : f32x2{__builtin_inff(), 0.f};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + 4 * SLOTS * u;
+            float mine = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                mine = fmaxf(mine, __uint_as_float(finite_magnitude(x[u][e])));
+                wrong |= !(x[u][e] - x[u][e] == 0.f);
+            }
+#pragma unroll
+            for (int d = L / 2; d > 0; d >>= 1) mine = fmaxf(mine, __shfl_xor(mine, d, 64));
+            top = fmaxf(top, mine);
+            if (mine > 0.f) least = fminf(least, mine);
+            const float sq = lanes_sum<L>(dot4(x[u], x[u]));
+            // (a square out of range: the largest magnitude times sqrt(D) instead)
+            norm = fmaxf(norm, sq < 1e37f && sq > 1e-30f ? sqrtf(sq) : fminf(mine * sqrtf((float)D), 1e38f));
+            if (j.job == kDO) {
+                const float delta = lanes_sum<L>(dot4(x[u], o[u]));
+                if (part == 0 && r < last)
+                    a.stats[(int64_t)j.bh * j.pad + r] = r >= j.lo && r < j.hi ? f32x2{a.lse[(int64_t)j.bh * a.s.queries + r] * kLog2e, delta} : f32x2{__builtin_inff(), 0.f};
+            }
         }
     }
-    top = wave_max_bits(top);
-    norm = wave_max(norm);
-    if (lane == 0) top_of[wave] = top, norm_of[wave] = norm;
+    const f32x4 mine{wave_max(top), wave_max(norm), -wave_max(-least), __any(wrong) ? 1.f : 0.f};
+    if (lane == 0) seen_of[wave] = mine;
     __syncthreads();
     if (threadIdx.x == 0) {
-        j.amax[(int64_t)j.bh * a.parts + blockIdx.x] = max(max(top_of[0], top_of[1]), max(top_of[2], top_of[3]));
-        if (j.norm) j.norm[(int64_t)j.bh * a.parts + blockIdx.x] = fmaxf(fmaxf(norm_of[0], norm_of[1]), fmaxf(norm_of[2], norm_of[3]));
+        f32x4 s = seen_of[0];
+        for (int w = 1; w < 4; ++w) s = f32x4{fmaxf(s[0], seen_of[w][0]), fmaxf(s[1], seen_of[w][1]), fminf(s[2], seen_of[w][2]), fmaxf(s[3], seen_of[w][3])};
+        j.seen[(int64_t)j.bh * a.parts + blockIdx.x] = s;
     }
 }
 
-// the scale of a head of an operand, and its largest row norm, in every lane
-__device__ __forceinline__ float head_scale(const uint32_t* __restrict amax, int parts, int64_t bh) {
-    const int lane = threadIdx.x & 63;
-    return split_scale(wave_max_bits(lane < parts ? amax[bh * parts + lane] : 0u));
-}
-__device__ __forceinline__ float head_scale(const TileArgs& a, int job, int64_t bh) { return head_scale(a.amax[job], a.parts, bh); } // job: a constant
-__device__ __forceinline__ float head_norm(const TileArgs& a, int job, int64_t bh) {
-    const int lane = threadIdx.x & 63;
-    return wave_max(lane < a.parts ? a.norm[job][bh * a.parts + lane] : 0.f);
-}
-
-// the halves: 8 values a thread
+// The halves of 64 rows, 8 values a thread; the first workgroup of a head leaves what the products need to know of it.
+// The halves hold a value to 2^-22 of itself and 2^-40 of the head's largest.  For keys and values that is taken while no row that is not zero is smaller than 2^-16 of the largest: 2^-24 of
+// each row's own.  Rows of q and dout enter scores, which need to be right against 1 (see beyond()), and sums over rows, which need to be right against the largest; rows of theirs may
+// be as small as 2^-24 of the largest (gradients of single positions are), with their own rows of dQ to 2^-16 of themselves there.
 template <int DP>
 __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
     constexpr int GROUPS = DP / 8, ROWS = 64;
     const HeadJob j = head_job(a, blockIdx.y);
-    const int length = attn_length(a.s, j.b), start = attn_start(a.s, j.b);
-    const bool query = j.job == kQ || j.job == kDO;
-    const int lo = query ? first_query(a.s, length, start) : 0, hi = query ? a.s.queries : used_keys(a.s, length, start);
-    if ((int)blockIdx.x * ROWS >= j.pad) return;
-    const float scale = head_scale(j.amax, a.parts, j.bh);
-    const AttnOperand& src = j.src;
-    const float* p = src.p + j.b * src.b + j.h * src.h;
+    if ((int)blockIdx.x * ROWS >= j.pad && blockIdx.x > 0) return;
+    const int lane = threadIdx.x & 63;
+    f32x4 s{0.f, 0.f, __builtin_inff(), 0.f};
+    if (lane < a.parts) s = j.seen[(int64_t)j.bh * a.parts + lane];
+    const float top = wave_max(s[0]), scale = split_scale(__float_as_uint(top));
+    if (blockIdx.x == 0) {
+        const float norm = wave_max(s[1]), least = -wave_max(-s[2]), wrong = wave_max(s[3]);
+        const bool key = j.job == kK || j.job == kV;
+        if (threadIdx.x == 0) j.head[j.bh] = f32x4{scale, norm, wrong > 0.f || top * (key ? 0x1p-16f : 0x1p-24f) > least ? 1.f : 0.f, 0.f};
+    }
+    const float* p = j.src.p + j.b * j.src.b + j.h * j.src.h;
     for (int x = threadIdx.x; x < ROWS * GROUPS; x += 256) {
         const int r = blockIdx.x * ROWS + x / GROUPS, d = x % GROUPS * 8;
         f16x8 h, l;
         f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        if (r >= lo && r < hi) {
-            const float* q = p + r * src.s + d * src.d;
+        if (r >= j.pad) break;
+        if (r >= j.lo && r < j.hi) {
+            const float* q = p + r * j.src.s + d * j.src.d;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                v[i] = src.d == 1 ? attn_load4<true>(q + 4 * i, 1, d / 4 + i, a.s.dim) : attn_load4<false>(q + 4 * i * src.d, src.d, d / 4 + i, a.s.dim);
+                v[i] = j.src.d == 1 ? attn_load4<true>(q + 4 * i, 1, d / 4 + i, a.s.dim) : attn_load4<false>(q + 4 * i * j.src.d, j.src.d, d / 4 + i, a.s.dim);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -187,12 +193,102 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
     }
 }
 
+// Whether a pair of heads is beyond the halves: a value that is not finite, keys or values of sizes too far apart, or scores above 2^16 (|q| |k| scale; their error would pass 2^-24).
+// Such heads are worked on row by row in fp32, where nothing that is not allowed can leave a trace.
+__device__ __forceinline__ bool beyond(const TileArgs& a, f32x4 q, f32x4 k, f32x4 v) { return q[2] + k[2] + v[2] > 0.f || !(q[1] * k[1] * fabsf(a.s.scale) < 65536.f); }
+
+__device__ __forceinline__ void store_part(float* to, int d, int D, f32x4 x) {
+    if (d + 3 < D) *(f32x4_u*)(to + d) = x;
+    else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < D) to[d + e] = x[e];
+}
+
+// ---- heads beyond the halves: a wavefront a row, or 64 / L keys ------------------------------------------------------------------------
+
+__device__ __forceinline__ f32x4 slow_load(const AttnOperand& o, int b, int64_t s, int h, int part, int D) {
+    return attn_load4<false>(o.p + b * o.b + s * o.s + h * o.h + 4 * part * o.d, o.d, part, D);
+}
+
+// a row's sum of p v (this lane's four values), its maximum and sum over the keys lo .. hi - 1
+template <int L>
+__device__ __forceinline__ f32x4 slow_forward(const TileArgs& a, int b, int h, int i, int lo, int hi, float& m, float& l) {
+    constexpr int SLOTS = 64 / L;
+    const int lane = threadIdx.x & 63, part = lane % L, D = a.s.dim, hk = h / a.s.group;
+    const f32x4 q = slow_load(a.src[kQ], b, i, h, part, D) * a.s.scale;
+    f32x4 o{0.f, 0.f, 0.f, 0.f};
+    m = kNone;
+    l = 0.f;
+    for (int j = lo + lane / L; __any(j < hi); j += SLOTS) {
+        const int jr = j < hi ? j : hi - 1;
+        const f32x4 k = slow_load(a.src[kK], b, jr, hk, part, D), v = slow_load(a.src[kV], b, jr, hk, part, D);
+        const float x = lanes_sum<L>(dot4(q, k));
+        if (j < hi) {
+            const float top = fmaxf(m, x), keep = below(m, top), p = below(x, top);
+            l = l * keep + p;
+            o = o * keep + p * v;
+            m = top;
+        }
+    }
+#pragma unroll
+    for (int d = L; d < 64; d <<= 1) {
+        const float om = __shfl_xor(m, d, 64), top = fmaxf(m, om), keep = below(m, top), okeep = below(om, top);
+        l = l * keep + __shfl_xor(l, d, 64) * okeep;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = o[e] * keep + __shfl_xor(o[e], d, 64) * okeep;
+        m = top;
+    }
+    return o;
+}
+
+// a row of dQ, without its factor scale
+template <int L>
+__device__ __forceinline__ f32x4 slow_dq(const TileArgs& a, int b, int h, int i, int limit, float lse, float delta) {
+    constexpr int SLOTS = 64 / L;
+    const int lane = threadIdx.x & 63, part = lane % L, D = a.s.dim, hk = h / a.s.group;
+    const f32x4 q = slow_load(a.src[kQ], b, i, h, part, D) * a.s.scale, g = slow_load(a.src[kDO], b, i, h, part, D);
+    f32x4 acc{0.f, 0.f, 0.f, 0.f};
+    for (int j = lane / L; __any(j < limit); j += SLOTS) {
+        const int jr = j < limit ? j : limit - 1;
+        const f32x4 k = slow_load(a.src[kK], b, jr, hk, part, D), v = slow_load(a.src[kV], b, jr, hk, part, D);
+        const float x = lanes_sum<L>(dot4(q, k)), dp = lanes_sum<L>(dot4(g, v));
+        if (j < limit) acc += __expf(x - lse) * (dp - delta) * k;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int d = L; d < 64; d <<= 1) acc[e] += __shfl_xor(acc[e], d, 64);
+    return acc;
+}
+
+// dK (without its factor scale) and dV of a key of this slot's, from the queries of head h
+template <int L>
+__device__ __forceinline__ void slow_dkv(const TileArgs& a, int b, int h, int j, int length, int start, f32x4& dk, f32x4& dv) {
+    const int part = (threadIdx.x & 63) % L, D = a.s.dim, hk = h / a.s.group, jr = j < a.s.keys ? j : a.s.keys - 1;
+    const int64_t bh = (int64_t)b * a.s.heads + h;
+    const f32x4 k = slow_load(a.src[kK], b, jr, hk, part, D), v = slow_load(a.src[kV], b, jr, hk, part, D);
+    dk = dv = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < a.s.queries; ++i) {
+        const int limit = attn_limit(length, start, i);
+        if (!__any(j < limit)) continue;
+        const f32x4 q = slow_load(a.src[kQ], b, i, h, part, D), g = slow_load(a.src[kDO], b, i, h, part, D);
+        const float x = lanes_sum<L>(dot4(q, k)) * a.s.scale, dp = lanes_sum<L>(dot4(g, v));
+        if (j < limit) {
+            const float p = __expf(x - a.lse[bh * a.s.queries + i]);
+            dv += p * g;
+            dk += p * (dp - a.stats[bh * row_pad(a.s.queries) + i][1]) * q;
+        }
+    }
+}
+
 // ---- tiles in LDS ------------------------------------------------------------------------------------------------------------------
 
 template <int DP>
 struct Tile {
     static constexpr int CH = DP / 4, KD = DP / 16, ND = DP / 32, BYTES = 32 * CH * 16, BLOCKS = BYTES / 1024;
     static constexpr bool WIDE = DP % 64 == 0;
+    static constexpr int LANES = DP <= 32 ? 8 : DP <= 64 ? 16 : 32; // of a row in fp32, four values each
 
     static __device__ __forceinline__ int swizzle(int row) { return WIDE ? (row & 1) | ((row >> 1) & 6) | ((row & 2) << 2) : (row >> 1) & 7; }
 
@@ -308,7 +404,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
     const int split = blockIdx.x % a.splits;
     head_and_block(blockIdx.x / a.splits, a.s.batch * a.s.heads, q_blocks, a.s.causal, true, &bh, &block);
     const int b = bh / a.s.heads, h = bh % a.s.heads, bk = b * a.s.kv_heads + h / a.s.group;
-    const int length = attn_length(a.s, b), start = attn_start(a.s, b);
+    const int length = __builtin_amdgcn_readfirstlane(attn_length(a.s, b)), start = __builtin_amdgcn_readfirstlane(attn_start(a.s, b));
     const int q0 = block * kRowPad + wave * 32, i = q0 + (lane & 31);
     const int limit = i < a.s.queries ? attn_limit(length, start, i) : 0;
     const int wave_last = q0 + 31 < a.s.queries ? q0 + 31 : a.s.queries - 1, block_last = (block + 1) * kRowPad < a.s.queries ? (block + 1) * kRowPad - 1 : a.s.queries - 1;
@@ -316,10 +412,29 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
     const int tiles = (attn_limit(length, start, block_last) + 31) / 32, per = (tiles + a.splits - 1) / a.splits;
     const int t0 = split * per < tiles ? split * per : tiles, t1 = t0 + per < tiles ? t0 + per : tiles;
 
+    const f32x4 head_q = a.head[kQ][bh], head_k = a.head[kK][bk], head_v = a.head[kV][bk];
+    if (__builtin_amdgcn_readfirstlane(beyond(a, head_q, head_k, head_v))) {
+        constexpr int L = T::LANES;
+        for (int r = q0; r < q0 + 32 && r < a.s.queries; ++r) {
+            float m, l;
+            const int most = attn_limit(length, start, r), hi = t1 * 32 < most ? t1 * 32 : most;
+            const f32x4 o = slow_forward<L>(a, b, h, r, t0 * 32, hi, m, l);
+            const int64_t row = (int64_t)bh * a.s.queries + r;
+            if (lane >= L) continue;
+            if (a.part) {
+                float* to = a.part + ((int64_t)split * a.s.batch * a.s.heads * a.s.queries + row) * (D + 2);
+                store_part(to, 4 * lane, D, o);
+                if (lane == 0) to[D] = m, to[D + 1] = l;
+            } else {
+                store_part(a.to + (((int64_t)b * a.s.queries + r) * a.s.heads + h) * D, 4 * lane, D, l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o / l);
+                if (lane == 0 && a.to_lse) a.to_lse[row] = l == 0.f ? kNone : m + logf(l);
+            }
+        }
+        return;
+    }
     f16x8 qh[T::KD], ql[T::KD];
     own_rows<DP>(qh, ql, a.split[kQ] + ((int64_t)bh * pad_q + q0) * DP, lane);
-    const float inv_v = 1.f / head_scale(a, kV, bk);
-    const float c = a.s.scale * kLog2e / head_scale(a, kQ, bh) / head_scale(a, kK, bk);
+    const float inv_v = 1.f / head_v[0], c = a.s.scale * kLog2e / head_q[0] / head_k[0];
     const float* const base[2] = {a.split[kK] + (int64_t)bk * pad_k * DP, a.split[kV] + (int64_t)bk * pad_k * DP};
     uint32_t off[LOADS];
     T::template offsets<2>(off, wave, lane);
@@ -417,21 +532,15 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int at = 32 * d + 8 * q + 4 * half;
-            const f32x4 x{o[d][4 * q] * factor, o[d][4 * q + 1] * factor, o[d][4 * q + 2] * factor, o[d][4 * q + 3] * factor};
-            if (at + 3 < D) *(f32x4_u*)(to + at) = x;
-            else
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (at + e < D) to[at + e] = x[e];
+            store_part(to, at, D, f32x4{o[d][4 * q] * factor, o[d][4 * q + 1] * factor, o[d][4 * q + 2] * factor, o[d][4 * q + 3] * factor});
         }
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------------------
 
-// 2^15 over the largest that |dS| can be, as a power of two
-__device__ __forceinline__ float ds_scale(const TileArgs& a, int64_t bh, int64_t bk) {
-    const float bound = 2.f * head_norm(a, kDO, bh) * head_norm(a, kV, bk);
-    const int e = (int)(__float_as_uint(fminf(bound, 1e38f)) >> 23) - 127 + 1; // bound < 2^e
+// 2^15 over the largest that |dS| can be, as a power of two, from the heads of dout and v
+__device__ __forceinline__ float ds_scale(f32x4 g, f32x4 v) {
+    const int e = (int)(__float_as_uint(fminf(2.f * g[1] * v[1], 1e38f)) >> 23) - 127 + 1; // the bound is below 2^e
     const int up = 15 - e;
     return __uint_as_float((uint32_t)((up > 126 ? 126 : up) + 127) << 23);
 }
@@ -441,14 +550,6 @@ __device__ __forceinline__ void store_gradient(const AttnOperand& g, int64_t at,
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (d + e < D) to[e * g.d] = accumulate ? to[e * g.d] + x[e] : x[e];
-}
-
-__device__ __forceinline__ void store_part(float* to, int d, int D, f32x4 x) {
-    if (d + 3 < D) *(f32x4_u*)(to + d) = x;
-    else
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (d + e < D) to[d + e] = x[e];
 }
 
 template <int DP>
@@ -461,18 +562,37 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(co
     int bh, block;
     head_and_block(blockIdx.x, a.s.batch * a.s.heads, k_blocks, a.s.causal, false, &bh, &block);
     const int b = bh / a.s.heads, h = bh % a.s.heads, hk = h / a.s.group, bk = b * a.s.kv_heads + hk;
-    const int length = attn_length(a.s, b), start = attn_start(a.s, b), keys = used_keys(a.s, length, start);
+    const int length = __builtin_amdgcn_readfirstlane(attn_length(a.s, b)), start = __builtin_amdgcn_readfirstlane(attn_start(a.s, b)), keys = used_keys(a.s, length, start);
     const int j0 = block * kRowPad + wave * 32, j = j0 + (lane & 31);
     // query i sees key j when i >= j - start and j < length
     const int see = a.s.causal ? j - start : 0;
     const int wave_first = a.s.causal && j0 - start > 0 ? j0 - start : 0, block_first = a.s.causal && block * kRowPad - start > 0 ? block * kRowPad - start : 0;
     const int t0 = block_first / 32, t1 = block * kRowPad < keys ? (a.s.queries + 31) / 32 : 0;
 
+    const f32x4 head_q = a.head[kQ][bh], head_k = a.head[kK][bk], head_v = a.head[kV][bk], head_g = a.head[kDO][bh];
+    if (__builtin_amdgcn_readfirstlane(beyond(a, head_q, head_k, head_v) || head_g[2] > 0.f)) {
+        constexpr int L = T::LANES;
+        for (int r = lane / L; r < 32 && __any(j0 + r < a.s.keys); r += 64 / L) {
+            f32x4 x, y;
+            const int key = j0 + r, d = 4 * (lane % L);
+            slow_dkv<L>(a, b, h, key, length, start, x, y);
+            if (key >= a.s.keys) continue;
+            x *= a.s.scale;
+            if (a.part_k) {
+                store_part(a.part_k + ((int64_t)bh * a.s.keys + key) * D, d, D, x);
+                store_part(a.part_v + ((int64_t)bh * a.s.keys + key) * D, d, D, y);
+                continue;
+            }
+            if (a.grad_k.p) store_gradient(a.grad_k, b * a.grad_k.b + hk * a.grad_k.h + key * a.grad_k.s, d, D, x, a.accumulate);
+            if (a.grad_v.p) store_gradient(a.grad_v, b * a.grad_v.b + hk * a.grad_v.h + key * a.grad_v.s, d, D, y, a.accumulate);
+        }
+        return;
+    }
     f16x8 kh[T::KD], kl[T::KD], vh[T::KD], vl[T::KD];
     own_rows<DP>(kh, kl, a.split[kK] + ((int64_t)bk * pad_k + j0) * DP, lane);
     own_rows<DP>(vh, vl, a.split[kV] + ((int64_t)bk * pad_k + j0) * DP, lane);
-    const float scale_q = head_scale(a, kQ, bh), scale_g = head_scale(a, kDO, bh), ds_up = ds_scale(a, bh, bk);
-    const float c = a.s.scale * kLog2e / scale_q / head_scale(a, kK, bk), inv_dp = 1.f / scale_g / head_scale(a, kV, bk);
+    const float scale_q = head_q[0], scale_g = head_g[0], ds_up = ds_scale(head_g, head_v);
+    const float c = a.s.scale * kLog2e / scale_q / head_k[0], inv_dp = 1.f / scale_g / head_v[0];
     const float* const base[2] = {a.split[kQ] + (int64_t)bh * pad_q * DP, a.split[kDO] + (int64_t)bh * pad_q * DP};
     const float* const stats = (const float*)(a.stats + (int64_t)bh * pad_q);
     uint32_t off[LOADS - 1];
@@ -609,18 +729,27 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(con
     int bh, block;
     head_and_block(blockIdx.x, a.s.batch * a.s.heads, q_blocks, a.s.causal, true, &bh, &block);
     const int b = bh / a.s.heads, h = bh % a.s.heads, bk = b * a.s.kv_heads + h / a.s.group;
-    const int length = attn_length(a.s, b), start = attn_start(a.s, b);
+    const int length = __builtin_amdgcn_readfirstlane(attn_length(a.s, b)), start = __builtin_amdgcn_readfirstlane(attn_start(a.s, b));
     const int q0 = block * kRowPad + wave * 32, i = q0 + (lane & 31);
     const int limit = i < a.s.queries ? attn_limit(length, start, i) : 0;
     const int wave_last = q0 + 31 < a.s.queries ? q0 + 31 : a.s.queries - 1, block_last = (block + 1) * kRowPad < a.s.queries ? (block + 1) * kRowPad - 1 : a.s.queries - 1;
     const int wave_most = q0 < a.s.queries ? attn_limit(length, start, wave_last) : 0, wave_least = wave_last == q0 + 31 ? attn_limit(length, start, q0) : 0;
     const int tiles = (attn_limit(length, start, block_last) + 31) / 32;
 
+    const f32x4 head_q = a.head[kQ][bh], head_k = a.head[kK][bk], head_v = a.head[kV][bk], head_g = a.head[kDO][bh];
+    if (__builtin_amdgcn_readfirstlane(beyond(a, head_q, head_k, head_v) || head_g[2] > 0.f)) {
+        constexpr int L = T::LANES;
+        for (int r = q0; r < q0 + 32 && r < a.s.queries; ++r) {
+            const f32x4 x = slow_dq<L>(a, b, h, r, attn_limit(length, start, r), a.lse[(int64_t)bh * a.s.queries + r], a.stats[(int64_t)bh * pad_q + r][1]);
+            if (lane < L) store_gradient(a.grad_q, b * a.grad_q.b + h * a.grad_q.h + r * a.grad_q.s, 4 * lane, D, x * a.s.scale, a.accumulate);
+        }
+        return;
+    }
     f16x8 qh[T::KD], ql[T::KD], gh[T::KD], gl[T::KD];
     own_rows<DP>(qh, ql, a.split[kQ] + ((int64_t)bh * pad_q + q0) * DP, lane);
     own_rows<DP>(gh, gl, a.split[kDO] + ((int64_t)bh * pad_q + q0) * DP, lane);
-    const float scale_k = head_scale(a, kK, bk), ds_up = ds_scale(a, bh, bk);
-    const float c = a.s.scale * kLog2e / head_scale(a, kQ, bh) / scale_k, inv_dp = 1.f / head_scale(a, kDO, bh) / head_scale(a, kV, bk);
+    const float scale_k = head_k[0], ds_up = ds_scale(head_g, head_v);
+    const float c = a.s.scale * kLog2e / head_q[0] / scale_k, inv_dp = 1.f / head_g[0] / head_v[0];
     const f32x2 stats = a.stats[(int64_t)bh * pad_q + i];
     const float lse2 = stats[0], delta = stats[1];
     const float* const base[2] = {a.split[kK] + (int64_t)bk * pad_k * DP, a.split[kV] + (int64_t)bk * pad_k * DP};
@@ -708,8 +837,8 @@ void plan_operands(TileArgs& a, Workspace& ws, int jobs) {
         const bool key = j == kK || j == kV;
         const int64_t heads = (int64_t)s.batch * (key ? s.kv_heads : s.heads);
         a.split[j] = ws.take<float>(heads * row_pad(key ? s.keys : s.queries) * padded_dim(s.dim));
-        a.amax[j] = ws.take<uint32_t>(heads * a.parts);
-        if (jobs == 4 && (j == kV || j == kDO)) a.norm[j] = ws.take<float>(heads * a.parts);
+        a.seen[j] = ws.take<f32x4>(heads * a.parts);
+        a.head[j] = ws.take<f32x4>(heads);
     }
 }
 

@@ -277,6 +277,30 @@ def test_keys_that_are_not_allowed_are_not_used(ops, bad, n):
         close(down(g), ref, 2 * RTOL_FRO, what)
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 1.0e30, 1.0e9])
+@pytest.mark.parametrize("where", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("dim", [16, 64, 96, 128])
+def test_a_row_out_of_the_ordinary_stays_with_what_sees_it(ops, where, bad, dim):
+    """One row of one head that is not finite, or far larger than all others: queries before it, keys behind it and the other heads are as without it."""
+    B, n, H, at = 2, 90, 2, 50
+    tensors = {name: randn(i, B, n, H, dim) for i, name in enumerate(("q", "k", "v", "dout"))}
+    want = attention_reference(tensors["q"], tensors["k"], tensors["v"], 0.2, True, None, None, tensors["dout"])
+    tensors[where][1, at, 0] = bad
+    Q, K, V, DO = (up(ops, tensors[name]) for name in ("q", "k", "v", "dout"))
+    o, lse = ops.A.attention(Q, K, V, scale=0.2, causal=True)
+    grads = ops.A.attention_backward(Q, K, V, o, lse, DO, scale=0.2, causal=True)
+    key = where in ("k", "v")
+    for got, ref, by_query, what in ((o, want[0], True, "out"), (grads[0], want[2][0], True, "grad_q"), (grads[1], want[2][1], False, "grad_k"), (grads[2], want[2][2], False, "grad_v")):
+        clean = np.ones((B, n, H), bool)
+        if by_query:
+            clean[1, at:, 0] = not key  # a key's row is seen by the queries from it on, a query's by itself
+            clean[1, at, 0] = False
+        else:
+            clean[1, :, 0] = False  # every key is seen by such a query, or shares the queries from it on
+            clean[1, at + 1:, 0] = not key
+        close(np.asarray(down(got))[clean], ref[clean], RTOL_FRO if what == "out" else 2 * RTOL_FRO, what)
+
+
 def test_attention_with_values_that_are_not_finite(ops):
     """An allowed key that is not a number reaches the queries that see it, and no other sequence or head."""
     B, n, H, D = 2, 80, 2, 32

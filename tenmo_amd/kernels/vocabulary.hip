@@ -23,7 +23,6 @@ constexpr int64_t kPieceValues = 256 << 20; // of G, 4 bytes each
 struct Source { // an operand in the order in which it is split: rows x cols
     const float* p;
     int64_t rows, cols, rs, cs;
-    const float* row_scale; // NULL: 1
 };
 
 struct VocabArgs {
@@ -39,31 +38,86 @@ __device__ __forceinline__ int64_t target_of(const VocabArgs& a, int64_t m) {
     return a.is64 ? ((const int64_t*)a.target)[m] : (int64_t)((const int32_t*)a.target)[m];
 }
 
-// ---- amax and split -------------------------------------------------------------------------------------------------------------
-
-struct SplitJobs {
-    Source src[2];
-    uint32_t* amax[2]; // kAmaxParts partial maxima
-    SplitMatrix dst[2];
+struct Upstream { // the gradient of the loss: of each row, or of the reduced one
+    const float* p;
+    int reduction;
+    const int32_t* valid_count;
 };
-
-// (picked by comparisons: an index that the compiler does not know would put the arguments into scratch memory)
-__device__ __forceinline__ Source source_of(const SplitJobs& j) {
-    const bool second = blockIdx.y != 0;
-    Source s;
-    s.p = second ? j.src[1].p : j.src[0].p;
-    s.rows = second ? j.src[1].rows : j.src[0].rows;
-    s.cols = second ? j.src[1].cols : j.src[0].cols;
-    s.rs = second ? j.src[1].rs : j.src[0].rs;
-    s.cs = second ? j.src[1].cs : j.src[0].cs;
-    s.row_scale = second ? j.src[1].row_scale : j.src[0].row_scale;
-    return s;
+// the factor of row m of the gradient; 0 where the target is ignore_index
+__device__ __forceinline__ float row_factor(const VocabArgs& a, const Upstream& u, int64_t m) {
+    if (target_of(a, m) == a.ignore) return 0.f;
+    const float s = u.p[u.reduction == 0 ? m : 0];
+    return u.reduction == 2 ? s / (float)(*u.valid_count > 1 ? *u.valid_count : 1) : s;
 }
 
-// four rows of a matrix at a time: four loads in flight a thread
-__global__ __launch_bounds__(256) void vocab_amax_kernel(const SplitJobs j) {
+// ---- amax and split -------------------------------------------------------------------------------------------------------------
+
+// W and, backward, H times its rows' factors have one scale each, since they are summed over along either axis: their largest values first, then the halves.  H itself has a scale of its own in
+// each row (a row is one column of the logits' product), so that no row loses anything to another; its halves come with the first launch.
+struct SplitArgs {
+    VocabArgs v;
+    Upstream up;
+    Source w, h;
+    uint32_t *amax_w, *amax_hs; // kAmaxParts partial maxima
+    SplitMatrix to_w, to_h, to_hs;
+    float* h_inverse; // [M]: 1 / the scale of a row of H
+};
+enum { kSplitW, kSplitH, kSplitHS }; // blockIdx.y
+
+__device__ __forceinline__ void split8(const float* x, float scale, float* to) {
+    f16x8 h, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        _Float16 hi, lo;
+        split_value(x[e] * scale, hi, lo);
+        h[e] = hi;
+        l[e] = lo;
+    }
+    *(f16x8*)to = h;
+    *(f16x8*)(to + 4) = l;
+}
+// columns c .. c + 7 of a row, zero behind the last
+__device__ __forceinline__ void load8(float (&x)[8], const float* p, int64_t cs, int64_t c, int64_t cols) {
+    if (cs == 1 && c + 7 < cols) {
+        const f32x4 a = *(const f32x4_u*)(p + c), b = *(const f32x4_u*)(p + c + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = c + e < cols ? p[(c + e) * cs] : 0.f;
+    }
+}
+
+// a wavefront a row
+__device__ __forceinline__ void split_h_rows(const SplitArgs& a) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < split_pad(a.h.rows); r += 4 * kAmaxParts) {
+        const bool in = r < a.h.rows;
+        const float* p = a.h.p + (in ? r : 0) * a.h.rs;
+        const int64_t cols = in ? a.h.cols : 0;
+        uint32_t top = 0;
+        float x[8];
+        for (int64_t c = lane * 8; c < a.to_h.pitch; c += 512) {
+            load8(x, p, a.h.cs, c, cols);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, finite_magnitude(x[e]));
+        }
+        const float scale = split_scale(wave_max_bits(top));
+        for (int64_t c = lane * 8; c < a.to_h.pitch; c += 512) {
+            load8(x, p, a.h.cs, c, cols);
+            split8(x, scale, a.to_h.p + r * a.to_h.pitch + c);
+        }
+        if (in && lane == 0) a.h_inverse[r] = 1.f / scale;
+    }
+}
+
+// four rows at a time: four loads in flight a thread
+__global__ __launch_bounds__(256) void vocab_amax_kernel(const SplitArgs a) {
     __shared__ uint32_t slots[4];
-    const Source s = source_of(j);
+    const int job = blockIdx.y;
+    if (job == kSplitH) return split_h_rows(a);
+    const bool hs = job == kSplitHS;
+    const Source s{hs ? a.h.p : a.w.p, hs ? a.h.rows : a.w.rows, hs ? a.h.cols : a.w.cols, hs ? a.h.rs : a.w.rs, hs ? a.h.cs : a.w.cs};
     uint32_t top = 0;
     for (int64_t r0 = blockIdx.x; r0 < s.rows; r0 += 4 * kAmaxParts) {
         const float* p[4];
@@ -72,28 +126,28 @@ __global__ __launch_bounds__(256) void vocab_amax_kernel(const SplitJobs j) {
         for (int u = 0; u < 4; ++u) { // (the last row again where there is none)
             const int64_t r = r0 + u * kAmaxParts < s.rows ? r0 + u * kAmaxParts : s.rows - 1;
             p[u] = s.p + r * s.rs;
-            scale[u] = s.row_scale ? s.row_scale[r] : 1.f;
+            scale[u] = hs ? row_factor(a.v, a.up, r) : 1.f;
         }
         int64_t c = threadIdx.x * 4;
         if (s.cs == 1)
             for (; c + 3 < s.cols; c += 1024) {
                 f32x4 x[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) x[u] = *(const f32x4_u*)(p[u] + c) * scale[u];
+                for (int u = 0; u < 4; ++u) x[u] = *(const f32x4_u*)(p[u] + c);
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top = max(top, finite_magnitude(x[u][e]));
+                    for (int e = 0; e < 4; ++e) top = max(top, finite_magnitude(scale[u] == 0.f ? 0.f : x[u][e] * scale[u]));
             }
         for (; c < s.cols; c += 1024)
             for (int e = 0; e < 4 && c + e < s.cols; ++e)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) top = max(top, finite_magnitude(p[u][(c + e) * s.cs] * scale[u]));
+                for (int u = 0; u < 4; ++u) top = max(top, finite_magnitude(scale[u] == 0.f ? 0.f : p[u][(c + e) * s.cs] * scale[u]));
     }
     top = wave_max_bits(top);
     if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) (blockIdx.y ? j.amax[1] : j.amax[0])[blockIdx.x] = max(max(slots[0], slots[1]), max(slots[2], slots[3]));
+    if (threadIdx.x == 0) (hs ? a.amax_hs : a.amax_w)[blockIdx.x] = max(max(slots[0], slots[1]), max(slots[2], slots[3]));
 }
 
 // the scale of a matrix, from its partial maxima, in every thread of a workgroup of 256
@@ -106,32 +160,23 @@ __device__ __forceinline__ float scale_from(const uint32_t* __restrict amax, uin
     return split_scale(max(max(slots[0], slots[1]), max(slots[2], slots[3])));
 }
 
-__global__ __launch_bounds__(256) void vocab_split_kernel(const SplitJobs j) {
+__global__ __launch_bounds__(256) void vocab_split_kernel(const SplitArgs a) {
     __shared__ uint32_t slots[4];
-    const Source s = source_of(j);
-    const SplitMatrix d{blockIdx.y ? j.dst[1].p : j.dst[0].p, blockIdx.y ? j.dst[1].pitch : j.dst[0].pitch, 0};
-    const float scale = scale_from(blockIdx.y ? j.amax[1] : j.amax[0], slots);
-    const int64_t groups = d.pitch / 8, all = split_pad(s.rows) * groups;
+    const bool hs = blockIdx.y != 0;
+    const Source s{hs ? a.h.p : a.w.p, hs ? a.h.rows : a.w.rows, hs ? a.h.cols : a.w.cols, hs ? a.h.rs : a.w.rs, hs ? a.h.cs : a.w.cs};
+    float* const to = hs ? a.to_hs.p : a.to_w.p;
+    const int64_t pitch = hs ? a.to_hs.pitch : a.to_w.pitch;
+    const float scale = scale_from(hs ? a.amax_hs : a.amax_w, slots);
+    const int64_t groups = pitch / 8, all = split_pad(s.rows) * groups;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / groups, c = (i - r * groups) * 8;
-        f16x8 h, l;
+        const float factor = r >= s.rows ? 0.f : hs ? row_factor(a.v, a.up, r) : 1.f;
         float x[8];
-        if (r < s.rows && s.cs == 1 && c + 7 < s.cols) {
-            const f32x4 a = *(const f32x4_u*)(s.p + r * s.rs + c), b = *(const f32x4_u*)(s.p + r * s.rs + c + 4);
-            for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
-        } else {
-            for (int e = 0; e < 8; ++e) x[e] = r < s.rows && c + e < s.cols ? s.p[r * s.rs + (c + e) * s.cs] : 0.f;
-        }
-        const float rscale = r < s.rows && s.row_scale ? s.row_scale[r] : 1.f;
-        for (int e = 0; e < 8; ++e) {
-            _Float16 hi, lo;
-            split_value(x[e] * rscale * scale, hi, lo);
-            h[e] = hi;
-            l[e] = lo;
-        }
-        float* to = d.p + r * d.pitch + c;
-        *(f16x8*)to = h;
-        *(f16x8*)(to + 4) = l;
+        load8(x, s.p + (r < s.rows ? r : 0) * s.rs, s.cs, c, factor == 0.f ? 0 : s.cols); // rows without a part in the gradient are zeros, whatever they hold
+        if (hs)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= factor;
+        split8(x, scale, to + r * pitch + c);
     }
 }
 
@@ -149,13 +194,14 @@ struct LogitArgs {
     VocabArgs v;
     int64_t first; // word of the piece's first row
     int64_t words; // of the piece
+    const float* h_inverse;
     // forward
     float2* part;      // [tile][token]: maximum and sum
     float* part_x;     // [tile][token]: sum of the logits, with label smoothing
     float* target_logit; // [token]
     // backward
     const float* lse;
-    const float* row_scale;
+    Upstream up;
     SplitMatrix g;
     float* part_db; // [2 * token tiles][V], with a wanted bias gradient
 };
@@ -163,16 +209,22 @@ struct LogitArgs {
 template <bool A_KMAJOR, bool GRAD>
 __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs p, const LogitArgs a) {
     __shared__ __align__(1024) float lds[kStages * kStageBytes / 4];
-    __shared__ uint32_t slots[2][4];
+    __shared__ uint32_t slots[4];
     int64_t tm, tn;
     tile_of(blockIdx.x, (uint32_t)p.tiles_m, (uint32_t)p.tiles_n, &tm, &tn);
     const int64_t m0 = tm * kTileM, n0 = tn * kTileN;
     f32x16 acc[4][2];
     split_tile<A_KMAJOR, true>(acc, lds, p.a, m0, p.M, p.b, n0, p.N, 0, p.k_steps);
-    const float inv = 1.f / scale_from(p.amax_a, slots[0]) / scale_from(p.amax_b, slots[1]);
+    const float inv_w = 1.f / scale_from(p.amax_a, slots);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int64_t v0 = m0 + (wave & 1) * 128 + 4 * half; // of the piece; register e of block i is v0 + 32 i + 8 (e / 4) + e % 4
     // logits in place
+    float inv[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int64_t token = n0 + (wave >> 1) * 64 + 32 * j + (lane & 31);
+        inv[j] = a.h_inverse[token < a.v.M ? token : a.v.M - 1]; // (applied after inv_w: the product of the two may be out of range)
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -186,7 +238,7 @@ __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs 
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j][4 * q + e] = acc[i][j][4 * q + e] * inv + bias[e];
+                for (int j = 0; j < 2; ++j) acc[i][j][4 * q + e] = acc[i][j][4 * q + e] * inv_w * inv[j] + bias[e];
         }
     const bool edge = m0 + kTileM > a.words;
     if (!GRAD) {
@@ -254,7 +306,7 @@ __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs 
             const int64_t token = n0 + (wave >> 1) * 64 + 32 * j + (lane & 31);
             const int64_t t = token < a.v.M ? target_of(a.v, token) : a.v.ignore;
             const bool valid = token < a.v.M && t != a.v.ignore;
-            const float lse = valid ? a.lse[token] : 0.f, row_scale = valid ? a.row_scale[token] : 0.f;
+            const float lse = valid ? a.lse[token] : 0.f, row_scale = valid && a.part_db ? row_factor(a.v, a.up, token) : 0.f;
             const int64_t at = t - a.first - v0;
             const bool store = token < split_pad(a.v.M);
             float* to = a.g.p + (store ? token : 0) * a.g.pitch;
@@ -422,35 +474,24 @@ __global__ __launch_bounds__(1024) void vocab_total_kernel(const VocabArgs v, co
     if (t == 0) *loss_sum = (float)s[0], *valid = c[0];
 }
 
-// scale_m: the factor of row m of the gradient
-__global__ __launch_bounds__(256) void vocab_row_scale_kernel(const VocabArgs v, const float* upstream, int reduction, const int32_t* valid, float* scale) {
-    const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (m >= v.M) return;
-    float s = 0.f;
-    if (target_of(v, m) != v.ignore) {
-        s = upstream[reduction == 0 ? m : 0];
-        if (reduction == 2) s /= (float)(*valid > 1 ? *valid : 1);
-    }
-    scale[m] = s;
-}
-
 // dH: the runs' sums added in order, times each row's factor
-__global__ __launch_bounds__(256) void vocab_dh_kernel(const float* __restrict part, int64_t runs, int64_t M, int64_t D, const float* __restrict row_scale, float* __restrict dh, int accumulate) {
-    const int64_t all = M * D;
+__global__ __launch_bounds__(256) void vocab_dh_kernel(const float* __restrict part, int64_t runs, const VocabArgs v, const Upstream up, float* __restrict dh, int accumulate) {
+    const int64_t D = v.D, all = v.M * D;
     for (int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; x < all; x += (int64_t)gridDim.x * 1024) {
         if (x + 3 < all) {
             f32x4 s = *(const f32x4*)(part + x);
             for (int64_t r = 1; r < runs; ++r) s += *(const f32x4_u*)(part + r * all + x);
             const int64_t m = x / D;
+            const float factor = row_factor(v, up, m);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] *= row_scale[x + e < (m + 1) * D ? m : (x + e) / D];
+            for (int e = 0; e < 4; ++e) s[e] *= x + e < (m + 1) * D ? factor : row_factor(v, up, (x + e) / D);
             if (accumulate) s += *(const f32x4_u*)(dh + x);
             *(f32x4_u*)(dh + x) = s;
         } else {
             for (int64_t y = x; y < all; ++y) {
                 float s = part[y];
                 for (int64_t r = 1; r < runs; ++r) s += part[r * all + y];
-                s *= row_scale[y / D];
+                s *= row_factor(v, up, y / D);
                 dh[y] = accumulate ? dh[y] + s : s;
             }
         }
@@ -469,9 +510,10 @@ __global__ __launch_bounds__(256) void vocab_db_kernel(const float* __restrict p
 
 struct Plan {
     SplitMatrix h, w, hs, g;
-    uint32_t *amax_h, *amax_w, *amax_hs;
+    uint32_t *amax_w, *amax_hs;
+    float* h_inverse;
     float2* part;
-    float *part_x, *target_logit, *row_scale, *part_db, *part_h;
+    float *part_x, *target_logit, *part_db, *part_h;
     int64_t piece; // words
     int64_t runs;  // of the words of a piece, in G W^T
 };
@@ -488,7 +530,7 @@ SplitMatrix take_split(Workspace& ws, int64_t rows, int64_t cols) {
 void plan_operands(Workspace& ws, Plan& p, int64_t M, int64_t D, int64_t V, bool word_rows) {
     p.h = take_split(ws, M, D);
     p.w = SplitMatrix{ws.take<float>(split_pad(V) * split_pad(D)), word_rows ? split_pad(D) : split_pad(V), word_rows ? V : D};
-    p.amax_h = ws.take<uint32_t>(kAmaxParts);
+    p.h_inverse = ws.take<float>(M);
     p.amax_w = ws.take<uint32_t>(kAmaxParts);
 }
 void plan_forward(Workspace& ws, Plan& p, int64_t M, int64_t D, int64_t V, bool word_rows) {
@@ -501,7 +543,6 @@ void plan_backward(Workspace& ws, Plan& p, int64_t M, int64_t D, int64_t V, bool
     plan_operands(ws, p, M, D, V, word_rows);
     p.hs = take_split(ws, M, D);
     p.amax_hs = ws.take<uint32_t>(kAmaxParts);
-    p.row_scale = ws.take<float>(M);
     p.part_db = ws.take<float>(2 * tiles_of(M, kTileN) * V);
     const int64_t most = std::max<int64_t>(kTileM, kPieceValues / split_pad(M) / kTileM * kTileM);
     p.piece = tiles_of(tiles_of(V, tiles_of(V, most)), kTileM) * kTileM; // pieces of equal size
@@ -530,18 +571,19 @@ int check_call(const tenmo_view* H, const tenmo_view* W, const float* bias, cons
     return 0;
 }
 
-Source source_h(const tenmo_view* H, const float* row_scale) { return Source{H->data + H->offset, H->shape[0], H->shape[1], H->strides[0], H->strides[1], row_scale}; }
+Source source_h(const tenmo_view* H) { return Source{H->data + H->offset, H->shape[0], H->shape[1], H->strides[0], H->strides[1]}; }
 bool rows_of_words(const tenmo_view* W) { return W->strides[0] == 1 && W->shape[0] > 1; }
 Source source_w(const tenmo_view* W) {
-    if (rows_of_words(W)) return Source{W->data + W->offset, W->shape[1], W->shape[0], W->strides[1], W->strides[0], nullptr};
-    return Source{W->data + W->offset, W->shape[0], W->shape[1], W->strides[0], W->strides[1], nullptr};
+    if (rows_of_words(W)) return Source{W->data + W->offset, W->shape[1], W->shape[0], W->strides[1], W->strides[0]};
+    return Source{W->data + W->offset, W->shape[0], W->shape[1], W->strides[0], W->strides[1]};
 }
 
-void launch_split(const SplitJobs& j, int jobs, const LibraryState& lib) {
-    int64_t groups = 0;
-    for (int i = 0; i < jobs; ++i) groups = std::max(groups, split_pad(j.src[i].rows) * j.dst[i].pitch / 8);
-    hipLaunchKernelGGL(vocab_amax_kernel, dim3(kAmaxParts, jobs), dim3(256), 0, lib.stream, j);
-    hipLaunchKernelGGL(vocab_split_kernel, dim3((unsigned)std::min<int64_t>(tiles_of(groups, 256), 16 * lib.cus), jobs), dim3(256), 0, lib.stream, j);
+// W and H, and H times its rows' factors where `hs` is wanted
+void launch_split(const Plan& p, const tenmo_view* H, const tenmo_view* W, const VocabArgs& v, const Upstream& up, bool hs, const LibraryState& lib) {
+    const SplitArgs a{v, up, source_w(W), source_h(H), p.amax_w, p.amax_hs, p.w, p.h, p.hs, p.h_inverse};
+    const int64_t groups = std::max(split_pad(a.w.rows) * p.w.pitch, split_pad(v.M) * p.h.pitch) / 8;
+    hipLaunchKernelGGL(vocab_amax_kernel, dim3(kAmaxParts, hs ? 3 : 2), dim3(256), 0, lib.stream, a);
+    hipLaunchKernelGGL(vocab_split_kernel, dim3((unsigned)std::min<int64_t>(tiles_of(groups, 256), 16 * lib.cus), hs ? 2 : 1), dim3(256), 0, lib.stream, a);
 }
 
 ProductArgs product(const SplitMatrix& a, const uint32_t* amax_a, const SplitMatrix& b, const uint32_t* amax_b, int64_t M, int64_t N, int64_t K) {
@@ -584,13 +626,10 @@ int tenmo_hip_vocabulary_loss_forward_f32(const tenmo_view* H, const tenmo_view*
         Plan p{};
         plan_forward(ws, p, v.M, v.D, v.V, word_rows);
         if (int rc = ws.check(who)) return rc;
-        SplitJobs j{};
-        j.src[0] = source_w(W); j.amax[0] = p.amax_w; j.dst[0] = p.w;
-        j.src[1] = source_h(H, nullptr); j.amax[1] = p.amax_h; j.dst[1] = p.h;
-        launch_split(j, 2, call.state);
-        const ProductArgs g = product(p.w, p.amax_w, p.h, p.amax_h, v.V, v.M, v.D);
+        launch_split(p, H, W, v, Upstream{}, false, call.state);
+        const ProductArgs g = product(p.w, p.amax_w, p.h, nullptr, v.V, v.M, v.D);
         LogitArgs a{};
-        a.v = v; a.words = v.V; a.part = p.part; a.part_x = label_smoothing > 0.f ? p.part_x : nullptr; a.target_logit = p.target_logit;
+        a.v = v; a.words = v.V; a.h_inverse = p.h_inverse; a.part = p.part; a.part_x = label_smoothing > 0.f ? p.part_x : nullptr; a.target_logit = p.target_logit;
         if (word_rows) hipLaunchKernelGGL((vocab_logits_kernel<true, false>), grid_of(g), dim3(256), 0, stream, g, a);
         else hipLaunchKernelGGL((vocab_logits_kernel<false, false>), grid_of(g), dim3(256), 0, stream, g, a);
         const JoinArgs jn{v, p.part, a.part_x, p.target_logit, g.tiles_m, per_sample_loss, lse};
@@ -639,15 +678,8 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
     Plan p{};
     if (v.M > 0) plan_backward(ws, p, v.M, v.D, v.V, word_rows);
     if (int rc = ws.check(who)) return rc;
-    if (v.M > 0) {
-        hipLaunchKernelGGL(vocab_row_scale_kernel, dim3((unsigned)tiles_of(v.M, 256)), dim3(256), 0, stream, v, upstream, (int)reduction, valid_count, p.row_scale);
-        SplitJobs j{};
-        j.src[0] = source_w(W); j.amax[0] = p.amax_w; j.dst[0] = p.w;
-        j.src[1] = source_h(H, nullptr); j.amax[1] = p.amax_h; j.dst[1] = p.h;
-        launch_split(j, 2, call.state);
-        j.src[0] = source_h(H, p.row_scale); j.amax[0] = p.amax_hs; j.dst[0] = p.hs;
-        if (grad_W) launch_split(j, 1, call.state);
-    }
+    const Upstream up{upstream, (int)reduction, valid_count};
+    if (v.M > 0) launch_split(p, H, W, v, up, grad_W != nullptr, call.state);
     const int64_t piece = v.M > 0 ? p.piece : v.V;
     int64_t runs = 0;
     for (int64_t first = 0; first < v.V; first += piece) {
@@ -656,9 +688,9 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
         G.pitch = split_pad(words);
         if (v.M > 0) {
             const SplitMatrix w = words_of(p.w, first, word_rows);
-            const ProductArgs g = product(w, p.amax_w, p.h, p.amax_h, words, v.M, v.D);
+            const ProductArgs g = product(w, p.amax_w, p.h, nullptr, words, v.M, v.D);
             LogitArgs a{};
-            a.v = v; a.first = first; a.words = words; a.lse = lse; a.row_scale = p.row_scale; a.g = G; a.part_db = grad_bias ? p.part_db : nullptr;
+            a.v = v; a.first = first; a.words = words; a.h_inverse = p.h_inverse; a.lse = lse; a.up = up; a.g = G; a.part_db = grad_bias ? p.part_db : nullptr;
             if (word_rows) hipLaunchKernelGGL((vocab_logits_kernel<true, true>), grid_of(g), dim3(256), 0, stream, g, a);
             else hipLaunchKernelGGL((vocab_logits_kernel<false, true>), grid_of(g), dim3(256), 0, stream, g, a);
         }
@@ -690,7 +722,7 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
         else hipLaunchKernelGGL(vocab_products_kernel<true>, grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
     }
     if (grad_H && v.M > 0)
-        hipLaunchKernelGGL(vocab_dh_kernel, dim3((unsigned)std::min<int64_t>(tiles_of(v.M * v.D, 1024), 8 * call.state.cus)), dim3(256), 0, stream, p.part_h, runs, v.M, v.D, p.row_scale, grad_H, add);
+        hipLaunchKernelGGL(vocab_dh_kernel, dim3((unsigned)std::min<int64_t>(tiles_of(v.M * v.D, 1024), 8 * call.state.cus)), dim3(256), 0, stream, p.part_h, runs, v, up, grad_H, add);
     if (grad_bias) hipLaunchKernelGGL(vocab_db_kernel, dim3((unsigned)tiles_of(v.V, 256)), dim3(256), 0, stream, p.part_db, v.M > 0 ? 2 * tiles_of(v.M, kTileN) : 0, v.V, grad_bias, add);
     return call.finish(sync);
 }

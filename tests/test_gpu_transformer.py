@@ -479,6 +479,29 @@ def test_vocabulary_loss_targets(ops):
     assert np.isnan(each[[3, 7]]).all() and not each[[11, 12]].any() and np.isfinite(np.delete(each, [3, 7])).all() and int(loss.valid_count.item()) == 18
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 1.0e30])
+def test_vocabulary_loss_rows_that_do_not_count(ops, bad):
+    """Whatever the hidden state of an ignored token holds, the others' losses and all gradients are as without it; and a row far larger than the others
+    takes nothing from their losses."""
+    m, d, v = 150, 48, 700
+    h, w, b = randn(1, m, d), randn(2, v, d) * 0.2, randn(3, v)
+    target = torch.arange(m)
+    target[[3, 149]] = -100
+    want = vocabulary_reference(h, w.t(), b, target, -100, 0.1, "mean", torch.ones(1))
+    h[3], h[149] = bad, -bad
+    H, W, B, T = up(ops, h), up(ops, w).transpose(), up(ops, b), target.cuda()
+    loss = ops.V.vocabulary_loss(H, W, B, T, label_smoothing=0.1)
+    assert np.abs(down(loss.per_sample).numpy() - want[0]).max() <= 2 * RTOL_FRO * np.abs(want[1]).max()
+    back = ops.V.vocabulary_loss_backward(H, W, B, T, loss, torch.ones(1, device="cuda"), label_smoothing=0.1)
+    for g, ref, what in zip(back, want[3], ("grad_h", "grad_w", "grad_bias")):
+        close(down(g), ref, 2 * RTOL_FRO, what)
+    if math.isfinite(bad):
+        target[3] = 5
+        loss = ops.V.vocabulary_loss(H, W, B, target.cuda(), label_smoothing=0.1)
+        keep = np.arange(m) != 3
+        assert np.abs(down(loss.per_sample).numpy() - want[0])[keep].max() <= 2 * RTOL_FRO * np.abs(want[1]).max()
+
+
 def test_vocabulary_loss_words_shut_out_by_the_bias(ops):
     """A bias of -inf gives a word no probability, and of its type's lowest value next to none; all but one: the loss of that one is zero."""
     m, d, v = 40, 32, 700

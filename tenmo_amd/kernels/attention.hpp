@@ -52,14 +52,6 @@ __device__ __forceinline__ f32x4 attn_load4(const float* p, int64_t ds, int part
     return x;
 }
 __device__ __forceinline__ float dot4(f32x4 a, f32x4 b) { return (a[0] * b[0] + a[1] * b[1]) + (a[2] * b[2] + a[3] * b[3]); }
-// the sum over the L lanes that hold one key or row
-template <int L>
-__device__ __forceinline__ float lanes_sum(float x) {
-#pragma unroll
-    for (int d = L / 2; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
-    return x;
-}
-
 struct AttnBackward {
     AttnShape s;
     AttnOperand q, k, v;           // q.p .. never written

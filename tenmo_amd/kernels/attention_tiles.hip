@@ -2,6 +2,8 @@
 //
 // Forward, a wavefront for 32 queries, 32 keys at a time:
 //   S^T = K Q^T (keys x queries), p = 2^(S c - m + 7) with c = scale log2(e), O^T += V^T P^T, l += sum p.
+// (Backward, a wavefront works on the up to three tiles of its workgroup that are beyond its own rows as on any other: leaving them out made the
+// compiler copy its sums, 250 instructions a tile.)
 // S^T comes out of the matrix units with a query in each lane (twice: the halves hold the keys 8 a + 0..3 and 8 a + 4..7), so the softmax needs one
 // exchange between lanes, and its registers are the operand of the second product as they are: the order in which that product takes the keys is free, and V is
 // fetched in the same one.  The running maximum m is renewed when a score passes it by 2^8 (p and the sums keep to the range of their types below that).
@@ -126,8 +128,7 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
                 mine = fmaxf(mine, __uint_as_float(finite_magnitude(x[u][e])));
                 wrong |= !(x[u][e] - x[u][e] == 0.f);
             }
-#pragma unroll
-            for (int d = L / 2; d > 0; d >>= 1) mine = fmaxf(mine, __shfl_xor(mine, d, 64));
+            mine = lanes_max<L>(mine);
             top = fmaxf(top, mine);
             if (mine > 0.f) least = fminf(least, mine);
             const float sq = lanes_sum<L>(dot4(x[u], x[u]));
@@ -347,6 +348,15 @@ __device__ __forceinline__ void split_mfma(f32x16& c, f16x8 ah, f16x8 al, f16x8 
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, c, 0, 0, 0);
 }
+// two of them in turn: no product waits for the one before it
+__device__ __forceinline__ void split_mfma2(f32x16& c, f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl, f32x16& d, f16x8 eh, f16x8 el, f16x8 fh, f16x8 fl) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, c, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_32x32x16_f16(el, fh, d, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, c, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_32x32x16_f16(eh, fl, d, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, c, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_32x32x16_f16(eh, fh, d, 0, 0, 0);
+}
 __device__ __forceinline__ f32x16 zero16() {
     f32x16 z;
 #pragma unroll
@@ -480,7 +490,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
         float top = s[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = halves_max(top);
         if (__any(top > m + kRenew)) { // (an m of -inf is passed by any score)
             const float now = top > m + kRenew ? top : m, keep = m == kNone ? 0.f : __builtin_amdgcn_exp2f(m - now);
             m = now;
@@ -513,7 +523,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
         }
         TENMO_PRODUCTS(6);
     }
-    l += __shfl_xor(l, 32, 64);
+    l = halves_sum(l);
     if (i >= a.s.queries) return;
     const int64_t row = (int64_t)bh * a.s.queries + i;
     float* to;
@@ -566,7 +576,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(co
     const int j0 = block * kRowPad + wave * 32, j = j0 + (lane & 31);
     // query i sees key j when i >= j - start and j < length
     const int see = a.s.causal ? j - start : 0;
-    const int wave_first = a.s.causal && j0 - start > 0 ? j0 - start : 0, block_first = a.s.causal && block * kRowPad - start > 0 ? block * kRowPad - start : 0;
+    const int block_first = a.s.causal && block * kRowPad - start > 0 ? block * kRowPad - start : 0;
     const int t0 = block_first / 32, t1 = block * kRowPad < keys ? (a.s.queries + 31) / 32 : 0;
 
     const f32x4 head_q = a.head[kQ][bh], head_k = a.head[kK][bk], head_v = a.head[kV][bk], head_g = a.head[kDO][bh];
@@ -621,12 +631,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(co
         const f32x4* st = (const f32x4*)(g_tile + T::BYTES) + 2 * half; // two rows each
         stage = stage == STAGES - 1 ? 0 : stage + 1;
         const int i0 = t * 32;
-        if (i0 + 31 < wave_first || j0 >= keys) continue;
+
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int ks = 0; ks < T::KD; ++ks) {
-            split_mfma(s, T::row_read(q_tile, row_off[0], ks), T::row_read(q_tile, row_off[1], ks), kh[ks], kl[ks]);
-            split_mfma(dp, T::row_read(g_tile, row_off[0], ks), T::row_read(g_tile, row_off[1], ks), vh[ks], vl[ks]);
+            split_mfma2(s, T::row_read(q_tile, row_off[0], ks), T::row_read(q_tile, row_off[1], ks), kh[ks], kl[ks],
+                        dp, T::row_read(g_tile, row_off[0], ks), T::row_read(g_tile, row_off[1], ks), vh[ks], vl[ks]);
         }
         f32x4 rows[8]; // lse and delta of the rows 8 q + 4 half + {0, 1}, {2, 3}
 #pragma unroll
@@ -646,10 +656,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(co
             dp[e] = dp[e] * inv_dp - rows[e >> 1][2 * (e & 1) + 1];
         }
         if (i0 < j0 + 31 - start || j0 + 32 > length) { // some pairs are not allowed: their p is 0, whatever the rest
-            const int from = see - i0 - 4 * half;
+            const int from = j < length ? see - i0 - 4 * half : 32;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const bool ok = reg_row(e) >= from && j < length;
+                const bool ok = reg_row(e) >= from;
                 s[e] = ok ? s[e] : kNone;
                 dp[e] = ok ? dp[e] : 0.f;
             }
@@ -667,8 +677,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(co
             halves(dp, t2, one, sh, sl);
 #pragma unroll
             for (int d = 0; d < T::ND; ++d) {
-                split_mfma(dv[d], T::column_read(g_tile, col_off[0], t2, d), T::column_read(g_tile, col_off[1], t2, d), ph, pl);
-                split_mfma(dk[d], T::column_read(q_tile, col_off[0], t2, d), T::column_read(q_tile, col_off[1], t2, d), sh, sl);
+                split_mfma2(dv[d], T::column_read(g_tile, col_off[0], t2, d), T::column_read(g_tile, col_off[1], t2, d), ph, pl,
+                            dk[d], T::column_read(q_tile, col_off[0], t2, d), T::column_read(q_tile, col_off[1], t2, d), sh, sl);
             }
         }
         TENMO_READS(16);
@@ -733,7 +743,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(con
     const int q0 = block * kRowPad + wave * 32, i = q0 + (lane & 31);
     const int limit = i < a.s.queries ? attn_limit(length, start, i) : 0;
     const int wave_last = q0 + 31 < a.s.queries ? q0 + 31 : a.s.queries - 1, block_last = (block + 1) * kRowPad < a.s.queries ? (block + 1) * kRowPad - 1 : a.s.queries - 1;
-    const int wave_most = q0 < a.s.queries ? attn_limit(length, start, wave_last) : 0, wave_least = wave_last == q0 + 31 ? attn_limit(length, start, q0) : 0;
+    const int wave_least = wave_last == q0 + 31 ? attn_limit(length, start, q0) : 0;
     const int tiles = (attn_limit(length, start, block_last) + 31) / 32;
 
     const f32x4 head_q = a.head[kQ][bh], head_k = a.head[kK][bk], head_v = a.head[kV][bk], head_g = a.head[kDO][bh];
@@ -775,12 +785,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(con
         const char* k_tile = (const char*)lds + stage * 2 * T::BYTES;
         const char* v_tile = k_tile + T::BYTES;
         stage = stage == STAGES - 1 ? 0 : stage + 1;
-        if (t * 32 >= wave_most) continue;
+
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int ks = 0; ks < T::KD; ++ks) {
-            split_mfma(s, T::row_read(k_tile, row_off[0], ks), T::row_read(k_tile, row_off[1], ks), qh[ks], ql[ks]);
-            split_mfma(dp, T::row_read(v_tile, row_off[0], ks), T::row_read(v_tile, row_off[1], ks), gh[ks], gl[ks]);
+            split_mfma2(s, T::row_read(k_tile, row_off[0], ks), T::row_read(k_tile, row_off[1], ks), qh[ks], ql[ks],
+                        dp, T::row_read(v_tile, row_off[0], ks), T::row_read(v_tile, row_off[1], ks), gh[ks], gl[ks]);
         }
         TENMO_READS(8);
 #pragma unroll
@@ -832,7 +842,7 @@ int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 9
 void plan_operands(TileArgs& a, Workspace& ws, int jobs) {
     const AttnShape& s = a.s;
     a.jobs = jobs;
-    a.parts = std::max(1, std::min(kHeadParts, (std::max(s.queries, s.keys) + 63) / 64));
+    a.parts = std::max(1, std::min(kHeadParts, (std::max(s.queries, s.keys) + 255) / 256));
     for (int j = 0; j < jobs; ++j) {
         const bool key = j == kK || j == kV;
         const int64_t heads = (int64_t)s.batch * (key ? s.kv_heads : s.heads);

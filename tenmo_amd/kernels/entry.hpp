@@ -101,17 +101,45 @@ inline int64_t elements(const tenmo_view* v) {
 }
 
 // ---- reductions ---------------------------------------------------------------------------------------------------------
+// Between lanes through the vector unit's own lane moves (no LDS): within quads, halves of 16, 16, then rows of 16 exchanged.  Every lane ends with the same
+// bits: each step adds the same two values in either order.
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+template <int CTRL>
+__device__ __forceinline__ float lane_move(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// f(this lane's group of L, the neighbouring one's) for L = 1, 2, 4 .. 64 / 2
+template <int L, class F>
+__device__ __forceinline__ float lanes_reduce(float v, F f) {
+    if (L >= 2) v = f(v, lane_move<0xB1>(v));   // quad_perm 1 0 3 2
+    if (L >= 4) v = f(v, lane_move<0x4E>(v));   // quad_perm 2 3 0 1
+    if (L >= 8) v = f(v, lane_move<0x141>(v));  // row_half_mirror
+    if (L >= 16) v = f(v, lane_move<0x140>(v)); // row_mirror
+    if (L >= 32) {
+        const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = f(__uint_as_float(x[0]), __uint_as_float(x[1]));
+    }
+    if (L >= 64) {
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = f(__uint_as_float(x[0]), __uint_as_float(x[1]));
+    }
     return v;
 }
-
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+// over each group of L lanes
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) { return lanes_reduce<L>(v, [](float a, float b) { return a + b; }); }
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) { return lanes_reduce<L>(v, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ float wave_sum(float v) { return lanes_sum<64>(v); }
+__device__ __forceinline__ float wave_max(float v) { return lanes_max<64>(v); }
+// of this lane and the one 32 further
+__device__ __forceinline__ float halves_max(float v) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
 }
 
 // The sum over W wavefronts of a workgroup, in every thread, the same bits in all of them.  `slots` holds W floats; calls that

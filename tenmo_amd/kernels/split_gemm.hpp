@@ -39,14 +39,8 @@ __device__ __forceinline__ uint32_t finite_magnitude(float x) {
     const uint32_t m = __float_as_uint(x) & 0x7fffffffu;
     return m < 0x7f800000u ? m : 0u;
 }
-__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t w = (uint32_t)__shfl_xor((int)v, o, 64);
-        v = v > w ? v : w;
-    }
-    return v;
-}
+// (of magnitudes: their order as floats is that of their bits)
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) { return __float_as_uint(wave_max(__uint_as_float(v))); }
 // The power of two that brings the magnitude with these bits into [2^14, 2^15); 1 for zero.
 __device__ __forceinline__ float split_scale(uint32_t bits) {
     if (bits == 0) return 1.f;

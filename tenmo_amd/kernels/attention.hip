@@ -57,9 +57,21 @@ __global__ __launch_bounds__(256) void attn_zero_kernel(AttnOperand g, int64_t n
     }
 }
 
-// Rows or tiles: a tile is 32 queries against 32 keys, and its operands take two launches first.
-bool forward_by_rows(const AttnShape& s) { return s.queries <= 16; }
-bool backward_by_rows(const AttnShape& s) { return s.queries <= 48 || s.keys <= 48; }
+// Rows or tiles.  Rows work at D / 5 million pairs of a query and a key a microsecond less, tiles pay 7 us and one more pass over the operands before they begin: by these
+// sums, fitted to 150 shapes of D = 32, 64, 128 with 2 to 256 queries, 32 to 8192 keys and 8 to 512 heads.  Where the two meet, either is within a fifth of the other; at
+// [1, 8 x 64, 64 keys] rows take 13 us and tiles 20, at [32,16 x 64, 256 keys] 470 and 87.
+double padded(int dim) { return (dim + 31) / 32 * 32; }
+double pair_values(const AttnShape& s) { return (double)s.batch * s.heads * s.queries * s.keys * padded(s.dim); }
+bool forward_by_rows(const AttnShape& s) {
+    const double operands = (double)s.batch * padded(s.dim) * ((double)s.heads * s.queries + 2.0 * s.kv_heads * s.keys);
+    return pair_values(s) <= 37e6 + 18.0 * operands;
+}
+// Backward, where the rows' kernels also read the other side again for each row, one after the other: short sequences alone ([1, 8 x 64] with 128 queries and keys: 32 us by
+// rows, 46 by tiles; with 256: 68 and 60).
+bool backward_by_rows(const AttnShape& s) {
+    const double operands = 2.0 * s.batch * padded(s.dim) * ((double)s.heads * s.queries + (double)s.kv_heads * s.keys);
+    return s.queries <= 256 && s.keys <= 256 && pair_values(s) <= 20e6 + 6.0 * operands;
+}
 
 void forward_plan(const AttnShape& s, const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, float* out, float* lse, Workspace& ws, const LibraryState& lib, bool launch) {
     if (forward_by_rows(s)) attn_rows_forward(s, q, k, v, out, lse, ws, lib.cus, lib.stream, launch);

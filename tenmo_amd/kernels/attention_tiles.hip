@@ -444,7 +444,10 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
     }
     f16x8 qh[T::KD], ql[T::KD];
     own_rows<DP>(qh, ql, a.split[kQ] + ((int64_t)bh * pad_q + q0) * DP, lane);
-    const float inv_v = 1.f / head_v[0], c = a.s.scale * kLog2e / head_q[0] / head_k[0];
+    const float inv_v = 1.f / head_v[0], c = fabsf(a.s.scale) * kLog2e / head_q[0] / head_k[0];
+    if (a.s.scale < 0.f) // the maximum is taken before the factor, which has to keep the order
+#pragma unroll
+        for (int ks = 0; ks < T::KD; ++ks) qh[ks] = -qh[ks], ql[ks] = -ql[ks];
     const float* const base[2] = {a.split[kK] + (int64_t)bk * pad_k * DP, a.split[kV] + (int64_t)bk * pad_k * DP};
     uint32_t off[LOADS];
     T::template offsets<2>(off, wave, lane);
@@ -480,17 +483,17 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
             TENMO_READS(2);
         }
         TENMO_PRODUCTS(6);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] *= c;
-        if (t * 32 + 32 > wave_least) {
+        float by = c;
+        if (t * 32 + 32 > wave_least) { // (the factor first: it may be 0, and -inf has to stay what it is)
             const int left = limit - t * 32 - 4 * half;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = reg_row(e) < left ? s[e] : kNone;
+            for (int e = 0; e < 16; ++e) s[e] = reg_row(e) < left ? s[e] * c : kNone;
+            by = 1.f;
         }
         float top = s[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-        top = halves_max(top);
+        top = halves_max(top) * by;
         if (__any(top > m + kRenew)) { // (an m of -inf is passed by any score)
             const float now = top > m + kRenew ? top : m, keep = m == kNone ? 0.f : __builtin_amdgcn_exp2f(m - now);
             m = now;
@@ -504,7 +507,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            s[e] = __builtin_amdgcn_exp2f(s[e] + shift);
+            s[e] = __builtin_amdgcn_exp2f(s[e] * by + shift);
             sum += s[e];
         }
         l += sum;

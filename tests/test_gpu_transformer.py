@@ -194,6 +194,13 @@ ATTENTION = [  # batch, queries, keys, heads, kv_heads, dim, causal, lengths, st
     (1, 333, 333, 8, 2, 96, True, None, None),
     (1, 700, 513, 2, 1, 64, False, None, None),
     (2, 129, 257, 3, 3, 72, True, [-5, 400], [1000000, -1000000]),
+    (9, 65, 65, 8, 2, 33, True, [65, 64, 0, 1, 33, 65, 50, 2, 32], None),
+    (8, 160, 96, 16, 8, 64, True, None, None),     # the first 64 queries have no keys
+    (6, 97, 290, 16, 16, 20, True, [290, 100, 64, 0, 289, 97], [193, 3, -33, 10, 192, 0]),
+    (4, 130, 400, 16, 16, 100, False, [1, 257, 399, 128], None),
+    (1, 300, 300, 24, 3, 128, True, None, None),
+    (3, 384, 384, 8, 8, 64, True, [384, 255, 129], None),
+    (1, 100, 9000, 8, 8, 64, True, [8190], [8090]),  # few query tiles: the keys in runs
 ]
 
 
@@ -230,10 +237,10 @@ def test_attention(ops, case):
         assert [s is not None for s in some] == [i == skip for i in range(3)] and torch.equal(down(some[skip]), down(got[skip]))
 
 
-@pytest.mark.parametrize("n", [1, 40, 150])
+@pytest.mark.parametrize("n", [1, 40, 150, 600])
 def test_attention_of_strided_operands(ops, n):
     """Slices of a joint projection, heads before positions, every second value of d, a batch that is one sequence repeated (stride 0)."""
-    B, H, Hk, D, m = 2, 4, 2, 24, 150
+    B, H, Hk, D, m = 2, 4, 2, 24, max(150, n)
     qkv = randn(3, B, m, (H + 2 * Hk) * D)
     packed = (qkv[:, m - n:, :H * D].unflatten(2, (H, D)), qkv[:, :, H * D:(H + Hk) * D].unflatten(2, (Hk, D)), qkv[:, :, (H + Hk) * D:].unflatten(2, (Hk, D)))
     swapped = tuple(randn(4 + i, B, h, s, D).transpose(1, 2) for i, (h, s) in enumerate(((H, n), (Hk, m), (Hk, m))))
@@ -258,10 +265,10 @@ def test_attention_of_strided_operands(ops, n):
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 3.0e38])
-@pytest.mark.parametrize("n", [1, 70])
+@pytest.mark.parametrize("n", [1, 70, 100])
 def test_keys_that_are_not_allowed_are_not_used(ops, bad, n):
     """Whatever lies behind a sequence's keys, or ahead of a query, leaves no trace."""
-    B, m, H, D = 2, 140, 2, 64
+    B, m, H, D = 2, 140, 2 if n < 100 else 64, 64
     q, k, v, dout = randn(1, B, n, H, D), randn(2, B, m, H, D), randn(3, B, m, H, D), randn(4, B, n, H, D)
     lengths, starts = [100, 37], [100 - n, 20 - n]
     want = attention_reference(q, k, v, 0.1, True, lengths, starts, dout)
@@ -282,7 +289,7 @@ def test_keys_that_are_not_allowed_are_not_used(ops, bad, n):
 @pytest.mark.parametrize("dim", [16, 64, 96, 128])
 def test_a_row_out_of_the_ordinary_stays_with_what_sees_it(ops, where, bad, dim):
     """One row of one head that is not finite, or far larger than all others: queries before it, keys behind it and the other heads are as without it."""
-    B, n, H, at = 2, 90, 2, 50
+    B, n, H, at = 2, 200, 24, 120
     tensors = {name: randn(i, B, n, H, dim) for i, name in enumerate(("q", "k", "v", "dout"))}
     want = attention_reference(tensors["q"], tensors["k"], tensors["v"], 0.2, True, None, None, tensors["dout"])
     tensors[where][1, at, 0] = bad
@@ -313,6 +320,25 @@ def test_attention_with_values_that_are_not_finite(ops):
     close(o, want, RTOL_FRO, "the others")
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30, 2.0 ** -120])
+@pytest.mark.parametrize("n", [3, 160])
+def test_attention_scales(ops, n, scale):
+    """No scale (every allowed key counts the same), a negative one, and ones that no score survives."""
+    q, k, v, dout = (randn(i, 1, n, 2, 64) for i in range(4))
+    want, want_lse, grads = attention_reference(q, k, v, scale, True, None, None, dout)
+    for reps in (1, 40):  # enough heads for either kernel
+        Qr, Kr, Vr, DOr = (up(ops, t.repeat(reps, 1, 1, 1)) for t in (q, k, v, dout))
+        o, lse = ops.A.attention(Qr, Kr, Vr, scale=scale, causal=True)
+        close(down(o)[-1], want[0], RTOL_FRO, "out")
+        close(down(lse)[-1], want_lse[0], RTOL_FRO, "lse")
+        got = ops.A.attention_backward(Qr, Kr, Vr, o, lse, DOr, scale=scale, causal=True)
+        for g, ref, what in zip(got, grads, ("grad_q", "grad_k", "grad_v")):
+            if what == "grad_v" or abs(scale) > 1e-20:
+                close(down(g)[-1], ref[0], 2 * RTOL_FRO, what)
+            else:
+                assert np.abs(down(g)[-1].numpy()).max() <= abs(scale) * 1e4
+
+
 def test_attention_extreme_scores(ops):
     """Scores of thousands and values over 40 powers of two: the maximum is taken off before the exponential, and the sums have fp32's range."""
     B, n, H, D = 1, 96, 2, 64
@@ -320,21 +346,22 @@ def test_attention_extreme_scores(ops):
     v[:, :, 1] *= 2.0 ** 40
     dout[:, :, 0] *= 2.0 ** -40
     want = attention_reference(q, k, v, 1.0, True, None, None, dout)
-    Q, K, V, DO = (up(ops, t) for t in (q, k, v, dout))
-    o, lse = ops.A.attention(Q, K, V, scale=1.0, causal=True)
     # The magnitudes of a score's 64 products add up to 64 * 16 * 16 * 0.64 * 2 = 21000 at most; 12 roundings of 2^-24 of that are 2^-6, in the exponent and so
     # relative in p.  Nearly every p is 0 or 1, and a gradient p (dP - delta) cancels where it is 1: its error is measured against p (|dP| + |delta|).
     tol = 2.0 ** -6
-    close(down(lse), want[1], RTOL_FRO, "lse")
-    got = ops.A.attention_backward(Q, K, V, o, lse, DO, scale=1.0, causal=True)
-    for h in range(H):
-        close(down(o)[:, :, h], want[0][:, :, h], tol, "out")
-        close(down(got[2])[:, :, h], want[2][2][:, :, h], tol, "grad_v")
-        qh, kh, vh, gh = (t[0, :, h].double().numpy() for t in (q, k, v, dout))
-        p = np.tril(np.exp(np.minimum(qh @ kh.T - want[1][0, h][:, None], 0.0)))
-        terms = p * (np.abs(gh @ vh.T) + np.abs((gh * want[0][0, :, h]).sum(1))[:, None])
-        for g, ref, size, what in ((got[0], want[2][0], terms @ np.abs(kh), "grad_q"), (got[1], want[2][1], terms.T @ np.abs(qh), "grad_k")):
-            assert np.linalg.norm(down(g)[0, :, h].numpy() - ref[0, :, h]) <= tol * np.linalg.norm(size), what
+    for reps in (1, 60):  # enough heads for either kernel
+        Q, K, V, DO = (up(ops, t.repeat(reps, 1, 1, 1)) for t in (q, k, v, dout))
+        o, lse = ops.A.attention(Q, K, V, scale=1.0, causal=True)
+        close(down(lse)[-1], want[1][0], RTOL_FRO, "lse")
+        got = [down(g)[-1] for g in ops.A.attention_backward(Q, K, V, o, lse, DO, scale=1.0, causal=True)]
+        for h in range(H):
+            close(down(o)[-1, :, h], want[0][0, :, h], tol, "out")
+            close(got[2][:, h], want[2][2][0, :, h], tol, "grad_v")
+            qh, kh, vh, gh = (t[0, :, h].double().numpy() for t in (q, k, v, dout))
+            p = np.tril(np.exp(np.minimum(qh @ kh.T - want[1][0, h][:, None], 0.0)))
+            terms = p * (np.abs(gh @ vh.T) + np.abs((gh * want[0][0, :, h]).sum(1))[:, None])
+            for g, ref, size, what in ((got[0], want[2][0], terms @ np.abs(kh), "grad_q"), (got[1], want[2][1], terms.T @ np.abs(qh), "grad_k")):
+                assert np.linalg.norm(g[:, h].numpy() - ref[0, :, h]) <= tol * np.linalg.norm(size), what
 
 
 def test_attention_without_keys_or_queries(ops):
@@ -350,7 +377,7 @@ def test_attention_without_keys_or_queries(ops):
     assert not down(gk).any() and not down(gv).any()
 
 
-@pytest.mark.parametrize("n", [1, 130])
+@pytest.mark.parametrize("n", [1, 130, 2300])
 def test_attention_offsets_past_32_bits(ops, n):
     """A cache whose positions lie 2^24 values apart: the last of 300 is more than 2^32 values behind the first."""
     m, D, pitch = 300, 64, 1 << 24
@@ -442,8 +469,8 @@ def test_vocabulary_loss(ops, case):
 
 
 def test_vocabulary_loss_in_several_pieces(ops, monkeypatch):
-    """Tokens enough for more than one piece of the vocabulary: 2^27 values of G are 20480 tokens times 6553 words."""
-    m, d, v = 20480, 32, 9001
+    """Tokens enough for more than one piece of the vocabulary: 2^28 values of G are 20480 tokens times 13107 words."""
+    m, d, v = 20480, 32, 14001
     h, w, b = randn(1, m, d).cuda(), (randn(2, v, d) * 0.3).cuda(), randn(3, v).cuda()
     target = torch.randint(0, v, (m,), generator=torch.Generator().manual_seed(1)).cuda()
     x = h.double() @ w.double().t() + b.double()
@@ -614,8 +641,8 @@ def call_all(ops, s):
 
 
 def state_of(ops, seed):
-    s = {n: up(ops, randn(seed + i, *shape)) for i, (n, shape) in enumerate((("x", (70, 96)), ("w", (96,)), ("q", (2, 200, 4, 64)), ("k", (2, 200, 2, 64)), ("v", (2, 200, 2, 64)),
-                                                                             ("q1", (2, 1, 4, 64)), ("h", (200, 80)), ("e", (900, 80)), ("b", (900,))))}
+    s = {n: up(ops, randn(seed + i, *shape)) for i, (n, shape) in enumerate((("x", (70, 96)), ("w", (96,)), ("q", (2, 400, 8, 64)), ("k", (2, 400, 2, 64)), ("v", (2, 400, 2, 64)),
+                                                                             ("q1", (2, 1, 8, 64)), ("h", (200, 80)), ("e", (900, 80)), ("b", (900,))))}
     s["t"] = torch.randint(0, 900, (200,), generator=torch.Generator().manual_seed(seed)).cuda()
     s["one"] = torch.ones(1, device="cuda")
     return s

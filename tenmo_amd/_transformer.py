@@ -50,37 +50,35 @@ def load() -> C.CDLL:
     return L
 
 
-class Launch:
-    """``with Launch(buffer, ...) as L:`` — the library initialised, every operand on its device, its stream joined with the current one."""
+def enter(*operands: Optional[NDBuffer]):
+    """(library, token): the library initialised, every operand on its device, its stream behind the current one.  ``leave(token)`` puts the
+    current stream behind the library's."""
+    _lib.init()
+    for b in operands:
+        if b is not None and b.storage.get_device() != 0:  # _lib.init's device
+            raise TenmoHipError(-3, f"operand on {b.storage.device}: the library runs on device 0")
+    L = _bound or load()
+    current, own = _current_stream(0), L.tenmo_hip_get_stream() or 0
+    if current == own or (current == 0 and _follows_default(L, own)):
+        return L, None
+    stream, library = torch.cuda.current_stream(0), torch.cuda.ExternalStream(own, device=0)
+    library.wait_stream(stream)
+    return L, (stream, library)
 
-    __slots__ = ("_join",)
 
-    def __init__(self, *operands: Optional[NDBuffer]):
-        _lib.init()
-        for b in operands:
-            if b is not None and b.storage.get_device() != 0:  # _lib.init's device
-                raise TenmoHipError(-3, f"operand on {b.storage.device}: the library runs on device 0")
+def leave(token) -> None:
+    if token is not None:
+        current, library = token
+        current.wait_stream(library)
 
-    def __enter__(self) -> C.CDLL:
-        L = _bound or load()
-        current, own = torch._C._cuda_getCurrentRawStream(0), L.tenmo_hip_get_stream() or 0
-        self._join = None
-        if current != own and not (current == 0 and self._follows_default(L, own)):
-            stream, library = torch.cuda.current_stream(0), torch.cuda.ExternalStream(own, device=0)
-            library.wait_stream(stream)
-            self._join = (stream, library)
-        return L
 
-    @staticmethod
-    def _follows_default(L: C.CDLL, stream: int) -> bool:
-        """Whether the stream is ordered with the default stream by itself (it was not created as a non-blocking one)."""
-        flags = C.c_uint(1)
-        return L.hipStreamGetFlags(stream, C.byref(flags)) == 0 and flags.value == 0
+_current_stream = torch._C._cuda_getCurrentRawStream
 
-    def __exit__(self, *exc) -> None:
-        if self._join is not None:
-            current, library = self._join
-            current.wait_stream(library)
+
+def _follows_default(L: C.CDLL, stream: int) -> bool:
+    """Whether the stream is ordered with the default stream by itself (it was not created as a non-blocking one)."""
+    flags = C.c_uint(1)
+    return L.hipStreamGetFlags(stream, C.byref(flags)) == 0 and flags.value == 0
 
 
 def empty(like: NDBuffer, *shape: int) -> NDBuffer:
@@ -90,7 +88,7 @@ def empty(like: NDBuffer, *shape: int) -> NDBuffer:
         strides.append(n)
         n *= s
     b = NDBuffer.__new__(NDBuffer)  # (what the constructor checks holds here)
-    b.storage = torch.empty(n or 1, dtype=torch.float32, device=like.storage.device)
+    b.storage = like.storage.new_empty(n or 1)
     b.shape, b.strides, b.offset = shape, tuple(reversed(strides)), 0
     return b
 
@@ -113,7 +111,7 @@ def workspace(like: NDBuffer, nbytes: int):
     check(nbytes)
     if nbytes == 0:
         return None, None, 0
-    t = torch.empty(nbytes, dtype=torch.uint8, device=like.storage.device)
+    t = like.storage.new_empty((nbytes + 3) // 4)
     return t, t.data_ptr(), nbytes
 
 
@@ -122,10 +120,9 @@ def address(b: Optional[NDBuffer]) -> Optional[int]:
     return None if b is None else b.storage.data_ptr() + 4 * b.offset
 
 
-def dense(b: Optional[NDBuffer], shape, what: str) -> Optional[NDBuffer]:
-    if b is not None and (tuple(b.shape) != tuple(shape) or not b.is_contiguous()):
-        raise TenmoHipError(-2, f"{what} must be dense with shape {tuple(shape)}, got shape {b.shape} with strides {b.strides}")
-    return b
+def dense(b: Optional[NDBuffer], shape: tuple, what: str) -> None:
+    if b is not None and (b.shape != shape or not (b.strides == (1,) or b.is_contiguous())):
+        raise TenmoHipError(-2, f"{what} must be dense with shape {shape}, got shape {b.shape} with strides {b.strides}")
 
 
 def device_ints(t: Optional[torch.Tensor], n: int, what: str, dtypes=(torch.int32,)) -> Optional[int]:

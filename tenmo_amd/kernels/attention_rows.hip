@@ -134,28 +134,34 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const RowsArgs a) {
     }
 }
 
-// The runs of one row joined: 4 wavefronts, each with every fourth run, two values of d a lane.
-__global__ __launch_bounds__(256) void attn_join_kernel(const AttnShape s, const float* __restrict part, int splits, float* __restrict out, float* __restrict lse) {
-    __shared__ float keep_of[kMostRuns], sum_of[4], o_of[4][128];
+// The runs of one row joined: W wavefronts, each with every W-th run, two values of d a lane.
+template <int W>
+__global__ __launch_bounds__(64 * W) void attn_join_kernel(const AttnShape s, const float* __restrict part, int splits, float* __restrict out, float* __restrict lse) {
+    __shared__ float keep_of[kMostRuns], sum_of[kMostRuns], slots[2][W], o_of[W][128];
     const int D = s.dim, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t row = blockIdx.x, pitch = (int64_t)s.batch * s.heads * s.queries * (D + 2);
     const float* __restrict p = part + row * (D + 2);
     float top = kNone;
-    for (int t = threadIdx.x; t < splits; t += 256) top = fmaxf(top, keep_of[t] = p[t * pitch + D]);
+    for (int t = threadIdx.x; t < splits; t += 64 * W) {
+        keep_of[t] = p[t * pitch + D];
+        sum_of[t] = p[t * pitch + D + 1];
+        top = fmaxf(top, keep_of[t]);
+    }
     top = wave_max(top);
-    if (lane == 0) sum_of[wave] = top;
+    if (lane == 0) slots[0][wave] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(sum_of[0], sum_of[1]), fmaxf(sum_of[2], sum_of[3]));
-    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, slots[0][w]);
     float sum = 0.f;
-    for (int t = threadIdx.x; t < splits; t += 256) {
+    for (int t = threadIdx.x; t < splits; t += 64 * W) {
         const float keep = below(keep_of[t], top);
-        sum += keep * p[t * pitch + D + 1];
+        sum += keep * sum_of[t];
         keep_of[t] = keep;
     }
-    sum = group_sum<4>(sum, sum_of); // (a barrier: keep_of is whole)
+    sum = group_sum<W>(sum, slots[1]); // (a barrier: keep_of is whole)
     float o[2] = {0.f, 0.f};
-    for (int t = wave; t < splits; t += 4)
+#pragma unroll 8
+    for (int t = wave; t < splits; t += W)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
             if (lane + 64 * e < D) o[e] += keep_of[t] * p[t * pitch + lane + 64 * e];
@@ -164,7 +170,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnShape s, const
     __syncthreads();
     const int i = (int)(row % s.queries), h = (int)(row / s.queries % s.heads), d = threadIdx.x;
     const int64_t b = row / s.queries / s.heads;
-    if (d < D) out[((b * s.queries + i) * s.heads + h) * D + d] = sum == 0.f ? 0.f : ((o_of[0][d] + o_of[1][d]) + (o_of[2][d] + o_of[3][d])) / sum;
+    if (d < D) {
+        float x = o_of[0][d];
+        for (int w = 1; w < W; ++w) x += o_of[w][d];
+        out[((b * s.queries + i) * s.heads + h) * D + d] = sum == 0.f ? 0.f : x / sum;
+    }
     if (d == 0 && lse) lse[row] = sum == 0.f ? kNone : top + logf(sum);
 }
 
@@ -319,7 +329,10 @@ void attn_rows_forward(const AttnShape& s, const AttnOperand& q, const AttnOpera
 }
 
 void attn_join(const AttnShape& s, const float* part, int splits, float* out, float* lse, hipStream_t stream) {
-    hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)((int64_t)s.batch * s.heads * s.queries)), dim3(256), 0, stream, s, part, splits, out, lse);
+    const dim3 grid((unsigned)((int64_t)s.batch * s.heads * s.queries));
+    // many runs of few rows: one load of each wavefront's runs after another is what takes the time (128 runs of 32 rows: 19 us with 4 wavefronts)
+    if (splits > 16) hipLaunchKernelGGL(attn_join_kernel<16>, grid, dim3(1024), 0, stream, s, part, splits, out, lse);
+    else hipLaunchKernelGGL(attn_join_kernel<4>, grid, dim3(256), 0, stream, s, part, splits, out, lse);
 }
 
 } // namespace tenmo

@@ -308,6 +308,7 @@ __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs 
             const bool valid = token < a.v.M && t != a.v.ignore;
             const float lse = valid ? a.lse[token] : 0.f, row_scale = valid && a.part_db ? row_factor(a.v, a.up, token) : 0.f;
             const int64_t at = t - a.first - v0;
+            const bool here = __any(at >= 0 && at < 128); // a target among this wavefront's words: one in six at 50257 words
             const bool store = token < split_pad(a.v.M);
             float* to = a.g.p + (store ? token : 0) * a.g.pitch;
 #pragma unroll
@@ -319,7 +320,7 @@ __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs 
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float g = __expf(acc[i][j][4 * q + e] - lse) - smooth;
-                        if (at == 32 * i + 8 * q + e) g -= 1.f - a.v.ls;
+                        if (here && at == 32 * i + 8 * q + e) g -= 1.f - a.v.ls;
                         g = valid && v + e < a.words ? g : 0.f;
                         if (a.part_db) db[16 * i + 4 * q + e] += g * row_scale;
                         _Float16 hi, lo;

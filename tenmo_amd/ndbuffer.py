@@ -36,8 +36,8 @@ class NDBuffer:
         if storage.dtype != torch.float32 or storage.dim() != 1 or not storage.is_cuda:
             raise TenmoHipError(-3, "NDBuffer storage must be a flat fp32 device tensor")
         self.storage = storage
-        self.shape = tuple(int(s) for s in shape)
-        self.strides = tuple(int(s) for s in strides) if strides is not None else default_strides(self.shape)
+        self.shape = tuple(map(int, shape))
+        self.strides = tuple(map(int, strides)) if strides is not None else default_strides(self.shape)
         self.offset = int(offset)
         if len(self.shape) != len(self.strides):
             raise TenmoHipError(-2, "shape and strides differ in rank")

@@ -2,6 +2,7 @@
 The arithmetic is the library's (``tenmo_hip_layer_norm_*``, include/tenmo_hip_transformer.h)."""
 from __future__ import annotations
 
+import math
 from typing import List, Optional, Sequence, Tuple
 
 from . import _transformer as _t
@@ -14,7 +15,7 @@ def _rows(x: NDBuffer) -> Tuple[int, int]:
     if x.rank() < 1:
         raise TenmoHipError(-2, "layer_norm: needs at least one axis")
     n = x.shape[-1]
-    return (x.numels() // n if n else 0), n
+    return math.prod(x.shape[:-1]) if n else 0, n
 
 
 def layer_norm(x: NDBuffer, weight: Optional[NDBuffer] = None, bias: Optional[NDBuffer] = None, eps: float = 1e-5,
@@ -23,11 +24,12 @@ def layer_norm(x: NDBuffer, weight: Optional[NDBuffer] = None, bias: Optional[ND
     rows, n = _rows(x)
     _t.dense(weight, (n,), "layer_norm: weight")
     _t.dense(bias, (n,), "layer_norm: bias")
-    with _t.Launch(x, weight, bias) as L:
-        out = _t.empty(x, *x.shape)
-        mean, rstd = (_t.empty(x, rows), _t.empty(x, rows)) if statistics else (None, None)
-        check(L.tenmo_hip_layer_norm_forward_f32(_t.view(x), _t.address(weight), _t.address(bias), eps, out.data_ptr(),
-                                                 _t.address(mean), _t.address(rstd), 1 if sync else 0))
+    L, joined = _t.enter(x, weight, bias)
+    out = _t.empty(x, *x.shape)
+    mean, rstd = (_t.empty(x, rows), _t.empty(x, rows)) if statistics else (None, None)
+    check(L.tenmo_hip_layer_norm_forward_f32(_t.view(x), _t.address(weight), _t.address(bias), eps, out.data_ptr(),
+                                             _t.address(mean), _t.address(rstd), 1 if sync else 0))
+    _t.leave(joined)
     return out, mean, rstd
 
 
@@ -46,12 +48,13 @@ def layer_norm_backward(x: NDBuffer, weight: Optional[NDBuffer], mean: NDBuffer,
     if into is not None:
         for g, shape, what in zip(into, (x.shape, (n,), (n,)), ("grad_x", "grad_weight", "grad_bias")):
             _t.dense(g, shape, "layer_norm_backward: " + what)
-    with _t.Launch(x, weight, mean, rstd, dy, *(into or ())) as L:
-        gx, gw, gb = into if into is not None else (_t.empty(x, *x.shape) if need_x else None, _t.empty(x, n) if need_weight else None,
-                                                    _t.empty(x, n) if need_bias else None)
-        _, ws, size = _keep = _t.workspace(x, L.tenmo_hip_layer_norm_backward_workspace_bytes(rows, n) if gw is not None or gb is not None else 0)
-        check(L.tenmo_hip_layer_norm_backward_f32(_t.view(x), _t.address(weight), _t.address(mean), _t.address(rstd), _t.address(dy),
-                                                  _t.address(gx), _t.address(gw), _t.address(gb), 0 if into is None else 1, ws, size, 1 if sync else 0))
+    L, joined = _t.enter(x, weight, mean, rstd, dy, *(into or ()))
+    gx, gw, gb = into if into is not None else (_t.empty(x, *x.shape) if need_x else None, _t.empty(x, n) if need_weight else None,
+                                                _t.empty(x, n) if need_bias else None)
+    _, ws, size = _keep = _t.workspace(x, L.tenmo_hip_layer_norm_backward_workspace_bytes(rows, n) if gw is not None or gb is not None else 0)
+    check(L.tenmo_hip_layer_norm_backward_f32(_t.view(x), _t.address(weight), _t.address(mean), _t.address(rstd), _t.address(dy),
+                                              _t.address(gx), _t.address(gw), _t.address(gb), 0 if into is None else 1, ws, size, 1 if sync else 0))
+    _t.leave(joined)
     return gx, gw, gb
 
 

@@ -14,8 +14,9 @@
 //   queries: a wavefront for 32 queries, over their keys: S^T, dP^T, dS^T; dQ^T += K^T dS^T.
 // Seven products for the five that one pass with atomics would need.
 //
-// Two launches bring the operands into split form first: the largest magnitude of each head (of the rows that count), then the halves, head by head,
-// rows padded to 128 and D to DP = 32, 64, 96 or 128 with zeros; rows that no allowed pair touches are zeros too, whatever the operand holds there.
+// Two launches bring the operands that are read in tiles into split form first: the largest magnitude of each head (of the rows that count), then the halves, head by head,
+// rows padded to 128 and D to DP = 32, 64, 96 or 128 with zeros; rows that no allowed pair touches are zeros too, whatever the operand holds there.  Forward, a wavefront's own rows of q
+// are split as they are read, with a scale of their own each ([8,1024,12,64]: 14 us less beforehand, 4 more in the product; backward, where all four are there, it costs 11).
 // dS has |dS| <= 2 max |dO_i| max |V_j| (norms of rows), which gives its scale before it is known.
 //
 // LDS tile: 32 rows of DP / 4 chunks of 16 bytes, chunk c = 2 * (d / 8) + kind at slot c ^ swizzle(row); read by rows (16 bytes a lane: 16 rows in 16 different slots of the
@@ -36,12 +37,12 @@ constexpr float kRenew = 8.f;
 
 __host__ __device__ constexpr int row_pad(int n) { return (n + kRowPad - 1) / kRowPad * kRowPad; }
 
-enum { kQ, kK, kV, kDO };
+enum { kK, kV, kQ, kDO }; // forward the first two are split beforehand, backward all of them
 
 struct TileArgs {
     AttnShape s;
-    AttnOperand src[4]; // q, k, v, dout
-    int jobs;           // 3 or 4 of them
+    AttnOperand src[4];
+    int jobs;           // operands that are split beforehand
     int parts;
     float* split[4];    // [batch][heads][rows padded][DP]
     f32x4* seen[4];     // [batch * heads][parts]: of a run of rows, the largest finite magnitude, the largest norm of a row, the smallest largest magnitude of a row
@@ -73,9 +74,9 @@ struct HeadJob {
 __device__ __forceinline__ HeadJob head_job(const TileArgs& a, int y) {
     HeadJob j;
     const int q = a.s.batch * a.s.heads, k = a.s.batch * a.s.kv_heads;
-    j.job = y < q ? kQ : y < q + k ? kK : y < q + 2 * k ? kV : kDO;
+    j.job = y < k ? kK : y < 2 * k ? kV : y < 2 * k + q ? kQ : kDO;
     const bool key = j.job == kK || j.job == kV;
-    j.bh = j.job == kQ ? y : j.job == kK ? y - q : j.job == kV ? y - q - k : y - q - 2 * k;
+    j.bh = j.job == kK ? y : j.job == kV ? y - k : j.job == kQ ? y - 2 * k : y - 2 * k - q;
     j.heads = key ? a.s.kv_heads : a.s.heads;
     j.b = j.bh / j.heads;
     j.h = j.bh - j.b * j.heads;
@@ -153,8 +154,8 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
 
 // The halves of 64 rows, 8 values a thread; the first workgroup of a head leaves what the products need to know of it.
 // The halves hold a value to 2^-22 of itself and 2^-40 of the head's largest.  For keys and values that is taken while no row that is not zero is smaller than 2^-16 of the largest: 2^-24 of
-// each row's own.  Rows of q and dout enter scores, which need to be right against 1 (see beyond()), and sums over rows, which need to be right against the largest; rows of theirs may
-// be as small as 2^-24 of the largest (gradients of single positions are), with their own rows of dQ to 2^-16 of themselves there.
+// each row's own.  Rows of q and dout, backward, enter scores, which need to be right against 1 (see beyond()), and sums over rows, which need to be right against the largest; rows of
+// theirs may be as small as 2^-24 of the largest (gradients of single positions are), with a dQ of their own to 2^-16 of itself there.
 template <int DP>
 __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
     constexpr int GROUPS = DP / 8, ROWS = 64;
@@ -194,8 +195,8 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
     }
 }
 
-// Whether a pair of heads is beyond the halves: a value that is not finite, keys or values of sizes too far apart, or scores above 2^16 (|q| |k| scale; their error would pass 2^-24).
-// Such heads are worked on row by row in fp32, where nothing that is not allowed can leave a trace.
+// Heads beyond the halves are worked on row by row in fp32, where nothing that is not allowed can leave a trace: those with keys or values that are not finite, or of sizes too far apart;
+// and backward the same of q and dout, and scores above 2^16 (|q| |k| scale; with one scale for all rows of q their error would pass 2^-24).
 __device__ __forceinline__ bool beyond(const TileArgs& a, f32x4 q, f32x4 k, f32x4 v) { return q[2] + k[2] + v[2] > 0.f || !(q[1] * k[1] * fabsf(a.s.scale) < 65536.f); }
 
 __device__ __forceinline__ void store_part(float* to, int d, int D, f32x4 x) {
@@ -388,6 +389,41 @@ __device__ __forceinline__ void own_rows(f16x8 (&h)[DP / 16], f16x8 (&l)[DP / 16
         l[ks] = *(const f16x8*)(p + 16 * ks + 4);
     }
 }
+// The same from the fp32 operand, a row a lane (and the other half of it 32 lanes further), each with a scale of its own, which is returned: a row of these is a column of the
+// product, so none loses anything to another.  Rows that are not `in` are zeros and not read.  *norm: the row's.
+template <int DP>
+__device__ __forceinline__ float own_split(f16x8 (&h)[DP / 16], f16x8 (&l)[DP / 16], const AttnOperand& o, int b, int i, int head, bool in, int D, float* norm) {
+    constexpr int KD = DP / 16;
+    const int half = (threadIdx.x & 63) >> 5;
+    const float* p = o.p + b * o.b + (in ? i : 0) * o.s + head * o.h;
+    f32x4 x[KD][2];
+    float top = 0.f, sq = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KD; ++ks)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int part = 4 * ks + 2 * half + u;
+            x[ks][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (in) x[ks][u] = o.d == 1 ? attn_load4<true>(p + 4 * part, 1, part, D) : attn_load4<false>(p + 4 * part * o.d, o.d, part, D);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, __uint_as_float(finite_magnitude(x[ks][u][e])));
+            sq += dot4(x[ks][u], x[ks][u]);
+        }
+    top = halves_max(top);
+    sq = halves_sum(sq);
+    *norm = sq < 1e37f && sq > 1e-30f ? sqrtf(sq) : fminf(top * sqrtf((float)D), 1e38f); // (a square out of range: the largest magnitude times sqrt(D) instead)
+    const float scale = split_scale(__float_as_uint(top));
+#pragma unroll
+    for (int ks = 0; ks < KD; ++ks)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            _Float16 hi, lo;
+            split_value(x[ks][e >> 2][e & 3] * scale, hi, lo);
+            h[ks][e] = hi;
+            l[ks][e] = lo;
+        }
+    return scale;
+}
 // register e of a product is row 8 (e / 4) + 4 (lane / 32) + e % 4
 __device__ __forceinline__ int reg_row(int e) { return 8 * (e >> 2) + (e & 3); }
 
@@ -422,8 +458,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
     const int tiles = (attn_limit(length, start, block_last) + 31) / 32, per = (tiles + a.splits - 1) / a.splits;
     const int t0 = split * per < tiles ? split * per : tiles, t1 = t0 + per < tiles ? t0 + per : tiles;
 
-    const f32x4 head_q = a.head[kQ][bh], head_k = a.head[kK][bk], head_v = a.head[kV][bk];
-    if (__builtin_amdgcn_readfirstlane(beyond(a, head_q, head_k, head_v))) {
+    const f32x4 head_k = a.head[kK][bk], head_v = a.head[kV][bk];
+    if (__builtin_amdgcn_readfirstlane(head_k[2] + head_v[2] > 0.f)) {
         constexpr int L = T::LANES;
         for (int r = q0; r < q0 + 32 && r < a.s.queries; ++r) {
             float m, l;
@@ -443,8 +479,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
         return;
     }
     f16x8 qh[T::KD], ql[T::KD];
-    own_rows<DP>(qh, ql, a.split[kQ] + ((int64_t)bh * pad_q + q0) * DP, lane);
-    const float inv_v = 1.f / head_v[0], c = fabsf(a.s.scale) * kLog2e / head_q[0] / head_k[0];
+    float norm_q;
+    const float scale_q = own_split<DP>(qh, ql, a.src[kQ], b, i, h, limit > 0, D, &norm_q);
+    const float inv_v = 1.f / head_v[0], c = fabsf(a.s.scale) * kLog2e / scale_q / head_k[0];
     if (a.s.scale < 0.f) // the maximum is taken before the factor, which has to keep the order
 #pragma unroll
         for (int ks = 0; ks < T::KD; ++ks) qh[ks] = -qh[ks], ql[ks] = -ql[ks];
@@ -551,9 +588,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
 
 // ---- backward ------------------------------------------------------------------------------------------------------------------------
 
-// 2^15 over the largest that |dS| can be, as a power of two, from the heads of dout and v
-__device__ __forceinline__ float ds_scale(f32x4 g, f32x4 v) {
-    const int e = (int)(__float_as_uint(fminf(2.f * g[1] * v[1], 1e38f)) >> 23) - 127 + 1; // the bound is below 2^e
+// 2^15 over the largest that |dS| can be, as a power of two, from the norms of dout and v
+__device__ __forceinline__ float ds_scale(float norm_g, float norm_v) {
+    const int e = (int)(__float_as_uint(fminf(2.f * norm_g * norm_v, 1e38f)) >> 23) - 127 + 1; // the bound is below 2^e
     const int up = 15 - e;
     return __uint_as_float((uint32_t)((up > 126 ? 126 : up) + 127) << 23);
 }
@@ -604,7 +641,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(co
     f16x8 kh[T::KD], kl[T::KD], vh[T::KD], vl[T::KD];
     own_rows<DP>(kh, kl, a.split[kK] + ((int64_t)bk * pad_k + j0) * DP, lane);
     own_rows<DP>(vh, vl, a.split[kV] + ((int64_t)bk * pad_k + j0) * DP, lane);
-    const float scale_q = head_q[0], scale_g = head_g[0], ds_up = ds_scale(head_g, head_v);
+    const float scale_q = head_q[0], scale_g = head_g[0], ds_up = ds_scale(head_g[1], head_v[1]);
     const float c = a.s.scale * kLog2e / scale_q / head_k[0], inv_dp = 1.f / scale_g / head_v[0];
     const float* const base[2] = {a.split[kQ] + (int64_t)bh * pad_q * DP, a.split[kDO] + (int64_t)bh * pad_q * DP};
     const float* const stats = (const float*)(a.stats + (int64_t)bh * pad_q);
@@ -761,7 +798,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(con
     f16x8 qh[T::KD], ql[T::KD], gh[T::KD], gl[T::KD];
     own_rows<DP>(qh, ql, a.split[kQ] + ((int64_t)bh * pad_q + q0) * DP, lane);
     own_rows<DP>(gh, gl, a.split[kDO] + ((int64_t)bh * pad_q + q0) * DP, lane);
-    const float scale_k = head_k[0], ds_up = ds_scale(head_g, head_v);
+    const float scale_k = head_k[0], ds_up = ds_scale(head_g[1], head_v[1]);
     const float c = a.s.scale * kLog2e / head_q[0] / scale_k, inv_dp = 1.f / head_g[0] / head_v[0];
     const f32x2 stats = a.stats[(int64_t)bh * pad_q + i];
     const float lse2 = stats[0], delta = stats[1];
@@ -845,7 +882,7 @@ int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 9
 void plan_operands(TileArgs& a, Workspace& ws, int jobs) {
     const AttnShape& s = a.s;
     a.jobs = jobs;
-    a.parts = std::max(1, std::min(kHeadParts, (std::max(s.queries, s.keys) + 255) / 256));
+    a.parts = std::max(1, std::min(kHeadParts, (std::max(jobs == 2 ? 0 : s.queries, s.keys) + 255) / 256));
     for (int j = 0; j < jobs; ++j) {
         const bool key = j == kK || j == kV;
         const int64_t heads = (int64_t)s.batch * (key ? s.kv_heads : s.heads);
@@ -858,9 +895,9 @@ void plan_operands(TileArgs& a, Workspace& ws, int jobs) {
 template <int DP, int L>
 void launch_operands(const TileArgs& a, hipStream_t stream) {
     const AttnShape& s = a.s;
-    const unsigned heads = (unsigned)(s.batch * (s.heads * (a.jobs - 2) + s.kv_heads * 2));
+    const unsigned heads = (unsigned)(s.batch * (s.heads * (a.jobs - 2) + s.kv_heads * 2)); // (jobs: 2 or 4)
     hipLaunchKernelGGL(attn_amax_kernel<L>, dim3(a.parts, heads), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(attn_split_kernel<DP>, dim3((unsigned)(std::max(row_pad(s.queries), row_pad(s.keys)) / 64), heads), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(attn_split_kernel<DP>, dim3((unsigned)(std::max(a.jobs == 2 ? 0 : row_pad(s.queries), std::max(row_pad(s.keys), 64)) / 64), heads), dim3(256), 0, stream, a);
 }
 
 template <int DP, int L>
@@ -891,7 +928,7 @@ void attn_tiles_forward(const AttnShape& s, const AttnOperand& q, const AttnOper
     a.s = s;
     a.src[kQ] = q; a.src[kK] = k; a.src[kV] = v;
     a.to = out; a.to_lse = lse;
-    plan_operands(a, ws, 3);
+    plan_operands(a, ws, 2);
     // two workgroups a CU fill it; a run of fewer than 256 keys is not worth its part of the join
     const int64_t groups = (int64_t)s.batch * s.heads * (row_pad(s.queries) / kRowPad);
     a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(2LL * cus / groups, std::min(s.keys / 256, kMostRuns)));

@@ -8,6 +8,8 @@
  * allocates or copies to the host: every entry can be captured into a HIP graph (with sync = 0), which then owns the use of the
  * workspace given to it; two calls that may run at the same time need two workspaces.
  *
+ * Sizes beyond what a launch holds are refused with TENMO_ERR_UNSUPPORTED: each entry says which.
+ *
  * Gradients: with accumulate = 0 they are written, with accumulate != 0 added to what is there.  A NULL gradient is not computed.
  * Results do not depend on scheduling: the same inputs give the same bits.
  */
@@ -22,7 +24,7 @@ extern "C" {
 /* ---- layer norm ---------------------------------------------------------------------------------------------------------- */
 
 /* out[r, :] = (x[r, :] - mean[r]) * rstd[r] * weight + bias over the last axis of X (any strides, rank 1 to 8, N = its last extent >= 1),
- * mean and biased variance of each row, rstd = 1 / sqrt(variance + eps), eps >= 0.  weight, bias: N floats or NULL (1 and 0).
+ * mean and biased variance of each row, rstd = 1 / sqrt(variance + eps), eps >= 0, N up to 2^27.  weight, bias: N floats or NULL (1 and 0).
  * out: dense, X's shape.  mean, rstd: one float a row, or NULL (both) when no gradient is wanted. */
 int tenmo_hip_layer_norm_forward_f32(const tenmo_view* X, const float* weight, const float* bias, float eps,
                                      float* out, float* mean, float* rstd, int32_t sync);
@@ -37,11 +39,12 @@ int tenmo_hip_layer_norm_backward_f32(const tenmo_view* X, const float* weight, 
 /* ---- attention ------------------------------------------------------------------------------------------------------------ */
 
 /* Q [B, Sq, H, D], K and V [B, Sk, Hk, D] (views with any strides; H a multiple of Hk, query head h reads key head h / (H / Hk);
- * D of 1 to 128).  out[b, i, h, :] = sum over the allowed keys j of softmax_j(scale * q_i . k_j) * v_j, dense [B, Sq, H, D].
+ * D of 1 to 128; B * H up to 2^20, B * H * Sq up to 2^26, B * Hk * Sk up to 2^28).  out[b, i, h, :] = sum over the allowed keys j of softmax_j(scale * q_i . k_j) * v_j, dense [B, Sq, H, D].
  * Key j is allowed for query i of sequence b when j < key_lengths[b] (NULL: Sk; taken as 0 below 0 and as Sk above Sk) and, if causal != 0,
  * j <= i + query_starts[b] (the position of the first query; NULL: Sk - Sq, the queries are the last positions).  Both are device arrays
  * of B ints.  Keys that are not allowed are not used, whatever they hold; a query without keys gets zeros.
- * lse: NULL, or dense [B, H, Sq]: log of the sum of exp(scale * q_i . k_j) over the allowed keys (-inf without keys), for the backward call. */
+ * lse: NULL, or dense [B, H, Sq]: log of the sum of exp(scale * q_i . k_j) over the allowed keys (-inf without keys), for the backward call.
+ * The size of the workspace depends on the device: the function needs tenmo_hip_init, and returns a negative status without. */
 int64_t tenmo_hip_attention_forward_workspace_bytes(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim);
 int tenmo_hip_attention_forward_f32(const tenmo_view* Q, const tenmo_view* K, const tenmo_view* V, float scale, int32_t causal,
                                     const int32_t* key_lengths, const int32_t* query_starts, float* out, float* lse,
@@ -60,7 +63,8 @@ int tenmo_hip_attention_backward_f32(const tenmo_view* Q, const tenmo_view* K, c
 /* tenmo_hip_cross_entropy_forward_f32 of the logits H . W + bias without writing them: H [M, D] and W [D, V] are views of any strides (a weight
  * tied to an embedding [V, D] is its transposed view), bias V floats or NULL; target, ignore_index, label_smoothing, per_sample_loss [M],
  * loss_sum [1] and valid_count [1] as there (a target outside 0..V-1 that is not ignore_index gives NaN).  lse [M]: log of the sum of the
- * exponentials of each row of logits. */
+ * exponentials of each row of logits.  M and V up to 2^22, D up to 2^20, each product of two of them up to 2^38.  A row of H or a word of W that is not finite
+ * makes the results that it enters not finite; the hidden state of an ignored token enters its own lse alone. */
 int64_t tenmo_hip_vocabulary_loss_forward_workspace_bytes(int64_t tokens, int64_t dim, int64_t vocabulary);
 int tenmo_hip_vocabulary_loss_forward_f32(const tenmo_view* H, const tenmo_view* W, const float* bias, const void* target,
                                           int32_t target_is_int64, int64_t ignore_index, float label_smoothing,

@@ -43,7 +43,8 @@ struct TileArgs {
     AttnShape s;
     AttnOperand src[4];
     int jobs;           // operands that are split beforehand
-    int parts;
+    int parts;          // runs of a head's rows in the first launch
+    int split_blocks;   // workgroups a head in the second
     float* split[4];    // [batch][heads][rows padded][DP]
     f32x4* seen[4];     // [batch * heads][parts]: of a run of rows, the largest finite magnitude, the largest norm of a row, the smallest largest magnitude of a row
                         // that is not zero, and 1 if there is a value that is not finite
@@ -103,11 +104,12 @@ template <int L>
 __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
     constexpr int SLOTS = 64 / L, U = 4;
     __shared__ f32x4 seen_of[4];
-    const HeadJob j = head_job(a, blockIdx.y);
+    const int run = blockIdx.x % a.parts;
+    const HeadJob j = head_job(a, blockIdx.x / a.parts);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = lane % L, D = a.s.dim;
     const float* p = j.src.p + j.b * j.src.b + j.h * j.src.h + 4 * part * j.src.d;
     const int all = j.job == kDO ? j.pad : j.rows, per = (all + a.parts - 1) / a.parts;
-    const int first = blockIdx.x * per, last = first + per < all ? first + per : all;
+    const int first = run * per, last = first + per < all ? first + per : all;
     float top = 0.f, norm = 0.f, least = __builtin_inff();
     bool wrong = false;
     for (int r0 = first + wave * SLOTS + lane / L; __any(r0 < last); r0 += 4 * SLOTS * U) {
@@ -148,7 +150,7 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
     if (threadIdx.x == 0) {
         f32x4 s = seen_of[0];
         for (int w = 1; w < 4; ++w) s = f32x4{fmaxf(s[0], seen_of[w][0]), fmaxf(s[1], seen_of[w][1]), fminf(s[2], seen_of[w][2]), fmaxf(s[3], seen_of[w][3])};
-        j.seen[(int64_t)j.bh * a.parts + blockIdx.x] = s;
+        j.seen[(int64_t)j.bh * a.parts + run] = s;
     }
 }
 
@@ -159,20 +161,21 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
 template <int DP>
 __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
     constexpr int GROUPS = DP / 8, ROWS = 64;
-    const HeadJob j = head_job(a, blockIdx.y);
-    if ((int)blockIdx.x * ROWS >= j.pad && blockIdx.x > 0) return;
+    const int block = blockIdx.x % a.split_blocks;
+    const HeadJob j = head_job(a, blockIdx.x / a.split_blocks);
+    if (block * ROWS >= j.pad && block > 0) return;
     const int lane = threadIdx.x & 63;
     f32x4 s{0.f, 0.f, __builtin_inff(), 0.f};
     if (lane < a.parts) s = j.seen[(int64_t)j.bh * a.parts + lane];
     const float top = wave_max(s[0]), scale = split_scale(__float_as_uint(top));
-    if (blockIdx.x == 0) {
+    if (block == 0) {
         const float norm = wave_max(s[1]), least = -wave_max(-s[2]), wrong = wave_max(s[3]);
         const bool key = j.job == kK || j.job == kV;
         if (threadIdx.x == 0) j.head[j.bh] = f32x4{scale, norm, wrong > 0.f || top * (key ? 0x1p-16f : 0x1p-24f) > least ? 1.f : 0.f, 0.f};
     }
     const float* p = j.src.p + j.b * j.src.b + j.h * j.src.h;
     for (int x = threadIdx.x; x < ROWS * GROUPS; x += 256) {
-        const int r = blockIdx.x * ROWS + x / GROUPS, d = x % GROUPS * 8;
+        const int r = block * ROWS + x / GROUPS, d = x % GROUPS * 8;
         f16x8 h, l;
         f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
         if (r >= j.pad) break;
@@ -882,7 +885,8 @@ int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 9
 void plan_operands(TileArgs& a, Workspace& ws, int jobs) {
     const AttnShape& s = a.s;
     a.jobs = jobs;
-    a.parts = std::max(1, std::min(kHeadParts, (std::max(jobs == 2 ? 0 : s.queries, s.keys) + 255) / 256));
+    a.parts = std::max(1, std::min(kHeadParts, (std::max(jobs == 2 ? 0 : s.queries, s.keys) + 127) / 128));
+    a.split_blocks = std::max(jobs == 2 ? 0 : row_pad(s.queries), row_pad(s.keys)) / 64;
     for (int j = 0; j < jobs; ++j) {
         const bool key = j == kK || j == kV;
         const int64_t heads = (int64_t)s.batch * (key ? s.kv_heads : s.heads);
@@ -896,8 +900,8 @@ template <int DP, int L>
 void launch_operands(const TileArgs& a, hipStream_t stream) {
     const AttnShape& s = a.s;
     const unsigned heads = (unsigned)(s.batch * (s.heads * (a.jobs - 2) + s.kv_heads * 2)); // (jobs: 2 or 4)
-    hipLaunchKernelGGL(attn_amax_kernel<L>, dim3(a.parts, heads), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(attn_split_kernel<DP>, dim3((unsigned)(std::max(a.jobs == 2 ? 0 : row_pad(s.queries), std::max(row_pad(s.keys), 64)) / 64), heads), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(attn_amax_kernel<L>, dim3(heads * a.parts), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(attn_split_kernel<DP>, dim3(heads * a.split_blocks), dim3(256), 0, stream, a);
 }
 
 template <int DP, int L>

@@ -75,65 +75,67 @@ __global__ __launch_bounds__(256) void norm_forward_kernel(const NormForward a) 
     constexpr int T = W * 64;
     __shared__ float slots[2][4];
     const int t = threadIdx.x % T, n = (int)a.in.n;
-    const int64_t row = (int64_t)blockIdx.x * (256 / T) + threadIdx.x / T;
-    if (row >= a.in.rows) return; // W == 4: the whole workgroup; W == 1: no barrier follows
-    f32x4 x[V4];
-    load_row<T, V4>(x, norm_row(a.in, row), n, t);
-    float s = 0.f;
+    for (int64_t row = (int64_t)blockIdx.x * (256 / T) + threadIdx.x / T; row < a.in.rows; row += (int64_t)gridDim.x * (256 / T)) {
+        f32x4 x[V4];
+        load_row<T, V4>(x, norm_row(a.in, row), n, t);
+        float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < V4; ++k) s += (x[k][0] + x[k][1]) + (x[k][2] + x[k][3]);
-    const float mean = group_sum<W>(s, slots[0]) / (float)n;
-    s = 0.f;
+        for (int k = 0; k < V4; ++k) s += (x[k][0] + x[k][1]) + (x[k][2] + x[k][3]);
+        const float mean = group_sum<W>(s, slots[0]) / (float)n;
+        s = 0.f;
 #pragma unroll
-    for (int k = 0; k < V4; ++k)
+        for (int k = 0; k < V4; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float d = 4 * (t + T * k) + e < n ? x[k][e] - mean : 0.f;
-            x[k][e] = d;
-            s += d * d;
+            for (int e = 0; e < 4; ++e) {
+                const float d = 4 * (t + T * k) + e < n ? x[k][e] - mean : 0.f;
+                x[k][e] = d;
+                s += d * d;
+            }
+        const float rstd = 1.f / sqrtf(group_sum<W>(s, slots[1]) / (float)n + a.eps);
+        f32x4 w[V4];
+        if (a.weight) {
+            load_row<T, V4>(w, a.weight, n, t);
+#pragma unroll
+            for (int k = 0; k < V4; ++k) x[k] = x[k] * rstd * w[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < V4; ++k) x[k] = x[k] * rstd;
         }
-    const float rstd = 1.f / sqrtf(group_sum<W>(s, slots[1]) / (float)n + a.eps);
-    f32x4 w[V4];
-    if (a.weight) {
-        load_row<T, V4>(w, a.weight, n, t);
+        if (a.bias) {
+            load_row<T, V4>(w, a.bias, n, t);
 #pragma unroll
-        for (int k = 0; k < V4; ++k) x[k] = x[k] * rstd * w[k];
-    } else {
-#pragma unroll
-        for (int k = 0; k < V4; ++k) x[k] = x[k] * rstd;
-    }
-    if (a.bias) {
-        load_row<T, V4>(w, a.bias, n, t);
-#pragma unroll
-        for (int k = 0; k < V4; ++k) x[k] += w[k];
-    }
-    store_row<T, V4>(a.out + row * a.in.n, x, n, t);
-    if (t == 0 && a.mean) {
-        a.mean[row] = mean;
-        a.rstd[row] = rstd;
+            for (int k = 0; k < V4; ++k) x[k] += w[k];
+        }
+        store_row<T, V4>(a.out + row * a.in.n, x, n, t);
+        if (t == 0 && a.mean) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
     }
 }
 
 __global__ __launch_bounds__(256) void norm_forward_any_kernel(const NormForward a) {
     __shared__ float slots[2][4];
-    const int64_t row = blockIdx.x, n = a.in.n, cs = a.in.col_stride;
-    const float* __restrict p = norm_row(a.in, row);
-    float s = 0.f;
-    for (int64_t c = threadIdx.x; c < n; c += 256) s += p[c * cs];
-    const float mean = group_sum<4>(s, slots[0]) / (float)n;
-    s = 0.f;
-    for (int64_t c = threadIdx.x; c < n; c += 256) {
-        const float d = p[c * cs] - mean;
-        s += d * d;
-    }
-    const float rstd = 1.f / sqrtf(group_sum<4>(s, slots[1]) / (float)n + a.eps);
-    for (int64_t c = threadIdx.x; c < n; c += 256) {
-        const float y = (p[c * cs] - mean) * rstd * (a.weight ? a.weight[c] : 1.f);
-        a.out[row * n + c] = a.bias ? y + a.bias[c] : y;
-    }
-    if (threadIdx.x == 0 && a.mean) {
-        a.mean[row] = mean;
-        a.rstd[row] = rstd;
+    const int64_t n = a.in.n, cs = a.in.col_stride;
+    for (int64_t row = blockIdx.x; row < a.in.rows; row += gridDim.x) {
+        const float* __restrict p = norm_row(a.in, row);
+        float s = 0.f;
+        for (int64_t c = threadIdx.x; c < n; c += 256) s += p[c * cs];
+        const float mean = group_sum<4>(s, slots[0]) / (float)n;
+        s = 0.f;
+        for (int64_t c = threadIdx.x; c < n; c += 256) {
+            const float d = p[c * cs] - mean;
+            s += d * d;
+        }
+        const float rstd = 1.f / sqrtf(group_sum<4>(s, slots[1]) / (float)n + a.eps);
+        for (int64_t c = threadIdx.x; c < n; c += 256) {
+            const float y = (p[c * cs] - mean) * rstd * (a.weight ? a.weight[c] : 1.f);
+            a.out[row * n + c] = a.bias ? y + a.bias[c] : y;
+        }
+        if (threadIdx.x == 0 && a.mean) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
     }
 }
 
@@ -226,22 +228,24 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(const NormBackward a
 
 __global__ __launch_bounds__(256) void norm_backward_any_kernel(const NormBackward a) { // grad_x alone
     __shared__ float slots[2][4];
-    const int64_t row = blockIdx.x, n = a.in.n, cs = a.in.col_stride;
-    const float* __restrict p = norm_row(a.in, row);
-    const float* __restrict dy = a.dy + row * n;
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float c1 = 0.f, c2 = 0.f;
-    for (int64_t c = threadIdx.x; c < n; c += 256) {
-        const float g = dy[c] * (a.weight ? a.weight[c] : 1.f);
-        c1 += g;
-        c2 += g * ((p[c * cs] - mean) * rstd);
-    }
-    c1 = group_sum<4>(c1, slots[0]) / (float)n;
-    c2 = group_sum<4>(c2, slots[1]) / (float)n;
-    for (int64_t c = threadIdx.x; c < n; c += 256) {
-        const float g = dy[c] * (a.weight ? a.weight[c] : 1.f);
-        const float d = rstd * (g - c1 - (p[c * cs] - mean) * rstd * c2);
-        a.grad_x[row * n + c] = a.accumulate ? a.grad_x[row * n + c] + d : d;
+    const int64_t n = a.in.n, cs = a.in.col_stride;
+    for (int64_t row = blockIdx.x; row < a.in.rows; row += gridDim.x) {
+        const float* __restrict p = norm_row(a.in, row);
+        const float* __restrict dy = a.dy + row * n;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float c1 = 0.f, c2 = 0.f;
+        for (int64_t c = threadIdx.x; c < n; c += 256) {
+            const float g = dy[c] * (a.weight ? a.weight[c] : 1.f);
+            c1 += g;
+            c2 += g * ((p[c * cs] - mean) * rstd);
+        }
+        c1 = group_sum<4>(c1, slots[0]) / (float)n;
+        c2 = group_sum<4>(c2, slots[1]) / (float)n;
+        for (int64_t c = threadIdx.x; c < n; c += 256) {
+            const float g = dy[c] * (a.weight ? a.weight[c] : 1.f);
+            const float d = rstd * (g - c1 - (p[c * cs] - mean) * rstd * c2);
+            a.grad_x[row * n + c] = a.accumulate ? a.grad_x[row * n + c] + d : d;
+        }
     }
 }
 
@@ -304,7 +308,7 @@ int norm_rows(const tenmo_view* X, const char* who, NormRows* r) {
             r->stride[r->rank++] = X->strides[d];
         }
     }
-    if (r->rows > 0x7fffffffLL || r->n > 0x7fffffffLL) return refuse(TENMO_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows or columns", who);
+    if (r->n > 1 << 27) return refuse(TENMO_ERR_UNSUPPORTED, "%s: more than 2^27 columns", who);
     return 0;
 }
 
@@ -312,6 +316,9 @@ int norm_rows(const tenmo_view* X, const char* who, NormRows* r) {
 constexpr int64_t kNormWorkgroups = 768;
 int64_t norm_rows_at_a_time(int64_t n) { return n <= 1024 ? 4 : 1; }
 int64_t norm_parts(int64_t rows, int64_t n) { return std::max<int64_t>(1, std::min<int64_t>((rows + norm_rows_at_a_time(n) - 1) / norm_rows_at_a_time(n), kNormWorkgroups)); }
+
+// a workgroup a row, or four, up to what a launch may hold; beyond that they take further ones
+unsigned norm_grid(int64_t groups) { return (unsigned)std::min<int64_t>(groups, 1 << 22); }
 
 template <class Args>
 using NormKernel = void (*)(Args);
@@ -354,9 +361,9 @@ int tenmo_hip_layer_norm_forward_f32(const tenmo_view* X, const float* weight, c
     a.weight = weight; a.bias = bias; a.eps = eps; a.out = out; a.mean = mean; a.rstd = rstd;
     if (a.in.n <= 8192 && (a.in.col_stride == 1 || a.in.n == 1)) {
         const int64_t rows_at_a_time = norm_rows_at_a_time(a.in.n);
-        hipLaunchKernelGGL(norm_forward_for(a.in.n), dim3((unsigned)((a.in.rows + rows_at_a_time - 1) / rows_at_a_time)), dim3(256), 0, call.state.stream, a);
+        hipLaunchKernelGGL(norm_forward_for(a.in.n), dim3(norm_grid((a.in.rows + rows_at_a_time - 1) / rows_at_a_time)), dim3(256), 0, call.state.stream, a);
     } else {
-        hipLaunchKernelGGL(norm_forward_any_kernel, dim3((unsigned)a.in.rows), dim3(256), 0, call.state.stream, a);
+        hipLaunchKernelGGL(norm_forward_any_kernel, dim3(norm_grid(a.in.rows)), dim3(256), 0, call.state.stream, a);
     }
     return call.finish(sync);
 }
@@ -392,7 +399,7 @@ int tenmo_hip_layer_norm_backward_f32(const tenmo_view* X, const float* weight, 
         if (n <= 8192 && (a.in.col_stride == 1 || n == 1)) {
             hipLaunchKernelGGL(norm_backward_for(n), dim3((unsigned)norm_parts(a.in.rows, n)), dim3(256), 0, stream, a);
         } else {
-            if (grad_X) hipLaunchKernelGGL(norm_backward_any_kernel, dim3((unsigned)a.in.rows), dim3(256), 0, stream, a);
+            if (grad_X) hipLaunchKernelGGL(norm_backward_any_kernel, dim3(norm_grid(a.in.rows)), dim3(256), 0, stream, a);
             if (a.partial) hipLaunchKernelGGL(norm_columns_any_kernel, dim3((unsigned)((n + 255) / 256), (unsigned)a.parts), dim3(256), 0, stream, a);
         }
     }

@@ -558,7 +558,9 @@ void plan_backward(Workspace& ws, Plan& p, int64_t M, int64_t D, int64_t V, bool
 
 int check_sizes(int64_t M, int64_t D, int64_t V, const char* who) {
     if (M < 0 || D < 1 || V < 1) return refuse(TENMO_ERR_INVALID_SHAPE, "%s: needs tokens >= 0, a dimension >= 1 and a vocabulary >= 1", who);
-    if (M > 1 << 22 || D > 1 << 20 || V > 1 << 22) return refuse(TENMO_ERR_UNSUPPORTED, "%s: more than 2^22 tokens, 2^20 dimensions or 2^22 words", who);
+    const int64_t most = (int64_t)1 << 38; // a launch holds 2^32 threads: 2^24 tiles of 2^15 values
+    if (M > 1 << 22 || D > 1 << 20 || V > 1 << 22 || M * V > most || D * V > most || M * D > most)
+        return refuse(TENMO_ERR_UNSUPPORTED, "%s: more than 2^22 tokens, 2^20 dimensions, 2^22 words or 2^38 values of a matrix", who);
     return 0;
 }
 

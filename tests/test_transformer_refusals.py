@@ -51,7 +51,7 @@ def test_layer_norm_refusals():
     refused(ARGUMENT, "eps", norm_forward(eps=float("nan")))
     refused(ARGUMENT, "null out", norm_forward(out=None))
     refused(ARGUMENT, "mean and rstd", norm_forward(mean=None))
-    refused(UNSUPPORTED, "2^31", norm_forward(view((1 << 32, 2), (2, 1))))
+    refused(UNSUPPORTED, "2^27", norm_forward(view((2, (1 << 27) + 1))))
     L = _transformer.load()
     refused(ARGUMENT, "null X", L.tenmo_hip_layer_norm_forward_f32(None, P, P, 1e-5, P, P, P, 0))
     refused(ARGUMENT, "null pointer", L.tenmo_hip_layer_norm_backward_f32(view((4, 8)), P, None, P, P, P, P, P, 0, P, 1 << 20, 0))
@@ -70,7 +70,9 @@ def test_attention_refusals():
     refused(SHAPE, "multiple", attn_forward(k=(2, 5, 0, 16)))
     refused(UNSUPPORTED, "head size 129", attn_forward(q=(2, 3, 4, 129), k=(2, 5, 2, 129)))
     refused(UNSUPPORTED, "head size 0", attn_forward(q=(2, 3, 4, 0), k=(2, 5, 2, 0)))
-    refused(UNSUPPORTED, "2^30", attn_forward(q=(1 << 15, 1 << 15, 4, 16), k=(1 << 15, 5, 2, 16)))
+    refused(UNSUPPORTED, "2^26", attn_forward(q=(1 << 15, 1 << 15, 4, 16), k=(1 << 15, 5, 2, 16)))
+    refused(UNSUPPORTED, "2^20", attn_forward(q=(1 << 19, 1, 4, 16), k=(1 << 19, 5, 2, 16)))
+    refused(UNSUPPORTED, "2^28", attn_forward(q=(1, 1, 4, 16), k=(1, 1 << 28, 2, 16)))
     refused(ARGUMENT, "scale", attn_forward(scale=float("inf")))
     refused(ARGUMENT, "null out", attn_forward(out=None))
     L = _transformer.load()
@@ -100,6 +102,7 @@ def test_vocabulary_loss_refusals():
     refused(SHAPE, "inner dims", forward(w=(7, 10)))
     refused(SHAPE, "vocabulary >= 1", forward(w=(8, 0)))
     refused(UNSUPPORTED, "words", forward(w=(8, (1 << 22) + 1)))
+    refused(UNSUPPORTED, "2^38", forward(h=(1 << 20, 8), w=(8, 1 << 20)))
     refused(ARGUMENT, "label_smoothing", forward(smoothing=1.5))
     refused(ARGUMENT, "label_smoothing", forward(smoothing=float("nan")))
     refused(ARGUMENT, "null pointer", forward(target=None))

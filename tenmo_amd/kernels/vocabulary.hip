@@ -5,12 +5,13 @@
 //   dH = scale (G W^T),  dW = (scale H)^T G,  db = sum_m scale_m G
 //
 // Bound: the matrix units, 2 M V D flop forward, 6 M V D backward (the logits again, dH, dW).  All three products run as split fp16 products
-// (split_gemm.hpp).
+// (split_gemm.hpp); up to 64 tokens, where reading W is the bound, the kernels of vocabulary_few.hip take their place.
 //   * forward: tiles of 256 words x 128 tokens; the words of a token lie in the registers of two lanes, so that a tile's maximum and sum of a token take
 //     one exchange, and 8 bytes a token and tile leave the chip instead of 1 KiB of logits.  A second launch joins the tiles of a token in a fixed order.
 //   * backward: a piece of the vocabulary at a time; the tiles of the first launch end as G in split form (|G| <= 1, so its scale is known beforehand: 2^14),
 //     which the second launch multiplies with W and with H.  The piece is as large as 1 GiB of G allows.
 #include "split_gemm.hpp"
+#include "vocabulary.hpp"
 
 #include <algorithm>
 
@@ -24,31 +25,6 @@ struct Source { // an operand in the order in which it is split: rows x cols
     const float* p;
     int64_t rows, cols, rs, cs;
 };
-
-struct VocabArgs {
-    int64_t M, V, D;
-    const float* bias;
-    const void* target;
-    int is64;
-    int64_t ignore;
-    float ls;
-};
-
-__device__ __forceinline__ int64_t target_of(const VocabArgs& a, int64_t m) {
-    return a.is64 ? ((const int64_t*)a.target)[m] : (int64_t)((const int32_t*)a.target)[m];
-}
-
-struct Upstream { // the gradient of the loss: of each row, or of the reduced one
-    const float* p;
-    int reduction;
-    const int32_t* valid_count;
-};
-// the factor of row m of the gradient; 0 where the target is ignore_index
-__device__ __forceinline__ float row_factor(const VocabArgs& a, const Upstream& u, int64_t m) {
-    if (target_of(a, m) == a.ignore) return 0.f;
-    const float s = u.p[u.reduction == 0 ? m : 0];
-    return u.reduction == 2 ? s / (float)(*u.valid_count > 1 ? *u.valid_count : 1) : s;
-}
 
 // ---- amax and split -------------------------------------------------------------------------------------------------------------
 
@@ -575,6 +551,7 @@ int check_call(const tenmo_view* H, const tenmo_view* W, const float* bias, cons
 }
 
 Source source_h(const tenmo_view* H) { return Source{H->data + H->offset, H->shape[0], H->shape[1], H->strides[0], H->strides[1]}; }
+Operand2 operand(const tenmo_view* x) { return Operand2{x->data + x->offset, x->strides[0], x->strides[1]}; }
 bool rows_of_words(const tenmo_view* W) { return W->strides[0] == 1 && W->shape[0] > 1; }
 Source source_w(const tenmo_view* W) {
     if (rows_of_words(W)) return Source{W->data + W->offset, W->shape[1], W->shape[0], W->strides[1], W->strides[0]};
@@ -592,6 +569,7 @@ void launch_split(const Plan& p, const tenmo_view* H, const tenmo_view* W, const
 ProductArgs product(const SplitMatrix& a, const uint32_t* amax_a, const SplitMatrix& b, const uint32_t* amax_b, int64_t M, int64_t N, int64_t K) {
     return ProductArgs{a, b, amax_a, amax_b, M, N, split_pad(K) / kStepK, tiles_of(M, kTileM), tiles_of(N, kTileN), split_pad(K) / kStepK, 0};
 }
+dim3 grid_of_dh(const VocabArgs& v, const LibraryState& lib) { return dim3((unsigned)std::min<int64_t>(tiles_of(v.M * v.D, 1024), 8 * lib.cus)); }
 dim3 grid_of(const ProductArgs& p) { return dim3((unsigned)(p.tiles_m * p.tiles_n)); }
 
 // the words `first` .. of the split W
@@ -608,7 +586,9 @@ int64_t tenmo_hip_vocabulary_loss_forward_workspace_bytes(int64_t tokens, int64_
     if (int rc = check_sizes(tokens, dim, vocabulary, "tenmo_hip_vocabulary_loss_forward_workspace_bytes")) return rc;
     Workspace ws(nullptr, 0);
     Plan p{};
-    if (tokens) plan_forward(ws, p, tokens, dim, vocabulary, true);
+    FewPlan few{};
+    if (tokens > kFewTokens) plan_forward(ws, p, tokens, dim, vocabulary, true);
+    else if (tokens) few_plan_forward(ws, few, VocabArgs{tokens, vocabulary, dim, nullptr, nullptr, 0, 0, 0.f});
     return ws.used();
 }
 
@@ -623,9 +603,16 @@ int tenmo_hip_vocabulary_loss_forward_f32(const tenmo_view* H, const tenmo_view*
     Call call(who);
     if (int rc = call.begin()) return rc;
     const hipStream_t stream = call.state.stream;
-    if (v.M > 0) {
+    Workspace ws(workspace, workspace_bytes);
+    if (v.M > 0 && v.M <= kFewTokens) {
+        FewPlan p{};
+        few_plan_forward(ws, p, v);
+        if (int rc = ws.check(who)) return rc;
+        few_forward(p, v, operand(H), operand(W), stream);
+        const JoinArgs jn{v, p.part, label_smoothing > 0.f ? p.part_x : nullptr, p.target_logit, p.tiles, per_sample_loss, lse};
+        hipLaunchKernelGGL(vocab_join_kernel, dim3(1), dim3(1024), 0, stream, jn);
+    } else if (v.M > 0) {
         const bool word_rows = rows_of_words(W);
-        Workspace ws(workspace, workspace_bytes);
         Plan p{};
         plan_forward(ws, p, v.M, v.D, v.V, word_rows);
         if (int rc = ws.check(who)) return rc;
@@ -646,7 +633,9 @@ int64_t tenmo_hip_vocabulary_loss_backward_workspace_bytes(int64_t tokens, int64
     if (int rc = check_sizes(tokens, dim, vocabulary, "tenmo_hip_vocabulary_loss_backward_workspace_bytes")) return rc;
     Workspace ws(nullptr, 0);
     Plan p{};
-    if (tokens) plan_backward(ws, p, tokens, dim, vocabulary, true);
+    FewPlan few{};
+    if (tokens > kFewTokens) plan_backward(ws, p, tokens, dim, vocabulary, true);
+    else if (tokens) few_plan_backward(ws, few, VocabArgs{tokens, vocabulary, dim, nullptr, nullptr, 0, 0, 0.f});
     return ws.used();
 }
 
@@ -678,10 +667,18 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
     const int64_t gw_d = grad_W ? grad_W->strides[0] : 0, gw_v = grad_W ? grad_W->strides[1] : 0;
     const bool word_rows = rows_of_words(W);
     Workspace ws(workspace, workspace_bytes);
+    const Upstream up{upstream, (int)reduction, valid_count};
+    if (v.M > 0 && v.M <= kFewTokens) {
+        FewPlan p{};
+        few_plan_backward(ws, p, v);
+        if (int rc = ws.check(who)) return rc;
+        few_backward(p, v, operand(H), operand(W), lse, up, grad_H != nullptr, gw, gw_d, gw_v, grad_bias, add, stream);
+        if (grad_H) hipLaunchKernelGGL(vocab_dh_kernel, grid_of_dh(v, call.state), dim3(256), 0, stream, p.part_h, p.runs, v, up, grad_H, add);
+        return call.finish(sync);
+    }
     Plan p{};
     if (v.M > 0) plan_backward(ws, p, v.M, v.D, v.V, word_rows);
     if (int rc = ws.check(who)) return rc;
-    const Upstream up{upstream, (int)reduction, valid_count};
     if (v.M > 0) launch_split(p, H, W, v, up, grad_W != nullptr, call.state);
     const int64_t piece = v.M > 0 ? p.piece : v.V;
     int64_t runs = 0;
@@ -725,7 +722,7 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
         else hipLaunchKernelGGL(vocab_products_kernel<true>, grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
     }
     if (grad_H && v.M > 0)
-        hipLaunchKernelGGL(vocab_dh_kernel, dim3((unsigned)std::min<int64_t>(tiles_of(v.M * v.D, 1024), 8 * call.state.cus)), dim3(256), 0, stream, p.part_h, runs, v, up, grad_H, add);
+        hipLaunchKernelGGL(vocab_dh_kernel, grid_of_dh(v, call.state), dim3(256), 0, stream, p.part_h, runs, v, up, grad_H, add);
     if (grad_bias) hipLaunchKernelGGL(vocab_db_kernel, dim3((unsigned)tiles_of(v.V, 256)), dim3(256), 0, stream, p.part_db, v.M > 0 ? 2 * tiles_of(v.M, kTileN) : 0, v.V, grad_bias, add);
     return call.finish(sync);
 }

@@ -1,0 +1,329 @@
+// The vocabulary loss for up to 64 tokens: what bounds it is reading W (and writing dW), so it is read as it is, in fp32, by the fp32 matrix instruction.
+//
+//   forward   x = H W: a workgroup for 128 words and 32 tokens, or 64 and 64, over all of D; its maximum and sum of each token leave the chip.
+//   backward  the same product again, ending as G in fp32 [tokens, words]; dH = G W^T, the words cut into runs with a sum each;
+//             dW = (scale H)^T G, tiles of 128 x 64 whose whole reduction (the tokens) lies in LDS.
+//
+// The split form of the products (vocabulary.hip) reads W three times and writes it once before it begins, which its rate pays back from 65 tokens up.  Forward and backward
+// with W as an embedding [words, D], here against the split form:
+//       768 x 50257:  1 token 55 + 160 us against 146 + 272;  32 tokens 55 + 181 against 144 + 273;  64 tokens 91 + 251 against 146 + 284
+//      1600 x 8000:   1 token 57 +  97 us against 100 + 145;  64 tokens 56 + 121 against 101 + 154
+//       128 x 1000:   1 token 21 +  30 us against  28 +  41;  64 tokens 21 +  35 against  28 +  45
+// One read of the first W (154 MB) takes 30 us at the rate of a copy, its backward (W twice, dW once) 92 us.
+// Both products with W have the matrix in the rows of the instruction's result and the tokens in its columns: rows r of 32 in LDS, K-major ([row][k], 32 k and 4 of padding: a
+// float4 of four k a lane, 16 rows in 16 different bank groups) where the memory runs along k, MN-major ([k][row]) where it runs along r.
+#include "vocabulary.hpp"
+
+#include <algorithm>
+
+namespace tenmo {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+constexpr int KC = 32;       // k a step
+constexpr int PITCH = KC + 4;
+
+enum { kLoss, kGrad, kHidden };
+
+struct FewArgs {
+    VocabArgs v;
+    Operand2 a;          // rows x k: W transposed, or W
+    int64_t rows, k;     // rows of the result: words, or D
+    Operand2 b;          // tokens x k: H, or G
+    int64_t run;         // k of a run
+    float2* part;
+    float *part_x, *target_logit;
+    const float* lse;
+    float* out;          // G [tokens][words], or [runs][tokens][D]
+};
+
+// ROWS x KC of an operand on the way into LDS, ROWS * KC / 256 values a thread
+template <int ROWS, bool KMAJOR>
+struct Staged {
+    static constexpr int N = ROWS * KC / 1024; // groups of four
+    f32x4 x[N];
+    __device__ __forceinline__ void load(const Operand2& o, int64_t r0, int64_t rows, int64_t k0, int64_t k_end) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int y = threadIdx.x + 256 * i;
+            const int64_t r = r0 + (KMAJOR ? y / (KC / 4) : y % (ROWS / 4) * 4), k = k0 + (KMAJOR ? y % (KC / 4) * 4 : y / (ROWS / 4));
+            x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (r >= rows || k >= k_end) continue;
+            const float* p = o.p + r * o.r + k * o.c;
+            const int64_t left = KMAJOR ? k_end - k : rows - r, step = KMAJOR ? o.c : o.r;
+            if (step == 1 && left >= 4) x[i] = *(const f32x4_u*)p;
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < left) x[i][e] = p[e * step];
+        }
+    }
+    __device__ __forceinline__ void store(float* lds) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int y = threadIdx.x + 256 * i;
+            if (KMAJOR) *(f32x4*)(lds + y / (KC / 4) * PITCH + y % (KC / 4) * 4) = x[i];
+            else *(f32x4*)(lds + y / (ROWS / 4) * (ROWS + 4) + y % (ROWS / 4) * 4) = x[i];
+        }
+    }
+    static constexpr int FLOATS = KMAJOR ? ROWS * PITCH : KC * (ROWS + 4);
+    // the four k of this half of the wavefront, of eight from k8, for row `row`
+    static __device__ __forceinline__ f32x4 read(const float* lds, int row, int k8, int half) {
+        if (KMAJOR) return *(const f32x4*)(lds + row * PITCH + k8 + 4 * half);
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = lds[(k8 + 4 * half + e) * (ROWS + 4) + row];
+        return y;
+    }
+};
+
+template <int TOKENS, int MODE, bool A_KMAJOR>
+__global__ __launch_bounds__(256) void few_kernel(const FewArgs a) {
+    constexpr int ROWS = TOKENS == 32 ? 128 : 64;
+    using A = Staged<ROWS, A_KMAJOR>;
+    using B = Staged<TOKENS, true>;
+    __shared__ __align__(16) float lds_a[2][A::FLOATS], lds_b[2][B::FLOATS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int row_block = TOKENS == 32 ? wave : wave & 1, token_block = TOKENS == 32 ? 0 : wave >> 1;
+    const int64_t tiles = (a.rows + ROWS - 1) / ROWS, run = MODE == kHidden ? blockIdx.x / tiles : 0;
+    const int64_t r0 = (blockIdx.x - run * tiles) * ROWS, k0 = run * a.run, k_end = MODE == kHidden && k0 + a.run < a.k ? k0 + a.run : a.k;
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+    A sa;
+    B sb;
+    sa.load(a.a, r0, a.rows, k0, k_end);
+    sb.load(a.b, 0, a.v.M, k0, k_end);
+    int stage = 0;
+    for (int64_t k = k0; k < k_end; k += KC, stage ^= 1) {
+        sa.store(lds_a[stage]);
+        sb.store(lds_b[stage]);
+        __syncthreads();
+        if (k + KC < k_end) { // on the way while this step is multiplied; its place in LDS was read a step ago
+            sa.load(a.a, r0, a.rows, k + KC, k_end);
+            sb.load(a.b, 0, a.v.M, k + KC, k_end);
+        }
+#pragma unroll
+        for (int k8 = 0; k8 < KC; k8 += 8) {
+            const f32x4 x = A::read(lds_a[stage], 32 * row_block + (lane & 31), k8, half), y = B::read(lds_b[stage], 32 * token_block + (lane & 31), k8, half);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[s], y[s], acc, 0, 0, 0);
+        }
+    }
+    // register e: row 8 (e / 4) + 4 half + e % 4 of the block, column lane % 32
+    const int64_t row0 = r0 + 32 * row_block + 4 * half, token = 32 * token_block + (lane & 31);
+    if (MODE == kHidden) {
+        if (token >= a.v.M) return;
+        float* to = a.out + (run * a.v.M + token) * a.rows;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int64_t r = row0 + 8 * q;
+            if (r + 3 < a.rows) *(f32x4_u*)(to + r) = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (r + e < a.rows) to[r + e] = acc[4 * q + e];
+        }
+        return;
+    }
+    const int64_t at = (token < a.v.M ? target_of(a.v, token) : a.v.ignore) - row0; // the target's place from this lane's first word
+    if (a.v.bias)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int64_t r = row0 + 8 * (e >> 2) + (e & 3);
+            if (r < a.rows) acc[e] += a.v.bias[r];
+        }
+    if (MODE == kLoss) {
+        __shared__ float join[3][ROWS / 32][TOKENS];
+        float top = -__builtin_inff(), sum = 0.f, sx = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const bool in = row0 + 8 * (e >> 2) + (e & 3) < a.rows;
+            sx += in ? acc[e] : 0.f;
+            acc[e] = in ? acc[e] : -__builtin_inff();
+            top = fmaxf(top, acc[e]);
+        }
+        top = halves_max(top);
+        const float base = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            sum += __expf(acc[e] - base);
+            if (token < a.v.M && at == 8 * (e >> 2) + (e & 3)) a.target_logit[token] = acc[e];
+        }
+        sum = halves_sum(sum);
+        sx = halves_sum(sx);
+        const int col = 32 * token_block + (lane & 31);
+        if (half == 0) join[0][row_block][col] = top, join[1][row_block][col] = sum, join[2][row_block][col] = sx;
+        __syncthreads();
+        const int t = threadIdx.x;
+        if (t < TOKENS && t < a.v.M) {
+            float m = join[0][0][t], s = 0.f, x = 0.f;
+#pragma unroll
+            for (int w = 1; w < ROWS / 32; ++w) m = fmaxf(m, join[0][w][t]);
+            const float b = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+            for (int w = 0; w < ROWS / 32; ++w) s += join[1][w][t] * __expf(join[0][w][t] - b), x += join[2][w][t];
+            a.part[blockIdx.x * a.v.M + t] = make_float2(m, s);
+            if (a.part_x) a.part_x[blockIdx.x * a.v.M + t] = x;
+        }
+        return;
+    }
+    if (token >= a.v.M) return;
+    const bool valid = target_of(a.v, token) != a.v.ignore;
+    const float lse = a.lse[token], smooth = a.v.ls / (float)a.v.V;
+    float* to = a.out + token * a.v.V;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        f32x4 g;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            g[e] = __expf(acc[4 * q + e] - lse) - smooth;
+            if (at == 8 * q + e) g[e] -= 1.f - a.v.ls;
+            g[e] = valid ? g[e] : 0.f;
+        }
+        const int64_t r = row0 + 8 * q;
+        if (r + 3 < a.rows) *(f32x4_u*)(to + r) = g;
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (r + e < a.rows) to[r + e] = g[e];
+    }
+}
+
+// dW: rows i of the result (words, or D) by columns j, the one with unit stride; X [tokens][i] and Y [tokens][j] in LDS whole
+struct FewWeight {
+    VocabArgs v;
+    Upstream up;
+    Operand2 x, y;
+    int x_is_h;       // the hidden states are X, or else Y: their rows are multiplied by their factors
+    int64_t rows, cols;
+    float* out;
+    int64_t rs, cs;
+    int accumulate;
+};
+
+template <int TOKENS>
+__global__ __launch_bounds__(256) void few_weight_kernel(const FewWeight a) {
+    constexpr int I = 128, J = 64;
+    __shared__ float lx[TOKENS][I + 4], ly[TOKENS][J + 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int64_t tiles_j = (a.cols + J - 1) / J, i0 = blockIdx.x / tiles_j * I, j0 = blockIdx.x % tiles_j * J;
+    auto fill = [&](float* to, int width, const Operand2& o, int64_t c0, int64_t cols, bool is_h) {
+        for (int y = threadIdx.x; y < TOKENS * width / 4; y += 256) {
+            const int m = y / (width / 4), c = y % (width / 4) * 4;
+            f32x4 x{0.f, 0.f, 0.f, 0.f};
+            const int64_t left = cols - c0 - c;
+            const float factor = m >= a.v.M || left <= 0 ? 0.f : is_h ? row_factor(a.v, a.up, m) : 1.f;
+            if (factor != 0.f) { // rows without a part in the gradient are zeros, whatever they hold
+                const float* p = o.p + m * o.r + (c0 + c) * o.c;
+                if (o.c == 1 && left >= 4) x = *(const f32x4_u*)p;
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e < left) x[e] = p[e * o.c];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[m * (width + 4) + c + e] = x[e] * factor;
+        }
+    };
+    fill(&lx[0][0], I, a.x, i0, a.rows, a.x_is_h);
+    fill(&ly[0][0], J, a.y, j0, a.cols, !a.x_is_h);
+    __syncthreads();
+    f32x16 acc[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[b][e] = 0.f;
+#pragma unroll 4
+    for (int m = 0; m < TOKENS; m += 2) {
+        const float x = lx[m + half][32 * wave + (lane & 31)];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, ly[m + half][32 * b + (lane & 31)], acc[b], 0, 0, 0);
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int64_t i = i0 + 32 * wave + 8 * (e >> 2) + 4 * half + (e & 3), j = j0 + 32 * b + (lane & 31);
+            if (i >= a.rows || j >= a.cols) continue;
+            float* to = a.out + i * a.rs + j * a.cs;
+            *to = a.accumulate ? *to + acc[b][e] : acc[b][e];
+        }
+}
+
+// db: the tokens in order
+__global__ __launch_bounds__(256) void few_bias_kernel(const VocabArgs v, const Upstream up, const float* __restrict g, float* db, int accumulate) {
+    const int64_t word = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (word >= v.V) return;
+    float s = 0.f;
+    for (int64_t m = 0; m < v.M; ++m) s += g[m * v.V + word] * row_factor(v, up, m);
+    db[word] = accumulate ? db[word] + s : s;
+}
+
+int64_t up_to(int64_t n, int64_t t) { return (n + t - 1) / t; }
+int64_t rows_a_tile(int64_t tokens) { return tokens <= 32 ? 128 : 64; }
+
+template <int MODE>
+void launch_few(const FewArgs& a, int64_t grid, hipStream_t stream) {
+    const bool k_major = a.a.c == 1 || a.a.r != 1;
+    if (a.v.M <= 32) {
+        if (k_major) hipLaunchKernelGGL((few_kernel<32, MODE, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((few_kernel<32, MODE, false>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+    } else {
+        if (k_major) hipLaunchKernelGGL((few_kernel<64, MODE, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((few_kernel<64, MODE, false>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+    }
+}
+
+} // namespace
+
+void few_plan_forward(Workspace& ws, FewPlan& p, const VocabArgs& v) {
+    p.tiles = up_to(v.V, rows_a_tile(v.M));
+    p.part = ws.take<float2>(p.tiles * v.M);
+    p.part_x = ws.take<float>(p.tiles * v.M);
+    p.target_logit = ws.take<float>(v.M);
+}
+
+void few_plan_backward(Workspace& ws, FewPlan& p, const VocabArgs& v) {
+    p.g = ws.take<float>(v.M * v.V);
+    // four workgroups a CU, of at least 256 words each
+    p.run = up_to(up_to(v.V, std::max<int64_t>(1, std::min(1024 / up_to(v.D, rows_a_tile(v.M)), v.V / 256))), KC) * KC;
+    p.runs = up_to(v.V, p.run);
+    p.part_h = ws.take<float>(p.runs * v.M * v.D);
+}
+
+void few_forward(const FewPlan& p, const VocabArgs& v, const Operand2& h, const Operand2& w, hipStream_t stream) {
+    FewArgs a{};
+    a.v = v;
+    a.a = Operand2{w.p, w.c, w.r}; a.rows = v.V; a.k = v.D; a.b = h;
+    a.part = p.part; a.part_x = v.ls > 0.f ? p.part_x : nullptr; a.target_logit = p.target_logit;
+    launch_few<kLoss>(a, p.tiles, stream);
+}
+
+void few_backward(const FewPlan& p, const VocabArgs& v, const Operand2& h, const Operand2& w, const float* lse, const Upstream& up, bool want_h,
+                  float* grad_w, int64_t gw_d, int64_t gw_v, float* grad_bias, int accumulate, hipStream_t stream) {
+    FewArgs a{};
+    a.v = v; a.lse = lse;
+    a.a = Operand2{w.p, w.c, w.r}; a.rows = v.V; a.k = v.D; a.b = h;
+    a.out = p.g;
+    launch_few<kGrad>(a, up_to(v.V, rows_a_tile(v.M)), stream);
+    const Operand2 g{p.g, v.V, 1};
+    if (want_h) {
+        a.a = w; a.rows = v.D; a.k = v.V; a.b = g;
+        a.run = p.run;
+        a.out = p.part_h;
+        launch_few<kHidden>(a, up_to(v.D, rows_a_tile(v.M)) * p.runs, stream);
+    }
+    if (grad_w) {
+        FewWeight f{};
+        f.v = v; f.up = up; f.out = grad_w; f.accumulate = accumulate;
+        if (gw_d == 1 || gw_v != 1) { f.x = g; f.y = h; f.rows = v.V; f.cols = v.D; f.rs = gw_v; f.cs = gw_d; }
+        else { f.x = h; f.y = g; f.x_is_h = 1; f.rows = v.D; f.cols = v.V; f.rs = gw_d; f.cs = gw_v; }
+        const dim3 grid((unsigned)(up_to(f.rows, 128) * up_to(f.cols, 64)));
+        if (v.M <= 32) hipLaunchKernelGGL(few_weight_kernel<32>, grid, dim3(256), 0, stream, f);
+        else hipLaunchKernelGGL(few_weight_kernel<64>, grid, dim3(256), 0, stream, f);
+    }
+    if (grad_bias) hipLaunchKernelGGL(few_bias_kernel, dim3((unsigned)up_to(v.V, 256)), dim3(256), 0, stream, v, up, p.g, grad_bias, accumulate);
+}
+
+} // namespace tenmo

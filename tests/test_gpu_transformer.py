@@ -417,6 +417,12 @@ VOCABULARY = [  # tokens, dim, vocabulary, weight, bias, reduction, smoothing, i
     (1, 7, 3, "dense", True, "mean", 0.1, False),
     (5, 16, 17, "tied", True, "none", 0.0, True),
     (64, 128, 1000, "tied", False, "mean", 0.0, True),
+    (2, 50, 4099, "tied", True, "mean", 0.1, True),
+    (31, 257, 129, "strided", True, "sum", 0.0, True),
+    (32, 96, 1281, "dense", True, "none", 0.1, False),
+    (33, 31, 640, "tied", True, "mean", 0.0, True),
+    (63, 130, 1025, "dense", True, "sum", 0.3, True),
+    (65, 64, 1000, "tied", True, "mean", 0.1, True),
     (128, 64, 256, "dense", True, "mean", 0.0, False),
     (129, 100, 257, "dense", True, "sum", 0.1, True),
     (255, 33, 511, "tied", True, "none", 0.2, False),
@@ -506,16 +512,17 @@ def test_vocabulary_loss_targets(ops):
     assert np.isnan(each[[3, 7]]).all() and not each[[11, 12]].any() and np.isfinite(np.delete(each, [3, 7])).all() and int(loss.valid_count.item()) == 18
 
 
+@pytest.mark.parametrize("m", [12, 50, 150])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, 1.0e30])
-def test_vocabulary_loss_rows_that_do_not_count(ops, bad):
+def test_vocabulary_loss_rows_that_do_not_count(ops, bad, m):
     """Whatever the hidden state of an ignored token holds, the others' losses and all gradients are as without it; and a row far larger than the others
     takes nothing from their losses."""
-    m, d, v = 150, 48, 700
+    d, v = 48, 700
     h, w, b = randn(1, m, d), randn(2, v, d) * 0.2, randn(3, v)
     target = torch.arange(m)
-    target[[3, 149]] = -100
+    target[[3, m - 1]] = -100
     want = vocabulary_reference(h, w.t(), b, target, -100, 0.1, "mean", torch.ones(1))
-    h[3], h[149] = bad, -bad
+    h[3], h[m - 1] = bad, -bad
     H, W, B, T = up(ops, h), up(ops, w).transpose(), up(ops, b), target.cuda()
     loss = ops.V.vocabulary_loss(H, W, B, T, label_smoothing=0.1)
     assert np.abs(down(loss.per_sample).numpy() - want[0]).max() <= 2 * RTOL_FRO * np.abs(want[1]).max()
@@ -529,9 +536,10 @@ def test_vocabulary_loss_rows_that_do_not_count(ops, bad):
         assert np.abs(down(loss.per_sample).numpy() - want[0])[keep].max() <= 2 * RTOL_FRO * np.abs(want[1]).max()
 
 
-def test_vocabulary_loss_words_shut_out_by_the_bias(ops):
+@pytest.mark.parametrize("m", [20, 40, 100])
+def test_vocabulary_loss_words_shut_out_by_the_bias(ops, m):
     """A bias of -inf gives a word no probability, and of its type's lowest value next to none; all but one: the loss of that one is zero."""
-    m, d, v = 40, 32, 700
+    d, v = 32, 700
     h, w, b = randn(1, m, d), randn(2, d, v), randn(3, v)
     b[600:] = -math.inf
     b[300:400] = torch.finfo(torch.float32).min
@@ -547,10 +555,11 @@ def test_vocabulary_loss_words_shut_out_by_the_bias(ops):
     assert np.abs(down(loss.per_sample).numpy()).max() <= RTOL_FRO * 10
 
 
+@pytest.mark.parametrize("m", [50, 100])
 @pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -30, 2.0 ** 60])
-def test_vocabulary_loss_scales(ops, scale):
+def test_vocabulary_loss_scales(ops, scale, m):
     """Hidden states and weights far from one whose products are ordinary: the halves are scaled by the largest value."""
-    m, d, v = 50, 64, 600
+    d, v = 64, 600
     h, w, target = randn(1, m, d) * scale, randn(2, d, v) * 0.2 / scale, torch.arange(m)
     want = vocabulary_reference(h, w, None, target, -100, 0.0, "sum", torch.ones(1))
     H, W, T, one = up(ops, h), up(ops, w), target.cuda(), torch.ones(1, device="cuda")

@@ -457,6 +457,7 @@ __global__ __launch_bounds__(256) void vocab_dh_kernel(const float* __restrict p
     for (int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; x < all; x += (int64_t)gridDim.x * 1024) {
         if (x + 3 < all) {
             f32x4 s = *(const f32x4*)(part + x);
+#pragma unroll 8
             for (int64_t r = 1; r < runs; ++r) s += *(const f32x4_u*)(part + r * all + x);
             const int64_t m = x / D;
             const float factor = row_factor(v, up, m);

@@ -6,9 +6,9 @@
 //
 // The split form of the products (vocabulary.hip) reads W three times and writes it once before it begins, which its rate pays back from 65 tokens up.  Forward and backward
 // with W as an embedding [words, D], here against the split form:
-//       768 x 50257:  1 token 55 + 160 us against 146 + 272;  32 tokens 55 + 181 against 144 + 273;  64 tokens 91 + 251 against 146 + 284
-//      1600 x 8000:   1 token 57 +  97 us against 100 + 145;  64 tokens 56 + 121 against 101 + 154
-//       128 x 1000:   1 token 21 +  30 us against  28 +  41;  64 tokens 21 +  35 against  28 +  45
+//       768 x 50257:  1 token 61 + 133 us against 146 + 271;  32 tokens 59 + 146 against 144 + 274;  64 tokens 88 + 203 against 146 + 284
+//      1600 x 8000:   1 token 67 + 104 us against 100 + 145;  64 tokens 51 + 104 against 101 + 154
+//       128 x 1000:   1 token 22 +  25 us against  27 +  42;  64 tokens 22 +  25 against  28 +  45
 // One read of the first W (154 MB) takes 30 us at the rate of a copy, its backward (W twice, dW once) 92 us.
 // Both products with W have the matrix in the rows of the instruction's result and the tokens in its columns: rows r of 32 in LDS, K-major ([row][k], 32 k and 4 of padding: a
 // float4 of four k a lane, 16 rows in 16 different bank groups) where the memory runs along k, MN-major ([k][row]) where it runs along r.
@@ -42,23 +42,37 @@ template <int ROWS, bool KMAJOR>
 struct Staged {
     static constexpr int N = ROWS * KC / 1024; // groups of four
     f32x4 x[N];
+    // Rows behind the last are the last again (their products are not stored).  No branch of a lane's own: one would wait for the loads before it.
     __device__ __forceinline__ void load(const Operand2& o, int64_t r0, int64_t rows, int64_t k0, int64_t k_end) {
+        const bool wide = KMAJOR ? o.c == 1 && k0 + KC <= k_end : o.r == 1 && r0 + ROWS <= rows;
+        if (wide) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int y = threadIdx.x + 256 * i;
-            const int64_t r = r0 + (KMAJOR ? y / (KC / 4) : y % (ROWS / 4) * 4), k = k0 + (KMAJOR ? y % (KC / 4) * 4 : y / (ROWS / 4));
-            x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (r >= rows || k >= k_end) continue;
-            const float* p = o.p + r * o.r + k * o.c;
-            const int64_t left = KMAJOR ? k_end - k : rows - r, step = KMAJOR ? o.c : o.r;
-            if (step == 1 && left >= 4) x[i] = *(const f32x4_u*)p;
-            else
+            for (int i = 0; i < N; ++i) {
+                const int y = threadIdx.x + 256 * i;
+                const int64_t r = r0 + (KMAJOR ? y / (KC / 4) : y % (ROWS / 4) * 4), k = k0 + (KMAJOR ? y % (KC / 4) * 4 : y / (ROWS / 4));
+                x[i] = *(const f32x4_u*)(o.p + (KMAJOR && r >= rows ? rows - 1 : r) * o.r + (!KMAJOR && k >= k_end ? k_end - 1 : k) * o.c);
+            }
+        } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e < left) x[i][e] = p[e * step];
+            for (int i = 0; i < N; ++i) {
+                const int y = threadIdx.x + 256 * i;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int64_t r = r0 + (KMAJOR ? y / (KC / 4) : y % (ROWS / 4) * 4 + e), k = k0 + (KMAJOR ? y % (KC / 4) * 4 + e : y / (ROWS / 4));
+                    x[i][e] = o.p[(r >= rows ? rows - 1 : r) * o.r + (k >= k_end ? k_end - 1 : k) * o.c];
+                }
+            }
         }
     }
-    __device__ __forceinline__ void store(float* lds) const {
+    // k of what was loaded, and its end: zeros behind it
+    __device__ __forceinline__ void store(float* lds, int64_t k0, int64_t k_end) {
+        if (k0 + KC > k_end)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int y = threadIdx.x + 256 * i;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][e] = k0 + (KMAJOR ? y % (KC / 4) * 4 + e : y / (ROWS / 4)) < k_end ? x[i][e] : 0.f;
+            }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int y = threadIdx.x + 256 * i;
@@ -96,8 +110,8 @@ __global__ __launch_bounds__(256) void few_kernel(const FewArgs a) {
     sb.load(a.b, 0, a.v.M, k0, k_end);
     int stage = 0;
     for (int64_t k = k0; k < k_end; k += KC, stage ^= 1) {
-        sa.store(lds_a[stage]);
-        sb.store(lds_b[stage]);
+        sa.store(lds_a[stage], k, k_end);
+        sb.store(lds_b[stage], k, k_end);
         __syncthreads();
         if (k + KC < k_end) { // on the way while this step is multiplied; its place in LDS was read a step ago
             sa.load(a.a, r0, a.rows, k + KC, k_end);
@@ -202,32 +216,56 @@ struct FewWeight {
     int accumulate;
 };
 
+// columns c0 .. c0 + WIDTH of every token, on the way into LDS
+template <int TOKENS, int WIDTH>
+struct TokenRows {
+    static constexpr int N = TOKENS * WIDTH / 1024;
+    f32x4 x[N];
+    // columns behind the last are the last again (their products are not stored), and so are tokens
+    __device__ __forceinline__ void load(const Operand2& o, int64_t tokens, int64_t c0, int64_t cols) {
+        const bool wide = o.c == 1 && c0 + WIDTH <= cols;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int y = threadIdx.x + 256 * i, m = y / (WIDTH / 4);
+            const int64_t c = c0 + y % (WIDTH / 4) * 4;
+            const float* p = o.p + (m >= tokens ? tokens - 1 : m) * o.r;
+            if (wide) x[i] = *(const f32x4_u*)(p + c);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][e] = p[(c + e >= cols ? cols - 1 : c + e) * o.c];
+        }
+    }
+    // times the rows' factors: rows without a part in the gradient are zeros, whatever they hold
+    __device__ __forceinline__ void store(float* lds, const float* factors) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int y = threadIdx.x + 256 * i, m = y / (WIDTH / 4);
+            const float f = factors[m];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i][e] = f == 0.f ? 0.f : x[i][e] * f;
+            *(f32x4*)(lds + m * (WIDTH + 4) + y % (WIDTH / 4) * 4) = x[i];
+        }
+    }
+};
+
 template <int TOKENS>
 __global__ __launch_bounds__(256) void few_weight_kernel(const FewWeight a) {
     constexpr int I = 128, J = 64;
-    __shared__ float lx[TOKENS][I + 4], ly[TOKENS][J + 4];
+    __shared__ __align__(16) float lx[TOKENS][I + 4], ly[TOKENS][J + 4], factors[2][TOKENS]; // of G: one for every token
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int64_t tiles_j = (a.cols + J - 1) / J, i0 = blockIdx.x / tiles_j * I, j0 = blockIdx.x % tiles_j * J;
-    auto fill = [&](float* to, int width, const Operand2& o, int64_t c0, int64_t cols, bool is_h) {
-        for (int y = threadIdx.x; y < TOKENS * width / 4; y += 256) {
-            const int m = y / (width / 4), c = y % (width / 4) * 4;
-            f32x4 x{0.f, 0.f, 0.f, 0.f};
-            const int64_t left = cols - c0 - c;
-            const float factor = m >= a.v.M || left <= 0 ? 0.f : is_h ? row_factor(a.v, a.up, m) : 1.f;
-            if (factor != 0.f) { // rows without a part in the gradient are zeros, whatever they hold
-                const float* p = o.p + m * o.r + (c0 + c) * o.c;
-                if (o.c == 1 && left >= 4) x = *(const f32x4_u*)p;
-                else
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (e < left) x[e] = p[e * o.c];
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) to[m * (width + 4) + c + e] = x[e] * factor;
-        }
-    };
-    fill(&lx[0][0], I, a.x, i0, a.rows, a.x_is_h);
-    fill(&ly[0][0], J, a.y, j0, a.cols, !a.x_is_h);
+    TokenRows<TOKENS, I> x;
+    TokenRows<TOKENS, J> y;
+    x.load(a.x, a.v.M, i0, a.rows);
+    y.load(a.y, a.v.M, j0, a.cols);
+    if (threadIdx.x < TOKENS) { // each once: it hangs on three loads in a row
+        const bool in = threadIdx.x < a.v.M;
+        factors[0][threadIdx.x] = in ? 1.f : 0.f;
+        factors[1][threadIdx.x] = in ? row_factor(a.v, a.up, threadIdx.x) : 0.f;
+    }
+    __syncthreads();
+    x.store(&lx[0][0], factors[a.x_is_h]);
+    y.store(&ly[0][0], factors[!a.x_is_h]);
     __syncthreads();
     f32x16 acc[2];
 #pragma unroll
@@ -236,9 +274,9 @@ __global__ __launch_bounds__(256) void few_weight_kernel(const FewWeight a) {
         for (int e = 0; e < 16; ++e) acc[b][e] = 0.f;
 #pragma unroll 4
     for (int m = 0; m < TOKENS; m += 2) {
-        const float x = lx[m + half][32 * wave + (lane & 31)];
+        const float left = lx[m + half][32 * wave + (lane & 31)];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, ly[m + half][32 * b + (lane & 31)], acc[b], 0, 0, 0);
+        for (int b = 0; b < 2; ++b) acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(left, ly[m + half][32 * b + (lane & 31)], acc[b], 0, 0, 0);
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -286,8 +324,8 @@ void few_plan_forward(Workspace& ws, FewPlan& p, const VocabArgs& v) {
 
 void few_plan_backward(Workspace& ws, FewPlan& p, const VocabArgs& v) {
     p.g = ws.take<float>(v.M * v.V);
-    // four workgroups a CU, of at least 256 words each
-    p.run = up_to(up_to(v.V, std::max<int64_t>(1, std::min(1024 / up_to(v.D, rows_a_tile(v.M)), v.V / 256))), KC) * KC;
+    // four workgroups a CU, of at least 64 words each
+    p.run = up_to(up_to(v.V, std::max<int64_t>(1, std::min(1024 / up_to(v.D, rows_a_tile(v.M)), v.V / 64))), KC) * KC;
     p.runs = up_to(v.V, p.run);
     p.part_h = ws.take<float>(p.runs * v.M * v.D);
 }

@@ -56,20 +56,20 @@ __global__ __launch_bounds__(256) void attn_zero_kernel(AttnOperand g, int64_t n
     }
 }
 
-// Rows or tiles.  Rows work at D / 5 million pairs of a query and a key a microsecond less, tiles pay 7 us and one more pass over the operands before they begin: by these
-// sums, fitted to 150 shapes of D = 32, 64, 128 with 2 to 256 queries, 32 to 8192 keys and 8 to 512 heads.  Where the two meet, either is within a fifth of the other; at
-// [1, 8 x 64, 64 keys] rows take 13 us and tiles 20, at [32,16 x 64, 256 keys] 470 and 87.
+// Rows or tiles.  Rows cost by pairs of a query and a key, tiles begin with two launches and one more pass over the operands: by these sums, fitted to 264 launches of
+// D = 32, 64, 128 with 2 to 512 queries, 64 to 8192 keys and 8 to 512 heads.  No choice costs more than 1.39 of the other there, and 1 % in the mean; at [1, 8 x 64, 64 keys] rows take
+// 13 us and tiles 20, at [32,16 x 64, 256 keys] 382 and 74.
 double padded(int dim) { return (dim + 31) / 32 * 32; }
 double pair_values(const AttnShape& s) { return (double)s.batch * s.heads * s.queries * s.keys * padded(s.dim); }
 bool forward_by_rows(const AttnShape& s) {
     const double operands = (double)s.batch * padded(s.dim) * ((double)s.heads * s.queries + 2.0 * s.kv_heads * s.keys);
-    return pair_values(s) <= 37e6 + 18.0 * operands;
+    return pair_values(s) <= 60e6 + 15.0 * operands;
 }
-// Backward, where the rows' kernels also read the other side again for each row, one after the other: short sequences alone ([1, 8 x 64] with 128 queries and keys: 32 us by
-// rows, 46 by tiles; with 256: 68 and 60).
+// Backward, where a wavefront or a slot of it takes the other side's rows one after the other: 1024 of them at most ([1, 8 x 64]: 128 queries and keys take 24 us by rows and 46 by tiles,
+// 512 of both 115 and 74).
 bool backward_by_rows(const AttnShape& s) {
     const double operands = 2.0 * s.batch * padded(s.dim) * ((double)s.heads * s.queries + (double)s.kv_heads * s.keys);
-    return s.queries <= 256 && s.keys <= 256 && pair_values(s) <= 20e6 + 6.0 * operands;
+    return s.queries <= 1024 && s.keys <= 1024 && pair_values(s) <= 40e6 + 3.0 * operands;
 }
 
 void forward_plan(const AttnShape& s, const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, float* out, float* lse, Workspace& ws, const LibraryState& lib, bool launch) {

@@ -41,15 +41,43 @@ constexpr float kNone = -__builtin_inff(); // the maximum and the logarithm of t
 // maximum by t comes out with a relative error of (t + 2) 2^-24, where its weight is exp(-t).
 __device__ __forceinline__ float below(float a, float m) { return __expf(a - (m == kNone ? 0.f : m)); }
 
-// Four values of d, of which the first is 4 * part, from p (that value's place): 16 bytes where they are there and adjacent, else one by one, zero behind the last.
-template <bool UNIT>
-__device__ __forceinline__ f32x4 attn_load4(const float* p, int64_t ds, int part, int D) {
-    if (UNIT && 4 * part + 3 < D) return *(const f32x4_u*)p;
-    f32x4 x{0.f, 0.f, 0.f, 0.f};
+// Four values of d of a row, of which the first is 4 * part; zero behind the last.  Three ways, none with a branch of a lane's own: where lanes part, each waits for the loads that the others
+// have under way.  What a lane has no values for it reads at the row's end and drops.
+enum { kLoadAny, kLoadWhole, kLoadTail }; // any stride; adjacent values, a multiple of four of them; adjacent values, four at least
+__device__ __host__ __forceinline__ int attn_kind(int64_t d, int D) { return d != 1 || D < 4 ? kLoadAny : D % 4 ? kLoadTail : kLoadWhole; }
+template <int KIND>
+__device__ __forceinline__ f32x4 attn_load4(const float* row, int64_t ds, int part, int D) {
+    const int at = 4 * part;
+    f32x4 x;
+    if (KIND == kLoadWhole) {
+        x = *(const f32x4_u*)(row + (at < D ? at : 0));
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (4 * part + e < D) x[e] = p[e * ds];
+        for (int e = 0; e < 4; ++e) x[e] = at < D ? x[e] : 0.f;
+    } else if (KIND == kLoadTail) { // the last group is read with values of the one before it, and moved down
+        x = *(const f32x4_u*)(row + (at < D - 4 ? at : D - 4));
+        const int by = at - (D - 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float y = by <= 0 ? x[e] : 0.f;
+#pragma unroll
+            for (int f = e + 1; f < 4; ++f) y = by == f - e ? x[f] : y;
+            x[e] = y;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = row[(at + e < D ? at + e : D - 1) * ds];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = at + e < D ? x[e] : 0.f;
+    }
     return x;
+}
+template <int KIND> struct LoadKind { static constexpr int value = KIND; };
+// f with the kind as a constant: one branch, that all lanes take together, around all loads of a kind
+template <class F>
+__device__ __forceinline__ void attn_with_kind(int kind, F f) {
+    if (kind == kLoadWhole) f(LoadKind<kLoadWhole>{});
+    else if (kind == kLoadTail) f(LoadKind<kLoadTail>{});
+    else f(LoadKind<kLoadAny>{});
 }
 __device__ __forceinline__ float dot4(f32x4 a, f32x4 b) { return (a[0] * b[0] + a[1] * b[1]) + (a[2] * b[2] + a[3] * b[3]); }
 struct AttnBackward {

@@ -27,7 +27,7 @@ struct RowsArgs {
     int splits, row_blocks;
 };
 
-template <int L, int R, bool UNIT> // lanes a key, rows a workgroup, unit stride along d
+template <int L, int R, int KIND> // lanes a key, rows a workgroup, how rows are loaded
 __global__ __launch_bounds__(256) void attn_rows_kernel(const RowsArgs a) {
     constexpr int SLOTS = 64 / L, U = R > 4 ? 2 : 4;
     __shared__ float join_m[4][SLOTS][R], join_l[4][SLOTS][R];
@@ -47,9 +47,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const RowsArgs a) {
     for (int r = 0; r < R; ++r) {
         const int row = row0 + r < rows ? row0 + r : rows - 1;
         const int h = hk * a.s.group + row / a.s.queries, i = row % a.s.queries;
-        const float* p = a.q.p + b * a.q.b + i * a.q.s + h * a.q.h;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[r][e] = 4 * part + e < D ? p[(4 * part + e) * a.q.d] * a.s.scale : 0.f;
+        q[r] = attn_load4<KIND>(a.q.p + b * a.q.b + i * a.q.s + h * a.q.h, a.q.d, part, D) * a.s.scale;
         limit[r] = attn_limit(length, start, i);
         least = limit[r] < least ? limit[r] : least;
         most = limit[r] > most ? limit[r] : most;
@@ -62,15 +60,15 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const RowsArgs a) {
     f32x4 o[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) m[r] = kNone, l[r] = 0.f, o[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const float* kp = a.k.p + b * a.k.b + hk * a.k.h + 4 * part * a.k.d;
-    const float* vp = a.v.p + b * a.v.b + hk * a.v.h + 4 * part * a.v.d;
+    const float* kp = a.k.p + b * a.k.b + hk * a.k.h;
+    const float* vp = a.v.p + b * a.v.b + hk * a.v.h;
     for (int j0 = lo + wave * SLOTS + slot; __any(j0 < hi); j0 += 4 * SLOTS * U) {
         f32x4 k[U], v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) { // a slot without a key of its own reads the run's last one and does not use it
             const int64_t j = j0 + 4 * SLOTS * u < hi ? j0 + 4 * SLOTS * u : hi - 1;
-            k[u] = attn_load4<UNIT>(kp + j * a.k.s, a.k.d, part, D);
-            v[u] = attn_load4<UNIT>(vp + j * a.v.s, a.v.d, part, D);
+            k[u] = attn_load4<KIND>(kp + j * a.k.s, a.k.d, part, D);
+            v[u] = attn_load4<KIND>(vp + j * a.v.s, a.v.d, part, D);
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -178,16 +176,20 @@ __global__ __launch_bounds__(64 * W) void attn_join_kernel(const AttnShape s, co
     if (d == 0 && lse) lse[row] = sum == 0.f ? kNone : top + logf(sum);
 }
 
+int kind_of(const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, int D) { return attn_kind(q.d == 1 && k.d == 1 ? v.d : 0, D); }
+
 template <int L, int R>
-void launch_rows(const RowsArgs& a, bool unit, unsigned grid, hipStream_t stream) {
-    if (unit) hipLaunchKernelGGL((attn_rows_kernel<L, R, true>), dim3(grid), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((attn_rows_kernel<L, R, false>), dim3(grid), dim3(256), 0, stream, a);
+void launch_rows(const RowsArgs& a, unsigned grid, hipStream_t stream) {
+    const int kind = kind_of(a.q, a.k, a.v, a.s.dim);
+    if (kind == kLoadWhole) hipLaunchKernelGGL((attn_rows_kernel<L, R, kLoadWhole>), dim3(grid), dim3(256), 0, stream, a);
+    else if (kind == kLoadTail) hipLaunchKernelGGL((attn_rows_kernel<L, R, kLoadTail>), dim3(grid), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attn_rows_kernel<L, R, kLoadAny>), dim3(grid), dim3(256), 0, stream, a);
 }
 template <int L>
-void launch_rows(const RowsArgs& a, int r, bool unit, unsigned grid, hipStream_t stream) {
-    if (r == 1) launch_rows<L, 1>(a, unit, grid, stream);
-    else if (r <= 4) launch_rows<L, 4>(a, unit, grid, stream);
-    else launch_rows<L, 8>(a, unit, grid, stream);
+void launch_rows(const RowsArgs& a, int r, unsigned grid, hipStream_t stream) {
+    if (r == 1) launch_rows<L, 1>(a, grid, stream);
+    else if (r <= 4) launch_rows<L, 4>(a, grid, stream);
+    else launch_rows<L, 8>(a, grid, stream);
 }
 
 // Backward.  Rows: s and dP = dout . v again for each allowed key, p = exp(s - lse), dS = p (dP - delta) with delta = dout . out; dq = scale sum_j dS k_j.
@@ -207,7 +209,7 @@ __device__ __forceinline__ void add_to(const AttnOperand& g, int64_t at, int par
         }
 }
 
-template <int L, bool UNIT>
+template <int L, int KIND>
 __global__ __launch_bounds__(256) void attn_rows_dq_kernel(const RowsBackward a) { // a wavefront a row
     constexpr int SLOTS = 64 / L, U = 2;
     const AttnShape& s = a.b.s;
@@ -216,22 +218,22 @@ __global__ __launch_bounds__(256) void attn_rows_dq_kernel(const RowsBackward a)
     if (row >= (int64_t)s.batch * s.heads * s.queries) return;
     const int i = (int)(row % s.queries), h = (int)(row / s.queries % s.heads), b = (int)(row / s.queries / s.heads), hk = h / s.group;
     const int limit = attn_limit(attn_length(s, b), attn_start(s, b), i);
-    const int64_t dense = (((int64_t)b * s.queries + i) * s.heads + h) * D + 4 * part;
-    const f32x4 q = attn_load4<false>(a.b.q.p + b * a.b.q.b + i * a.b.q.s + h * a.b.q.h + 4 * part * a.b.q.d, a.b.q.d, part, D) * s.scale;
-    const f32x4 g = attn_load4<true>(a.b.dout + dense, 1, part, D), o = attn_load4<true>(a.b.out + dense, 1, part, D);
+    const int64_t dense = (((int64_t)b * s.queries + i) * s.heads + h) * D;
+    const f32x4 q = attn_load4<KIND>(a.b.q.p + b * a.b.q.b + i * a.b.q.s + h * a.b.q.h, a.b.q.d, part, D) * s.scale;
+    const f32x4 g = attn_load4<KIND>(a.b.dout + dense, 1, part, D), o = attn_load4<KIND>(a.b.out + dense, 1, part, D);
     const float delta = lanes_sum<L>(dot4(g, o)), lse = a.b.lse[row];
     if (lane == 0) a.delta[row] = delta;
     if (!a.b.grad_q.p) return;
-    const float* kp = a.b.k.p + b * a.b.k.b + hk * a.b.k.h + 4 * part * a.b.k.d;
-    const float* vp = a.b.v.p + b * a.b.v.b + hk * a.b.v.h + 4 * part * a.b.v.d;
+    const float* kp = a.b.k.p + b * a.b.k.b + hk * a.b.k.h;
+    const float* vp = a.b.v.p + b * a.b.v.b + hk * a.b.v.h;
     f32x4 acc{0.f, 0.f, 0.f, 0.f};
     for (int j0 = slot; __any(j0 < limit); j0 += SLOTS * U) {
         f32x4 k[U], v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t j = j0 + SLOTS * u < limit ? j0 + SLOTS * u : limit - 1;
-            k[u] = attn_load4<UNIT>(kp + j * a.b.k.s, a.b.k.d, part, D);
-            v[u] = attn_load4<UNIT>(vp + j * a.b.v.s, a.b.v.d, part, D);
+            k[u] = attn_load4<KIND>(kp + j * a.b.k.s, a.b.k.d, part, D);
+            v[u] = attn_load4<KIND>(vp + j * a.b.v.s, a.b.v.d, part, D);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -247,9 +249,9 @@ __global__ __launch_bounds__(256) void attn_rows_dq_kernel(const RowsBackward a)
 }
 
 // dv_j = sum_i p_ij dout_i, dk_j = scale sum_i dS_ij q_i over the queries of the heads that share the key's: a slot a key, the queries dealt to the 4 wavefronts.
-template <int L, bool UNIT>
+template <int L, int KIND>
 __global__ __launch_bounds__(256) void attn_rows_dkv_kernel(const RowsBackward a) {
-    constexpr int SLOTS = 64 / L;
+    constexpr int SLOTS = 64 / L, U = 4;
     __shared__ f32x4 join[2][4][SLOTS][L];
     const AttnShape& s = a.b.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slot = lane / L, part = lane % L, D = s.dim;
@@ -258,20 +260,33 @@ __global__ __launch_bounds__(256) void attn_rows_dkv_kernel(const RowsBackward a
     const int hk = rest % s.kv_heads, b = rest / s.kv_heads;
     const int length = attn_length(s, b), start = attn_start(s, b);
     const int64_t jr = j < s.keys ? j : s.keys - 1;
-    const f32x4 k = attn_load4<UNIT>(a.b.k.p + b * a.b.k.b + hk * a.b.k.h + jr * a.b.k.s + 4 * part * a.b.k.d, a.b.k.d, part, D);
-    const f32x4 v = attn_load4<UNIT>(a.b.v.p + b * a.b.v.b + hk * a.b.v.h + jr * a.b.v.s + 4 * part * a.b.v.d, a.b.v.d, part, D);
+    const f32x4 k = attn_load4<KIND>(a.b.k.p + b * a.b.k.b + hk * a.b.k.h + jr * a.b.k.s, a.b.k.d, part, D);
+    const f32x4 v = attn_load4<KIND>(a.b.v.p + b * a.b.v.b + hk * a.b.v.h + jr * a.b.v.s, a.b.v.d, part, D);
     f32x4 dk{0.f, 0.f, 0.f, 0.f}, dv = dk;
+    // the first query that sees the first of these keys
+    const int first = j - slot < length ? (j - slot > start ? j - slot - start : 0) : s.queries;
     for (int h = hk * s.group; h < (hk + 1) * s.group; ++h)
-        for (int i = wave; i < s.queries; i += 4) {
-            if (!__any(j < attn_limit(length, start, i))) continue;
-            const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
-            const f32x4 q = attn_load4<false>(a.b.q.p + b * a.b.q.b + i * a.b.q.s + h * a.b.q.h + 4 * part * a.b.q.d, a.b.q.d, part, D);
-            const f32x4 g = attn_load4<true>(a.b.dout + (((int64_t)b * s.queries + i) * s.heads + h) * D + 4 * part, 1, part, D);
-            const float x = lanes_sum<L>(dot4(q, k)) * s.scale, dp = lanes_sum<L>(dot4(g, v));
-            if (j >= attn_limit(length, start, i)) continue;
-            const float p = __expf(x - a.b.lse[row]);
-            dv += p * g;
-            dk += p * (dp - a.delta[row]) * q;
+        for (int i0 = first + wave; i0 < s.queries; i0 += 4 * U) {
+            f32x4 q[U], g[U];
+            float lse[U], delta[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) { // (the last query again where there is none)
+                const int i = i0 + 4 * u < s.queries ? i0 + 4 * u : s.queries - 1;
+                const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
+                q[u] = attn_load4<KIND>(a.b.q.p + b * a.b.q.b + i * a.b.q.s + h * a.b.q.h, a.b.q.d, part, D);
+                g[u] = attn_load4<KIND>(a.b.dout + (((int64_t)b * s.queries + i) * s.heads + h) * D, 1, part, D);
+                lse[u] = a.b.lse[row];
+                delta[u] = a.delta[row];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + 4 * u;
+                const float x = lanes_sum<L>(dot4(q[u], k)) * s.scale, dp = lanes_sum<L>(dot4(g[u], v));
+                if (i >= s.queries || j >= attn_limit(length, start, i)) continue; // its row may hold anything
+                const float p = __expf(x - lse[u]);
+                dv += p * g[u];
+                dk += p * (dp - delta[u]) * q[u];
+            }
         }
     join[0][wave][slot][part] = dk;
     join[1][wave][slot][part] = dv;
@@ -283,13 +298,17 @@ __global__ __launch_bounds__(256) void attn_rows_dkv_kernel(const RowsBackward a
     if (a.b.grad_v.p) add_to(a.b.grad_v, b * a.b.grad_v.b + j * a.b.grad_v.s + hk * a.b.grad_v.h, part, D, dv, a.b.accumulate);
 }
 
+template <int L, int KIND>
+void launch_rows_backward(const RowsBackward& a, unsigned row_grid, unsigned key_grid, hipStream_t stream) {
+    hipLaunchKernelGGL((attn_rows_dq_kernel<L, KIND>), dim3(row_grid), dim3(256), 0, stream, a);
+    if (a.b.grad_k.p || a.b.grad_v.p) hipLaunchKernelGGL((attn_rows_dkv_kernel<L, KIND>), dim3(key_grid), dim3(256), 0, stream, a);
+}
 template <int L>
-void launch_rows_backward(const RowsBackward& a, bool unit, unsigned row_grid, unsigned key_grid, hipStream_t stream) {
-    if (unit) hipLaunchKernelGGL((attn_rows_dq_kernel<L, true>), dim3(row_grid), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((attn_rows_dq_kernel<L, false>), dim3(row_grid), dim3(256), 0, stream, a);
-    if (!a.b.grad_k.p && !a.b.grad_v.p) return;
-    if (unit) hipLaunchKernelGGL((attn_rows_dkv_kernel<L, true>), dim3(key_grid), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((attn_rows_dkv_kernel<L, false>), dim3(key_grid), dim3(256), 0, stream, a);
+void launch_rows_backward(const RowsBackward& a, unsigned row_grid, unsigned key_grid, hipStream_t stream) {
+    const int kind = kind_of(a.b.q, a.b.k, a.b.v, a.b.s.dim);
+    if (kind == kLoadWhole) launch_rows_backward<L, kLoadWhole>(a, row_grid, key_grid, stream);
+    else if (kind == kLoadTail) launch_rows_backward<L, kLoadTail>(a, row_grid, key_grid, stream);
+    else launch_rows_backward<L, kLoadAny>(a, row_grid, key_grid, stream);
 }
 
 } // namespace
@@ -303,10 +322,9 @@ void attn_rows_backward(const AttnBackward& b, Workspace& ws, hipStream_t stream
     const int slots = b.s.dim <= 32 ? 8 : b.s.dim <= 64 ? 4 : 2;
     a.key_blocks = (b.s.keys + slots - 1) / slots;
     const unsigned row_grid = (unsigned)((rows + 3) / 4), key_grid = (unsigned)((int64_t)b.s.batch * b.s.kv_heads * a.key_blocks);
-    const bool unit = b.k.d == 1 && b.v.d == 1;
-    if (b.s.dim <= 32) launch_rows_backward<8>(a, unit, row_grid, key_grid, stream);
-    else if (b.s.dim <= 64) launch_rows_backward<16>(a, unit, row_grid, key_grid, stream);
-    else launch_rows_backward<32>(a, unit, row_grid, key_grid, stream);
+    if (b.s.dim <= 32) launch_rows_backward<8>(a, row_grid, key_grid, stream);
+    else if (b.s.dim <= 64) launch_rows_backward<16>(a, row_grid, key_grid, stream);
+    else launch_rows_backward<32>(a, row_grid, key_grid, stream);
 }
 
 void attn_rows_forward(const AttnShape& s, const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, float* out, float* lse,
@@ -321,10 +339,9 @@ void attn_rows_forward(const AttnShape& s, const AttnOperand& q, const AttnOpera
     if (a.splits > 1) a.part = ws.take<float>((int64_t)a.splits * s.batch * s.heads * s.queries * (s.dim + 2));
     if (!launch) return;
     const unsigned grid = (unsigned)(groups * a.splits);
-    const bool unit = k.d == 1 && v.d == 1;
-    if (s.dim <= 32) launch_rows<8>(a, r, unit, grid, stream);
-    else if (s.dim <= 64) launch_rows<16>(a, r, unit, grid, stream);
-    else launch_rows<32>(a, r, unit, grid, stream);
+    if (s.dim <= 32) launch_rows<8>(a, r, grid, stream);
+    else if (s.dim <= 64) launch_rows<16>(a, r, grid, stream);
+    else launch_rows<32>(a, r, grid, stream);
     if (a.splits > 1) attn_join(s, a.part, a.splits, out, lse, stream);
 }
 

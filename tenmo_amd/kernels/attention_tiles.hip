@@ -107,24 +107,30 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
     const int run = blockIdx.x % a.parts;
     const HeadJob j = head_job(a, blockIdx.x / a.parts);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = lane % L, D = a.s.dim;
-    const float* p = j.src.p + j.b * j.src.b + j.h * j.src.h + 4 * part * j.src.d;
+    const float* p = j.src.p + j.b * j.src.b + j.h * j.src.h;
     const int all = j.job == kDO ? j.pad : j.rows, per = (all + a.parts - 1) / a.parts;
     const int first = run * per, last = first + per < all ? first + per : all;
     float top = 0.f, norm = 0.f, least = __builtin_inff();
     bool wrong = false;
     for (int r0 = first + wave * SLOTS + lane / L; __any(r0 < last); r0 += 4 * SLOTS * U) {
         f32x4 x[U], o[U];
+        // (a row that does not count is read as one that does, or as the first)
+        auto row_at = [&](int u) { const int r = r0 + 4 * SLOTS * u; return r >= j.lo && r < j.hi ? r : j.lo < j.hi ? j.lo : 0; };
+        attn_with_kind(attn_kind(j.src.d, D), [&](auto kind) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = attn_load4<kind.value>(p + row_at(u) * j.src.s, j.src.d, part, D);
+        });
+        if (j.job == kDO)
+            attn_with_kind(attn_kind(1, D), [&](auto kind) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) o[u] = attn_load4<kind.value>(a.out + (((int64_t)j.b * a.s.queries + row_at(u)) * a.s.heads + j.h) * D, 1, part, D);
+            });
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int r = r0 + 4 * SLOTS * u;
             const bool in = r < last && r >= j.lo && r < j.hi;
-            x[u] = o[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (in) x[u] = j.src.d == 1 ? attn_load4<true>(p + r * j.src.s, 1, part, D) : attn_load4<false>(p + r * j.src.s, j.src.d, part, D);
-            if (in && j.job == kDO) o[u] = attn_load4<true>(a.out + (((int64_t)j.b * a.s.queries + r) * a.s.heads + j.h) * D + 4 * part, 1, part, D);
-        }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int r = r0 + 4 * SLOTS * u;
+            for (int e = 0; e < 4; ++e) x[u][e] = in ? x[u][e] : 0.f;
             float mine = 0.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -138,9 +144,11 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
             // (a square out of range: the largest magnitude times sqrt(D) instead)
             norm = fmaxf(norm, sq < 1e37f && sq > 1e-30f ? sqrtf(sq) : fminf(mine * sqrtf((float)D), 1e38f));
             if (j.job == kDO) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[u][e] = in ? o[u][e] : 0.f;
                 const float delta = lanes_sum<L>(dot4(x[u], o[u]));
                 if (part == 0 && r < last)
-                    a.stats[(int64_t)j.bh * j.pad + r] = r >= j.lo && r < j.hi ? f32x2{a.lse[(int64_t)j.bh * a.s.queries + r] * kLog2e, delta} : f32x2{__builtin_inff(), 0.f};
+                    a.stats[(int64_t)j.bh * j.pad + r] = in ? f32x2{a.lse[(int64_t)j.bh * a.s.queries + r] * kLog2e, delta} : f32x2{__builtin_inff(), 0.f};
             }
         }
     }
@@ -160,7 +168,7 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
 // theirs may be as small as 2^-24 of the largest (gradients of single positions are), with a dQ of their own to 2^-16 of itself there.
 template <int DP>
 __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
-    constexpr int GROUPS = DP / 8, ROWS = 64;
+    constexpr int GROUPS = DP / 8, ROWS = 64, N = ROWS * GROUPS / 256;
     const int block = blockIdx.x % a.split_blocks;
     const HeadJob j = head_job(a, blockIdx.x / a.split_blocks);
     if (block * ROWS >= j.pad && block > 0) return;
@@ -174,25 +182,29 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
         if (threadIdx.x == 0) j.head[j.bh] = f32x4{scale, norm, wrong > 0.f || top * (key ? 0x1p-16f : 0x1p-24f) > least ? 1.f : 0.f, 0.f};
     }
     const float* p = j.src.p + j.b * j.src.b + j.h * j.src.h;
-    for (int x = threadIdx.x; x < ROWS * GROUPS; x += 256) {
-        const int r = block * ROWS + x / GROUPS, d = x % GROUPS * 8;
-        f16x8 h, l;
-        f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        if (r >= j.pad) break;
-        if (r >= j.lo && r < j.hi) {
-            const float* q = p + r * j.src.s + d * j.src.d;
+    if (j.pad == 0) return;
+    f32x4 v[N][2];
+    attn_with_kind(attn_kind(j.src.d, a.s.dim), [&](auto kind) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                v[i] = j.src.d == 1 ? attn_load4<true>(q + 4 * i, 1, d / 4 + i, a.s.dim) : attn_load4<false>(q + 4 * i * j.src.d, j.src.d, d / 4 + i, a.s.dim);
+        for (int i = 0; i < N; ++i) {
+            const int x = threadIdx.x + 256 * i, r = block * ROWS + x / GROUPS, at = r >= j.lo && r < j.hi ? r : j.lo < j.hi ? j.lo : 0;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) v[i][u] = attn_load4<kind.value>(p + at * j.src.s, j.src.d, x % GROUPS * 2 + u, a.s.dim);
         }
+    });
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int x = threadIdx.x + 256 * i, r = block * ROWS + x / GROUPS;
+        const bool in = r >= j.lo && r < j.hi;
+        f16x8 h, l;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             _Float16 hi16, lo16;
-            split_value(v[e >> 2][e & 3] * scale, hi16, lo16);
+            split_value(in ? v[i][e >> 2][e & 3] * scale : 0.f, hi16, lo16);
             h[e] = hi16;
             l[e] = lo16;
         }
-        float* to = j.split + ((int64_t)j.bh * j.pad + r) * DP + d;
+        float* to = j.split + ((int64_t)j.bh * j.pad + r) * DP + x % GROUPS * 8;
         *(f16x8*)to = h;
         *(f16x8*)(to + 4) = l;
     }
@@ -213,7 +225,7 @@ __device__ __forceinline__ void store_part(float* to, int d, int D, f32x4 x) {
 // ---- heads beyond the halves: a wavefront a row, or 64 / L keys ------------------------------------------------------------------------
 
 __device__ __forceinline__ f32x4 slow_load(const AttnOperand& o, int b, int64_t s, int h, int part, int D) {
-    return attn_load4<false>(o.p + b * o.b + s * o.s + h * o.h + 4 * part * o.d, o.d, part, D);
+    return attn_load4<kLoadAny>(o.p + b * o.b + s * o.s + h * o.h, o.d, part, D);
 }
 
 // a row's sum of p v (this lane's four values), its maximum and sum over the keys lo .. hi - 1
@@ -393,7 +405,7 @@ __device__ __forceinline__ void own_rows(f16x8 (&h)[DP / 16], f16x8 (&l)[DP / 16
     }
 }
 // The same from the fp32 operand, a row a lane (and the other half of it 32 lanes further), each with a scale of its own, which is returned: a row of these is a column of the
-// product, so none loses anything to another.  Rows that are not `in` are zeros and not read.  *norm: the row's.
+// product, so none loses anything to another.  Rows that are not `in` are zeros.  *norm: the row's.
 template <int DP>
 __device__ __forceinline__ float own_split(f16x8 (&h)[DP / 16], f16x8 (&l)[DP / 16], const AttnOperand& o, int b, int i, int head, bool in, int D, float* norm) {
     constexpr int KD = DP / 16;
@@ -401,13 +413,18 @@ __device__ __forceinline__ float own_split(f16x8 (&h)[DP / 16], f16x8 (&l)[DP / 
     const float* p = o.p + b * o.b + (in ? i : 0) * o.s + head * o.h;
     f32x4 x[KD][2];
     float top = 0.f, sq = 0.f;
+    attn_with_kind(attn_kind(o.d, D), [&](auto kind) {
+#pragma unroll
+        for (int ks = 0; ks < KD; ++ks)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) x[ks][u] = attn_load4<kind.value>(p, o.d, 4 * ks + 2 * half + u, D);
+    });
 #pragma unroll
     for (int ks = 0; ks < KD; ++ks)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int part = 4 * ks + 2 * half + u;
-            x[ks][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (in) x[ks][u] = o.d == 1 ? attn_load4<true>(p + 4 * part, 1, part, D) : attn_load4<false>(p + 4 * part * o.d, o.d, part, D);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[ks][u][e] = in ? x[ks][u][e] : 0.f; // whatever the row holds
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = fmaxf(top, __uint_as_float(finite_magnitude(x[ks][u][e])));
             sq += dot4(x[ks][u], x[ks][u]);
@@ -765,9 +782,9 @@ __global__ __launch_bounds__(256) void attn_group_kernel(const TileArgs a) {
     for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.x * 256) {
         const int d = (int)(x % quads) * 4;
         const int64_t row = x / quads, bk = row / a.s.keys, j = row - bk * a.s.keys, b = bk / a.s.kv_heads, hk = bk - b * a.s.kv_heads;
-        const float* p = part + (((b * a.s.heads + hk * a.s.group) * a.s.keys) + j) * D + d;
-        f32x4 sum = attn_load4<true>(p, 1, d / 4, D);
-        for (int i = 1; i < a.s.group; ++i) sum += attn_load4<true>(p + (int64_t)i * a.s.keys * D, 1, d / 4, D);
+        const float* p = part + (((b * a.s.heads + hk * a.s.group) * a.s.keys) + j) * D;
+        f32x4 sum = attn_load4<kLoadAny>(p, 1, d / 4, D);
+        for (int i = 1; i < a.s.group; ++i) sum += attn_load4<kLoadAny>(p + (int64_t)i * a.s.keys * D, 1, d / 4, D);
         store_gradient(g, b * g.b + hk * g.h + j * g.s, d, D, sum, a.accumulate);
     }
 }

@@ -39,7 +39,7 @@ int tenmo_hip_layer_norm_backward_f32(const tenmo_view* X, const float* weight, 
 /* ---- attention ------------------------------------------------------------------------------------------------------------ */
 
 /* Q [B, Sq, H, D], K and V [B, Sk, Hk, D] (views with any strides; H a multiple of Hk, query head h reads key head h / (H / Hk);
- * D of 1 to 128; B * H up to 2^20, B * H * Sq up to 2^26, B * Hk * Sk up to 2^28).  out[b, i, h, :] = sum over the allowed keys j of softmax_j(scale * q_i . k_j) * v_j, dense [B, Sq, H, D].
+ * D of 1 to 128; B * H up to 2^20, B * H * Sq up to 2^25, B * Hk * Sk up to 2^27).  out[b, i, h, :] = sum over the allowed keys j of softmax_j(scale * q_i . k_j) * v_j, dense [B, Sq, H, D].
  * Key j is allowed for query i of sequence b when j < key_lengths[b] (NULL: Sk; taken as 0 below 0 and as Sk above Sk) and, if causal != 0,
  * j <= i + query_starts[b] (the position of the first query; NULL: Sk - Sq, the queries are the last positions).  Both are device arrays
  * of B ints.  Keys that are not allowed are not used, whatever they hold; a query without keys gets zeros.
@@ -51,7 +51,7 @@ int tenmo_hip_attention_forward_f32(const tenmo_view* Q, const tenmo_view* K, co
                                     void* workspace, int64_t workspace_bytes, int32_t sync);
 /* Gradients for the upstream gradient dOut (dense [B, Sq, H, D]); out and lse as the forward call with the same arguments left them.  The
  * probabilities are computed again.  grad_Q, grad_K, grad_V: views of the shapes of Q, K, V with strides of their own (no two elements
- * at one place), written through; grad_K and grad_V sum over the query heads that share a key head. */
+ * of the three at one place), written through; grad_K and grad_V sum over the query heads that share a key head. */
 int64_t tenmo_hip_attention_backward_workspace_bytes(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim);
 int tenmo_hip_attention_backward_f32(const tenmo_view* Q, const tenmo_view* K, const tenmo_view* V, float scale, int32_t causal,
                                      const int32_t* key_lengths, const int32_t* query_starts, const float* out, const float* lse,

@@ -47,7 +47,7 @@ def attention_backward(q: NDBuffer, k: NDBuffer, v: NDBuffer, out: NDBuffer, lse
                        key_lengths: Optional[torch.Tensor] = None, query_starts: Optional[torch.Tensor] = None, need: Sequence[bool] = (True, True, True),
                        into: Optional[Sequence[Optional[NDBuffer]]] = None, sync: bool = False) -> Tuple[Optional[NDBuffer], Optional[NDBuffer], Optional[NDBuffer]]:
     """(grad_q, grad_k, grad_v) for the upstream gradient dout (dense, out's shape), with out and lse of the forward call and its other
-    arguments; those not needed are None.  ``into``: three buffers of the shapes of q, k and v (any strides, no two elements at one place) or None each, which are
+    arguments; those not needed are None.  ``into``: three buffers of the shapes of q, k and v (any strides, no two elements of the three at one place) or None each, which are
     added to instead."""
     sizes = _sizes(q, k, v)
     batch, queries, _, heads, _, dim = sizes

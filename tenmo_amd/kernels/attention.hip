@@ -9,9 +9,9 @@ int attn_shape(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int6
     if (batch < 0 || queries < 0 || keys < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads)
         return refuse(TENMO_ERR_INVALID_SHAPE, "%s: %lld query heads for %lld key heads: a multiple of them is needed", who, (long long)heads, (long long)kv_heads);
     if (dim < 1 || dim > 128) return refuse(TENMO_ERR_UNSUPPORTED, "%s: head size %lld, 1 to 128 are supported", who, (long long)dim);
-    const int64_t rows = 1 << 26, sequences = 1 << 20; // (each below what makes the next product overflow)
-    if (batch > sequences || heads > sequences || batch * heads > sequences || queries > rows || keys > rows || batch * heads * queries > rows || batch * kv_heads * keys > 4 * rows)
-        return refuse(TENMO_ERR_UNSUPPORTED, "%s: more than 2^20 heads of sequences, 2^26 rows of queries or 2^28 of keys", who);
+    const int64_t sequences = 1 << 20, rows = 1 << 25, keys_most = 1 << 27; // (each below what makes the next product overflow)
+    if (batch > sequences || heads > sequences || batch * heads > sequences || queries > rows || keys > keys_most || batch * heads * queries > rows || batch * kv_heads * keys > keys_most)
+        return refuse(TENMO_ERR_UNSUPPORTED, "%s: more than 2^20 heads of sequences, 2^25 rows of queries or 2^27 of keys", who);
     s->batch = (int)batch; s->queries = (int)queries; s->keys = (int)keys; s->heads = (int)heads; s->kv_heads = (int)kv_heads; s->dim = (int)dim;
     s->group = (int)(heads / kv_heads);
     return 0;

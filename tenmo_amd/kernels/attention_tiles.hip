@@ -44,7 +44,6 @@ struct TileArgs {
     AttnOperand src[4];
     int jobs;           // operands that are split beforehand
     int parts;          // runs of a head's rows in the first launch
-    int split_blocks;   // workgroups a head in the second
     float* split[4];    // [batch][heads][rows padded][DP]
     f32x4* seen[4];     // [batch * heads][parts]: of a run of rows, the largest finite magnitude, the largest norm of a row, the smallest largest magnitude of a row
                         // that is not zero, and 1 if there is a value that is not finite
@@ -169,20 +168,21 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
 template <int DP>
 __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
     constexpr int GROUPS = DP / 8, ROWS = 64, N = ROWS * GROUPS / 256;
-    const int block = blockIdx.x % a.split_blocks;
-    const HeadJob j = head_job(a, blockIdx.x / a.split_blocks);
-    if (block * ROWS >= j.pad && block > 0) return;
+    // the heads of K and V first
+    const uint32_t key_blocks = row_pad(a.s.keys) / ROWS, query_blocks = row_pad(a.s.queries) / ROWS, key_heads = 2 * a.s.batch * a.s.kv_heads;
+    const bool key = blockIdx.x < key_heads * key_blocks;
+    const uint32_t id = key ? blockIdx.x : blockIdx.x - key_heads * key_blocks, blocks = key ? key_blocks : query_blocks;
+    const int block = id % blocks;
+    const HeadJob j = head_job(a, (key ? 0 : key_heads) + id / blocks);
     const int lane = threadIdx.x & 63;
     f32x4 s{0.f, 0.f, __builtin_inff(), 0.f};
     if (lane < a.parts) s = j.seen[(int64_t)j.bh * a.parts + lane];
     const float top = wave_max(s[0]), scale = split_scale(__float_as_uint(top));
     if (block == 0) {
         const float norm = wave_max(s[1]), least = -wave_max(-s[2]), wrong = wave_max(s[3]);
-        const bool key = j.job == kK || j.job == kV;
         if (threadIdx.x == 0) j.head[j.bh] = f32x4{scale, norm, wrong > 0.f || top * (key ? 0x1p-16f : 0x1p-24f) > least ? 1.f : 0.f, 0.f};
     }
     const float* p = j.src.p + j.b * j.src.b + j.h * j.src.h;
-    if (j.pad == 0) return;
     f32x4 v[N][2];
     attn_with_kind(attn_kind(j.src.d, a.s.dim), [&](auto kind) {
 #pragma unroll
@@ -899,11 +899,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(con
 
 int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 
+int all_heads(const AttnShape& s, int jobs) { return s.batch * (s.heads * (jobs - 2) + s.kv_heads * 2); } // (jobs: 2 or 4)
+
 void plan_operands(TileArgs& a, Workspace& ws, int jobs) {
     const AttnShape& s = a.s;
     a.jobs = jobs;
-    a.parts = std::max(1, std::min(kHeadParts, (std::max(jobs == 2 ? 0 : s.queries, s.keys) + 127) / 128));
-    a.split_blocks = std::max(jobs == 2 ? 0 : row_pad(s.queries), row_pad(s.keys)) / 64;
+    // 128 rows a workgroup, while they are fewer than a launch holds
+    a.parts = std::max(1, std::min(std::min(kHeadParts, (1 << 23) / all_heads(s, jobs)), (std::max(jobs == 2 ? 0 : s.queries, s.keys) + 127) / 128));
     for (int j = 0; j < jobs; ++j) {
         const bool key = j == kK || j == kV;
         const int64_t heads = (int64_t)s.batch * (key ? s.kv_heads : s.heads);
@@ -916,9 +918,9 @@ void plan_operands(TileArgs& a, Workspace& ws, int jobs) {
 template <int DP, int L>
 void launch_operands(const TileArgs& a, hipStream_t stream) {
     const AttnShape& s = a.s;
-    const unsigned heads = (unsigned)(s.batch * (s.heads * (a.jobs - 2) + s.kv_heads * 2)); // (jobs: 2 or 4)
-    hipLaunchKernelGGL(attn_amax_kernel<L>, dim3(heads * a.parts), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(attn_split_kernel<DP>, dim3(heads * a.split_blocks), dim3(256), 0, stream, a);
+    const int64_t rows = (int64_t)s.batch * ((int64_t)s.heads * (a.jobs - 2) * row_pad(s.queries) + (int64_t)s.kv_heads * 2 * row_pad(s.keys));
+    hipLaunchKernelGGL(attn_amax_kernel<L>, dim3((unsigned)(all_heads(s, a.jobs) * a.parts)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(attn_split_kernel<DP>, dim3((unsigned)(rows / 64)), dim3(256), 0, stream, a);
 }
 
 template <int DP, int L>

@@ -201,6 +201,9 @@ ATTENTION = [  # batch, queries, keys, heads, kv_heads, dim, causal, lengths, st
     (1, 300, 300, 24, 3, 128, True, None, None),
     (3, 384, 384, 8, 8, 64, True, [384, 255, 129], None),
     (1, 100, 9000, 8, 8, 64, True, [8190], [8090]),  # few query tiles: the keys in runs
+    (8, 300, 310, 16, 8, 20, True, [310, 299, 0, 1, 64, 65, 300, 128], [10, 10, 10, -299, 0, -3, 200, 5]),
+    (3, 700, 260, 12, 4, 65, True, [260, 17, 0], None),  # the first 440 queries have no keys
+    (2, 260, 1500, 12, 4, 127, False, [1500, 700], None),
 ]
 
 
@@ -289,7 +292,7 @@ def test_keys_that_are_not_allowed_are_not_used(ops, bad, n):
 @pytest.mark.parametrize("dim", [16, 64, 96, 128])
 def test_a_row_out_of_the_ordinary_stays_with_what_sees_it(ops, where, bad, dim):
     """One row of one head that is not finite, or far larger than all others: queries before it, keys behind it and the other heads are as without it."""
-    B, n, H, at = 2, 200, 24, 120
+    B, n, H, at = 2, 200, 24 if dim > 32 else 48, 120  # enough for the kernels in tiles
     tensors = {name: randn(i, B, n, H, dim) for i, name in enumerate(("q", "k", "v", "dout"))}
     want = attention_reference(tensors["q"], tensors["k"], tensors["v"], 0.2, True, None, None, tensors["dout"])
     tensors[where][1, at, 0] = bad
@@ -349,7 +352,7 @@ def test_attention_extreme_scores(ops):
     # The magnitudes of a score's 64 products add up to 64 * 16 * 16 * 0.64 * 2 = 21000 at most; 12 roundings of 2^-24 of that are 2^-6, in the exponent and so
     # relative in p.  Nearly every p is 0 or 1, and a gradient p (dP - delta) cancels where it is 1: its error is measured against p (|dP| + |delta|).
     tol = 2.0 ** -6
-    for reps in (1, 60):  # enough heads for either kernel
+    for reps in (1, 150):  # enough heads for either kernel
         Q, K, V, DO = (up(ops, t.repeat(reps, 1, 1, 1)) for t in (q, k, v, dout))
         o, lse = ops.A.attention(Q, K, V, scale=1.0, causal=True)
         close(down(lse)[-1], want[1][0], RTOL_FRO, "lse")
@@ -377,7 +380,7 @@ def test_attention_without_keys_or_queries(ops):
     assert not down(gk).any() and not down(gv).any()
 
 
-@pytest.mark.parametrize("n", [1, 130, 2300])
+@pytest.mark.parametrize("n", [1, 130, 2300, 5000])
 def test_attention_offsets_past_32_bits(ops, n):
     """A cache whose positions lie 2^24 values apart: the last of 300 is more than 2^32 values behind the first."""
     m, D, pitch = 300, 64, 1 << 24
@@ -646,6 +649,9 @@ def call_all(ops, s):
         out += [o, lse, *ops.A.attention_backward(q, s["k"], s["v"], o, lse, q, causal=True)]
     loss = ops.V.vocabulary_loss(s["h"], s["e"].transpose(), s["b"], s["t"])
     out += [loss.per_sample, loss.lse, loss.loss_sum, *ops.V.vocabulary_loss_backward(s["h"], s["e"].transpose(), s["b"], s["t"], loss, s["one"])]
+    few = ops.NDBuffer(s["h"].storage, (40, 80))
+    loss = ops.V.vocabulary_loss(few, s["e"].transpose(), s["b"], s["t"][:40])
+    out += [loss.per_sample, loss.lse, loss.loss_sum, *ops.V.vocabulary_loss_backward(few, s["e"].transpose(), s["b"], s["t"][:40], loss, s["one"])]
     return out
 
 

@@ -70,9 +70,9 @@ def test_attention_refusals():
     refused(SHAPE, "multiple", attn_forward(k=(2, 5, 0, 16)))
     refused(UNSUPPORTED, "head size 129", attn_forward(q=(2, 3, 4, 129), k=(2, 5, 2, 129)))
     refused(UNSUPPORTED, "head size 0", attn_forward(q=(2, 3, 4, 0), k=(2, 5, 2, 0)))
-    refused(UNSUPPORTED, "2^26", attn_forward(q=(1 << 15, 1 << 15, 4, 16), k=(1 << 15, 5, 2, 16)))
+    refused(UNSUPPORTED, "2^25", attn_forward(q=(1 << 15, 1 << 15, 4, 16), k=(1 << 15, 5, 2, 16)))
     refused(UNSUPPORTED, "2^20", attn_forward(q=(1 << 19, 1, 4, 16), k=(1 << 19, 5, 2, 16)))
-    refused(UNSUPPORTED, "2^28", attn_forward(q=(1, 1, 4, 16), k=(1, 1 << 28, 2, 16)))
+    refused(UNSUPPORTED, "2^27", attn_forward(q=(1, 1, 4, 16), k=(1, 1 << 28, 2, 16)))
     refused(ARGUMENT, "scale", attn_forward(scale=float("inf")))
     refused(ARGUMENT, "null out", attn_forward(out=None))
     L = _transformer.load()

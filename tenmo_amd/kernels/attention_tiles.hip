@@ -623,14 +623,18 @@ __device__ __forceinline__ void store_gradient(const AttnOperand& g, int64_t at,
 }
 
 template <int DP>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(const TileArgs a) {
+struct Backward {
+    static constexpr int STAGES = DP <= 64 ? 3 : 2, STAGE = 2 * Tile<DP>::BYTES + 1024; // two tiles, and the rows' lse and delta
+};
+
+template <int DP>
+__device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) {
     using T = Tile<DP>;
-    constexpr int STAGES = DP <= 64 ? 3 : 2, LOADS = 2 * T::BLOCKS / 4 + 1, STAGE = 2 * T::BYTES + 1024;
-    __shared__ __align__(1024) float lds[STAGES * STAGE / 4];
+    constexpr int STAGES = Backward<DP>::STAGES, STAGE = Backward<DP>::STAGE, LOADS = 2 * T::BLOCKS / 4 + 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, D = a.s.dim;
     const int pad_q = row_pad(a.s.queries), pad_k = row_pad(a.s.keys), k_blocks = pad_k / kRowPad;
     int bh, block;
-    head_and_block(blockIdx.x, a.s.batch * a.s.heads, k_blocks, a.s.causal, false, &bh, &block);
+    head_and_block(id, a.s.batch * a.s.heads, k_blocks, a.s.causal, false, &bh, &block);
     const int b = bh / a.s.heads, h = bh % a.s.heads, hk = h / a.s.group, bk = b * a.s.kv_heads + hk;
     const int length = __builtin_amdgcn_readfirstlane(attn_length(a.s, b)), start = __builtin_amdgcn_readfirstlane(attn_start(a.s, b)), keys = used_keys(a.s, length, start);
     const int j0 = block * kRowPad + wave * 32, j = j0 + (lane & 31);
@@ -771,33 +775,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dkv_kernel(co
         }
 }
 
-// dK and dV of a key head: the parts of the query heads that share it, in order
-__global__ __launch_bounds__(256) void attn_group_kernel(const TileArgs a) {
-    const int D = a.s.dim, quads = (D + 3) / 4;
-    const AttnOperand g{blockIdx.y ? a.grad_v.p : a.grad_k.p, blockIdx.y ? a.grad_v.b : a.grad_k.b, blockIdx.y ? a.grad_v.s : a.grad_k.s,
-                        blockIdx.y ? a.grad_v.h : a.grad_k.h, blockIdx.y ? a.grad_v.d : a.grad_k.d};
-    if (!g.p) return;
-    const float* __restrict part = blockIdx.y ? a.part_v : a.part_k;
-    const int64_t all = (int64_t)a.s.batch * a.s.kv_heads * a.s.keys * quads;
-    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.x * 256) {
-        const int d = (int)(x % quads) * 4;
-        const int64_t row = x / quads, bk = row / a.s.keys, j = row - bk * a.s.keys, b = bk / a.s.kv_heads, hk = bk - b * a.s.kv_heads;
-        const float* p = part + (((b * a.s.heads + hk * a.s.group) * a.s.keys) + j) * D;
-        f32x4 sum = attn_load4<kLoadAny>(p, 1, d / 4, D);
-        for (int i = 1; i < a.s.group; ++i) sum += attn_load4<kLoadAny>(p + (int64_t)i * a.s.keys * D, 1, d / 4, D);
-        store_gradient(g, b * g.b + hk * g.h + j * g.s, d, D, sum, a.accumulate);
-    }
-}
-
 template <int DP>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(const TileArgs a) {
+__device__ __forceinline__ void tile_dq(const TileArgs& a, int id, float* lds) {
     using T = Tile<DP>;
-    constexpr int STAGES = DP <= 64 ? 3 : 2, LOADS = 2 * T::BLOCKS / 4;
-    __shared__ __align__(1024) float lds[STAGES * 2 * T::BYTES / 4];
+    constexpr int STAGES = Backward<DP>::STAGES, LOADS = 2 * T::BLOCKS / 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, D = a.s.dim;
     const int pad_q = row_pad(a.s.queries), pad_k = row_pad(a.s.keys), q_blocks = pad_q / kRowPad;
     int bh, block;
-    head_and_block(blockIdx.x, a.s.batch * a.s.heads, q_blocks, a.s.causal, true, &bh, &block);
+    head_and_block(id, a.s.batch * a.s.heads, q_blocks, a.s.causal, true, &bh, &block);
     const int b = bh / a.s.heads, h = bh % a.s.heads, bk = b * a.s.kv_heads + h / a.s.group;
     const int length = __builtin_amdgcn_readfirstlane(attn_length(a.s, b)), start = __builtin_amdgcn_readfirstlane(attn_start(a.s, b));
     const int q0 = block * kRowPad + wave * 32, i = q0 + (lane & 31);
@@ -895,6 +880,32 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_dq_kernel(con
         }
 }
 
+// Both in one launch, the blocks of keys (four products a tile) before the blocks of queries (three): neither needs the other, and the ends of the first, when the chip empties, are filled by the second.
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_backward_kernel(const TileArgs a, int key_blocks) {
+    __shared__ __align__(1024) float lds[Backward<DP>::STAGES * Backward<DP>::STAGE / 4];
+    if ((int)blockIdx.x < key_blocks) tile_dkv<DP>(a, blockIdx.x, lds);
+    else tile_dq<DP>(a, blockIdx.x - key_blocks, lds);
+}
+
+// dK and dV of a key head: the parts of the query heads that share it, in order
+__global__ __launch_bounds__(256) void attn_group_kernel(const TileArgs a) {
+    const int D = a.s.dim, quads = (D + 3) / 4;
+    const AttnOperand g{blockIdx.y ? a.grad_v.p : a.grad_k.p, blockIdx.y ? a.grad_v.b : a.grad_k.b, blockIdx.y ? a.grad_v.s : a.grad_k.s,
+                        blockIdx.y ? a.grad_v.h : a.grad_k.h, blockIdx.y ? a.grad_v.d : a.grad_k.d};
+    if (!g.p) return;
+    const float* __restrict part = blockIdx.y ? a.part_v : a.part_k;
+    const int64_t all = (int64_t)a.s.batch * a.s.kv_heads * a.s.keys * quads;
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.x * 256) {
+        const int d = (int)(x % quads) * 4;
+        const int64_t row = x / quads, bk = row / a.s.keys, j = row - bk * a.s.keys, b = bk / a.s.kv_heads, hk = bk - b * a.s.kv_heads;
+        const float* p = part + (((b * a.s.heads + hk * a.s.group) * a.s.keys) + j) * D;
+        f32x4 sum = attn_load4<kLoadAny>(p, 1, d / 4, D);
+        for (int i = 1; i < a.s.group; ++i) sum += attn_load4<kLoadAny>(p + (int64_t)i * a.s.keys * D, 1, d / 4, D);
+        store_gradient(g, b * g.b + hk * g.h + j * g.s, d, D, sum, a.accumulate);
+    }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
 
 int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
@@ -937,13 +948,12 @@ template <int DP, int L>
 void launch_backward(const TileArgs& a, hipStream_t stream) {
     launch_operands<DP, L>(a, stream);
     const AttnShape& s = a.s;
-    if (a.grad_k.p || a.grad_v.p)
-        hipLaunchKernelGGL(attn_tile_dkv_kernel<DP>, dim3((unsigned)(s.batch * s.heads * (row_pad(s.keys) / kRowPad))), dim3(256), 0, stream, a);
+    const int blocks_of_keys = a.grad_k.p || a.grad_v.p ? s.batch * s.heads * (row_pad(s.keys) / kRowPad) : 0, blocks_of_queries = a.grad_q.p ? s.batch * s.heads * (row_pad(s.queries) / kRowPad) : 0;
+    hipLaunchKernelGGL(attn_tile_backward_kernel<DP>, dim3((unsigned)(blocks_of_keys + blocks_of_queries)), dim3(256), 0, stream, a, blocks_of_keys);
     if ((a.grad_k.p || a.grad_v.p) && a.part_k) {
         const int64_t quads = (int64_t)s.batch * s.kv_heads * s.keys * ((s.dim + 3) / 4);
         hipLaunchKernelGGL(attn_group_kernel, dim3((unsigned)std::min<int64_t>((quads + 255) / 256, 4096), 2), dim3(256), 0, stream, a);
     }
-    if (a.grad_q.p) hipLaunchKernelGGL(attn_tile_dq_kernel<DP>, dim3((unsigned)(s.batch * s.heads * (row_pad(s.queries) / kRowPad))), dim3(256), 0, stream, a);
 }
 
 } // namespace

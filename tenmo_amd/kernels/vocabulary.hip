@@ -5,7 +5,7 @@
 //   dH = scale (G W^T),  dW = (scale H)^T G,  db = sum_m scale_m G
 //
 // Bound: the matrix units, 2 M V D flop forward, 6 M V D backward (the logits again, dH, dW).  All three products run as split fp16 products
-// (split_gemm.hpp); up to 64 tokens, where reading W is the bound, the kernels of vocabulary_few.hip take their place.
+// (split_gemm.hpp); for few tokens or a small W, where reading W or latency is the bound, the kernels of vocabulary_few.hip take their place.
 //   * forward: tiles of 256 words x 128 tokens; the words of a token lie in the registers of two lanes, so that a tile's maximum and sum of a token take
 //     one exchange, and 8 bytes a token and tile leave the chip instead of 1 KiB of logits.  A second launch joins the tiles of a token in a fixed order.
 //   * backward: a piece of the vocabulary at a time; the tiles of the first launch end as G in split form (|G| <= 1, so its scale is known beforehand: 2^14),
@@ -476,6 +476,18 @@ __global__ __launch_bounds__(256) void vocab_dh_kernel(const float* __restrict p
     }
 }
 
+// dW of a piece: the runs' sums [rows][cols] added in order
+__global__ __launch_bounds__(256) void vocab_dw_kernel(const float* __restrict part, int64_t runs, int64_t rows, int64_t cols, const StoreArgs s) {
+    const int64_t all = rows * cols;
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.x * 256) {
+        float sum = part[x];
+#pragma unroll 8
+        for (int64_t r = 1; r < runs; ++r) sum += part[r * all + x];
+        float* to = s.c + x / cols * s.rs + x % cols * s.cs;
+        *to = s.accumulate ? *to + sum : sum;
+    }
+}
+
 __global__ __launch_bounds__(256) void vocab_db_kernel(const float* __restrict part, int64_t parts, int64_t V, float* db, int accumulate) {
     const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (v >= V) return;
@@ -491,9 +503,10 @@ struct Plan {
     uint32_t *amax_w, *amax_hs;
     float* h_inverse;
     float2* part;
-    float *part_x, *target_logit, *part_db, *part_h;
-    int64_t piece; // words
-    int64_t runs;  // of the words of a piece, in G W^T
+    float *part_x, *target_logit, *part_db, *part_h, *part_w;
+    int64_t piece;  // words
+    int64_t runs;   // of the words of a piece, in G W^T
+    int64_t w_runs; // of the tokens, in (scale H)^T G
 };
 
 int64_t tiles_of(int64_t n, int64_t t) { return (n + t - 1) / t; }
@@ -531,6 +544,9 @@ void plan_backward(Workspace& ws, Plan& p, int64_t M, int64_t D, int64_t V, bool
     const int64_t tiles = tiles_of(M, kTileM) * tiles_of(D, kTileN);
     p.runs = std::max<int64_t>(1, std::max(p.piece / std::max<int64_t>(M, 2048), std::min(p.piece / 128, 512 / tiles)));
     p.part_h = ws.take<float>(p.runs * M * D);
+    // The same of the tokens where the weight's gradient has few tiles (128 x 300, 16384 tokens: 92 us backward, 667 with one run)
+    p.w_runs = std::max<int64_t>(1, std::min(M / 128, 512 / (tiles_of(p.piece, kTileM) * tiles_of(D, kTileN))));
+    if (p.w_runs > 1) p.part_w = ws.take<float>(p.w_runs * p.piece * D);
 }
 
 int check_sizes(int64_t M, int64_t D, int64_t V, const char* who) {
@@ -586,10 +602,11 @@ extern "C" {
 int64_t tenmo_hip_vocabulary_loss_forward_workspace_bytes(int64_t tokens, int64_t dim, int64_t vocabulary) {
     if (int rc = check_sizes(tokens, dim, vocabulary, "tenmo_hip_vocabulary_loss_forward_workspace_bytes")) return rc;
     Workspace ws(nullptr, 0);
+    if (tokens == 0) return 0;
     Plan p{};
     FewPlan few{};
-    if (tokens > kFewTokens) plan_forward(ws, p, tokens, dim, vocabulary, true);
-    else if (tokens) few_plan_forward(ws, few, VocabArgs{tokens, vocabulary, dim, nullptr, nullptr, 0, 0, 0.f});
+    if (few_for_forward(tokens, dim, vocabulary)) few_plan_forward(ws, few, VocabArgs{tokens, vocabulary, dim, nullptr, nullptr, 0, 0, 0.f});
+    else plan_forward(ws, p, tokens, dim, vocabulary, true);
     return ws.used();
 }
 
@@ -605,13 +622,13 @@ int tenmo_hip_vocabulary_loss_forward_f32(const tenmo_view* H, const tenmo_view*
     if (int rc = call.begin()) return rc;
     const hipStream_t stream = call.state.stream;
     Workspace ws(workspace, workspace_bytes);
-    if (v.M > 0 && v.M <= kFewTokens) {
+    if (v.M > 0 && few_for_forward(v.M, v.D, v.V)) {
         FewPlan p{};
         few_plan_forward(ws, p, v);
         if (int rc = ws.check(who)) return rc;
         few_forward(p, v, operand(H), operand(W), stream);
         const JoinArgs jn{v, p.part, label_smoothing > 0.f ? p.part_x : nullptr, p.target_logit, p.tiles, per_sample_loss, lse};
-        hipLaunchKernelGGL(vocab_join_kernel, dim3(1), dim3(1024), 0, stream, jn);
+        hipLaunchKernelGGL(vocab_join_kernel, dim3((unsigned)tiles_of(v.M, 64)), dim3(1024), 0, stream, jn);
     } else if (v.M > 0) {
         const bool word_rows = rows_of_words(W);
         Plan p{};
@@ -633,10 +650,11 @@ int tenmo_hip_vocabulary_loss_forward_f32(const tenmo_view* H, const tenmo_view*
 int64_t tenmo_hip_vocabulary_loss_backward_workspace_bytes(int64_t tokens, int64_t dim, int64_t vocabulary) {
     if (int rc = check_sizes(tokens, dim, vocabulary, "tenmo_hip_vocabulary_loss_backward_workspace_bytes")) return rc;
     Workspace ws(nullptr, 0);
+    if (tokens == 0) return 0;
     Plan p{};
     FewPlan few{};
-    if (tokens > kFewTokens) plan_backward(ws, p, tokens, dim, vocabulary, true);
-    else if (tokens) few_plan_backward(ws, few, VocabArgs{tokens, vocabulary, dim, nullptr, nullptr, 0, 0, 0.f});
+    if (few_for_backward(tokens, dim, vocabulary)) few_plan_backward(ws, few, VocabArgs{tokens, vocabulary, dim, nullptr, nullptr, 0, 0, 0.f});
+    else plan_backward(ws, p, tokens, dim, vocabulary, true);
     return ws.used();
 }
 
@@ -669,7 +687,7 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
     const bool word_rows = rows_of_words(W);
     Workspace ws(workspace, workspace_bytes);
     const Upstream up{upstream, (int)reduction, valid_count};
-    if (v.M > 0 && v.M <= kFewTokens) {
+    if (v.M > 0 && few_for_backward(v.M, v.D, v.V)) {
         FewPlan p{};
         few_plan_backward(ws, p, v);
         if (int rc = ws.check(who)) return rc;
@@ -717,10 +735,21 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
             }
             w_tiles = dw.tiles_m * dw.tiles_n;
         }
+        const StoreArgs to_w = sw;
+        int64_t w_runs = 1;
+        if (grad_W && p.w_runs > 1) {
+            dw.run_steps = tiles_of(dw.k_steps, p.w_runs);
+            dw.run_stride = dw.M * dw.N;
+            w_runs = tiles_of(dw.k_steps, dw.run_steps);
+            w_tiles *= w_runs;
+            sw = StoreArgs{p.part_w, dw.N, 1, 0};
+        }
         if (h_tiles + w_tiles == 0) continue;
         const dim3 grid((unsigned)(h_tiles + w_tiles));
         if (word_rows) hipLaunchKernelGGL(vocab_products_kernel<false>, grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
         else hipLaunchKernelGGL(vocab_products_kernel<true>, grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
+        if (grad_W && p.w_runs > 1)
+            hipLaunchKernelGGL(vocab_dw_kernel, dim3((unsigned)std::min<int64_t>(tiles_of(dw.run_stride, 256), 8 * call.state.cus)), dim3(256), 0, stream, p.part_w, w_runs, dw.M, dw.N, to_w);
     }
     if (grad_H && v.M > 0)
         hipLaunchKernelGGL(vocab_dh_kernel, grid_of_dh(v, call.state), dim3(256), 0, stream, p.part_h, runs, v, up, grad_H, add);

@@ -35,8 +35,9 @@ struct Operand2 { // element (r, c) of a view of rank 2
     int64_t r, c;
 };
 
-// ---- few tokens: vocabulary_few.hip ----
-constexpr int kFewTokens = 64; // up to here the fp32 matrix instruction keeps up with reading W
+// ---- few tokens, or a small W: vocabulary_few.hip ----
+bool few_for_forward(int64_t tokens, int64_t dim, int64_t words);
+bool few_for_backward(int64_t tokens, int64_t dim, int64_t words);
 struct FewPlan {
     float2* part;       // [tiles][tokens], forward
     float *part_x, *target_logit;

@@ -1,14 +1,14 @@
-// The vocabulary loss for up to 64 tokens: what bounds it is reading W (and writing dW), so it is read as it is, in fp32, by the fp32 matrix instruction.
+// The vocabulary loss for few tokens, or a small W: what bounds it is reading W (and writing dW), or latency, so W is read as it is, in fp32, by the fp32 matrix instruction.
 //
 //   forward   x = H W: a workgroup for 128 words and 32 tokens, or 64 and 64, over all of D; its maximum and sum of each token leave the chip.
 //   backward  the same product again, ending as G in fp32 [tokens, words]; dH = G W^T, the words cut into runs with a sum each;
-//             dW = (scale H)^T G, tiles of 128 x 64 whose whole reduction (the tokens) lies in LDS.
+//             dW = (scale H)^T G, tiles of 128 x 64, the tokens in blocks of 64 through LDS.
 //
-// The split form of the products (vocabulary.hip) reads W three times and writes it once before it begins, which its rate pays back from 65 tokens up.  Forward and backward
-// with W as an embedding [words, D], here against the split form:
-//       768 x 50257:  1 token 61 + 133 us against 146 + 271;  32 tokens 59 + 146 against 144 + 274;  64 tokens 88 + 203 against 146 + 284
-//      1600 x 8000:   1 token 67 + 104 us against 100 + 145;  64 tokens 51 + 104 against 101 + 154
-//       128 x 1000:   1 token 22 +  25 us against  27 +  42;  64 tokens 22 +  25 against  28 +  45
+// The split form of the products (vocabulary.hip) reads W three times and writes it once before it begins, which its rate pays back only for many tokens and a large W.  Forward and
+// backward with W as an embedding [words, D], here against the split form:
+//       768 x 50257:    1 token 61 + 133 us against 146 + 271;   64 tokens 88 + 206 against 142 + 266;   256 tokens 221 + 610 against 173 + 367
+//      1600 x 4000:    64 tokens 50 +  87 us against  91 + 128;  256 tokens 53 + 146 against  91 + 167;  512 tokens  85 + 248 against  92 + 188
+//       128 x 1000:    64 tokens 25 +  27 us against  31 +  45;  256 tokens 25 +  41 against  30 +  52;  512 tokens  25 +  61 against  30 +  54
 // One read of the first W (154 MB) takes 30 us at the rate of a copy, its backward (W twice, dW once) 92 us.
 // Both products with W have the matrix in the rows of the instruction's result and the tokens in its columns: rows r of 32 in LDS, K-major ([row][k], 32 k and 4 of padding: a
 // float4 of four k a lane, 16 rows in 16 different bank groups) where the memory runs along k, MN-major ([k][row]) where it runs along r.
@@ -99,15 +99,17 @@ __global__ __launch_bounds__(256) void few_kernel(const FewArgs a) {
     __shared__ __align__(16) float lds_a[2][A::FLOATS], lds_b[2][B::FLOATS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int row_block = TOKENS == 32 ? wave : wave & 1, token_block = TOKENS == 32 ? 0 : wave >> 1;
-    const int64_t tiles = (a.rows + ROWS - 1) / ROWS, run = MODE == kHidden ? blockIdx.x / tiles : 0;
-    const int64_t r0 = (blockIdx.x - run * tiles) * ROWS, k0 = run * a.run, k_end = MODE == kHidden && k0 + a.run < a.k ? k0 + a.run : a.k;
+    // the blocks of tokens that share a tile of W lie next to each other
+    const int64_t tiles = (a.rows + ROWS - 1) / ROWS, token_blocks = (a.v.M + TOKENS - 1) / TOKENS, id = blockIdx.x / token_blocks;
+    const int64_t t0 = (blockIdx.x - id * token_blocks) * TOKENS, run = MODE == kHidden ? id / tiles : 0, tile = id - run * tiles;
+    const int64_t r0 = tile * ROWS, k0 = run * a.run, k_end = MODE == kHidden && k0 + a.run < a.k ? k0 + a.run : a.k;
     f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
     A sa;
     B sb;
     sa.load(a.a, r0, a.rows, k0, k_end);
-    sb.load(a.b, 0, a.v.M, k0, k_end);
+    sb.load(a.b, t0, a.v.M, k0, k_end);
     int stage = 0;
     for (int64_t k = k0; k < k_end; k += KC, stage ^= 1) {
         sa.store(lds_a[stage], k, k_end);
@@ -115,7 +117,7 @@ __global__ __launch_bounds__(256) void few_kernel(const FewArgs a) {
         __syncthreads();
         if (k + KC < k_end) { // on the way while this step is multiplied; its place in LDS was read a step ago
             sa.load(a.a, r0, a.rows, k + KC, k_end);
-            sb.load(a.b, 0, a.v.M, k + KC, k_end);
+            sb.load(a.b, t0, a.v.M, k + KC, k_end);
         }
 #pragma unroll
         for (int k8 = 0; k8 < KC; k8 += 8) {
@@ -125,7 +127,7 @@ __global__ __launch_bounds__(256) void few_kernel(const FewArgs a) {
         }
     }
     // register e: row 8 (e / 4) + 4 half + e % 4 of the block, column lane % 32
-    const int64_t row0 = r0 + 32 * row_block + 4 * half, token = 32 * token_block + (lane & 31);
+    const int64_t row0 = r0 + 32 * row_block + 4 * half, token = t0 + 32 * token_block + (lane & 31);
     if (MODE == kHidden) {
         if (token >= a.v.M) return;
         float* to = a.out + (run * a.v.M + token) * a.rows;
@@ -170,15 +172,15 @@ __global__ __launch_bounds__(256) void few_kernel(const FewArgs a) {
         if (half == 0) join[0][row_block][col] = top, join[1][row_block][col] = sum, join[2][row_block][col] = sx;
         __syncthreads();
         const int t = threadIdx.x;
-        if (t < TOKENS && t < a.v.M) {
+        if (t < TOKENS && t0 + t < a.v.M) {
             float m = join[0][0][t], s = 0.f, x = 0.f;
 #pragma unroll
             for (int w = 1; w < ROWS / 32; ++w) m = fmaxf(m, join[0][w][t]);
             const float b = m == -__builtin_inff() ? 0.f : m;
 #pragma unroll
             for (int w = 0; w < ROWS / 32; ++w) s += join[1][w][t] * __expf(join[0][w][t] - b), x += join[2][w][t];
-            a.part[blockIdx.x * a.v.M + t] = make_float2(m, s);
-            if (a.part_x) a.part_x[blockIdx.x * a.v.M + t] = x;
+            a.part[tile * a.v.M + t0 + t] = make_float2(m, s);
+            if (a.part_x) a.part_x[tile * a.v.M + t0 + t] = x;
         }
         return;
     }
@@ -221,14 +223,14 @@ template <int TOKENS, int WIDTH>
 struct TokenRows {
     static constexpr int N = TOKENS * WIDTH / 1024;
     f32x4 x[N];
-    // columns behind the last are the last again (their products are not stored), and so are tokens
-    __device__ __forceinline__ void load(const Operand2& o, int64_t tokens, int64_t c0, int64_t cols) {
+    // tokens t0 ..; columns behind the last are the last again (their products are not stored), and so are tokens
+    __device__ __forceinline__ void load(const Operand2& o, int64_t t0, int64_t tokens, int64_t c0, int64_t cols) {
         const bool wide = o.c == 1 && c0 + WIDTH <= cols;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int y = threadIdx.x + 256 * i, m = y / (WIDTH / 4);
             const int64_t c = c0 + y % (WIDTH / 4) * 4;
-            const float* p = o.p + (m >= tokens ? tokens - 1 : m) * o.r;
+            const float* p = o.p + (t0 + m >= tokens ? tokens - 1 : t0 + m) * o.r;
             if (wide) x[i] = *(const f32x4_u*)(p + c);
             else
 #pragma unroll
@@ -256,27 +258,33 @@ __global__ __launch_bounds__(256) void few_weight_kernel(const FewWeight a) {
     const int64_t tiles_j = (a.cols + J - 1) / J, i0 = blockIdx.x / tiles_j * I, j0 = blockIdx.x % tiles_j * J;
     TokenRows<TOKENS, I> x;
     TokenRows<TOKENS, J> y;
-    x.load(a.x, a.v.M, i0, a.rows);
-    y.load(a.y, a.v.M, j0, a.cols);
-    if (threadIdx.x < TOKENS) { // each once: it hangs on three loads in a row
-        const bool in = threadIdx.x < a.v.M;
-        factors[0][threadIdx.x] = in ? 1.f : 0.f;
-        factors[1][threadIdx.x] = in ? row_factor(a.v, a.up, threadIdx.x) : 0.f;
-    }
-    __syncthreads();
-    x.store(&lx[0][0], factors[a.x_is_h]);
-    y.store(&ly[0][0], factors[!a.x_is_h]);
-    __syncthreads();
     f32x16 acc[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[b][e] = 0.f;
+    x.load(a.x, 0, a.v.M, i0, a.rows);
+    y.load(a.y, 0, a.v.M, j0, a.cols);
+    for (int64_t t0 = 0; t0 < a.v.M; t0 += TOKENS) {
+        if (threadIdx.x < TOKENS) { // each once: it hangs on three loads in a row
+            const int64_t m = t0 + threadIdx.x;
+            factors[0][threadIdx.x] = m < a.v.M ? 1.f : 0.f;
+            factors[1][threadIdx.x] = m < a.v.M ? row_factor(a.v, a.up, m) : 0.f;
+        }
+        __syncthreads(); // (and the block before is multiplied)
+        x.store(&lx[0][0], factors[a.x_is_h]);
+        y.store(&ly[0][0], factors[!a.x_is_h]);
+        __syncthreads();
+        if (t0 + TOKENS < a.v.M) {
+            x.load(a.x, t0 + TOKENS, a.v.M, i0, a.rows);
+            y.load(a.y, t0 + TOKENS, a.v.M, j0, a.cols);
+        }
 #pragma unroll 4
-    for (int m = 0; m < TOKENS; m += 2) {
-        const float left = lx[m + half][32 * wave + (lane & 31)];
+        for (int m = 0; m < TOKENS; m += 2) {
+            const float left = lx[m + half][32 * wave + (lane & 31)];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(left, ly[m + half][32 * b + (lane & 31)], acc[b], 0, 0, 0);
+            for (int b = 0; b < 2; ++b) acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(left, ly[m + half][32 * b + (lane & 31)], acc[b], 0, 0, 0);
+        }
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -289,20 +297,35 @@ __global__ __launch_bounds__(256) void few_weight_kernel(const FewWeight a) {
         }
 }
 
-// db: the tokens in order
-__global__ __launch_bounds__(256) void few_bias_kernel(const VocabArgs v, const Upstream up, const float* __restrict g, float* db, int accumulate) {
-    const int64_t word = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (word >= v.V) return;
+// db of 64 words: each of the 16 wavefronts takes every 16th token, then their sums are added in order
+__global__ __launch_bounds__(1024) void few_bias_kernel(const VocabArgs v, const Upstream up, const float* __restrict g, float* db, int accumulate) {
+    __shared__ float sums[16][64], factors[1024];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t word = (int64_t)blockIdx.x * 64 + lane, column = word < v.V ? word : v.V - 1;
     float s = 0.f;
-    for (int64_t m = 0; m < v.M; ++m) s += g[m * v.V + word] * row_factor(v, up, m);
+    for (int64_t m0 = 0; m0 < v.M; m0 += 1024) {
+        if (m0) __syncthreads();
+        if (m0 + threadIdx.x < v.M) factors[threadIdx.x] = row_factor(v, up, m0 + threadIdx.x);
+        __syncthreads();
+        const int many = v.M - m0 < 1024 ? (int)(v.M - m0) : 1024;
+#pragma unroll 8
+        for (int m = wave; m < many; m += 16) s += g[(m0 + m) * v.V + column] * factors[m];
+    }
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave || word >= v.V) return;
+    for (int w = 1; w < 16; ++w) s += sums[w][lane];
     db[word] = accumulate ? db[word] + s : s;
 }
 
 int64_t up_to(int64_t n, int64_t t) { return (n + t - 1) / t; }
 int64_t rows_a_tile(int64_t tokens) { return tokens <= 32 ? 128 : 64; }
 
+int64_t token_blocks(int64_t tokens) { return tokens <= 32 ? 1 : up_to(tokens, 64); }
+
 template <int MODE>
-void launch_few(const FewArgs& a, int64_t grid, hipStream_t stream) {
+void launch_few(const FewArgs& a, int64_t tiles, hipStream_t stream) {
+    const int64_t grid = tiles * token_blocks(a.v.M);
     const bool k_major = a.a.c == 1 || a.a.r != 1;
     if (a.v.M <= 32) {
         if (k_major) hipLaunchKernelGGL((few_kernel<32, MODE, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
@@ -315,6 +338,15 @@ void launch_few(const FewArgs& a, int64_t grid, hipStream_t stream) {
 
 } // namespace
 
+// By the values of W that blocks of 64 tokens read, fitted to 237 sizes (64 to 16384 tokens, 32 to 1600 dimensions, 300 to 50257 words): no choice costs more than 1.09 of the other;
+// backward each block of tokens also takes a turn in dW's sum.
+bool few_for_forward(int64_t tokens, int64_t dim, int64_t words) {
+    return tokens <= 64 || (double)token_blocks(tokens) * dim * words <= 8e6 + 20e3 * dim + 1.6 * dim * words;
+}
+bool few_for_backward(int64_t tokens, int64_t dim, int64_t words) {
+    return tokens <= 64 || token_blocks(tokens) * ((double)dim * words + 3e6) <= 20e6 + 20e3 * dim + 0.5 * dim * words;
+}
+
 void few_plan_forward(Workspace& ws, FewPlan& p, const VocabArgs& v) {
     p.tiles = up_to(v.V, rows_a_tile(v.M));
     p.part = ws.take<float2>(p.tiles * v.M);
@@ -325,7 +357,7 @@ void few_plan_forward(Workspace& ws, FewPlan& p, const VocabArgs& v) {
 void few_plan_backward(Workspace& ws, FewPlan& p, const VocabArgs& v) {
     p.g = ws.take<float>(v.M * v.V);
     // four workgroups a CU, of at least 64 words each
-    p.run = up_to(up_to(v.V, std::max<int64_t>(1, std::min(1024 / up_to(v.D, rows_a_tile(v.M)), v.V / 64))), KC) * KC;
+    p.run = up_to(up_to(v.V, std::max<int64_t>(1, std::min(1024 / (up_to(v.D, rows_a_tile(v.M)) * token_blocks(v.M)), v.V / 64))), KC) * KC;
     p.runs = up_to(v.V, p.run);
     p.part_h = ws.take<float>(p.runs * v.M * v.D);
 }
@@ -361,7 +393,7 @@ void few_backward(const FewPlan& p, const VocabArgs& v, const Operand2& h, const
         if (v.M <= 32) hipLaunchKernelGGL(few_weight_kernel<32>, grid, dim3(256), 0, stream, f);
         else hipLaunchKernelGGL(few_weight_kernel<64>, grid, dim3(256), 0, stream, f);
     }
-    if (grad_bias) hipLaunchKernelGGL(few_bias_kernel, dim3((unsigned)up_to(v.V, 256)), dim3(256), 0, stream, v, up, p.g, grad_bias, accumulate);
+    if (grad_bias) hipLaunchKernelGGL(few_bias_kernel, dim3((unsigned)up_to(v.V, 64)), dim3(1024), 0, stream, v, up, p.g, grad_bias, accumulate);
 }
 
 } // namespace tenmo

@@ -432,6 +432,13 @@ VOCABULARY = [  # tokens, dim, vocabulary, weight, bias, reduction, smoothing, i
     (300, 130, 2049, "strided", True, "mean", 0.1, True),
     (77, 769, 1500, "tied", True, "mean", 1.0, True),
     (513, 48, 5003, "dense", False, "none", 0.0, True),
+    (1900, 65, 12001, "tied", True, "mean", 0.1, False),
+    (2500, 100, 8003, "dense", True, "sum", 0.1, True),
+    (4100, 33, 9000, "strided", True, "none", 0.0, True),
+    (2000, 769, 1501, "tied", False, "mean", 1.0, True),
+    (3000, 40, 130, "tied", True, "none", 0.1, True),     # few tiles of the weight's gradient: the tokens in runs
+    (3001, 150, 300, "strided", False, "mean", 0.0, True),
+    (1500, 130, 1500, "dense", True, "mean", 0.0, True),  # forward and backward by different kernels
 ]
 
 
@@ -515,12 +522,12 @@ def test_vocabulary_loss_targets(ops):
     assert np.isnan(each[[3, 7]]).all() and not each[[11, 12]].any() and np.isfinite(np.delete(each, [3, 7])).all() and int(loss.valid_count.item()) == 18
 
 
-@pytest.mark.parametrize("m", [12, 50, 150])
+@pytest.mark.parametrize("m, v", [(12, 700), (50, 700), (150, 700), (2100, 9000)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, 1.0e30])
-def test_vocabulary_loss_rows_that_do_not_count(ops, bad, m):
+def test_vocabulary_loss_rows_that_do_not_count(ops, bad, m, v):
     """Whatever the hidden state of an ignored token holds, the others' losses and all gradients are as without it; and a row far larger than the others
     takes nothing from their losses."""
-    d, v = 48, 700
+    d = 48
     h, w, b = randn(1, m, d), randn(2, v, d) * 0.2, randn(3, v)
     target = torch.arange(m)
     target[[3, m - 1]] = -100
@@ -539,14 +546,14 @@ def test_vocabulary_loss_rows_that_do_not_count(ops, bad, m):
         assert np.abs(down(loss.per_sample).numpy() - want[0])[keep].max() <= 2 * RTOL_FRO * np.abs(want[1]).max()
 
 
-@pytest.mark.parametrize("m", [20, 40, 100])
-def test_vocabulary_loss_words_shut_out_by_the_bias(ops, m):
+@pytest.mark.parametrize("m, v", [(20, 700), (40, 700), (100, 700), (2300, 12000)])
+def test_vocabulary_loss_words_shut_out_by_the_bias(ops, m, v):
     """A bias of -inf gives a word no probability, and of its type's lowest value next to none; all but one: the loss of that one is zero."""
-    d, v = 32, 700
+    d = 32
     h, w, b = randn(1, m, d), randn(2, d, v), randn(3, v)
     b[600:] = -math.inf
     b[300:400] = torch.finfo(torch.float32).min
-    target = torch.arange(m)
+    target = torch.arange(m) % 300
     want = vocabulary_reference(h, w, b, target, -100, 0.0, "sum", torch.ones(1))
     H, W, B, T, one = up(ops, h), up(ops, w), up(ops, b), target.cuda(), torch.ones(1, device="cuda")
     loss = ops.V.vocabulary_loss(H, W, B, T)
@@ -558,11 +565,11 @@ def test_vocabulary_loss_words_shut_out_by_the_bias(ops, m):
     assert np.abs(down(loss.per_sample).numpy()).max() <= RTOL_FRO * 10
 
 
-@pytest.mark.parametrize("m", [50, 100])
+@pytest.mark.parametrize("m, v", [(50, 600), (100, 600), (1700, 9000)])
 @pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -30, 2.0 ** 60])
-def test_vocabulary_loss_scales(ops, scale, m):
+def test_vocabulary_loss_scales(ops, scale, m, v):
     """Hidden states and weights far from one whose products are ordinary: the halves are scaled by the largest value."""
-    d, v = 64, 600
+    d = 64
     h, w, target = randn(1, m, d) * scale, randn(2, d, v) * 0.2 / scale, torch.arange(m)
     want = vocabulary_reference(h, w, None, target, -100, 0.0, "sum", torch.ones(1))
     H, W, T, one = up(ops, h), up(ops, w), target.cuda(), torch.ones(1, device="cuda")
@@ -657,8 +664,8 @@ def call_all(ops, s):
 
 def state_of(ops, seed):
     s = {n: up(ops, randn(seed + i, *shape)) for i, (n, shape) in enumerate((("x", (70, 96)), ("w", (96,)), ("q", (2, 400, 8, 64)), ("k", (2, 400, 2, 64)), ("v", (2, 400, 2, 64)),
-                                                                             ("q1", (2, 1, 8, 64)), ("h", (200, 80)), ("e", (900, 80)), ("b", (900,))))}
-    s["t"] = torch.randint(0, 900, (200,), generator=torch.Generator().manual_seed(seed)).cuda()
+                                                                             ("q1", (2, 1, 8, 64)), ("h", (1700, 80)), ("e", (9000, 80)), ("b", (9000,))))}
+    s["t"] = torch.randint(0, 9000, (1700,), generator=torch.Generator().manual_seed(seed)).cuda()
     s["one"] = torch.ones(1, device="cuda")
     return s
 

@@ -69,7 +69,8 @@ bool forward_by_rows(const AttnShape& s) {
 // other, and 1 % in the mean; [1, 8 x 64]: 128 queries and keys take 23 us by rows and 31 by tiles, 512 of both 114 and 49.
 bool backward_by_rows(const AttnShape& s) {
     const double operands = 2.0 * s.batch * padded(s.dim) * ((double)s.heads * s.queries + (double)s.kv_heads * s.keys);
-    return s.queries <= 1024 && s.keys <= 1024 && pair_values(s) + 600.0 * padded(s.dim) * s.keys <= 40e6 + 4.0 * operands;
+    const bool fits = (int64_t)s.batch * s.kv_heads * s.keys < 1 << 24; // a launch: half as many workgroups at the most
+    return fits && s.queries <= 1024 && s.keys <= 1024 && pair_values(s) + 600.0 * padded(s.dim) * s.keys <= 40e6 + 4.0 * operands;
 }
 
 void forward_plan(const AttnShape& s, const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, float* out, float* lse, Workspace& ws, const LibraryState& lib, bool launch) {
@@ -78,8 +79,8 @@ void forward_plan(const AttnShape& s, const AttnOperand& q, const AttnOperand& k
 }
 
 void backward_plan(const AttnBackward& b, Workspace& ws, const LibraryState& lib, bool launch) {
-    if (backward_by_rows(b.s)) attn_rows_backward(b, ws, lib.stream, launch);
-    else attn_tiles_backward(b, ws, lib.stream, launch);
+    if (!backward_by_rows(b.s)) attn_tiles_backward(b, ws, lib.stream, launch);
+    else if (launch) attn_rows_backward(b, lib.stream);
 }
 
 } // namespace

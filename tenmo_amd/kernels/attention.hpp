@@ -92,7 +92,7 @@ struct AttnBackward {
 void attn_rows_forward(const AttnShape&, const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, float* out, float* lse,
                        Workspace& ws, int cus, hipStream_t stream, bool launch);
 
-void attn_rows_backward(const AttnBackward&, Workspace& ws, hipStream_t stream, bool launch);
+void attn_rows_backward(const AttnBackward&, hipStream_t stream); // needs no workspace
 constexpr int kMostRuns = 1024;
 // joins `splits` runs of keys: part [splits][batch][heads][queries][dim + 2] holds each run's sum of p v, its maximum and its sum of p
 void attn_join(const AttnShape&, const float* part, int splits, float* out, float* lse, hipStream_t stream);

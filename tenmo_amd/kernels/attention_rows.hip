@@ -192,12 +192,13 @@ void launch_rows(const RowsArgs& a, int r, unsigned grid, hipStream_t stream) {
     else launch_rows<L, 8>(a, grid, stream);
 }
 
-// Backward.  Rows: s and dP = dout . v again for each allowed key, p = exp(s - lse), dS = p (dP - delta) with delta = dout . out; dq = scale sum_j dS k_j.
-// Two launches, of rows and of keys; what bounds them at the sizes they are taken for is latency.
+// Backward: s and dP = dout . v again for each allowed pair, p = exp(s - lse), dS = p (dP - delta) with delta = dout . out; dq = scale sum_j dS k_j over a row's keys,
+// dv_j = sum_i p_ij dout_i and dk_j = scale sum_i dS_ij q_i over the queries of the heads that share a key's.  What bounds it at the sizes it is taken for is latency, so both are one launch: the
+// blocks of keys work delta out of out again (a call of [2,33,4,32]: 17.7 us, 21.9 in two launches; [1,128,8,128]: 19.2, 28.4).
 struct RowsBackward {
     AttnBackward b;
-    float* delta; // [batch][heads][queries], written by the rows' launch, read by the keys'
-    int row_blocks, key_blocks;
+    int key_blocks;  // of a key head
+    int key_groups;  // workgroups of keys, before those of rows
 };
 
 __device__ __forceinline__ void add_to(const AttnOperand& g, int64_t at, int part, int D, f32x4 x, int accumulate) {
@@ -210,11 +211,11 @@ __device__ __forceinline__ void add_to(const AttnOperand& g, int64_t at, int par
 }
 
 template <int L, int KIND>
-__global__ __launch_bounds__(256) void attn_rows_dq_kernel(const RowsBackward a) { // a wavefront a row
+__device__ __forceinline__ void rows_dq(const RowsBackward& a, int id) { // a wavefront a row
     constexpr int SLOTS = 64 / L, U = 2;
     const AttnShape& s = a.b.s;
     const int lane = threadIdx.x & 63, slot = lane / L, part = lane % L, D = s.dim;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t row = (int64_t)id * 4 + (threadIdx.x >> 6);
     if (row >= (int64_t)s.batch * s.heads * s.queries) return;
     const int i = (int)(row % s.queries), h = (int)(row / s.queries % s.heads), b = (int)(row / s.queries / s.heads), hk = h / s.group;
     const int limit = attn_limit(attn_length(s, b), attn_start(s, b), i);
@@ -222,8 +223,6 @@ __global__ __launch_bounds__(256) void attn_rows_dq_kernel(const RowsBackward a)
     const f32x4 q = attn_load4<KIND>(a.b.q.p + b * a.b.q.b + i * a.b.q.s + h * a.b.q.h, a.b.q.d, part, D) * s.scale;
     const f32x4 g = attn_load4<KIND>(a.b.dout + dense, 1, part, D), o = attn_load4<KIND>(a.b.out + dense, 1, part, D);
     const float delta = lanes_sum<L>(dot4(g, o)), lse = a.b.lse[row];
-    if (lane == 0) a.delta[row] = delta;
-    if (!a.b.grad_q.p) return;
     const float* kp = a.b.k.p + b * a.b.k.b + hk * a.b.k.h;
     const float* vp = a.b.v.p + b * a.b.v.b + hk * a.b.v.h;
     f32x4 acc{0.f, 0.f, 0.f, 0.f};
@@ -248,14 +247,14 @@ __global__ __launch_bounds__(256) void attn_rows_dq_kernel(const RowsBackward a)
     if (slot == 0) add_to(a.b.grad_q, b * a.b.grad_q.b + i * a.b.grad_q.s + h * a.b.grad_q.h, part, D, acc * s.scale, a.b.accumulate);
 }
 
-// dv_j = sum_i p_ij dout_i, dk_j = scale sum_i dS_ij q_i over the queries of the heads that share the key's: a slot a key, the queries dealt to the 4 wavefronts.
+// a slot a key, the queries dealt to the 4 wavefronts, four of each at a time
 template <int L, int KIND>
-__global__ __launch_bounds__(256) void attn_rows_dkv_kernel(const RowsBackward a) {
+__device__ __forceinline__ void rows_dkv(const RowsBackward& a, int id) {
     constexpr int SLOTS = 64 / L, U = 4;
     __shared__ f32x4 join[2][4][SLOTS][L];
     const AttnShape& s = a.b.s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slot = lane / L, part = lane % L, D = s.dim;
-    int rest = blockIdx.x;
+    int rest = id;
     const int j = rest % a.key_blocks * SLOTS + slot; rest /= a.key_blocks;
     const int hk = rest % s.kv_heads, b = rest / s.kv_heads;
     const int length = attn_length(s, b), start = attn_start(s, b);
@@ -267,25 +266,26 @@ __global__ __launch_bounds__(256) void attn_rows_dkv_kernel(const RowsBackward a
     const int first = j - slot < length ? (j - slot > start ? j - slot - start : 0) : s.queries;
     for (int h = hk * s.group; h < (hk + 1) * s.group; ++h)
         for (int i0 = first + wave; i0 < s.queries; i0 += 4 * U) {
-            f32x4 q[U], g[U];
-            float lse[U], delta[U];
+            f32x4 q[U], g[U], o[U];
+            float lse[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) { // (the last query again where there is none)
                 const int i = i0 + 4 * u < s.queries ? i0 + 4 * u : s.queries - 1;
                 const int64_t row = ((int64_t)b * s.heads + h) * s.queries + i;
                 q[u] = attn_load4<KIND>(a.b.q.p + b * a.b.q.b + i * a.b.q.s + h * a.b.q.h, a.b.q.d, part, D);
-                g[u] = attn_load4<KIND>(a.b.dout + (((int64_t)b * s.queries + i) * s.heads + h) * D, 1, part, D);
+                const int64_t dense = (((int64_t)b * s.queries + i) * s.heads + h) * D;
+                g[u] = attn_load4<KIND>(a.b.dout + dense, 1, part, D);
+                o[u] = attn_load4<KIND>(a.b.out + dense, 1, part, D);
                 lse[u] = a.b.lse[row];
-                delta[u] = a.delta[row];
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int i = i0 + 4 * u;
-                const float x = lanes_sum<L>(dot4(q[u], k)) * s.scale, dp = lanes_sum<L>(dot4(g[u], v));
+                const float x = lanes_sum<L>(dot4(q[u], k)) * s.scale, dp = lanes_sum<L>(dot4(g[u], v)), delta = lanes_sum<L>(dot4(g[u], o[u]));
                 if (i >= s.queries || j >= attn_limit(length, start, i)) continue; // its row may hold anything
                 const float p = __expf(x - lse[u]);
                 dv += p * g[u];
-                dk += p * (dp - delta[u]) * q[u];
+                dk += p * (dp - delta) * q[u];
             }
         }
     join[0][wave][slot][part] = dk;
@@ -299,32 +299,32 @@ __global__ __launch_bounds__(256) void attn_rows_dkv_kernel(const RowsBackward a
 }
 
 template <int L, int KIND>
-void launch_rows_backward(const RowsBackward& a, unsigned row_grid, unsigned key_grid, hipStream_t stream) {
-    hipLaunchKernelGGL((attn_rows_dq_kernel<L, KIND>), dim3(row_grid), dim3(256), 0, stream, a);
-    if (a.b.grad_k.p || a.b.grad_v.p) hipLaunchKernelGGL((attn_rows_dkv_kernel<L, KIND>), dim3(key_grid), dim3(256), 0, stream, a);
+__global__ __launch_bounds__(256) void attn_rows_backward_kernel(const RowsBackward a) {
+    if ((int)blockIdx.x < a.key_groups) rows_dkv<L, KIND>(a, blockIdx.x);
+    else rows_dq<L, KIND>(a, blockIdx.x - a.key_groups);
 }
+
 template <int L>
-void launch_rows_backward(const RowsBackward& a, unsigned row_grid, unsigned key_grid, hipStream_t stream) {
+void launch_rows_backward(const RowsBackward& a, unsigned grid, hipStream_t stream) {
     const int kind = kind_of(a.b.q, a.b.k, a.b.v, a.b.s.dim);
-    if (kind == kLoadWhole) launch_rows_backward<L, kLoadWhole>(a, row_grid, key_grid, stream);
-    else if (kind == kLoadTail) launch_rows_backward<L, kLoadTail>(a, row_grid, key_grid, stream);
-    else launch_rows_backward<L, kLoadAny>(a, row_grid, key_grid, stream);
+    if (kind == kLoadWhole) hipLaunchKernelGGL((attn_rows_backward_kernel<L, kLoadWhole>), dim3(grid), dim3(256), 0, stream, a);
+    else if (kind == kLoadTail) hipLaunchKernelGGL((attn_rows_backward_kernel<L, kLoadTail>), dim3(grid), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attn_rows_backward_kernel<L, kLoadAny>), dim3(grid), dim3(256), 0, stream, a);
 }
 
 } // namespace
 
-void attn_rows_backward(const AttnBackward& b, Workspace& ws, hipStream_t stream, bool launch) {
+void attn_rows_backward(const AttnBackward& b, hipStream_t stream) {
     RowsBackward a{};
     a.b = b;
-    const int64_t rows = (int64_t)b.s.batch * b.s.heads * b.s.queries;
-    a.delta = ws.take<float>(rows);
-    if (!launch) return;
     const int slots = b.s.dim <= 32 ? 8 : b.s.dim <= 64 ? 4 : 2;
     a.key_blocks = (b.s.keys + slots - 1) / slots;
-    const unsigned row_grid = (unsigned)((rows + 3) / 4), key_grid = (unsigned)((int64_t)b.s.batch * b.s.kv_heads * a.key_blocks);
-    if (b.s.dim <= 32) launch_rows_backward<8>(a, row_grid, key_grid, stream);
-    else if (b.s.dim <= 64) launch_rows_backward<16>(a, row_grid, key_grid, stream);
-    else launch_rows_backward<32>(a, row_grid, key_grid, stream);
+    a.key_groups = b.grad_k.p || b.grad_v.p ? b.s.batch * b.s.kv_heads * a.key_blocks : 0;
+    const int row_groups = b.grad_q.p ? (int)(((int64_t)b.s.batch * b.s.heads * b.s.queries + 3) / 4) : 0;
+    const unsigned grid = (unsigned)(a.key_groups + row_groups);
+    if (b.s.dim <= 32) launch_rows_backward<8>(a, grid, stream);
+    else if (b.s.dim <= 64) launch_rows_backward<16>(a, grid, stream);
+    else launch_rows_backward<32>(a, grid, stream);
 }
 
 void attn_rows_forward(const AttnShape& s, const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, float* out, float* lse,

@@ -393,6 +393,8 @@ struct JoinArgs {
     const float *part_x, *target_logit;
     int64_t tiles;
     float *loss, *lse;
+    float* loss_sum; // with one workgroup: the sum of the losses as well, and the tokens that count
+    int32_t* valid_count;
 };
 
 // 64 tokens a workgroup, the tiles of each dealt to the 16 wavefronts
@@ -412,23 +414,33 @@ __global__ __launch_bounds__(1024) void vocab_join_kernel(const JoinArgs a) {
     }
     s[0][wave][lane] = top; s[1][wave][lane] = sum; s[2][wave][lane] = sx;
     __syncthreads();
-    if (wave || token >= M) return;
-    for (int w = 1; w < 16; ++w) top = fmaxf(top, s[0][w][lane]);
-    const float base = top == -__builtin_inff() ? 0.f : top;
-    sum = sx = 0.f;
-    for (int w = 0; w < 16; ++w) sum += s[1][w][lane] * __expf(s[0][w][lane] - base), sx += s[2][w][lane];
-    const float lse = base + logf(sum);
-    a.lse[token] = lse;
-    const int64_t t = target_of(a.v, token);
+    if (wave) return;
     float loss = 0.f;
-    if (t != a.v.ignore) {
-        if (t < 0 || t >= a.v.V) loss = __builtin_nanf("");
-        else {
-            loss = lse - a.target_logit[token];
-            if (a.v.ls > 0.f) loss = (1.f - a.v.ls) * loss + a.v.ls * (lse - sx / (float)a.v.V);
+    bool counts = false;
+    if (token < M) {
+        for (int w = 1; w < 16; ++w) top = fmaxf(top, s[0][w][lane]);
+        const float base = top == -__builtin_inff() ? 0.f : top;
+        sum = sx = 0.f;
+        for (int w = 0; w < 16; ++w) sum += s[1][w][lane] * __expf(s[0][w][lane] - base), sx += s[2][w][lane];
+        const float lse = base + logf(sum);
+        a.lse[token] = lse;
+        const int64_t t = target_of(a.v, token);
+        counts = t != a.v.ignore;
+        if (counts) {
+            if (t < 0 || t >= a.v.V) loss = __builtin_nanf("");
+            else {
+                loss = lse - a.target_logit[token];
+                if (a.v.ls > 0.f) loss = (1.f - a.v.ls) * loss + a.v.ls * (lse - sx / (float)a.v.V);
+            }
         }
+        a.loss[token] = loss;
     }
-    a.loss[token] = loss;
+    if (!a.loss_sum) return;
+    double total = loss;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d, 64);
+    const int many = __popcll(__ballot(counts));
+    if (lane == 0) *a.loss_sum = (float)total, *a.valid_count = many;
 }
 
 // The sum of the rows' losses (in 64 bits, a fixed order) and the number of rows that count: one workgroup.
@@ -627,7 +639,7 @@ int tenmo_hip_vocabulary_loss_forward_f32(const tenmo_view* H, const tenmo_view*
         few_plan_forward(ws, p, v);
         if (int rc = ws.check(who)) return rc;
         few_forward(p, v, operand(H), operand(W), stream);
-        const JoinArgs jn{v, p.part, label_smoothing > 0.f ? p.part_x : nullptr, p.target_logit, p.tiles, per_sample_loss, lse};
+        const JoinArgs jn{v, p.part, label_smoothing > 0.f ? p.part_x : nullptr, p.target_logit, p.tiles, per_sample_loss, lse, v.M <= 64 ? loss_sum : nullptr, valid_count};
         hipLaunchKernelGGL(vocab_join_kernel, dim3((unsigned)tiles_of(v.M, 64)), dim3(1024), 0, stream, jn);
     } else if (v.M > 0) {
         const bool word_rows = rows_of_words(W);
@@ -640,10 +652,10 @@ int tenmo_hip_vocabulary_loss_forward_f32(const tenmo_view* H, const tenmo_view*
         a.v = v; a.words = v.V; a.h_inverse = p.h_inverse; a.part = p.part; a.part_x = label_smoothing > 0.f ? p.part_x : nullptr; a.target_logit = p.target_logit;
         if (word_rows) hipLaunchKernelGGL((vocab_logits_kernel<true, false>), grid_of(g), dim3(256), 0, stream, g, a);
         else hipLaunchKernelGGL((vocab_logits_kernel<false, false>), grid_of(g), dim3(256), 0, stream, g, a);
-        const JoinArgs jn{v, p.part, a.part_x, p.target_logit, g.tiles_m, per_sample_loss, lse};
+        const JoinArgs jn{v, p.part, a.part_x, p.target_logit, g.tiles_m, per_sample_loss, lse, v.M <= 64 ? loss_sum : nullptr, valid_count};
         hipLaunchKernelGGL(vocab_join_kernel, dim3((unsigned)tiles_of(v.M, 64)), dim3(1024), 0, stream, jn);
     }
-    hipLaunchKernelGGL(vocab_total_kernel, dim3(1), dim3(1024), 0, stream, v, per_sample_loss, loss_sum, valid_count);
+    if (v.M == 0 || v.M > 64) hipLaunchKernelGGL(vocab_total_kernel, dim3(1), dim3(1024), 0, stream, v, per_sample_loss, loss_sum, valid_count);
     return call.finish(sync);
 }
 

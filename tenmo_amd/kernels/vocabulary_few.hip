@@ -6,9 +6,9 @@
 //
 // The split form of the products (vocabulary.hip) reads W three times and writes it once before it begins, which its rate pays back only for many tokens and a large W.  Forward and
 // backward with W as an embedding [words, D], here against the split form:
-//       768 x 50257:    1 token 61 + 133 us against 146 + 271;   64 tokens 88 + 206 against 142 + 266;   256 tokens 221 + 610 against 173 + 367
+//       768 x 50257:    1 token 57 + 131 us against 146 + 271;   64 tokens 84 + 193 against 142 + 266;   256 tokens 221 + 610 against 173 + 367
 //      1600 x 4000:    64 tokens 50 +  87 us against  91 + 128;  256 tokens 53 + 146 against  91 + 167;  512 tokens  85 + 248 against  92 + 188
-//       128 x 1000:    64 tokens 25 +  27 us against  31 +  45;  256 tokens 25 +  41 against  30 +  52;  512 tokens  25 +  61 against  30 +  54
+//       128 x 1000:    64 tokens 20 +  23 us against  31 +  45;  256 tokens 25 +  41 against  30 +  52;  512 tokens  25 +  61 against  30 +  54
 // One read of the first W (154 MB) takes 30 us at the rate of a copy, its backward (W twice, dW once) 92 us.
 // Both products with W have the matrix in the rows of the instruction's result and the tokens in its columns: rows r of 32 in LDS, K-major ([row][k], 32 k and 4 of padding: a
 // float4 of four k a lane, 16 rows in 16 different bank groups) where the memory runs along k, MN-major ([k][row]) where it runs along r.
@@ -91,17 +91,25 @@ struct Staged {
     }
 };
 
-template <int TOKENS, int MODE, bool A_KMAJOR>
-__global__ __launch_bounds__(256) void few_kernel(const FewArgs a) {
-    constexpr int ROWS = TOKENS == 32 ? 128 : 64;
+template <int TOKENS, bool A_KMAJOR>
+struct FewTile {
+    static constexpr int ROWS = TOKENS == 32 ? 128 : 64;
     using A = Staged<ROWS, A_KMAJOR>;
     using B = Staged<TOKENS, true>;
-    __shared__ __align__(16) float lds_a[2][A::FLOATS], lds_b[2][B::FLOATS];
+    static constexpr int FLOATS = 2 * (A::FLOATS + B::FLOATS);
+};
+
+template <int TOKENS, int MODE, bool A_KMAJOR>
+__device__ __forceinline__ void few_product(const FewArgs& a, int64_t group, float* lds) {
+    using Tile = FewTile<TOKENS, A_KMAJOR>;
+    constexpr int ROWS = Tile::ROWS;
+    using A = typename Tile::A;
+    using B = typename Tile::B;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int row_block = TOKENS == 32 ? wave : wave & 1, token_block = TOKENS == 32 ? 0 : wave >> 1;
     // the blocks of tokens that share a tile of W lie next to each other
-    const int64_t tiles = (a.rows + ROWS - 1) / ROWS, token_blocks = (a.v.M + TOKENS - 1) / TOKENS, id = blockIdx.x / token_blocks;
-    const int64_t t0 = (blockIdx.x - id * token_blocks) * TOKENS, run = MODE == kHidden ? id / tiles : 0, tile = id - run * tiles;
+    const int64_t tiles = (a.rows + ROWS - 1) / ROWS, token_blocks = (a.v.M + TOKENS - 1) / TOKENS, id = group / token_blocks;
+    const int64_t t0 = (group - id * token_blocks) * TOKENS, run = MODE == kHidden ? id / tiles : 0, tile = id - run * tiles;
     const int64_t r0 = tile * ROWS, k0 = run * a.run, k_end = MODE == kHidden && k0 + a.run < a.k ? k0 + a.run : a.k;
     f32x16 acc;
 #pragma unroll
@@ -112,8 +120,9 @@ __global__ __launch_bounds__(256) void few_kernel(const FewArgs a) {
     sb.load(a.b, t0, a.v.M, k0, k_end);
     int stage = 0;
     for (int64_t k = k0; k < k_end; k += KC, stage ^= 1) {
-        sa.store(lds_a[stage], k, k_end);
-        sb.store(lds_b[stage], k, k_end);
+        float *const lds_a = lds + stage * A::FLOATS, *const lds_b = lds + 2 * A::FLOATS + stage * B::FLOATS;
+        sa.store(lds_a, k, k_end);
+        sb.store(lds_b, k, k_end);
         __syncthreads();
         if (k + KC < k_end) { // on the way while this step is multiplied; its place in LDS was read a step ago
             sa.load(a.a, r0, a.rows, k + KC, k_end);
@@ -121,7 +130,7 @@ __global__ __launch_bounds__(256) void few_kernel(const FewArgs a) {
         }
 #pragma unroll
         for (int k8 = 0; k8 < KC; k8 += 8) {
-            const f32x4 x = A::read(lds_a[stage], 32 * row_block + (lane & 31), k8, half), y = B::read(lds_b[stage], 32 * token_block + (lane & 31), k8, half);
+            const f32x4 x = A::read(lds_a, 32 * row_block + (lane & 31), k8, half), y = B::read(lds_b, 32 * token_block + (lane & 31), k8, half);
 #pragma unroll
             for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[s], y[s], acc, 0, 0, 0);
         }
@@ -206,6 +215,12 @@ __global__ __launch_bounds__(256) void few_kernel(const FewArgs a) {
     }
 }
 
+template <int TOKENS, int MODE, bool A_KMAJOR>
+__global__ __launch_bounds__(256) void few_kernel(const FewArgs a) {
+    __shared__ __align__(16) float lds[FewTile<TOKENS, A_KMAJOR>::FLOATS];
+    few_product<TOKENS, MODE, A_KMAJOR>(a, blockIdx.x, lds);
+}
+
 // dW: rows i of the result (words, or D) by columns j, the one with unit stride; X [tokens][i] and Y [tokens][j] in LDS whole
 struct FewWeight {
     VocabArgs v;
@@ -250,12 +265,16 @@ struct TokenRows {
     }
 };
 
+constexpr int kWeightI = 128, kWeightJ = 64;
 template <int TOKENS>
-__global__ __launch_bounds__(256) void few_weight_kernel(const FewWeight a) {
-    constexpr int I = 128, J = 64;
-    __shared__ __align__(16) float lx[TOKENS][I + 4], ly[TOKENS][J + 4], factors[2][TOKENS]; // of G: one for every token
+constexpr int kWeightFloats = TOKENS * (kWeightI + 4 + kWeightJ + 4 + 2);
+
+template <int TOKENS>
+__device__ __forceinline__ void few_weight(const FewWeight& a, int64_t id, float* lds) {
+    constexpr int I = kWeightI, J = kWeightJ;
+    float *const lx = lds, *const ly = lds + TOKENS * (I + 4), *const factors = ly + TOKENS * (J + 4); // [0 ..] of G: one for every token; [TOKENS ..] of H
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const int64_t tiles_j = (a.cols + J - 1) / J, i0 = blockIdx.x / tiles_j * I, j0 = blockIdx.x % tiles_j * J;
+    const int64_t tiles_j = (a.cols + J - 1) / J, i0 = id / tiles_j * I, j0 = id % tiles_j * J;
     TokenRows<TOKENS, I> x;
     TokenRows<TOKENS, J> y;
     f32x16 acc[2];
@@ -268,12 +287,12 @@ __global__ __launch_bounds__(256) void few_weight_kernel(const FewWeight a) {
     for (int64_t t0 = 0; t0 < a.v.M; t0 += TOKENS) {
         if (threadIdx.x < TOKENS) { // each once: it hangs on three loads in a row
             const int64_t m = t0 + threadIdx.x;
-            factors[0][threadIdx.x] = m < a.v.M ? 1.f : 0.f;
-            factors[1][threadIdx.x] = m < a.v.M ? row_factor(a.v, a.up, m) : 0.f;
+            factors[threadIdx.x] = m < a.v.M ? 1.f : 0.f;
+            factors[TOKENS + threadIdx.x] = m < a.v.M ? row_factor(a.v, a.up, m) : 0.f;
         }
         __syncthreads(); // (and the block before is multiplied)
-        x.store(&lx[0][0], factors[a.x_is_h]);
-        y.store(&ly[0][0], factors[!a.x_is_h]);
+        x.store(lx, factors + (a.x_is_h ? TOKENS : 0));
+        y.store(ly, factors + (a.x_is_h ? 0 : TOKENS));
         __syncthreads();
         if (t0 + TOKENS < a.v.M) {
             x.load(a.x, t0 + TOKENS, a.v.M, i0, a.rows);
@@ -281,9 +300,9 @@ __global__ __launch_bounds__(256) void few_weight_kernel(const FewWeight a) {
         }
 #pragma unroll 4
         for (int m = 0; m < TOKENS; m += 2) {
-            const float left = lx[m + half][32 * wave + (lane & 31)];
+            const float left = lx[(m + half) * (I + 4) + 32 * wave + (lane & 31)];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(left, ly[m + half][32 * b + (lane & 31)], acc[b], 0, 0, 0);
+            for (int b = 0; b < 2; ++b) acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(left, ly[(m + half) * (J + 4) + 32 * b + (lane & 31)], acc[b], 0, 0, 0);
         }
     }
 #pragma unroll
@@ -295,6 +314,15 @@ __global__ __launch_bounds__(256) void few_weight_kernel(const FewWeight a) {
             float* to = a.out + i * a.rs + j * a.cs;
             *to = a.accumulate ? *to + acc[b][e] : acc[b][e];
         }
+}
+
+// dH's runs (the first workgroups) and dW in one launch: neither needs the other
+template <int TOKENS, bool A_KMAJOR>
+__global__ __launch_bounds__(256) void few_gradients_kernel(const FewArgs h, uint32_t h_groups, const FewWeight w) {
+    constexpr int FLOATS = FewTile<TOKENS, A_KMAJOR>::FLOATS > kWeightFloats<TOKENS> ? FewTile<TOKENS, A_KMAJOR>::FLOATS : kWeightFloats<TOKENS>;
+    __shared__ __align__(16) float lds[FLOATS];
+    if (blockIdx.x < h_groups) few_product<TOKENS, kHidden, A_KMAJOR>(h, blockIdx.x, lds);
+    else few_weight<TOKENS>(w, blockIdx.x - h_groups, lds);
 }
 
 // db of 64 words: each of the 16 wavefronts takes every 16th token, then their sums are added in order
@@ -323,15 +351,16 @@ int64_t rows_a_tile(int64_t tokens) { return tokens <= 32 ? 128 : 64; }
 
 int64_t token_blocks(int64_t tokens) { return tokens <= 32 ? 1 : up_to(tokens, 64); }
 
+bool k_major(const FewArgs& a) { return a.a.c == 1 || a.a.r != 1; }
+
 template <int MODE>
 void launch_few(const FewArgs& a, int64_t tiles, hipStream_t stream) {
     const int64_t grid = tiles * token_blocks(a.v.M);
-    const bool k_major = a.a.c == 1 || a.a.r != 1;
     if (a.v.M <= 32) {
-        if (k_major) hipLaunchKernelGGL((few_kernel<32, MODE, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+        if (k_major(a)) hipLaunchKernelGGL((few_kernel<32, MODE, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
         else hipLaunchKernelGGL((few_kernel<32, MODE, false>), dim3((unsigned)grid), dim3(256), 0, stream, a);
     } else {
-        if (k_major) hipLaunchKernelGGL((few_kernel<64, MODE, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+        if (k_major(a)) hipLaunchKernelGGL((few_kernel<64, MODE, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
         else hipLaunchKernelGGL((few_kernel<64, MODE, false>), dim3((unsigned)grid), dim3(256), 0, stream, a);
     }
 }
@@ -378,20 +407,23 @@ void few_backward(const FewPlan& p, const VocabArgs& v, const Operand2& h, const
     a.out = p.g;
     launch_few<kGrad>(a, up_to(v.V, rows_a_tile(v.M)), stream);
     const Operand2 g{p.g, v.V, 1};
-    if (want_h) {
-        a.a = w; a.rows = v.D; a.k = v.V; a.b = g;
-        a.run = p.run;
-        a.out = p.part_h;
-        launch_few<kHidden>(a, up_to(v.D, rows_a_tile(v.M)) * p.runs, stream);
-    }
-    if (grad_w) {
-        FewWeight f{};
-        f.v = v; f.up = up; f.out = grad_w; f.accumulate = accumulate;
-        if (gw_d == 1 || gw_v != 1) { f.x = g; f.y = h; f.rows = v.V; f.cols = v.D; f.rs = gw_v; f.cs = gw_d; }
-        else { f.x = h; f.y = g; f.x_is_h = 1; f.rows = v.D; f.cols = v.V; f.rs = gw_d; f.cs = gw_v; }
-        const dim3 grid((unsigned)(up_to(f.rows, 128) * up_to(f.cols, 64)));
-        if (v.M <= 32) hipLaunchKernelGGL(few_weight_kernel<32>, grid, dim3(256), 0, stream, f);
-        else hipLaunchKernelGGL(few_weight_kernel<64>, grid, dim3(256), 0, stream, f);
+    a.a = w; a.rows = v.D; a.k = v.V; a.b = g;
+    a.run = p.run;
+    a.out = p.part_h;
+    FewWeight f{};
+    f.v = v; f.up = up; f.out = grad_w; f.accumulate = accumulate;
+    if (gw_d == 1 || gw_v != 1) { f.x = g; f.y = h; f.rows = v.V; f.cols = v.D; f.rs = gw_v; f.cs = gw_d; }
+    else { f.x = h; f.y = g; f.x_is_h = 1; f.rows = v.D; f.cols = v.V; f.rs = gw_d; f.cs = gw_v; }
+    const int64_t h_groups = want_h ? up_to(v.D, rows_a_tile(v.M)) * p.runs * token_blocks(v.M) : 0, w_groups = grad_w ? up_to(f.rows, kWeightI) * up_to(f.cols, kWeightJ) : 0;
+    if (h_groups + w_groups > 0) {
+        const dim3 grid((unsigned)(h_groups + w_groups));
+        if (v.M <= 32) {
+            if (k_major(a)) hipLaunchKernelGGL((few_gradients_kernel<32, true>), grid, dim3(256), 0, stream, a, (uint32_t)h_groups, f);
+            else hipLaunchKernelGGL((few_gradients_kernel<32, false>), grid, dim3(256), 0, stream, a, (uint32_t)h_groups, f);
+        } else {
+            if (k_major(a)) hipLaunchKernelGGL((few_gradients_kernel<64, true>), grid, dim3(256), 0, stream, a, (uint32_t)h_groups, f);
+            else hipLaunchKernelGGL((few_gradients_kernel<64, false>), grid, dim3(256), 0, stream, a, (uint32_t)h_groups, f);
+        }
     }
     if (grad_bias) hipLaunchKernelGGL(few_bias_kernel, dim3((unsigned)up_to(v.V, 64)), dim3(1024), 0, stream, v, up, p.g, grad_bias, accumulate);
 }

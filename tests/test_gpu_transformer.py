@@ -738,9 +738,9 @@ def test_a_workspace_that_is_too_small_is_refused(ops):
     assert L.tenmo_hip_layer_norm_backward_f32(v, p, p, p, p, None, p, None, 0, p + 4, need, 0) == -3 and b"aligned" in L.tenmo_hip_last_error()
     need = L.tenmo_hip_vocabulary_loss_forward_workspace_bytes(300, 64, 300)
     assert L.tenmo_hip_vocabulary_loss_forward_f32(v, C.byref(x.transpose().c_view()), None, p, 1, -100, 0.0, p, p, p, p, p, need - 1, 0) == -3
-    q = up(ops, randn(1, 2, 40, 2, 64))
+    q = up(ops, randn(1, 2, 400, 8, 64))
     qv = C.byref(q.c_view())
-    need = L.tenmo_hip_attention_backward_workspace_bytes(2, 40, 40, 2, 2, 64)
+    need = L.tenmo_hip_attention_backward_workspace_bytes(2, 400, 400, 8, 8, 64)
     assert need > 0 and L.tenmo_hip_attention_backward_f32(qv, qv, qv, 0.1, 0, None, None, p, p, p, qv, None, None, 0, p, need - 1, 0) == -3
 
 

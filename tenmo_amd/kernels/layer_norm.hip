@@ -10,7 +10,7 @@
 //   * loads and stores are 16 bytes whatever the row's alignment (global memory needs 4): rows of odd length cost split cache lines,
 //     not instructions.
 //   * backward: each wavefront (or workgroup) takes every G-th row and keeps the sums of its columns for dw and db in registers; a row of partial sums a workgroup
-//     goes to the workspace, and a second launch adds them in a fixed order.
+//     goes to the workspace, and a second launch adds them in a fixed order.  For few rows workgroups of columns in the one launch take their place.
 #include "entry.hpp"
 
 #include <algorithm>
@@ -143,14 +143,41 @@ struct NormBackward {
     NormRows in;
     const float *weight, *mean, *rstd, *dy;
     float *grad_x, *grad_weight, *grad_bias;
-    float* partial; // [parts][2][n]: sums of dy * xhat and of dy; NULL when neither is wanted
+    float* partial; // [parts][2][n]: sums of dy * xhat and of dy; NULL when neither is wanted, or the launch has workgroups for them
     int64_t parts;
     int accumulate;
+    int64_t row_groups; // workgroups of rows; those behind them take 16 columns of dw and db each
 };
+
+// dw and db of 16 columns over all rows: 16 rows at a time, eight of each thread's in flight, their sums added in order
+__device__ __forceinline__ void norm_columns(const NormBackward& a, int64_t group) {
+    __shared__ float sums[2][16][16];
+    const int64_t n = a.in.n, column = group * 16 + (threadIdx.x & 15), c = column < n ? column : n - 1;
+    const int slot = threadIdx.x >> 4;
+    float sw = 0.f, sb = 0.f;
+#pragma unroll 8
+    for (int64_t row = slot; row < a.in.rows; row += 16) {
+        const float dy = a.dy[row * n + c];
+        sw += dy * ((norm_row(a.in, row)[c * a.in.col_stride] - a.mean[row]) * a.rstd[row]);
+        sb += dy;
+    }
+    sums[0][slot][threadIdx.x & 15] = sw;
+    sums[1][slot][threadIdx.x & 15] = sb;
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    const int which = threadIdx.x >> 4, i = threadIdx.x & 15;
+    float* out = which ? a.grad_bias : a.grad_weight;
+    if (!out || column >= n) return;
+    float s = sums[which][0][i];
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += sums[which][k][i];
+    out[c] = a.accumulate ? out[c] + s : s;
+}
 
 // A row's x and dy are read while the row before it is worked on, where the registers allow.
 template <int W, int V4>
 __global__ __launch_bounds__(256) void norm_backward_kernel(const NormBackward a) {
+    if (blockIdx.x >= a.row_groups) return norm_columns(a, blockIdx.x - a.row_groups);
     constexpr int T = W * 64, R = 256 / T; // rows a workgroup works on at a time
     constexpr bool AHEAD = V4 <= 4;
     __shared__ float slots[2][2][4];
@@ -169,7 +196,7 @@ __global__ __launch_bounds__(256) void norm_backward_kernel(const NormBackward a
         next_mean = a.mean[row];
         next_rstd = a.rstd[row];
     };
-    const int64_t first = (int64_t)blockIdx.x * R + threadIdx.x / T, stride = (int64_t)gridDim.x * R;
+    const int64_t first = (int64_t)blockIdx.x * R + threadIdx.x / T, stride = a.row_groups * R;
     if (AHEAD && first < a.in.rows) load(first);
     for (int64_t row = first; row < a.in.rows; row += stride, turn ^= 1) {
         if (!AHEAD) load(row);
@@ -317,6 +344,10 @@ constexpr int64_t kNormWorkgroups = 768;
 int64_t norm_rows_at_a_time(int64_t n) { return n <= 1024 ? 4 : 1; }
 int64_t norm_parts(int64_t rows, int64_t n) { return std::max<int64_t>(1, std::min<int64_t>((rows + norm_rows_at_a_time(n) - 1) / norm_rows_at_a_time(n), kNormWorkgroups)); }
 
+// Few rows: dw and db by workgroups of their own in the same launch, which read x and dy again, instead of a launch behind it (a backward call of 256 rows of 768: 14.6 us, 17.9 with the
+// join; [1024, 768] 14.0 and 17.7, [2048, 768] 36.7 and 30.6 waited for, [512, 8000] 45.7 and 43.2).
+bool norm_columns_in_launch(int64_t rows, int64_t n) { return rows <= 1024 && rows * n <= 1 << 21; }
+
 // a workgroup a row, or four, up to what a launch may hold; beyond that they take further ones
 unsigned norm_grid(int64_t groups) { return (unsigned)std::min<int64_t>(groups, 1 << 22); }
 
@@ -389,21 +420,23 @@ int tenmo_hip_layer_norm_backward_f32(const tenmo_view* X, const float* weight, 
     a.grad_x = grad_X; a.grad_weight = grad_weight; a.grad_bias = grad_bias; a.accumulate = accumulate ? 1 : 0;
     const hipStream_t stream = call.state.stream;
     const int64_t n = a.in.n;
-    if (grad_weight || grad_bias) {
+    const bool by_rows = n <= 8192 && (a.in.col_stride == 1 || n == 1), columns_too = by_rows && a.in.rows > 0 && norm_columns_in_launch(a.in.rows, n) && (grad_weight || grad_bias);
+    if ((grad_weight || grad_bias) && !columns_too) {
         Workspace ws(workspace, workspace_bytes);
         a.parts = a.in.rows ? norm_parts(a.in.rows, n) : 0;
         a.partial = ws.take<float>(2 * a.parts * n);
         if (int rc = ws.check(who)) return rc;
     }
     if (a.in.rows > 0) {
-        if (n <= 8192 && (a.in.col_stride == 1 || n == 1)) {
-            hipLaunchKernelGGL(norm_backward_for(n), dim3((unsigned)norm_parts(a.in.rows, n)), dim3(256), 0, stream, a);
+        if (by_rows) {
+            a.row_groups = grad_X || !columns_too ? norm_parts(a.in.rows, n) : 0;
+            hipLaunchKernelGGL(norm_backward_for(n), dim3((unsigned)(a.row_groups + (columns_too ? (n + 15) / 16 : 0))), dim3(256), 0, stream, a);
         } else {
             if (grad_X) hipLaunchKernelGGL(norm_backward_any_kernel, dim3(norm_grid(a.in.rows)), dim3(256), 0, stream, a);
             if (a.partial) hipLaunchKernelGGL(norm_columns_any_kernel, dim3((unsigned)((n + 255) / 256), (unsigned)a.parts), dim3(256), 0, stream, a);
         }
     }
-    if (grad_weight || grad_bias) hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)((n + 63) / 64), 2), dim3(1024), 0, stream, a);
+    if ((grad_weight || grad_bias) && !columns_too) hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)((n + 63) / 64), 2), dim3(1024), 0, stream, a);
     return call.finish(sync);
 }
 

@@ -79,7 +79,7 @@ def norm_reference(x, w, b, eps, dy):
 
 
 NORM_SHAPES = [(1, 1), (3, 1), (1, 5), (1, 768), (7, 64), (5, 255), (9, 256), (4, 257), (130, 512), (33, 769), (2, 3, 1023), (515, 1024), (6, 1025), (1030, 2049), (3, 4097), (2, 8192),
-               (3, 8193), (2, 20001)]
+               (3, 8193), (2, 20001), (1500, 300), (2100, 1000), (1200, 5000), (4099, 33), (1025, 2)]
 
 
 @pytest.mark.parametrize("shape", NORM_SHAPES, ids=str)
@@ -110,6 +110,16 @@ def test_layer_norm(ops, shape, affine):
             close(down(t), down(g).double().numpy() + old, 2.0 ** -23, "accumulated")
     y2, none, _ = ops.N.layer_norm(X, W, B, 1e-5, statistics=False)
     assert none is None and torch.equal(down(y2), down(y))
+
+
+@pytest.mark.parametrize("shape", [(20, 300), (3000, 300), (5, 9000)], ids=str)
+def test_layer_norm_one_gradient_at_a_time(ops, shape):
+    x, dy, w = up(ops, randn(1, *shape)), up(ops, randn(2, *shape)), up(ops, randn(3, shape[1]))
+    y, mean, rstd = ops.N.layer_norm(x, w, w)
+    all_of_them = [down(g) for g in ops.N.layer_norm_backward(x, w, mean, rstd, dy)]
+    for i in range(3):
+        some = ops.N.layer_norm_backward(x, w, mean, rstd, dy, need_x=i == 0, need_weight=i == 1, need_bias=i == 2)
+        assert [g is not None for g in some] == [i == j for j in range(3)] and torch.equal(down(some[i]), all_of_them[i])
 
 
 @pytest.mark.parametrize("view", ["rows", "axes", "columns", "column"])
@@ -729,15 +739,16 @@ def test_a_workspace_that_is_too_small_is_refused(ops):
     from tenmo_amd import _transformer
 
     L = _transformer.load()
-    x = up(ops, randn(1, 300, 64))
+    x = up(ops, randn(1, 3000, 64))
     v = C.byref(x.c_view())
     p = x.data_ptr()
-    need = L.tenmo_hip_layer_norm_backward_workspace_bytes(300, 64)
+    need = L.tenmo_hip_layer_norm_backward_workspace_bytes(3000, 64)
     for ws, size in ((p, need - 1), (None, need)):
         assert L.tenmo_hip_layer_norm_backward_f32(v, p, p, p, p, None, p, None, 0, ws, size, 0) == -3 and b"workspace" in L.tenmo_hip_last_error()
     assert L.tenmo_hip_layer_norm_backward_f32(v, p, p, p, p, None, p, None, 0, p + 4, need, 0) == -3 and b"aligned" in L.tenmo_hip_last_error()
+    h = up(ops, randn(1, 300, 64))
     need = L.tenmo_hip_vocabulary_loss_forward_workspace_bytes(300, 64, 300)
-    assert L.tenmo_hip_vocabulary_loss_forward_f32(v, C.byref(x.transpose().c_view()), None, p, 1, -100, 0.0, p, p, p, p, p, need - 1, 0) == -3
+    assert L.tenmo_hip_vocabulary_loss_forward_f32(C.byref(h.c_view()), C.byref(h.transpose().c_view()), None, p, 1, -100, 0.0, p, p, p, p, p, need - 1, 0) == -3
     q = up(ops, randn(1, 2, 400, 8, 64))
     qv = C.byref(q.c_view())
     need = L.tenmo_hip_attention_backward_workspace_bytes(2, 400, 400, 8, 8, 64)

@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256) void attn_zero_kernel(AttnOperand g, int64_t n
 }
 
 // Rows or tiles.  Rows cost by pairs of a query and a key, tiles begin with two launches and one more pass over the operands: by these sums, fitted to 264 launches of
-// D = 32, 64, 128 with 2 to 512 queries, 64 to 8192 keys and 8 to 512 heads.  No choice costs more than 1.38 of the other there, and 1 % in the mean; at [1, 8 x 64, 64 keys] rows take
+// D = 32, 64, 128 with 2 to 512 queries, 64 to 8192 keys and 8 to 512 heads.  No choice costs more than 1.4 of the other there, and 1 % in the mean; at [1, 8 x 64, 64 keys] rows take
 // 13 us and tiles 20, at [32,16 x 64, 256 keys] 382 and 74.
 double padded(int dim) { return (dim + 31) / 32 * 32; }
 double pair_values(const AttnShape& s) { return (double)s.batch * s.heads * s.queries * s.keys * padded(s.dim); }
@@ -65,12 +65,12 @@ bool forward_by_rows(const AttnShape& s) {
     const double operands = (double)s.batch * padded(s.dim) * ((double)s.heads * s.queries + 2.0 * s.kv_heads * s.keys);
     return pair_values(s) <= 60e6 + 15.0 * operands;
 }
-// Backward, where a wavefront takes the keys of its row one after the other, two a slot at a time: that chain counts besides, 1024 of them at most.  No choice costs more than 1.30 of the
-// other, and 1 % in the mean; [1, 8 x 64]: 128 queries and keys take 23 us by rows and 31 by tiles, 512 of both 114 and 49.
+// Backward, where a wavefront takes the keys of its row one after the other, two a slot at a time: that chain counts besides, 1024 of them at most.  No choice costs more than 1.34 of the
+// other, and 1 % in the mean; [1, 8 x 64]: 128 queries and keys take 18 us by rows and 31 by tiles, 512 of both 83 and 49.
 bool backward_by_rows(const AttnShape& s) {
     const double operands = 2.0 * s.batch * padded(s.dim) * ((double)s.heads * s.queries + (double)s.kv_heads * s.keys);
     const bool fits = (int64_t)s.batch * s.kv_heads * s.keys < 1 << 24; // a launch: half as many workgroups at the most
-    return fits && s.queries <= 1024 && s.keys <= 1024 && pair_values(s) + 600.0 * padded(s.dim) * s.keys <= 40e6 + 4.0 * operands;
+    return fits && s.queries <= 1024 && s.keys <= 1024 && pair_values(s) + 800.0 * padded(s.dim) * s.keys <= 60e6 + 2.0 * operands;
 }
 
 void forward_plan(const AttnShape& s, const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, float* out, float* lse, Workspace& ws, const LibraryState& lib, bool launch) {

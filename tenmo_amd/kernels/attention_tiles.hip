@@ -14,9 +14,11 @@
 //   queries: a wavefront for 32 queries, over their keys: S^T, dP^T, dS^T; dQ^T += K^T dS^T.
 // Seven products for the five that one pass with atomics would need.
 //
-// Two launches bring the operands that are read in tiles into split form first: the largest magnitude of each head (of the rows that count), then the halves, head by head,
-// rows padded to 128 and D to DP = 32, 64, 96 or 128 with zeros; rows that no allowed pair touches are zeros too, whatever the operand holds there.  Forward, a wavefront's own rows of q
-// are split as they are read, with a scale of their own each ([8,1024,12,64]: 14 us less beforehand, 4 more in the product; backward, where all four are there, it costs 11).
+// The operands that are read in tiles are brought into split form first, head by head, rows padded to 128 and D to DP = 32, 64, 96 or 128 with zeros; rows that no allowed pair touches are
+// zeros too, whatever the operand holds there.
+//   * forward, K and V in one launch: 64 rows have a scale of their own (one read, where a scale of the whole head takes a launch before: [8,1024,12,64] 84 -> 71 us, [4,777,16,80] 73 -> 59).
+//     A wavefront's own rows of q are split as they are read, with a scale of their own each.
+//   * backward, all four in two launches: the largest magnitude of each head (of the rows that count), then the halves.
 // dS has |dS| <= 2 max |dO_i| max |V_j| (norms of rows), which gives its scale before it is known.
 //
 // LDS tile: 32 rows of DP / 4 chunks of 16 bytes, chunk c = 2 * (d / 8) + kind at slot c ^ swizzle(row); read by rows (16 bytes a lane: 16 rows in 16 different slots of the
@@ -42,7 +44,6 @@ enum { kK, kV, kQ, kDO }; // forward the first two are split beforehand, backwar
 struct TileArgs {
     AttnShape s;
     AttnOperand src[4];
-    int jobs;           // operands that are split beforehand
     int parts;          // runs of a head's rows in the first launch
     float* split[4];    // [batch][heads][rows padded][DP]
     f32x4* seen[4];     // [batch * heads][parts]: of a run of rows, the largest finite magnitude, the largest norm of a row, the smallest largest magnitude of a row
@@ -51,6 +52,7 @@ struct TileArgs {
     const float *out, *lse;
     f32x2* stats;        // [batch][heads][queries padded] (and 128 behind the last): lse log2(e) (+inf where there is none: no probability), and dO . O
     // forward
+    float* scale[2];     // [batch * heads][blocks of 64 rows]: 1 / the scale of K, the scale of V; `seen` is of these blocks too
     float *to, *to_lse, *part;
     int splits;
     // backward
@@ -208,6 +210,88 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
         *(f16x8*)to = h;
         *(f16x8*)(to + 4) = l;
     }
+}
+
+// of a power of two
+__device__ __forceinline__ float power_inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
+__device__ __forceinline__ float lane_value(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
+
+// Forward, K and V in one launch: a workgroup reads 64 rows, 4 values a lane and L lanes a row, and gives them a scale of their own.
+template <int DP, int L>
+__global__ __launch_bounds__(256) void attn_prepare_kernel(const TileArgs a) {
+    constexpr int SLOTS = 64 / L, U = L / 4, ROWS = 64; // U * 4 * SLOTS rows
+    __shared__ f32x4 seen_of[4];
+    const int blocks = row_pad(a.s.keys) / ROWS, block = blockIdx.x % blocks;
+    const HeadJob j = head_job(a, blockIdx.x / blocks);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = lane % L, D = a.s.dim;
+    const float* p = j.src.p + j.b * j.src.b + j.h * j.src.h;
+    auto row_of = [&](int u) { return block * ROWS + (u * 4 + wave) * SLOTS + lane / L; };
+    f32x4 x[U];
+    attn_with_kind(attn_kind(j.src.d, D), [&](auto kind) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = attn_load4<kind.value>(p + (row_of(u) < j.hi ? row_of(u) : 0) * j.src.s, j.src.d, part, D); // (a row that does not count is read as the first)
+    });
+    float top = 0.f, least = __builtin_inff();
+    bool wrong = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const bool in = row_of(u) < j.hi;
+        float mine = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[u][e] = in ? x[u][e] : 0.f;
+            mine = fmaxf(mine, __uint_as_float(finite_magnitude(x[u][e])));
+            wrong |= !(x[u][e] - x[u][e] == 0.f);
+        }
+        mine = lanes_max<L>(mine);
+        top = fmaxf(top, mine);
+        if (mine > 0.f) least = fminf(least, mine);
+    }
+    const f32x4 mine{wave_max(top), 0.f, -wave_max(-least), __any(wrong) ? 1.f : 0.f};
+    if (lane == 0) seen_of[wave] = mine;
+    __syncthreads();
+    f32x4 s = seen_of[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) s = f32x4{fmaxf(s[0], seen_of[w][0]), 0.f, fminf(s[2], seen_of[w][2]), fmaxf(s[3], seen_of[w][3])};
+    const float scale = split_scale(__float_as_uint(s[0]));
+    if (threadIdx.x == 0) {
+        j.seen[(int64_t)j.bh * blocks + block] = s;
+        (j.job == kK ? a.scale[kK] : a.scale[kV])[(int64_t)j.bh * blocks + block] = j.job == kK ? power_inverse(scale) : scale;
+    }
+    if (4 * part >= DP) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        f16x4 h, l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            _Float16 hi16, lo16;
+            split_value(x[u][e] * scale, hi16, lo16);
+            h[e] = hi16;
+            l[e] = lo16;
+        }
+        // 8 h, then 8 l: two lanes have four of each
+        float* to = j.split + ((int64_t)j.bh * j.pad + row_of(u)) * DP + part / 2 * 8 + part % 2 * 2;
+        *(f16x4*)to = h;
+        *(f16x4*)(to + 4) = l;
+    }
+}
+
+// Whether the halves do not hold K or V of this head: from what its blocks hold, in every lane
+__device__ __forceinline__ bool keys_beyond(const TileArgs& a, int bk) {
+    const int blocks = row_pad(a.s.keys) / 64, lane = threadIdx.x & 63;
+    bool bad = false;
+#pragma unroll
+    for (int job = 0; job < 2; ++job) {
+        float top = 0.f, least = __builtin_inff(), wrong = 0.f;
+        for (int i = lane; i < blocks; i += 64) {
+            const f32x4 s = a.seen[job][(int64_t)bk * blocks + i];
+            top = fmaxf(top, s[0]);
+            least = fminf(least, s[2]);
+            wrong = fmaxf(wrong, s[3]);
+        }
+        bad |= __any(wrong > 0.f) || wave_max(top) * 0x1p-16f > -wave_max(-least);
+    }
+    return bad;
 }
 
 // Heads beyond the halves are worked on row by row in fp32, where nothing that is not allowed can leave a trace: those with keys or values that are not finite, or of sizes too far apart;
@@ -478,8 +562,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
     const int tiles = (attn_limit(length, start, block_last) + 31) / 32, per = (tiles + a.splits - 1) / a.splits;
     const int t0 = split * per < tiles ? split * per : tiles, t1 = t0 + per < tiles ? t0 + per : tiles;
 
-    const f32x4 head_k = a.head[kK][bk], head_v = a.head[kV][bk];
-    if (__builtin_amdgcn_readfirstlane(head_k[2] + head_v[2] > 0.f)) {
+    if (__builtin_amdgcn_readfirstlane(keys_beyond(a, bk))) {
         constexpr int L = T::LANES;
         for (int r = q0; r < q0 + 32 && r < a.s.queries; ++r) {
             float m, l;
@@ -501,7 +584,17 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
     f16x8 qh[T::KD], ql[T::KD];
     float norm_q;
     const float scale_q = own_split<DP>(qh, ql, a.src[kQ], b, i, h, limit > 0, D, &norm_q);
-    const float inv_v = 1.f / head_v[0], c = fabsf(a.s.scale) * kLog2e / scale_q / head_k[0];
+    const float c_all = fabsf(a.s.scale) * kLog2e / scale_q;
+    const float *const scale_k = a.scale[kK] + (int64_t)bk * (pad_k / 64), *const scale_v = a.scale[kV] + (int64_t)bk * (pad_k / 64);
+    int unit = 127 << 23; // the bits of the power of two that V is multiplied by in the sums
+    float lane_k, lane_v; // of 64 blocks, one a lane
+    auto load_scales = [&](int t) {
+        const int i = (t >> 7) * 64 + lane < pad_k / 64 ? (t >> 7) * 64 + lane : 0;
+        lane_k = scale_k[i];
+        lane_v = scale_v[i];
+        asm volatile("" : "+v"(lane_k), "+v"(lane_v)); // waited for here: a wait in every tile would be one for the tiles that are on their way
+    };
+    load_scales(t0);
     if (a.s.scale < 0.f) // the maximum is taken before the factor, which has to keep the order
 #pragma unroll
         for (int ks = 0; ks < T::KD; ++ks) qh[ks] = -qh[ks], ql[ks] = -ql[ks];
@@ -530,6 +623,13 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
         const char* vs_tile = ks_tile + T::BYTES;
         stage = stage == STAGES - 1 ? 0 : stage + 1;
         if (t * 32 >= wave_most) continue; // nothing here for these 32 queries (every wavefront meets at the next barrier)
+        if (t % 128 == 0) load_scales(t);
+        // V of this block has a scale of its own: p makes up for it where that costs no more than 4 of its bits, else the sums do (by 2^16 at the most: keys_beyond())
+        const float c = c_all * lane_value(lane_k, (t >> 1) & 63);
+        const int scale = __builtin_amdgcn_readlane(__float_as_int(lane_v), (t >> 1) & 63), more = (scale - unit) >> 23;
+        const bool other = more < 0 || more > 4;
+        const float up = other ? __int_as_float((127 << 23) + scale - unit) : 1.f, less = kPBits - (other ? 0.f : (float)more), back = __int_as_float((127 + (other ? 0 : more)) << 23);
+        unit = other ? scale : unit;
         f32x16 s = zero16();
 #pragma unroll
         for (int ks = 0; ks < T::KD; ++ks) split_mfma(s, T::row_read(ks_tile, row_off[0], ks), T::row_read(ks_tile, row_off[1], ks), qh[ks], ql[ks]);
@@ -551,23 +651,23 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
 #pragma unroll
         for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
         top = halves_max(top) * by;
-        if (__any(top > m + kRenew)) { // (an m of -inf is passed by any score)
+        if (__any(top > m + kRenew) || other) { // (an m of -inf is passed by any score)
             const float now = top > m + kRenew ? top : m, keep = m == kNone ? 0.f : __builtin_amdgcn_exp2f(m - now);
             m = now;
             l *= keep;
 #pragma unroll
             for (int d = 0; d < T::ND; ++d)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[d][e] *= keep;
+                for (int e = 0; e < 16; ++e) o[d][e] *= keep * up;
         }
-        const float shift = kPBits - (m == kNone ? 0.f : m);
+        const float shift = less - (m == kNone ? 0.f : m);
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             s[e] = __builtin_amdgcn_exp2f(s[e] * by + shift);
             sum += s[e];
         }
-        l += sum;
+        l += sum * back;
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
             f16x8 ph, pl;
@@ -590,11 +690,11 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
     float factor;
     if (a.part) {
         to = a.part + ((int64_t)split * a.s.batch * a.s.heads * a.s.queries + row) * (D + 2);
-        factor = inv_v * (1.f / 128.f);
+        factor = power_inverse(__int_as_float(unit)) * (1.f / 128.f);
         if (half == 0) to[D] = m * kLn2, to[D + 1] = l * (1.f / 128.f);
     } else {
         to = a.to + (((int64_t)b * a.s.queries + i) * a.s.heads + h) * D;
-        factor = l == 0.f ? 0.f : inv_v / l;
+        factor = l == 0.f ? 0.f : power_inverse(__int_as_float(unit)) / l;
         if (half == 0 && a.to_lse) a.to_lse[row] = l == 0.f ? kNone : (m + __builtin_amdgcn_logf(l) - kPBits) * kLn2;
     }
 #pragma unroll
@@ -910,17 +1010,25 @@ __global__ __launch_bounds__(256) void attn_group_kernel(const TileArgs a) {
 
 int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 
-int all_heads(const AttnShape& s, int jobs) { return s.batch * (s.heads * (jobs - 2) + s.kv_heads * 2); } // (jobs: 2 or 4)
-
-void plan_operands(TileArgs& a, Workspace& ws, int jobs) {
+void plan_keys(TileArgs& a, Workspace& ws) {
     const AttnShape& s = a.s;
-    a.jobs = jobs;
-    // Runs of 128 rows, or, where that is fewer than four workgroups a CU, of the rows that one has in flight at once ([1,1024,12,64] forward: 43 us, 47 with 128; [8,1024,12,64]
-    // backward: 259 us, 256 with 128); no more than a launch holds.
-    const int heads_here = all_heads(s, jobs), longest = std::max(jobs == 2 ? 0 : s.queries, s.keys), once = 1024 / (s.dim <= 32 ? 8 : s.dim <= 64 ? 16 : 32);
-    const int run = (int64_t)heads_here * ((longest + 127) / 128) < 1024 ? once : 128;
-    a.parts = std::max(1, std::min(std::min(kHeadParts, (1 << 23) / heads_here), (longest + run - 1) / run));
-    for (int j = 0; j < jobs; ++j) {
+    const int64_t heads = (int64_t)s.batch * s.kv_heads, blocks = row_pad(s.keys) / 64;
+    for (int j = 0; j < 2; ++j) {
+        a.split[j] = ws.take<float>(heads * row_pad(s.keys) * padded_dim(s.dim));
+        a.seen[j] = ws.take<f32x4>(heads * blocks);
+        a.scale[j] = ws.take<float>(heads * blocks);
+    }
+}
+
+int all_heads(const AttnShape& s) { return 2 * s.batch * (s.heads + s.kv_heads); }
+
+void plan_operands(TileArgs& a, Workspace& ws) {
+    const AttnShape& s = a.s;
+    // Runs of 128 rows, or, where that is fewer than four workgroups a CU, of the rows that one has in flight at once ([8,1024,12,64]: 259 us, 256 with 128 rows); no more than a launch holds.
+    const int longest = std::max(s.queries, s.keys), once = 1024 / (s.dim <= 32 ? 8 : s.dim <= 64 ? 16 : 32);
+    const int run = (int64_t)all_heads(s) * ((longest + 127) / 128) < 1024 ? once : 128;
+    a.parts = std::max(1, std::min(std::min(kHeadParts, (1 << 23) / all_heads(s)), (longest + run - 1) / run));
+    for (int j = 0; j < 4; ++j) {
         const bool key = j == kK || j == kV;
         const int64_t heads = (int64_t)s.batch * (key ? s.kv_heads : s.heads);
         a.split[j] = ws.take<float>(heads * row_pad(key ? s.keys : s.queries) * padded_dim(s.dim));
@@ -930,24 +1038,18 @@ void plan_operands(TileArgs& a, Workspace& ws, int jobs) {
 }
 
 template <int DP, int L>
-void launch_operands(const TileArgs& a, hipStream_t stream) {
-    const AttnShape& s = a.s;
-    const int64_t rows = (int64_t)s.batch * ((int64_t)s.heads * (a.jobs - 2) * row_pad(s.queries) + (int64_t)s.kv_heads * 2 * row_pad(s.keys));
-    hipLaunchKernelGGL(attn_amax_kernel<L>, dim3((unsigned)(all_heads(s, a.jobs) * a.parts)), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(attn_split_kernel<DP>, dim3((unsigned)(rows / 64)), dim3(256), 0, stream, a);
-}
-
-template <int DP, int L>
 void launch_forward(const TileArgs& a, hipStream_t stream) {
-    launch_operands<DP, L>(a, stream);
     const AttnShape& s = a.s;
+    hipLaunchKernelGGL((attn_prepare_kernel<DP, L>), dim3((unsigned)(2 * s.batch * s.kv_heads * (row_pad(s.keys) / 64))), dim3(256), 0, stream, a);
     hipLaunchKernelGGL(attn_tile_forward_kernel<DP>, dim3((unsigned)(s.batch * s.heads * (row_pad(s.queries) / kRowPad) * a.splits)), dim3(256), 0, stream, a);
 }
 
 template <int DP, int L>
 void launch_backward(const TileArgs& a, hipStream_t stream) {
-    launch_operands<DP, L>(a, stream);
     const AttnShape& s = a.s;
+    const int64_t rows = 2LL * s.batch * ((int64_t)s.heads * row_pad(s.queries) + (int64_t)s.kv_heads * row_pad(s.keys));
+    hipLaunchKernelGGL(attn_amax_kernel<L>, dim3((unsigned)(all_heads(s) * a.parts)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(attn_split_kernel<DP>, dim3((unsigned)(rows / 64)), dim3(256), 0, stream, a);
     const int blocks_of_keys = a.grad_k.p || a.grad_v.p ? s.batch * s.heads * (row_pad(s.keys) / kRowPad) : 0, blocks_of_queries = a.grad_q.p ? s.batch * s.heads * (row_pad(s.queries) / kRowPad) : 0;
     hipLaunchKernelGGL(attn_tile_backward_kernel<DP>, dim3((unsigned)(blocks_of_keys + blocks_of_queries)), dim3(256), 0, stream, a, blocks_of_keys);
     if ((a.grad_k.p || a.grad_v.p) && a.part_k) {
@@ -964,7 +1066,7 @@ void attn_tiles_forward(const AttnShape& s, const AttnOperand& q, const AttnOper
     a.s = s;
     a.src[kQ] = q; a.src[kK] = k; a.src[kV] = v;
     a.to = out; a.to_lse = lse;
-    plan_operands(a, ws, 2);
+    plan_keys(a, ws);
     // two workgroups a CU fill it; a run of fewer than 256 keys is not worth its part of the join
     const int64_t groups = (int64_t)s.batch * s.heads * (row_pad(s.queries) / kRowPad);
     a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(2LL * cus / groups, std::min(s.keys / 256, kMostRuns)));
@@ -986,7 +1088,7 @@ void attn_tiles_backward(const AttnBackward& b, Workspace& ws, hipStream_t strea
     a.src[kDO] = AttnOperand{const_cast<float*>(b.dout), (int64_t)b.s.queries * b.s.heads * b.s.dim, (int64_t)b.s.heads * b.s.dim, b.s.dim, 1};
     a.out = b.out; a.lse = b.lse;
     a.grad_q = b.grad_q; a.grad_k = b.grad_k; a.grad_v = b.grad_v; a.accumulate = b.accumulate;
-    plan_operands(a, ws, 4);
+    plan_operands(a, ws);
     a.stats = ws.take<f32x2>((int64_t)b.s.batch * b.s.heads * row_pad(b.s.queries) + kRowPad);
     if (b.s.group > 1) {
         a.part_k = ws.take<float>((int64_t)b.s.batch * b.s.heads * b.s.keys * b.s.dim);

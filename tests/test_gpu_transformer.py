@@ -377,6 +377,24 @@ def test_attention_extreme_scores(ops):
                 assert np.linalg.norm(g[:, h].numpy() - ref[0, :, h]) <= tol * np.linalg.norm(size), what
 
 
+@pytest.mark.parametrize("H", [2, 40])
+def test_attention_blocks_of_keys_of_different_sizes(ops, H):
+    """Keys and values whose blocks of 64 lie up to 2^15 apart, each query with its weight in one block: every row of the result is right against its own size."""
+    B, n, m, D = 1, 300, 256, 64
+    q, k, v = randn(1, B, n, H, D), randn(2, B, m, H, D) * 0.2, randn(3, B, m, H, D)
+    q[..., :4] = k[..., :4] = 0.0
+    for b, size in enumerate((2.0 ** -6, 2.0 ** 7, 2.0 ** -8, 1.0)):
+        v[:, 64 * b:64 * b + 64] *= size
+        q[:, b::4, :, b] = 32.0 * 2.0 ** (b % 3 * 4)
+        k[:, 64 * b:64 * b + 64, :, b] = 2.0 ** -(b % 3 * 4)
+    want, want_lse, _ = attention_reference(q, k, v, 1.0, False, None, None, None)
+    o, lse = ops.A.attention(up(ops, q), up(ops, k), up(ops, v), scale=1.0)
+    close(down(lse), want_lse, RTOL_FRO, "lse")
+    # (a score of 32, made of products that cancel to a part in ten at the most, is right to 12 roundings of 2^-24 of 40, and so is its weight)
+    error = np.linalg.norm(down(o).numpy() - want, axis=-1) / np.linalg.norm(want, axis=-1)
+    assert error.max() <= 12 * 40 * 2.0 ** -24, error.max()
+
+
 def test_attention_without_keys_or_queries(ops):
     q, none = up(ops, randn(1, 2, 3, 2, 8)), ops.NDBuffer.empty((2, 0, 2, 8))
     o, lse = ops.A.attention(q, none, none)

@@ -403,15 +403,30 @@ __global__ __launch_bounds__(1024) void vocab_join_kernel(const JoinArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t token = (int64_t)blockIdx.x * 64 + lane, M = a.v.M;
     float top = -__builtin_inff(), sum = 0.f, sx = 0.f;
-    if (token < M) {
-        for (int64_t t = wave; t < a.tiles; t += 16) top = fmaxf(top, a.part[t * M + token].x);
-        const float base = top == -__builtin_inff() ? 0.f : top;
-        for (int64_t t = wave; t < a.tiles; t += 16) {
-            const float2 p = a.part[t * M + token];
-            sum += p.y * __expf(p.x - base);
-            if (a.part_x) sx += a.part_x[t * M + token];
+    constexpr int U = 8; // tiles in flight a thread (the last one again where there is none)
+    if (token < M)
+        for (int64_t t0 = wave; t0 < a.tiles; t0 += 16 * U) {
+            float2 p[U];
+            float x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t t = t0 + 16 * u < a.tiles ? t0 + 16 * u : a.tiles - 1;
+                p[u] = a.part[t * M + token];
+                x[u] = a.part_x ? a.part_x[t * M + token] : 0.f;
+            }
+            float now = top;
+#pragma unroll
+            for (int u = 0; u < U; ++u) now = fmaxf(now, p[u].x);
+            const float base = now == -__builtin_inff() ? 0.f : now;
+            sum *= __expf(top - base);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool in = t0 + 16 * u < a.tiles;
+                sum += in ? p[u].y * __expf(p[u].x - base) : 0.f;
+                sx += in ? x[u] : 0.f;
+            }
+            top = now;
         }
-    }
     s[0][wave][lane] = top; s[1][wave][lane] = sum; s[2][wave][lane] = sx;
     __syncthreads();
     if (wave) return;
@@ -469,7 +484,7 @@ __global__ __launch_bounds__(256) void vocab_dh_kernel(const float* __restrict p
     for (int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; x < all; x += (int64_t)gridDim.x * 1024) {
         if (x + 3 < all) {
             f32x4 s = *(const f32x4*)(part + x);
-#pragma unroll 8
+#pragma unroll 16
             for (int64_t r = 1; r < runs; ++r) s += *(const f32x4_u*)(part + r * all + x);
             const int64_t m = x / D;
             const float factor = row_factor(v, up, m);

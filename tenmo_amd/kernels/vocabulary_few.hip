@@ -385,8 +385,8 @@ void few_plan_forward(Workspace& ws, FewPlan& p, const VocabArgs& v) {
 
 void few_plan_backward(Workspace& ws, FewPlan& p, const VocabArgs& v) {
     p.g = ws.take<float>(v.M * v.V);
-    // four workgroups a CU, of at least 64 words each
-    p.run = up_to(up_to(v.V, std::max<int64_t>(1, std::min(1024 / (up_to(v.D, rows_a_tile(v.M)) * token_blocks(v.M)), v.V / 64))), KC) * KC;
+    // two workgroups a CU, of at least 64 words each
+    p.run = up_to(up_to(v.V, std::max<int64_t>(1, std::min(512 / (up_to(v.D, rows_a_tile(v.M)) * token_blocks(v.M)), v.V / 64))), KC) * KC;
     p.runs = up_to(v.V, p.run);
     p.part_h = ws.take<float>(p.runs * v.M * v.D);
 }

@@ -6,9 +6,9 @@
 //
 // The split form of the products (vocabulary.hip) reads W three times and writes it once before it begins, which its rate pays back only for many tokens and a large W.  Forward and
 // backward with W as an embedding [words, D], here against the split form:
-//       768 x 50257:    1 token 57 + 131 us against 146 + 271;   64 tokens 84 + 193 against 142 + 266;   256 tokens 221 + 610 against 173 + 367
+//       768 x 50257:    1 token 52 + 126 us against 146 + 271;   64 tokens 74 + 190 against 142 + 266;   256 tokens 221 + 610 against 173 + 367
 //      1600 x 4000:    64 tokens 50 +  87 us against  91 + 128;  256 tokens 53 + 146 against  91 + 167;  512 tokens  85 + 248 against  92 + 188
-//       128 x 1000:    64 tokens 20 +  23 us against  31 +  45;  256 tokens 25 +  41 against  30 +  52;  512 tokens  25 +  61 against  30 +  54
+//       128 x 1000:    64 tokens 19 +  22 us against  31 +  45;  256 tokens 25 +  41 against  30 +  52;  512 tokens  25 +  61 against  30 +  54
 // One read of the first W (154 MB) takes 30 us at the rate of a copy, its backward (W twice, dW once) 92 us.
 // Both products with W have the matrix in the rows of the instruction's result and the tokens in its columns: rows r of 32 in LDS, K-major ([row][k], 32 k and 4 of padding: a
 // float4 of four k a lane, 16 rows in 16 different bank groups) where the memory runs along k, MN-major ([k][row]) where it runs along r.

@@ -52,7 +52,7 @@ struct TileArgs {
     const float *out, *lse;
     f32x2* stats;        // [batch][heads][queries padded] (and 128 behind the last): lse log2(e) (+inf where there is none: no probability), and dO . O
     // forward
-    float* scale[2];     // [batch * heads][blocks of 64 rows]: 1 / the scale of K, the scale of V; `seen` is of these blocks too
+    float* scale[2];     // [batch * heads][blocks of 64 rows]: 1 / the scale of K, the scale of V or 0 where there are zeros alone; `seen` is of these blocks too
     float *to, *to_lse, *part;
     int splits;
     // backward
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(256) void attn_prepare_kernel(const TileArgs a) {
     const float scale = split_scale(__float_as_uint(s[0]));
     if (threadIdx.x == 0) {
         j.seen[(int64_t)j.bh * blocks + block] = s;
-        (j.job == kK ? a.scale[kK] : a.scale[kV])[(int64_t)j.bh * blocks + block] = j.job == kK ? power_inverse(scale) : scale;
+        (j.job == kK ? a.scale[kK] : a.scale[kV])[(int64_t)j.bh * blocks + block] = j.job == kK ? power_inverse(scale) : s[0] > 0.f ? scale : 0.f;
     }
     if (4 * part >= DP) return;
 #pragma unroll
@@ -626,7 +626,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
         if (t % 128 == 0) load_scales(t);
         // V of this block has a scale of its own: p makes up for it where that costs no more than 4 of its bits, else the sums do (by 2^16 at the most: keys_beyond())
         const float c = c_all * lane_value(lane_k, (t >> 1) & 63);
-        const int scale = __builtin_amdgcn_readlane(__float_as_int(lane_v), (t >> 1) & 63), more = (scale - unit) >> 23;
+        const int own = __builtin_amdgcn_readlane(__float_as_int(lane_v), (t >> 1) & 63), scale = own ? own : unit, more = (scale - unit) >> 23;
         const bool other = more < 0 || more > 4;
         const float up = other ? __int_as_float((127 << 23) + scale - unit) : 1.f, less = kPBits - (other ? 0.f : (float)more), back = __int_as_float((127 + (other ? 0 : more)) << 23);
         unit = other ? scale : unit;
@@ -690,19 +690,23 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
     float factor;
     if (a.part) {
         to = a.part + ((int64_t)split * a.s.batch * a.s.heads * a.s.queries + row) * (D + 2);
-        factor = power_inverse(__int_as_float(unit)) * (1.f / 128.f);
+        factor = 1.f / 128.f;
         if (half == 0) to[D] = m * kLn2, to[D + 1] = l * (1.f / 128.f);
     } else {
         to = a.to + (((int64_t)b * a.s.queries + i) * a.s.heads + h) * D;
-        factor = l == 0.f ? 0.f : power_inverse(__int_as_float(unit)) / l;
+        factor = l == 0.f ? 0.f : 1.f / l;
         if (half == 0 && a.to_lse) a.to_lse[row] = l == 0.f ? kNone : (m + __builtin_amdgcn_logf(l) - kPBits) * kLn2;
     }
+    const float inv_v = power_inverse(__int_as_float(unit)); // (by itself: its product with the factor may be too small for a float)
 #pragma unroll
     for (int d = 0; d < T::ND; ++d)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int at = 32 * d + 8 * q + 4 * half;
-            store_part(to, at, D, f32x4{o[d][4 * q] * factor, o[d][4 * q + 1] * factor, o[d][4 * q + 2] * factor, o[d][4 * q + 3] * factor});
+            f32x4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = o[d][4 * q + e] * factor * inv_v;
+            store_part(to, at, D, x);
         }
 }
 
@@ -854,7 +858,7 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
         TENMO_PRODUCTS(12);
     }
     if (j >= a.s.keys) return;
-    const float inv_dk = a.s.scale / ds_up / scale_q, inv_dv = 1.f / 16384.f / scale_g;
+    const float inv_ds = 1.f / ds_up, inv_q = 1.f / scale_q, inv_dv = 1.f / 16384.f / scale_g; // (one after the other: their product may be too small for a float)
     const int64_t at_k = b * a.grad_k.b + hk * a.grad_k.h + j * a.grad_k.s, at_v = b * a.grad_v.b + hk * a.grad_v.h + j * a.grad_v.s;
     const int64_t at_part = ((int64_t)bh * a.s.keys + j) * D;
 #pragma unroll
@@ -864,7 +868,7 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
             const int at = 32 * d + 8 * q + 4 * half;
             f32x4 x, y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = dk[d][4 * q + e] * inv_dk, y[e] = dv[d][4 * q + e] * inv_dv;
+            for (int e = 0; e < 4; ++e) x[e] = dk[d][4 * q + e] * a.s.scale * inv_q * inv_ds, y[e] = dv[d][4 * q + e] * inv_dv;
             if (a.part_k) {
                 store_part(a.part_k + at_part, at, D, x);
                 store_part(a.part_v + at_part, at, D, y);
@@ -967,7 +971,7 @@ __device__ __forceinline__ void tile_dq(const TileArgs& a, int id, float* lds) {
         TENMO_PRODUCTS(6);
     }
     if (i >= a.s.queries) return;
-    const float factor = a.s.scale / ds_up / scale_k;
+    const float inv_ds = 1.f / ds_up, inv_k = 1.f / scale_k;
     const int64_t at_q = b * a.grad_q.b + h * a.grad_q.h + i * a.grad_q.s;
 #pragma unroll
     for (int d = 0; d < T::ND; ++d)
@@ -975,7 +979,7 @@ __device__ __forceinline__ void tile_dq(const TileArgs& a, int id, float* lds) {
         for (int q = 0; q < 4; ++q) {
             f32x4 x;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = dq[d][4 * q + e] * factor;
+            for (int e = 0; e < 4; ++e) x[e] = dq[d][4 * q + e] * a.s.scale * inv_k * inv_ds;
             store_gradient(a.grad_q, at_q, 32 * d + 8 * q + 4 * half, D, x, a.accumulate);
         }
 }

@@ -352,6 +352,18 @@ def test_attention_scales(ops, n, scale):
                 assert np.abs(down(g)[-1].numpy()).max() <= abs(scale) * 1e4
 
 
+@pytest.mark.parametrize("size", [2.0 ** -108, 2.0 ** 90])
+@pytest.mark.parametrize("reps", [1, 60])
+def test_attention_gradients_of_any_size(ops, reps, size):
+    """Upstream gradients far from one: the gradients are those of one times as much."""
+    q, k, v, dout = (randn(i, 1, 160, 2, 64) for i in range(4))
+    want = attention_reference(q, k, v, 0.11, True, None, None, dout)[2]
+    Q, K, V, DO = (up(ops, t.repeat(reps, 1, 1, 1)) for t in (q, k, v, dout * size))
+    o, lse = ops.A.attention(Q, K, V, scale=0.11, causal=True)
+    for g, ref, what in zip(ops.A.attention_backward(Q, K, V, o, lse, DO, scale=0.11, causal=True), want, ("grad_q", "grad_k", "grad_v")):
+        close(down(g)[-1].double() / size, ref[0], 2 * RTOL_FRO, what)
+
+
 def test_attention_extreme_scores(ops):
     """Scores of thousands and values over 40 powers of two: the maximum is taken off before the exponential, and the sums have fp32's range."""
     B, n, H, D = 1, 96, 2, 64
@@ -377,16 +389,18 @@ def test_attention_extreme_scores(ops):
                 assert np.linalg.norm(g[:, h].numpy() - ref[0, :, h]) <= tol * np.linalg.norm(size), what
 
 
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -112])
 @pytest.mark.parametrize("H", [2, 40])
-def test_attention_blocks_of_keys_of_different_sizes(ops, H):
-    """Keys and values whose blocks of 64 lie up to 2^15 apart, each query with its weight in one block: every row of the result is right against its own size."""
+def test_attention_blocks_of_keys_of_different_sizes(ops, H, size):
+    """Keys and values whose blocks of 64 lie up to 2^15 apart, one of zeros among them, each query with its weight in one block: every row of the result is right against its own size."""
     B, n, m, D = 1, 300, 256, 64
     q, k, v = randn(1, B, n, H, D), randn(2, B, m, H, D) * 0.2, randn(3, B, m, H, D)
     q[..., :4] = k[..., :4] = 0.0
-    for b, size in enumerate((2.0 ** -6, 2.0 ** 7, 2.0 ** -8, 1.0)):
-        v[:, 64 * b:64 * b + 64] *= size
+    for b, factor in enumerate((2.0 ** -6, 2.0 ** 7, 2.0 ** -8, 1.0)):
+        v[:, 64 * b:64 * b + 64] *= size * factor
         q[:, b::4, :, b] = 32.0 * 2.0 ** (b % 3 * 4)
         k[:, 64 * b:64 * b + 64, :, b] = 2.0 ** -(b % 3 * 4)
+    k, v = (torch.cat((t[:, :128], 0.0 * t[:, :64], t[:, 128:]), 1) for t in (k, v))  # the zeros' scores are 0, the others' of a query 32 and near 0
     want, want_lse, _ = attention_reference(q, k, v, 1.0, False, None, None, None)
     o, lse = ops.A.attention(up(ops, q), up(ops, k), up(ops, v), scale=1.0)
     close(down(lse), want_lse, RTOL_FRO, "lse")

@@ -51,7 +51,8 @@ int tenmo_hip_attention_forward_f32(const tenmo_view* Q, const tenmo_view* K, co
                                     void* workspace, int64_t workspace_bytes, int32_t sync);
 /* Gradients for the upstream gradient dOut (dense [B, Sq, H, D]); out and lse as the forward call with the same arguments left them.  The
  * probabilities are computed again.  grad_Q, grad_K, grad_V: views of the shapes of Q, K, V with strides of their own (no two elements
- * of the three at one place), written through; grad_K and grad_V sum over the query heads that share a key head. */
+ * of the three at one place), written through; grad_K and grad_V sum over the query heads that share a key head.
+ * Where heads are shared, B * H * Sk up to 2^28. */
 int64_t tenmo_hip_attention_backward_workspace_bytes(int64_t batch, int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim);
 int tenmo_hip_attention_backward_f32(const tenmo_view* Q, const tenmo_view* K, const tenmo_view* V, float scale, int32_t causal,
                                      const int32_t* key_lengths, const int32_t* query_starts, const float* out, const float* lse,

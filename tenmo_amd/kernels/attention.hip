@@ -73,13 +73,20 @@ bool backward_by_rows(const AttnShape& s) {
     return fits && s.queries <= 1024 && s.keys <= 1024 && pair_values(s) + 800.0 * padded(s.dim) * s.keys <= 60e6 + 2.0 * operands;
 }
 
+// Tiles hold 2^24 workgroups a launch, and a part of each query head's share of dK and dV.
+int backward_fits(const AttnShape& s, const char* who) {
+    if (s.group > 1 && !backward_by_rows(s) && (int64_t)s.batch * s.heads * s.keys > 1 << 28)
+        return refuse(TENMO_ERR_UNSUPPORTED, "%s: more than 2^28 rows of keys over all query heads", who);
+    return 0;
+}
+
 void forward_plan(const AttnShape& s, const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, float* out, float* lse, Workspace& ws, const LibraryState& lib, bool launch) {
     if (forward_by_rows(s)) attn_rows_forward(s, q, k, v, out, lse, ws, lib.cus, lib.stream, launch);
     else attn_tiles_forward(s, q, k, v, out, lse, ws, lib.cus, lib.stream, launch);
 }
 
 void backward_plan(const AttnBackward& b, Workspace& ws, const LibraryState& lib, bool launch) {
-    if (!backward_by_rows(b.s)) attn_tiles_backward(b, ws, lib.stream, launch);
+    if (!backward_by_rows(b.s)) attn_tiles_backward(b, ws, lib.cus, lib.stream, launch);
     else if (launch) attn_rows_backward(b, lib.stream);
 }
 
@@ -124,6 +131,7 @@ int64_t tenmo_hip_attention_backward_workspace_bytes(int64_t batch, int64_t quer
     AttnBackward b{};
     LibraryState lib{};
     if (int rc = attn_shape(batch, queries, keys, heads, kv_heads, dim, "tenmo_hip_attention_backward_workspace_bytes", &b.s)) return rc;
+    if (int rc = backward_fits(b.s, "tenmo_hip_attention_backward_workspace_bytes")) return rc;
     if (int rc = library_state(&lib)) return rc;
     Workspace ws(nullptr, 0);
     if (batch > 0 && queries > 0 && keys > 0) backward_plan(b, ws, lib, false);
@@ -141,6 +149,7 @@ int tenmo_hip_attention_backward_f32(const tenmo_view* Q, const tenmo_view* K, c
     if (int rc = check_gradient(grad_K, K, who, "grad_K")) return rc;
     if (int rc = check_gradient(grad_V, V, who, "grad_V")) return rc;
     const AttnShape& s = b.s;
+    if (int rc = backward_fits(s, who)) return rc;
     if (s.batch > 0 && s.queries > 0 && s.keys > 0 && (!out || !lse || !dOut)) return refuse(TENMO_ERR_INVALID_ARGUMENT, "%s: null out, lse or dOut", who);
     Call call(who);
     if (int rc = call.begin()) return rc;

@@ -100,7 +100,7 @@ void attn_join(const AttnShape&, const float* part, int splits, float* out, floa
 // ---- attention_tiles.hip ----
 void attn_tiles_forward(const AttnShape&, const AttnOperand& q, const AttnOperand& k, const AttnOperand& v, float* out, float* lse,
                         Workspace& ws, int cus, hipStream_t stream, bool launch);
-void attn_tiles_backward(const AttnBackward&, Workspace& ws, hipStream_t stream, bool launch);
+void attn_tiles_backward(const AttnBackward&, Workspace& ws, int cus, hipStream_t stream, bool launch);
 
 } // namespace tenmo
 #endif

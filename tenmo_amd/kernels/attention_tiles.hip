@@ -58,7 +58,8 @@ struct TileArgs {
     // backward
     AttnOperand grad_q, grad_k, grad_v;
     int accumulate;
-    float *part_k, *part_v; // [batch][heads][keys][dim]: each query head's part where heads share a key head
+    int query_runs, key_runs;       // into which the queries of a block of keys, and the keys of a block of queries, are cut
+    float *part_k, *part_v, *part_q; // [runs][batch][heads][rows][dim]: the parts of each run and query head, where there is more than one
 };
 
 // first query row with a key, and the number of keys that some query may use
@@ -345,12 +346,12 @@ __device__ __forceinline__ f32x4 slow_forward(const TileArgs& a, int b, int h, i
 
 // a row of dQ, without its factor scale
 template <int L>
-__device__ __forceinline__ f32x4 slow_dq(const TileArgs& a, int b, int h, int i, int limit, float lse, float delta) {
+__device__ __forceinline__ f32x4 slow_dq(const TileArgs& a, int b, int h, int i, int lo, int limit, float lse, float delta) { // from the keys lo .. limit - 1
     constexpr int SLOTS = 64 / L;
     const int lane = threadIdx.x & 63, part = lane % L, D = a.s.dim, hk = h / a.s.group;
     const f32x4 q = slow_load(a.src[kQ], b, i, h, part, D) * a.s.scale, g = slow_load(a.src[kDO], b, i, h, part, D);
     f32x4 acc{0.f, 0.f, 0.f, 0.f};
-    for (int j = lane / L; __any(j < limit); j += SLOTS) {
+    for (int j = lo + lane / L; __any(j < limit); j += SLOTS) {
         const int jr = j < limit ? j : limit - 1;
         const f32x4 k = slow_load(a.src[kK], b, jr, hk, part, D), v = slow_load(a.src[kV], b, jr, hk, part, D);
         const float x = lanes_sum<L>(dot4(q, k)), dp = lanes_sum<L>(dot4(g, v));
@@ -363,14 +364,14 @@ __device__ __forceinline__ f32x4 slow_dq(const TileArgs& a, int b, int h, int i,
     return acc;
 }
 
-// dK (without its factor scale) and dV of a key of this slot's, from the queries of head h
+// dK (without its factor scale) and dV of a key of this slot's, from the queries lo .. hi - 1 of head h
 template <int L>
-__device__ __forceinline__ void slow_dkv(const TileArgs& a, int b, int h, int j, int length, int start, f32x4& dk, f32x4& dv) {
+__device__ __forceinline__ void slow_dkv(const TileArgs& a, int b, int h, int j, int length, int start, int lo, int hi, f32x4& dk, f32x4& dv) {
     const int part = (threadIdx.x & 63) % L, D = a.s.dim, hk = h / a.s.group, jr = j < a.s.keys ? j : a.s.keys - 1;
     const int64_t bh = (int64_t)b * a.s.heads + h;
     const f32x4 k = slow_load(a.src[kK], b, jr, hk, part, D), v = slow_load(a.src[kV], b, jr, hk, part, D);
     dk = dv = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < a.s.queries; ++i) {
+    for (int i = lo; i < hi; ++i) {
         const int limit = attn_limit(length, start, i);
         if (!__any(j < limit)) continue;
         const f32x4 q = slow_load(a.src[kQ], b, i, h, part, D), g = slow_load(a.src[kDO], b, i, h, part, D);
@@ -695,7 +696,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
     } else {
         to = a.to + (((int64_t)b * a.s.queries + i) * a.s.heads + h) * D;
         factor = l == 0.f ? 0.f : 1.f / l;
-        if (half == 0 && a.to_lse) a.to_lse[row] = l == 0.f ? kNone : (m + __builtin_amdgcn_logf(l) - kPBits) * kLn2;
+        // The 2^7 goes before the logarithm, which it would make larger and so coarser: an error here is one of all of the row's probabilities backward ([1,500..2000] 7e-7, so 3e-7)
+        if (half == 0 && a.to_lse) a.to_lse[row] = l == 0.f ? kNone : fmaf(m, kLn2, logf(l * (1.f / 128.f)));
     }
     const float inv_v = power_inverse(__int_as_float(unit)); // (by itself: its product with the factor may be too small for a float)
 #pragma unroll
@@ -738,14 +740,17 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, D = a.s.dim;
     const int pad_q = row_pad(a.s.queries), pad_k = row_pad(a.s.keys), k_blocks = pad_k / kRowPad;
     int bh, block;
-    head_and_block(id, a.s.batch * a.s.heads, k_blocks, a.s.causal, false, &bh, &block);
+    const int run = id % a.query_runs;
+    head_and_block(id / a.query_runs, a.s.batch * a.s.heads, k_blocks, a.s.causal, false, &bh, &block);
     const int b = bh / a.s.heads, h = bh % a.s.heads, hk = h / a.s.group, bk = b * a.s.kv_heads + hk;
     const int length = __builtin_amdgcn_readfirstlane(attn_length(a.s, b)), start = __builtin_amdgcn_readfirstlane(attn_start(a.s, b)), keys = used_keys(a.s, length, start);
     const int j0 = block * kRowPad + wave * 32, j = j0 + (lane & 31);
     // query i sees key j when i >= j - start and j < length
     const int see = a.s.causal ? j - start : 0;
     const int block_first = a.s.causal && block * kRowPad - start > 0 ? block * kRowPad - start : 0;
-    const int t0 = block_first / 32, t1 = block * kRowPad < keys ? (a.s.queries + 31) / 32 : 0;
+    const int first = block_first / 32, end = block * kRowPad < keys ? (a.s.queries + 31) / 32 : 0, per = end > first ? (end - first + a.query_runs - 1) / a.query_runs : 0;
+    const int t0 = first + run * per, t1 = t0 + per < end ? t0 + per : end;
+    const int64_t run_at = (int64_t)run * a.s.batch * a.s.heads * a.s.keys * D;
 
     const f32x4 head_q = a.head[kQ][bh], head_k = a.head[kK][bk], head_v = a.head[kV][bk], head_g = a.head[kDO][bh];
     if (__builtin_amdgcn_readfirstlane(beyond(a, head_q, head_k, head_v) || head_g[2] > 0.f)) {
@@ -753,12 +758,12 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
         for (int r = lane / L; r < 32 && __any(j0 + r < a.s.keys); r += 64 / L) {
             f32x4 x, y;
             const int key = j0 + r, d = 4 * (lane % L);
-            slow_dkv<L>(a, b, h, key, length, start, x, y);
+            slow_dkv<L>(a, b, h, key, length, start, t0 * 32, t1 * 32 < a.s.queries ? t1 * 32 : a.s.queries, x, y);
             if (key >= a.s.keys) continue;
             x *= a.s.scale;
             if (a.part_k) {
-                store_part(a.part_k + ((int64_t)bh * a.s.keys + key) * D, d, D, x);
-                store_part(a.part_v + ((int64_t)bh * a.s.keys + key) * D, d, D, y);
+                store_part(a.part_k + run_at + ((int64_t)bh * a.s.keys + key) * D, d, D, x);
+                store_part(a.part_v + run_at + ((int64_t)bh * a.s.keys + key) * D, d, D, y);
                 continue;
             }
             if (a.grad_k.p) store_gradient(a.grad_k, b * a.grad_k.b + hk * a.grad_k.h + key * a.grad_k.s, d, D, x, a.accumulate);
@@ -860,7 +865,7 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
     if (j >= a.s.keys) return;
     const float inv_ds = 1.f / ds_up, inv_q = 1.f / scale_q, inv_dv = 1.f / 16384.f / scale_g; // (one after the other: their product may be too small for a float)
     const int64_t at_k = b * a.grad_k.b + hk * a.grad_k.h + j * a.grad_k.s, at_v = b * a.grad_v.b + hk * a.grad_v.h + j * a.grad_v.s;
-    const int64_t at_part = ((int64_t)bh * a.s.keys + j) * D;
+    const int64_t at_part = run_at + ((int64_t)bh * a.s.keys + j) * D;
 #pragma unroll
     for (int d = 0; d < T::ND; ++d)
 #pragma unroll
@@ -886,21 +891,26 @@ __device__ __forceinline__ void tile_dq(const TileArgs& a, int id, float* lds) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, D = a.s.dim;
     const int pad_q = row_pad(a.s.queries), pad_k = row_pad(a.s.keys), q_blocks = pad_q / kRowPad;
     int bh, block;
-    head_and_block(id, a.s.batch * a.s.heads, q_blocks, a.s.causal, true, &bh, &block);
+    const int run = id % a.key_runs;
+    head_and_block(id / a.key_runs, a.s.batch * a.s.heads, q_blocks, a.s.causal, true, &bh, &block);
     const int b = bh / a.s.heads, h = bh % a.s.heads, bk = b * a.s.kv_heads + h / a.s.group;
     const int length = __builtin_amdgcn_readfirstlane(attn_length(a.s, b)), start = __builtin_amdgcn_readfirstlane(attn_start(a.s, b));
     const int q0 = block * kRowPad + wave * 32, i = q0 + (lane & 31);
     const int limit = i < a.s.queries ? attn_limit(length, start, i) : 0;
     const int wave_last = q0 + 31 < a.s.queries ? q0 + 31 : a.s.queries - 1, block_last = (block + 1) * kRowPad < a.s.queries ? (block + 1) * kRowPad - 1 : a.s.queries - 1;
     const int wave_least = wave_last == q0 + 31 ? attn_limit(length, start, q0) : 0;
-    const int tiles = (attn_limit(length, start, block_last) + 31) / 32;
+    const int tiles = (attn_limit(length, start, block_last) + 31) / 32, per = (tiles + a.key_runs - 1) / a.key_runs;
+    const int t0 = run * per < tiles ? run * per : tiles, t1 = t0 + per < tiles ? t0 + per : tiles;
+    float* const part = a.part_q ? a.part_q + ((int64_t)run * a.s.batch * a.s.heads + bh) * a.s.queries * D : nullptr;
 
     const f32x4 head_q = a.head[kQ][bh], head_k = a.head[kK][bk], head_v = a.head[kV][bk], head_g = a.head[kDO][bh];
     if (__builtin_amdgcn_readfirstlane(beyond(a, head_q, head_k, head_v) || head_g[2] > 0.f)) {
         constexpr int L = T::LANES;
         for (int r = q0; r < q0 + 32 && r < a.s.queries; ++r) {
-            const f32x4 x = slow_dq<L>(a, b, h, r, attn_limit(length, start, r), a.lse[(int64_t)bh * a.s.queries + r], a.stats[(int64_t)bh * pad_q + r][1]);
-            if (lane < L) store_gradient(a.grad_q, b * a.grad_q.b + h * a.grad_q.h + r * a.grad_q.s, 4 * lane, D, x * a.s.scale, a.accumulate);
+            const int most = attn_limit(length, start, r), hi = t1 * 32 < most ? t1 * 32 : most;
+            const f32x4 x = slow_dq<L>(a, b, h, r, t0 * 32, hi, a.lse[(int64_t)bh * a.s.queries + r], a.stats[(int64_t)bh * pad_q + r][1]);
+            if (part && lane < L) store_part(part + (int64_t)r * D, 4 * lane, D, x * a.s.scale);
+            else if (lane < L) store_gradient(a.grad_q, b * a.grad_q.b + h * a.grad_q.h + r * a.grad_q.s, 4 * lane, D, x * a.s.scale, a.accumulate);
         }
         return;
     }
@@ -924,13 +934,13 @@ __device__ __forceinline__ void tile_dq(const TileArgs& a, int id, float* lds) {
     f32x16 dq[T::ND];
 #pragma unroll
     for (int d = 0; d < T::ND; ++d) dq[d] = zero16();
-    if (tiles > 0) load(0, 0);
-    if (STAGES == 3 && tiles > 1) load(1, 1);
+    if (t0 < t1) load(t0, 0);
+    if (STAGES == 3 && t0 + 1 < t1) load(t0 + 1, 1);
     int stage = 0;
-    for (int t = 0; t < tiles; ++t) {
-        if (STAGES == 3 && t + 1 < tiles) stage_barrier<LOADS>();
+    for (int t = t0; t < t1; ++t) {
+        if (STAGES == 3 && t + 1 < t1) stage_barrier<LOADS>();
         else stage_barrier<0>();
-        if (t + STAGES - 1 < tiles) load(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+        if (t + STAGES - 1 < t1) load(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
         const char* k_tile = (const char*)lds + stage * 2 * T::BYTES;
         const char* v_tile = k_tile + T::BYTES;
         stage = stage == STAGES - 1 ? 0 : stage + 1;
@@ -980,7 +990,8 @@ __device__ __forceinline__ void tile_dq(const TileArgs& a, int id, float* lds) {
             f32x4 x;
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = dq[d][4 * q + e] * a.s.scale * inv_k * inv_ds;
-            store_gradient(a.grad_q, at_q, 32 * d + 8 * q + 4 * half, D, x, a.accumulate);
+            if (part) store_part(part + (int64_t)i * D, 32 * d + 8 * q + 4 * half, D, x);
+            else store_gradient(a.grad_q, at_q, 32 * d + 8 * q + 4 * half, D, x, a.accumulate);
         }
 }
 
@@ -992,20 +1003,24 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_tile_backward_kern
     else tile_dq<DP>(a, blockIdx.x - key_blocks, lds);
 }
 
-// dK and dV of a key head: the parts of the query heads that share it, in order
-__global__ __launch_bounds__(256) void attn_group_kernel(const TileArgs a) {
-    const int D = a.s.dim, quads = (D + 3) / 4;
-    const AttnOperand g{blockIdx.y ? a.grad_v.p : a.grad_k.p, blockIdx.y ? a.grad_v.b : a.grad_k.b, blockIdx.y ? a.grad_v.s : a.grad_k.s,
-                        blockIdx.y ? a.grad_v.h : a.grad_k.h, blockIdx.y ? a.grad_v.d : a.grad_k.d};
-    if (!g.p) return;
-    const float* __restrict part = blockIdx.y ? a.part_v : a.part_k;
-    const int64_t all = (int64_t)a.s.batch * a.s.kv_heads * a.s.keys * quads;
+// The parts of dK, dV (of the query heads that share a key head) and dQ, in order: blockIdx.y
+__global__ __launch_bounds__(256) void attn_parts_kernel(const TileArgs a) {
+    const int D = a.s.dim, quads = (D + 3) / 4, which = blockIdx.y;
+    const bool keys = which < 2;
+    const float* __restrict part = which == 0 ? a.part_k : which == 1 ? a.part_v : a.part_q;
+    const AttnOperand g{which == 0 ? a.grad_k.p : which == 1 ? a.grad_v.p : a.grad_q.p, which == 0 ? a.grad_k.b : which == 1 ? a.grad_v.b : a.grad_q.b,
+                        which == 0 ? a.grad_k.s : which == 1 ? a.grad_v.s : a.grad_q.s, which == 0 ? a.grad_k.h : which == 1 ? a.grad_v.h : a.grad_q.h,
+                        which == 0 ? a.grad_k.d : which == 1 ? a.grad_v.d : a.grad_q.d};
+    if (!g.p || !part) return;
+    const int heads = keys ? a.s.kv_heads : a.s.heads, rows = keys ? a.s.keys : a.s.queries, group = keys ? a.s.group : 1, runs = keys ? a.query_runs : a.key_runs;
+    const int64_t all = (int64_t)a.s.batch * heads * rows * quads, run_at = (int64_t)a.s.batch * a.s.heads * rows * D;
     for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.x * 256) {
         const int d = (int)(x % quads) * 4;
-        const int64_t row = x / quads, bk = row / a.s.keys, j = row - bk * a.s.keys, b = bk / a.s.kv_heads, hk = bk - b * a.s.kv_heads;
-        const float* p = part + (((b * a.s.heads + hk * a.s.group) * a.s.keys) + j) * D;
-        f32x4 sum = attn_load4<kLoadAny>(p, 1, d / 4, D);
-        for (int i = 1; i < a.s.group; ++i) sum += attn_load4<kLoadAny>(p + (int64_t)i * a.s.keys * D, 1, d / 4, D);
+        const int64_t row = x / quads, bh = row / rows, j = row - bh * rows, b = bh / heads, hk = bh - b * heads;
+        const float* p = part + ((b * a.s.heads + hk * group) * rows + j) * D;
+        f32x4 sum{0.f, 0.f, 0.f, 0.f};
+        for (int run = 0; run < runs; ++run)
+            for (int i = 0; i < group; ++i) sum += attn_load4<kLoadAny>(p + run * run_at + (int64_t)i * rows * D, 1, d / 4, D);
         store_gradient(g, b * g.b + hk * g.h + j * g.s, d, D, sum, a.accumulate);
     }
 }
@@ -1054,11 +1069,13 @@ void launch_backward(const TileArgs& a, hipStream_t stream) {
     const int64_t rows = 2LL * s.batch * ((int64_t)s.heads * row_pad(s.queries) + (int64_t)s.kv_heads * row_pad(s.keys));
     hipLaunchKernelGGL(attn_amax_kernel<L>, dim3((unsigned)(all_heads(s) * a.parts)), dim3(256), 0, stream, a);
     hipLaunchKernelGGL(attn_split_kernel<DP>, dim3((unsigned)(rows / 64)), dim3(256), 0, stream, a);
-    const int blocks_of_keys = a.grad_k.p || a.grad_v.p ? s.batch * s.heads * (row_pad(s.keys) / kRowPad) : 0, blocks_of_queries = a.grad_q.p ? s.batch * s.heads * (row_pad(s.queries) / kRowPad) : 0;
+    const int blocks_of_keys = a.grad_k.p || a.grad_v.p ? s.batch * s.heads * (row_pad(s.keys) / kRowPad) * a.query_runs : 0;
+    const int blocks_of_queries = a.grad_q.p ? s.batch * s.heads * (row_pad(s.queries) / kRowPad) * a.key_runs : 0;
     hipLaunchKernelGGL(attn_tile_backward_kernel<DP>, dim3((unsigned)(blocks_of_keys + blocks_of_queries)), dim3(256), 0, stream, a, blocks_of_keys);
-    if ((a.grad_k.p || a.grad_v.p) && a.part_k) {
-        const int64_t quads = (int64_t)s.batch * s.kv_heads * s.keys * ((s.dim + 3) / 4);
-        hipLaunchKernelGGL(attn_group_kernel, dim3((unsigned)std::min<int64_t>((quads + 255) / 256, 4096), 2), dim3(256), 0, stream, a);
+    const bool keys = a.part_k && blocks_of_keys, queries = a.part_q && blocks_of_queries;
+    if (keys || queries) {
+        const int64_t quads = (int64_t)s.batch * ((s.dim + 3) / 4) * std::max(keys ? (int64_t)s.kv_heads * s.keys : 0, queries ? (int64_t)s.heads * s.queries : 0);
+        hipLaunchKernelGGL(attn_parts_kernel, dim3((unsigned)std::min<int64_t>((quads + 255) / 256, 4096), queries ? 3 : 2), dim3(256), 0, stream, a);
     }
 }
 
@@ -1085,7 +1102,7 @@ void attn_tiles_forward(const AttnShape& s, const AttnOperand& q, const AttnOper
     if (a.splits > 1) attn_join(s, a.part, a.splits, out, lse, stream);
 }
 
-void attn_tiles_backward(const AttnBackward& b, Workspace& ws, hipStream_t stream, bool launch) {
+void attn_tiles_backward(const AttnBackward& b, Workspace& ws, int cus, hipStream_t stream, bool launch) {
     TileArgs a{};
     a.s = b.s;
     a.src[kQ] = b.q; a.src[kK] = b.k; a.src[kV] = b.v;
@@ -1094,10 +1111,21 @@ void attn_tiles_backward(const AttnBackward& b, Workspace& ws, hipStream_t strea
     a.grad_q = b.grad_q; a.grad_k = b.grad_k; a.grad_v = b.grad_v; a.accumulate = b.accumulate;
     plan_operands(a, ws);
     a.stats = ws.take<f32x2>((int64_t)b.s.batch * b.s.heads * row_pad(b.s.queries) + kRowPad);
-    if (b.s.group > 1) {
-        a.part_k = ws.take<float>((int64_t)b.s.batch * b.s.heads * b.s.keys * b.s.dim);
-        a.part_v = ws.take<float>((int64_t)b.s.batch * b.s.heads * b.s.keys * b.s.dim);
+    // A sum over many tiles is cut into runs, whose parts are added afterwards in order, for two reasons.  Few heads with few blocks leave CUs without a workgroup: runs are no longer than what three
+    // workgroups a CU would do if all tiles were dealt evenly (a tile of queries for a block of keys is four products, one of keys for a block of queries three), and 8 tiles at least, or the parts
+    // cost more.  Whole sums: [1,8192,8,64] for 500 keys 427 us, [1,2048,4,64] causal 121 us, [1,3000,6/2,128] 420 us; in runs 147, 66 and 386; with two workgroups a CU 141, 72 and 420, with four
+    // 149, 68 and 375.  And the accumulators round at each product, three for 16 rows: dK of 8192 queries has an error of 1.2e-6 of itself (2-norm) in one sum, and 0.9e-6 in runs of 128 tiles at the
+    // most; those cost 4 to 6 % ([1,8192,16/4,128] causal 2750 -> 2890 us).  No more than four of them for this, since their parts take memory.
+    const double heads = (double)b.s.batch * b.s.heads, query_tiles = (b.s.queries + 31) / 32, key_tiles = (b.s.keys + 31) / 32;
+    const double even = std::max(8.0, heads * (row_pad(b.s.keys) / kRowPad * query_tiles * 4.0 / 3.0 + row_pad(b.s.queries) / kRowPad * key_tiles) / (3.0 * cus));
+    auto runs = [&](double tiles) { return (int)std::max({1.0, tiles / even, std::min(4.0, std::ceil(tiles / 128))}); };
+    a.query_runs = runs(query_tiles);
+    a.key_runs = runs(key_tiles);
+    if (b.s.group > 1 || a.query_runs > 1) {
+        a.part_k = ws.take<float>(a.query_runs * (int64_t)b.s.batch * b.s.heads * b.s.keys * b.s.dim);
+        a.part_v = ws.take<float>(a.query_runs * (int64_t)b.s.batch * b.s.heads * b.s.keys * b.s.dim);
     }
+    if (a.key_runs > 1) a.part_q = ws.take<float>(a.key_runs * (int64_t)b.s.batch * b.s.heads * b.s.queries * b.s.dim);
     if (!launch) return;
     switch (padded_dim(b.s.dim)) {
         case 32: launch_backward<32, 8>(a, stream); break;

@@ -250,6 +250,62 @@ def test_attention(ops, case):
         assert [s is not None for s in some] == [i == skip for i in range(3)] and torch.equal(down(some[skip]), down(got[skip]))
 
 
+@pytest.mark.parametrize("case", [
+    (1, 2100, 130, 2, 1, 20, False, None, None),    # the queries of a block of keys in runs
+    (2, 1111, 257, 3, 3, 64, True, [257, 100], [-200, -1000]),
+    (1, 150, 3001, 2, 2, 40, True, [2900], [2000]),  # the keys of a block of queries in runs
+    (1, 1025, 1300, 4, 2, 128, True, None, None),   # both
+    (2, 900, 900, 2, 1, 96, True, [900, 0], None),
+], ids=lambda c: "-".join(str(x) for x in c[:7]))
+@pytest.mark.parametrize("bad", [None, "k", "q"])
+def test_attention_gradients_in_runs(ops, case, bad):
+    """Few heads: the parts of the runs add up, also into what is there, one gradient at a time, and for heads that are computed value by value (a value far out, of which p is nearly zero)."""
+    causal, lengths, starts = case[6:]
+    q, k, v, dout = attention_case(17, case)
+    if bad == "k":
+        k[0, 77, 0, 3] = 1.0e9
+        q[0, :, :case[3] // case[4], 3] = -q[0, :, :case[3] // case[4], 3].abs() - 0.01  # (so that the key has no weight)
+    elif bad == "q":
+        dout[0, 33, 0, 0] = 3.0e8
+    scale = 1.1 / math.sqrt(case[5])
+    want, _, grads = attention_reference(q, k, v, scale, causal, lengths, starts, dout)
+    Q, K, V, DO = (up(ops, t) for t in (q, k, v, dout))
+    mask = dict(scale=scale, causal=causal, key_lengths=ints(lengths), query_starts=ints(starts))
+    o, lse = ops.A.attention(Q, K, V, **mask)
+    close(down(o), want, RTOL_FRO, "out")
+    got = ops.A.attention_backward(Q, K, V, o, lse, DO, **mask)
+    base = [randn(40 + i, *t.shape) for i, t in enumerate((q, k, v))]
+    for skip, (g, ref, what) in enumerate(zip(got, grads, ("grad_q", "grad_k", "grad_v"))):
+        close(down(g), ref, 2 * RTOL_FRO, what)
+        some = ops.A.attention_backward(Q, K, V, o, lse, DO, need=[i == skip for i in range(3)], **mask)
+        assert torch.equal(down(some[skip]), down(g))
+    into = [up(ops, t) for t in base]
+    ops.A.attention_backward(Q, K, V, o, lse, DO, into=into, **mask)
+    for g, i, t in zip(got, into, base):
+        assert torch.equal(down(i), down(g) + t)
+
+
+def test_attention_gradients_of_long_sums(ops):
+    """Runs of 128 tiles at the most: the sums over a run round six times a tile, by half a step of the sum so far, which grows as a random walk does: sqrt(6 * 128 / 2) 2^-24 of the result."""
+    B, n, m, H, Hk, D = 1, 8192, 4000, 8, 2, 32
+    q, k, v, dout = (t.cuda() for t in attention_case(23, (B, n, m, H, Hk, D)))
+    Q, K, V, DO = (up(ops, t) for t in (q, k, v, dout))
+    o, lse = ops.A.attention(Q, K, V, scale=0.1)
+    got = [down(t) for t in ops.A.attention_backward(Q, K, V, o, lse, DO, scale=0.1)]
+    q, k, v, dout = (t.double().transpose(1, 2)[0].contiguous() for t in (q, k, v, dout))  # [heads, rows, D]
+    want = [torch.zeros_like(t) for t in (q, k, v)]
+    for h in range(H):
+        kk, vv = k[h * Hk // H], v[h * Hk // H]
+        p = torch.softmax(0.1 * (q[h] @ kk.t()), -1)
+        want[2][h * Hk // H] += p.t() @ dout[h]
+        ds = p * (dout[h] @ vv.t())
+        ds -= p * ds.sum(-1, keepdim=True)
+        want[0][h] = 0.1 * (ds @ kk)
+        want[1][h * Hk // H] += 0.1 * (ds.t() @ q[h])
+    for g, ref, what in zip(got, want, ("grad_q", "grad_k", "grad_v")):
+        close(g, ref.transpose(0, 1)[None].cpu().numpy(), math.sqrt(6 * 128 / 2) * 2.0 ** -24, what)
+
+
 @pytest.mark.parametrize("n", [1, 40, 150, 600])
 def test_attention_of_strided_operands(ops, n):
     """Slices of a joint projection, heads before positions, every second value of d, a batch that is one sequence repeated (stride 0)."""

@@ -87,6 +87,7 @@ def test_attention_refusals():
     refused(ARGUMENT, "null out, lse or dOut", backward(out=None))
     refused(SHAPE, "multiple", L.tenmo_hip_attention_forward_workspace_bytes(1, 1, 1, 3, 2, 16))
     refused(SHAPE, "multiple", L.tenmo_hip_attention_backward_workspace_bytes(-1, 1, 1, 2, 2, 16))
+    refused(UNSUPPORTED, "2^28", L.tenmo_hip_attention_backward_workspace_bytes(1, 8, (1 << 22) + 1, 64, 8, 16))
 
 
 def test_vocabulary_loss_refusals():

@@ -821,6 +821,40 @@ def test_captured_graphs(ops):
     assert all(torch.equal(x, y) for x, y in zip(bits(graphs[0][1]), want[1]))
 
 
+def test_a_captured_attention_whose_sums_run_in_parts(ops):
+    """Few heads, many rows: workspaces with the parts of each run, of two graphs replayed in turn and of eager calls between them."""
+    def call(s):
+        o, lse = ops.A.attention(s[0], s[1], s[2], causal=True)
+        return [o, lse, *ops.A.attention_backward(s[0], s[1], s[2], o, lse, s[3], causal=True)]
+
+    def state(seed):
+        return [up(ops, x) for x in attention_case(seed, (1, 1200, 900, 4, 2, 64))]
+
+    states = [state(seed) for seed in (50, 60)]
+    want = [bits(call(s)) for s in states]
+    torch.cuda.synchronize()
+    graphs = []
+    for s in states:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call(s)
+        graphs.append((g, out))
+    for turn in range(4):
+        for (g, out), ref in zip(graphs, want):
+            for o in out:
+                o.storage.fill_(7.0)
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(bits(out), ref)), turn
+        call(state(70 + turn))
+        torch.cuda.synchronize()
+    for g, _ in graphs:  # one behind the other, without a wait between them
+        g.replay()
+    torch.cuda.synchronize()
+    for (_, out), ref in zip(graphs, want):
+        assert all(torch.equal(x, y) for x, y in zip(bits(out), ref))
+
+
 def test_a_workspace_that_is_too_small_is_refused(ops):
     import ctypes as C
 

@@ -18,8 +18,15 @@
 // zeros too, whatever the operand holds there.
 //   * forward, K and V in one launch: 64 rows have a scale of their own (one read, where a scale of the whole head takes a launch before: [8,1024,12,64] 84 -> 71 us, [4,777,16,80] 73 -> 59).
 //     A wavefront's own rows of q are split as they are read, with a scale of their own each.
-//   * backward, all four in two launches: the largest magnitude of each head (of the rows that count), then the halves.
-// dS has |dS| <= 2 max |dO_i| max |V_j| (norms of rows), which gives its scale before it is known.
+//   * backward, all four in two launches: the largest magnitudes (of the rows that count), then the halves, with one scale a head for Q, K and V and one a row for dO.
+//
+// What a row of a gradient is summed from is held to the row's own sizes, however small they are against the head's (with one scale a head, keys of a weight of e^-18 got dK to 0.1 of itself,
+// and rows of dQ where dO is 2^-20 of the head's largest to 0.05):
+//   * a row of dO that is small against the head's largest has a scale a_i of its own, and P is taken times A / a_i (A: the head's scale): P dO is the same, and what the row adds is small in P
+//     instead.  The factor goes into the row's lse.
+//   * P and dS have a scale for each row of the result, which is a lane: a power of two that brings the largest so far into 2^10 .. 2^15, renewed, with the sums, when one passes it.
+//     Since it is known only when a tile is done, it costs a maximum of the tile's 16 values and a branch (the kernel at [8,1024,12,64] 187 us with and without, at [1,8192,16/4,128] 2967 and
+//     2960; with 2^12 in place of 2^10 scales are renewed more often: 194 and 3150, and with sums moved by the compiler, see scale_sums, 200 and 3670).
 //
 // LDS tile: 32 rows of DP / 4 chunks of 16 bytes, chunk c = 2 * (d / 8) + kind at slot c ^ swizzle(row); read by rows (16 bytes a lane: 16 rows in 16 different slots of the
 // banks) and by columns (the transposing read: 4 rows x 4 chunks in 16 different slots).
@@ -41,6 +48,10 @@ __host__ __device__ constexpr int row_pad(int n) { return (n + kRowPad - 1) / kR
 
 enum { kK, kV, kQ, kDO }; // forward the first two are split beforehand, backward all of them
 
+// Of a row of queries, backward, with a_i the scale of the row of dO and A the head's: lse log2(e) + log2(a_i / A) (+inf where there is no lse: no probability), dO . O times a_i / A, A / a_i, dO . O
+enum { kLseUp, kDeltaUp, kDown, kDelta, kStats };
+__device__ __forceinline__ int64_t stat_at(int64_t row, int which) { return (row >> 5) * (32 * kStats) + which * 32 + (row & 31); }
+
 struct TileArgs {
     AttnShape s;
     AttnOperand src[4];
@@ -48,9 +59,9 @@ struct TileArgs {
     float* split[4];    // [batch][heads][rows padded][DP]
     f32x4* seen[4];     // [batch * heads][parts]: of a run of rows, the largest finite magnitude, the largest norm of a row, the smallest largest magnitude of a row
                         // that is not zero, and 1 if there is a value that is not finite
-    f32x4* head[4];     // [batch * heads]: scale, largest norm of a row, 1 if the halves do not hold this head
+    f32x4* head[4];     // [batch * heads]: scale, largest norm of a row, 1 if the halves do not hold this head (backward)
     const float *out, *lse;
-    f32x2* stats;        // [batch][heads][queries padded] (and 128 behind the last): lse log2(e) (+inf where there is none: no probability), and dO . O
+    float* stats;        // backward, [batch][heads][queries padded / 32][kStats][32] (and 4 tiles behind the last)
     // forward
     float* scale[2];     // [batch * heads][blocks of 64 rows]: 1 / the scale of K, the scale of V or 0 where there are zeros alone; `seen` is of these blocks too
     float *to, *to_lse, *part;
@@ -101,7 +112,10 @@ __device__ __forceinline__ HeadJob head_job(const TileArgs& a, int y) {
     return j;
 }
 
-// What a run of a head's rows holds, and each row's lse and delta: L lanes a row, U rows in flight
+// of a power of two
+__device__ __forceinline__ float power_inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
+
+// What a run of a head's rows holds, and each row's lse, delta and largest magnitude of dO: L lanes a row, U rows in flight
 template <int L>
 __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
     constexpr int SLOTS = 64 / L, U = 4;
@@ -149,8 +163,12 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[u][e] = in ? o[u][e] : 0.f;
                 const float delta = lanes_sum<L>(dot4(x[u], o[u]));
-                if (part == 0 && r < last)
-                    a.stats[(int64_t)j.bh * j.pad + r] = in ? f32x2{a.lse[(int64_t)j.bh * a.s.queries + r] * kLog2e, delta} : f32x2{__builtin_inff(), 0.f};
+                if (part == 0 && r < last) {
+                    const int64_t row = (int64_t)j.bh * j.pad + r;
+                    a.stats[stat_at(row, kLseUp)] = in ? a.lse[(int64_t)j.bh * a.s.queries + r] * kLog2e : __builtin_inff();
+                    a.stats[stat_at(row, kDown)] = mine; // the next launch makes a scale of it
+                    a.stats[stat_at(row, kDelta)] = in ? delta : 0.f;
+                }
             }
         }
     }
@@ -165,9 +183,8 @@ __global__ __launch_bounds__(256) void attn_amax_kernel(const TileArgs a) {
 }
 
 // The halves of 64 rows, 8 values a thread; the first workgroup of a head leaves what the products need to know of it.
-// The halves hold a value to 2^-22 of itself and 2^-40 of the head's largest.  For keys and values that is taken while no row that is not zero is smaller than 2^-16 of the largest: 2^-24 of
-// each row's own.  Rows of q and dout, backward, enter scores, which need to be right against 1 (see beyond()), and sums over rows, which need to be right against the largest; rows of
-// theirs may be as small as 2^-24 of the largest (gradients of single positions are), with a dQ of their own to 2^-16 of itself there.
+// The halves hold a value to 2^-22 of itself and 2^-40 of the largest that has the same scale.  With one scale a head that is taken while no row that is not zero is smaller than 2^-16 of the
+// largest: 2^-24 of each row's own.  Rows of dout lie further apart (gradients of single positions do) and have a scale of their own.
 template <int DP>
 __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
     constexpr int GROUPS = DP / 8, ROWS = 64, N = ROWS * GROUPS / 256;
@@ -183,7 +200,7 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
     const float top = wave_max(s[0]), scale = split_scale(__float_as_uint(top));
     if (block == 0) {
         const float norm = wave_max(s[1]), least = -wave_max(-s[2]), wrong = wave_max(s[3]);
-        if (threadIdx.x == 0) j.head[j.bh] = f32x4{scale, norm, wrong > 0.f || top * (key ? 0x1p-16f : 0x1p-24f) > least ? 1.f : 0.f, 0.f};
+        if (threadIdx.x == 0) j.head[j.bh] = f32x4{scale, norm, wrong > 0.f || (j.job != kDO && top * 0x1p-16f > least) ? 1.f : 0.f, 0.f};
     }
     const float* p = j.src.p + j.b * j.src.b + j.h * j.src.h;
     f32x4 v[N][2];
@@ -195,6 +212,27 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
             for (int u = 0; u < 2; ++u) v[i][u] = attn_load4<kind.value>(p + at * j.src.s, j.src.d, x % GROUPS * 2 + u, a.s.dim);
         }
     });
+    float scales[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) scales[i] = scale;
+    if (j.job == kDO) { // (in the whole workgroup)
+#pragma unroll
+        for (int i = 0; i < N; ++i) { // (at most 2^120 times the head's, so that the quotient of the two is a float; 2^-12 of the largest is held to 2^-28 by the head's)
+            const float mine = a.stats[stat_at((int64_t)j.bh * j.pad + block * ROWS + (threadIdx.x + 256 * i) / GROUPS, kDown)];
+            if (mine > 0.f && mine < top * 0x1p-12f) scales[i] = fminf(split_scale(__float_as_uint(mine)), scale * 0x1p120f);
+        }
+        __syncthreads(); // each row's magnitude is read by all of its threads before one of them writes in its place
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int x = threadIdx.x + 256 * i;
+            if (x % GROUPS) continue;
+            const int64_t row = (int64_t)j.bh * j.pad + block * ROWS + x / GROUPS;
+            const float up = scales[i] * power_inverse(scale);
+            a.stats[stat_at(row, kLseUp)] += (float)((int)(__float_as_uint(up) >> 23) - 127);
+            a.stats[stat_at(row, kDeltaUp)] = a.stats[stat_at(row, kDelta)] * up;
+            a.stats[stat_at(row, kDown)] = power_inverse(up);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int x = threadIdx.x + 256 * i, r = block * ROWS + x / GROUPS;
@@ -203,7 +241,7 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             _Float16 hi16, lo16;
-            split_value(in ? v[i][e >> 2][e & 3] * scale : 0.f, hi16, lo16);
+            split_value(in ? v[i][e >> 2][e & 3] * scales[i] : 0.f, hi16, lo16);
             h[e] = hi16;
             l[e] = lo16;
         }
@@ -213,8 +251,6 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
     }
 }
 
-// of a power of two
-__device__ __forceinline__ float power_inverse(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
 __device__ __forceinline__ float lane_value(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
 
 // Forward, K and V in one launch: a workgroup reads 64 rows, 4 values a lane and L lanes a row, and gives them a scale of their own.
@@ -296,7 +332,7 @@ __device__ __forceinline__ bool keys_beyond(const TileArgs& a, int bk) {
 }
 
 // Heads beyond the halves are worked on row by row in fp32, where nothing that is not allowed can leave a trace: those with keys or values that are not finite, or of sizes too far apart;
-// and backward the same of q and dout, and scores above 2^16 (|q| |k| scale; with one scale for all rows of q their error would pass 2^-24).
+// and backward the same of q, dout that is not finite, and scores above 2^16 (|q| |k| scale; with one scale for all rows of q their error would pass 2^-24).
 __device__ __forceinline__ bool beyond(const TileArgs& a, f32x4 q, f32x4 k, f32x4 v) { return q[2] + k[2] + v[2] > 0.f || !(q[1] * k[1] * fabsf(a.s.scale) < 65536.f); }
 
 __device__ __forceinline__ void store_part(float* to, int d, int D, f32x4 x) {
@@ -379,7 +415,7 @@ __device__ __forceinline__ void slow_dkv(const TileArgs& a, int b, int h, int j,
         if (j < limit) {
             const float p = __expf(x - a.lse[bh * a.s.queries + i]);
             dv += p * g;
-            dk += p * (dp - a.stats[bh * row_pad(a.s.queries) + i][1]) * q;
+            dk += p * (dp - a.stats[stat_at(bh * row_pad(a.s.queries) + i, kDelta)]) * q;
         }
     }
 }
@@ -714,11 +750,40 @@ __global__ __launch_bounds__(256, 2) void attn_tile_forward_kernel(const TileArg
 
 // ---- backward ------------------------------------------------------------------------------------------------------------------------
 
-// 2^15 over the largest that |dS| can be, as a power of two, from the norms of dout and v
-__device__ __forceinline__ float ds_scale(float norm_g, float norm_v) {
-    const int e = (int)(__float_as_uint(fminf(2.f * norm_g * norm_v, 1e38f)) >> 23) - 127 + 1; // the bound is below 2^e
-    const int up = 15 - e;
-    return __uint_as_float((uint32_t)((up > 126 ? 126 : up) + 127) << 23);
+// The scale of what a lane's sums are made of: brings the largest so far into 2^10 .. 2^15
+struct Unit {
+    float scale = 0x1p126f, most = 0x1p-111f; // most: 2^15 / scale
+    // for a larger one (of both halves of the wavefront); gives what the sums are to be multiplied by
+    __device__ __forceinline__ float renew(float top) {
+        const int e = (int)(__float_as_uint(top) >> 23) - 127; // of top: -111 .. 128 where it is too large
+        const float now = top > most ? __uint_as_float((uint32_t)(10 - e + 127) << 23) : scale, by = now * power_inverse(scale);
+        scale = now;
+        most = 0x1p15f * power_inverse(now);
+        return by;
+    }
+};
+
+// Sums that lie in accumulation registers stay there: a plain product would have the compiler move them, or what it moves for them, in every tile (113 moves of 361 instructions at DP = 128).
+// Before the first read: the wait states behind a matrix instruction that wrote them; behind the last write: those before one that reads them.
+template <bool ACCUMULATION, int N>
+__device__ __forceinline__ void scale_sums(f32x16 (&x)[N], float by) {
+    if constexpr (ACCUMULATION) {
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+        for (int d = 0; d < N; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float v = x[d][e], t;
+                asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32_e32 %1, %2, %1\n\tv_accvgpr_write_b32 %0, %1" : "+a"(v), "=&v"(t) : "v"(by));
+                x[d][e] = v;
+            }
+        asm volatile("s_nop 7" ::: "memory");
+    } else {
+#pragma unroll
+        for (int d = 0; d < N; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[d][e] *= by;
+    }
 }
 
 __device__ __forceinline__ void store_gradient(const AttnOperand& g, int64_t at, int d, int D, f32x4 x, int accumulate) {
@@ -730,7 +795,7 @@ __device__ __forceinline__ void store_gradient(const AttnOperand& g, int64_t at,
 
 template <int DP>
 struct Backward {
-    static constexpr int STAGES = DP <= 64 ? 3 : 2, STAGE = 2 * Tile<DP>::BYTES + 1024; // two tiles, and the rows' lse and delta
+    static constexpr int STAGES = DP <= 64 ? 3 : 2, STAGE = 2 * Tile<DP>::BYTES + 1024; // two tiles, and what is known of the rows
 };
 
 template <int DP>
@@ -774,17 +839,17 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
     f16x8 kh[T::KD], kl[T::KD], vh[T::KD], vl[T::KD];
     own_rows<DP>(kh, kl, a.split[kK] + ((int64_t)bk * pad_k + j0) * DP, lane);
     own_rows<DP>(vh, vl, a.split[kV] + ((int64_t)bk * pad_k + j0) * DP, lane);
-    const float scale_q = head_q[0], scale_g = head_g[0], ds_up = ds_scale(head_g[1], head_v[1]);
+    const float scale_q = head_q[0], scale_g = head_g[0];
     const float c = a.s.scale * kLog2e / scale_q / head_k[0], inv_dp = 1.f / scale_g / head_v[0];
     const float* const base[2] = {a.split[kQ] + (int64_t)bh * pad_q * DP, a.split[kDO] + (int64_t)bh * pad_q * DP};
-    const float* const stats = (const float*)(a.stats + (int64_t)bh * pad_q);
+    const float* const stats = a.stats + (int64_t)bh * pad_q * kStats;
     uint32_t off[LOADS - 1];
     T::template offsets<2>(off, wave, lane);
     auto load = [&](int t, int stage) {
         const float* const src[2] = {base[0] + (int64_t)t * 32 * DP, base[1] + (int64_t)t * 32 * DP};
         T::template load<2>(lds, stage * STAGE, src, off, wave);
-        // the tile's 32 lse and delta, and 96 rows behind them that are not used: every wavefront brings the same
-        direct_load_16B(lds, stage * STAGE + 2 * T::BYTES, lane * 16, stats + (int64_t)t * 64);
+        // the tile's 32 rows, and the 32 behind them, which are not used: every wavefront brings the same
+        direct_load_16B(lds, stage * STAGE + 2 * T::BYTES, lane * 16, stats + (int64_t)t * (32 * kStats));
     };
     const uint32_t row_off[2] = {T::row_offset(lane, 0), T::row_offset(lane, 1)}, col_off[2] = {T::column_offset(lane, 0), T::column_offset(lane, 1)};
 
@@ -792,6 +857,7 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
     f32x16 dk[T::ND], dv[T::ND];
 #pragma unroll
     for (int d = 0; d < T::ND; ++d) dk[d] = dv[d] = zero16();
+    Unit unit_p, unit_s;
     if (t0 < t1) load(t0, 0);
     if (STAGES == 3 && t0 + 1 < t1) load(t0 + 1, 1);
     int stage = 0;
@@ -801,7 +867,7 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
         if (t + STAGES - 1 < t1) load(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
         const char* q_tile = (const char*)lds + stage * STAGE;
         const char* g_tile = q_tile + T::BYTES;
-        const f32x4* st = (const f32x4*)(g_tile + T::BYTES) + 2 * half; // two rows each
+        const f32x4* st = (const f32x4*)(g_tile + T::BYTES) + half; // four rows each
         stage = stage == STAGES - 1 ? 0 : stage + 1;
         const int i0 = t * 32;
 
@@ -811,9 +877,9 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
             split_mfma2(s, T::row_read(q_tile, row_off[0], ks), T::row_read(q_tile, row_off[1], ks), kh[ks], kl[ks],
                         dp, T::row_read(g_tile, row_off[0], ks), T::row_read(g_tile, row_off[1], ks), vh[ks], vl[ks]);
         }
-        f32x4 rows[8]; // lse and delta of the rows 8 q + 4 half + {0, 1}, {2, 3}
+        f32x4 lse[4], delta[4]; // of the rows 8 q + 4 half + 0..3
 #pragma unroll
-        for (int q = 0; q < 4; ++q) rows[2 * q] = st[4 * q], rows[2 * q + 1] = st[4 * q + 1];
+        for (int q = 0; q < 4; ++q) lse[q] = st[8 * kLseUp + 2 * q], delta[q] = st[8 * kDeltaUp + 2 * q];
         TENMO_READS(8);
 #pragma unroll
         for (int ks = 0; ks < T::KD - 2; ++ks) {
@@ -825,8 +891,8 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
         TENMO_PRODUCTS(6);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            s[e] = s[e] * c - rows[e >> 1][2 * (e & 1)];
-            dp[e] = dp[e] * inv_dp - rows[e >> 1][2 * (e & 1) + 1];
+            s[e] = s[e] * c - lse[e >> 2][e & 3];
+            dp[e] = dp[e] * inv_dp - delta[e >> 2][e & 3];
         }
         if (i0 < j0 + 31 - start || j0 + 32 > length) { // some pairs are not allowed: their p is 0, whatever the rest
             const int from = j < length ? see - i0 - 4 * half : 32;
@@ -837,12 +903,22 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
                 dp[e] = ok ? dp[e] : 0.f;
             }
         }
+        float top_p = 0.f, top_s = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const float p = __builtin_amdgcn_exp2f(s[e]);
-            dp[e] *= p * ds_up;
-            s[e] = p * 16384.f;
+            s[e] = __builtin_amdgcn_exp2f(s[e]);
+            dp[e] *= s[e];
+            top_p = fmaxf(top_p, s[e]);
+            top_s = fmaxf(top_s, fabsf(dp[e]));
         }
+        top_p = halves_max(top_p);
+        top_s = halves_max(top_s);
+        if (__any(top_p > unit_p.most || top_s > unit_s.most)) {
+            if (__any(top_p > unit_p.most)) scale_sums<(DP > 64)>(dv, unit_p.renew(top_p));
+            if (__any(top_s > unit_s.most)) scale_sums<(DP > 64)>(dk, unit_s.renew(top_s));
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] *= unit_p.scale, dp[e] *= unit_s.scale;
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
             f16x8 ph, pl, sh, sl;
@@ -863,7 +939,7 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
         TENMO_PRODUCTS(12);
     }
     if (j >= a.s.keys) return;
-    const float inv_ds = 1.f / ds_up, inv_q = 1.f / scale_q, inv_dv = 1.f / 16384.f / scale_g; // (one after the other: their product may be too small for a float)
+    const float inv_ds = power_inverse(unit_s.scale), inv_q = 1.f / scale_q, inv_p = power_inverse(unit_p.scale), inv_g = 1.f / scale_g; // (one after the other: their product may be too small for a float)
     const int64_t at_k = b * a.grad_k.b + hk * a.grad_k.h + j * a.grad_k.s, at_v = b * a.grad_v.b + hk * a.grad_v.h + j * a.grad_v.s;
     const int64_t at_part = run_at + ((int64_t)bh * a.s.keys + j) * D;
 #pragma unroll
@@ -873,7 +949,7 @@ __device__ __forceinline__ void tile_dkv(const TileArgs& a, int id, float* lds) 
             const int at = 32 * d + 8 * q + 4 * half;
             f32x4 x, y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = dk[d][4 * q + e] * a.s.scale * inv_q * inv_ds, y[e] = dv[d][4 * q + e] * inv_dv;
+            for (int e = 0; e < 4; ++e) x[e] = dk[d][4 * q + e] * a.s.scale * inv_q * inv_ds, y[e] = dv[d][4 * q + e] * inv_p * inv_g;
             if (a.part_k) {
                 store_part(a.part_k + at_part, at, D, x);
                 store_part(a.part_v + at_part, at, D, y);
@@ -908,7 +984,7 @@ __device__ __forceinline__ void tile_dq(const TileArgs& a, int id, float* lds) {
         constexpr int L = T::LANES;
         for (int r = q0; r < q0 + 32 && r < a.s.queries; ++r) {
             const int most = attn_limit(length, start, r), hi = t1 * 32 < most ? t1 * 32 : most;
-            const f32x4 x = slow_dq<L>(a, b, h, r, t0 * 32, hi, a.lse[(int64_t)bh * a.s.queries + r], a.stats[(int64_t)bh * pad_q + r][1]);
+            const f32x4 x = slow_dq<L>(a, b, h, r, t0 * 32, hi, a.lse[(int64_t)bh * a.s.queries + r], a.stats[stat_at((int64_t)bh * pad_q + r, kDelta)]);
             if (part && lane < L) store_part(part + (int64_t)r * D, 4 * lane, D, x * a.s.scale);
             else if (lane < L) store_gradient(a.grad_q, b * a.grad_q.b + h * a.grad_q.h + r * a.grad_q.s, 4 * lane, D, x * a.s.scale, a.accumulate);
         }
@@ -917,10 +993,9 @@ __device__ __forceinline__ void tile_dq(const TileArgs& a, int id, float* lds) {
     f16x8 qh[T::KD], ql[T::KD], gh[T::KD], gl[T::KD];
     own_rows<DP>(qh, ql, a.split[kQ] + ((int64_t)bh * pad_q + q0) * DP, lane);
     own_rows<DP>(gh, gl, a.split[kDO] + ((int64_t)bh * pad_q + q0) * DP, lane);
-    const float scale_k = head_k[0], ds_up = ds_scale(head_g[1], head_v[1]);
-    const float c = a.s.scale * kLog2e / head_q[0] / scale_k, inv_dp = 1.f / head_g[0] / head_v[0];
-    const f32x2 stats = a.stats[(int64_t)bh * pad_q + i];
-    const float lse2 = stats[0], delta = stats[1];
+    const float scale_k = head_k[0];
+    const float lse2 = limit > 0 ? a.lse[(int64_t)bh * a.s.queries + i] * kLog2e : __builtin_inff(), delta = a.stats[stat_at((int64_t)bh * pad_q + i, kDelta)];
+    const float c = a.s.scale * kLog2e / head_q[0] / scale_k, inv_dp = 1.f / head_g[0] / head_v[0] * a.stats[stat_at((int64_t)bh * pad_q + i, kDown)];
     const float* const base[2] = {a.split[kK] + (int64_t)bk * pad_k * DP, a.split[kV] + (int64_t)bk * pad_k * DP};
     uint32_t off[LOADS];
     T::template offsets<2>(off, wave, lane);
@@ -934,6 +1009,7 @@ __device__ __forceinline__ void tile_dq(const TileArgs& a, int id, float* lds) {
     f32x16 dq[T::ND];
 #pragma unroll
     for (int d = 0; d < T::ND; ++d) dq[d] = zero16();
+    Unit unit;
     if (t0 < t1) load(t0, 0);
     if (STAGES == 3 && t0 + 1 < t1) load(t0 + 1, 1);
     int stage = 0;
@@ -959,12 +1035,21 @@ __device__ __forceinline__ void tile_dq(const TileArgs& a, int id, float* lds) {
         }
         TENMO_PRODUCTS(12);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) dp[e] = __builtin_amdgcn_exp2f(s[e] * c - lse2) * (dp[e] * inv_dp - delta) * ds_up;
+        for (int e = 0; e < 16; ++e) dp[e] = __builtin_amdgcn_exp2f(s[e] * c - lse2) * (dp[e] * inv_dp - delta);
         if (t * 32 + 32 > wave_least) {
             const int left = limit - t * 32 - 4 * half;
 #pragma unroll
             for (int e = 0; e < 16; ++e) dp[e] = reg_row(e) < left ? dp[e] : 0.f;
         }
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(dp[e]));
+        top = halves_max(top);
+        if (__any(top > unit.most)) {
+            scale_sums<(DP > 64)>(dq, unit.renew(top));
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] *= unit.scale;
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
             f16x8 sh, sl;
@@ -981,7 +1066,7 @@ __device__ __forceinline__ void tile_dq(const TileArgs& a, int id, float* lds) {
         TENMO_PRODUCTS(6);
     }
     if (i >= a.s.queries) return;
-    const float inv_ds = 1.f / ds_up, inv_k = 1.f / scale_k;
+    const float inv_ds = power_inverse(unit.scale), inv_k = 1.f / scale_k;
     const int64_t at_q = b * a.grad_q.b + h * a.grad_q.h + i * a.grad_q.s;
 #pragma unroll
     for (int d = 0; d < T::ND; ++d)
@@ -1114,7 +1199,7 @@ void attn_tiles_backward(const AttnBackward& b, Workspace& ws, int cus, hipStrea
     a.out = b.out; a.lse = b.lse;
     a.grad_q = b.grad_q; a.grad_k = b.grad_k; a.grad_v = b.grad_v; a.accumulate = b.accumulate;
     plan_operands(a, ws);
-    a.stats = ws.take<f32x2>((int64_t)b.s.batch * b.s.heads * row_pad(b.s.queries) + kRowPad);
+    a.stats = ws.take<float>(kStats * ((int64_t)b.s.batch * b.s.heads * row_pad(b.s.queries) + kRowPad));
     // A sum over many tiles is cut into runs, whose parts are added afterwards in order, for two reasons.  Few heads with few blocks leave CUs without a workgroup: runs are no longer than what three
     // workgroups a CU would do if all tiles were dealt evenly (a tile of queries for a block of keys is four products, one of keys for a block of queries three), and 8 tiles at least, or the parts
     // cost more.  Whole sums: [1,8192,8,64] for 500 keys 427 us, [1,2048,4,64] causal 121 us, [1,3000,6/2,128] 420 us; in runs 147, 66 and 386; with two workgroups a CU 141, 72 and 420, with four

@@ -1,0 +1,109 @@
+"""Each row of a result of attention on its own, where sizes within a call lie far apart.
+
+A row is a sum of products.  Its error is measured against what enters it, the square root of the sum of the squares of its terms, so that neither the largest row of the call nor
+terms that cancel count.  Tolerances are those of whole results in test_gpu_transformer.py, 1e-5 and 2e-5 for gradients: a term is off by the roundings of its factors (2^-22 as two halves,
+2^-24 in fp32) and, where it holds a probability exp(-t), by that of its exponent, (t + 2 + |score|) 2^-24, which is 4e-6 at t = |score| = 32; the roundings of a sum have both signs.
+"""
+import math
+
+import pytest
+import torch
+
+from helpers import RTOL_FRO
+from test_gpu_transformer import down, ops, randn, up  # noqa: F401  (ops is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def rows_close(got, want, size, tol, what):
+    """|got - want| of each row (the last axis) against its size."""
+    got = got.double()
+    assert bool(torch.isfinite(got).all()), what
+    err = (got - want).norm(dim=-1)
+    worst = torch.where(size > 0, err / size.clamp(min=1e-300), torch.where(err > 0, math.inf, 0.0))
+    at = int(worst.argmax())
+    print(f"{what}: {worst.max():.2e} in row {at}, median {worst.median():.2e}", flush=True)
+    assert worst.max() <= tol, (what, at, float(worst.max()))
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------------------
+
+
+def attention_rows(q, k, v, scale, causal, dout):
+    """out and gradients of one sequence [1, n, H, D] in 64 bits, each with the sizes of its rows."""
+    n, m, group, D = q.shape[1], k.shape[1], q.shape[2] // k.shape[2], q.shape[3]
+    q, k, v, dout = (t[0].double().transpose(0, 1) for t in (q, k, v, dout))
+    kk, vv = (t.repeat_interleave(group, 0) for t in (k, v))
+    s = scale * q @ kk.transpose(1, 2)
+    if causal:
+        s = s.masked_fill(torch.arange(m)[None, :] > torch.arange(n)[:, None] + m - n, -math.inf)
+    p = torch.softmax(s, -1)
+    o, dp = p @ vv, dout @ vv.transpose(1, 2)
+    delta = (dout * o).sum(-1, keepdim=True)
+    ds = p * (dp - delta) * scale
+    dot = dout.norm(dim=-1, keepdim=True) * vv.norm(dim=-1)[:, None, :] / math.sqrt(D)  # the size of dp's own terms
+    ds2 = (p * (dp.abs() + delta.abs() + dot) * scale) ** 2
+    square = lambda t: (t ** 2).sum(-1, keepdim=True)  # noqa: E731
+    shared = lambda t: t.reshape(k.shape[0], group, *t.shape[1:]).sum(1)  # noqa: E731
+    want = [o, ds @ kk, shared(ds.transpose(1, 2) @ q), shared(p.transpose(1, 2) @ dout)]
+    size = [(p ** 2) @ square(vv), ds2 @ square(kk), shared(ds2.transpose(1, 2) @ square(q)), shared((p ** 2).transpose(1, 2) @ square(dout))]
+    return [t.transpose(0, 1)[None] for t in want], [t.transpose(0, 1)[None, ..., 0].sqrt() for t in size]
+
+
+def check_attention(ops, q, k, v, dout, scale, causal):
+    want, size = attention_rows(q, k, v, scale, causal, dout)
+    Q, K, V, DO = (up(ops, t) for t in (q, k, v, dout))
+    o, lse = ops.A.attention(Q, K, V, scale=scale, causal=causal)
+    grads = ops.A.attention_backward(Q, K, V, o, lse, DO, scale=scale, causal=causal)
+    rows_close(down(o), want[0], size[0], RTOL_FRO, "out")
+    for g, w, s, what in zip(grads, want[1:], size[1:], ("grad_q", "grad_k", "grad_v")):
+        rows_close(down(g), w, s, 2 * RTOL_FRO, what)
+
+
+SIZES = [  # queries, keys, heads, kv_heads, dim, causal
+    (600, 600, 4, 4, 64, True),
+    (600, 600, 4, 2, 64, False),
+    (333, 700, 8, 2, 128, True),
+    (1100, 1000, 4, 4, 32, False),
+    (400, 400, 6, 6, 80, True),
+    (70, 70, 2, 2, 64, True),  # by rows
+]
+
+
+@pytest.mark.parametrize("size", SIZES, ids=str)
+@pytest.mark.parametrize("where,factor", [("dout", 1e4), ("dout", 1e6), ("dout", 1e7), ("dout", 2.0 ** -10), ("dout", 2.0 ** -14), ("dout", 2.0 ** -20), ("dout", 2.0 ** -22), ("dout", 2.0 ** -40),
+                                          ("dout", 1e-30), ("v", 1e4), ("v", 6e4), ("v", 2.0 ** -14), ("k", 2.0 ** -14), ("q", 2.0 ** -14), ("q", 2.0 ** -20)], ids=str)
+@pytest.mark.parametrize("many", [False, True], ids=["one", "half"])
+def test_attention_rows_of_different_sizes(ops, size, where, factor, many):  # noqa: F811
+    """One row, or every row of the second half, times a factor: the others, and it, stay right by themselves."""
+    n, m, H, Hk, D, causal = size
+    t = {"q": randn(1, 1, n, H, D), "k": randn(2, 1, m, Hk, D), "v": randn(3, 1, m, Hk, D), "dout": randn(4, 1, n, H, D)}
+    rows = t[where].shape[1]
+    t[where][:, rows // 2 if many else rows // 3:rows if many else rows // 3 + 1] *= factor
+    check_attention(ops, t["q"], t["k"], t["v"], t["dout"], 1.0 / math.sqrt(D), causal)
+
+
+@pytest.mark.parametrize("size", SIZES, ids=str)
+@pytest.mark.parametrize("far", [8, 14, 18, 22, 30])
+def test_attention_keys_of_little_weight(ops, size, far):  # noqa: F811
+    """Keys that no query gives more than about e^-far: their gradients are sums of such probabilities alone."""
+    n, m, H, Hk, D, causal = size
+    q, k, v, dout = randn(5, 1, n, H, D), randn(6, 1, m, Hk, D), randn(7, 1, m, Hk, D), randn(8, 1, n, H, D)
+    scale = 1.0 / math.sqrt(D)
+    q[..., 0] = 3.0
+    k[:, 1::3, :, 0] = -far / (3.0 * scale)
+    check_attention(ops, q, k, v, dout, scale, causal)
+
+
+@pytest.mark.parametrize("size", SIZES, ids=str)
+@pytest.mark.parametrize("seed", [0, 1])
+def test_attention_values_far_out_of_little_weight(ops, size, seed):  # noqa: F811
+    """Values 2^15 times the others' at keys of so little weight that they do not make the result: what is lost of their probabilities would show in it."""
+    n, m, H, Hk, D, causal = size
+    q, k, v, dout = randn(9 + seed, 1, n, H, D), randn(19 + seed, 1, m, Hk, D), randn(29 + seed, 1, m, Hk, D), randn(39 + seed, 1, n, H, D)
+    scale = 1.0 / math.sqrt(D)
+    q[..., 0] = 3.0
+    v[:, 1::9] *= 2.0 ** 13
+    k[:, 1::9, :, 0] = -22.0 / (3.0 * scale)
+    check_attention(ops, q, k, v, dout, scale, causal)
+

@@ -500,12 +500,6 @@ __device__ __forceinline__ f32x16 zero16() {
     for (int e = 0; e < 16; ++e) z[e] = 0.f;
     return z;
 }
-// a 1 that the compiler takes for a variable: x * one - h, rounded to fp16, is one mixed-precision instruction, x - h converts twice
-__device__ __forceinline__ float variable_one() {
-    float one = 1.f;
-    asm volatile("" : "+v"(one));
-    return one;
-}
 // registers 8 t .. 8 t + 7 of a product as an operand
 __device__ __forceinline__ void halves(const f32x16& x, int t, float one, f16x8& h, f16x8& l) {
 #pragma unroll

@@ -56,6 +56,12 @@ __device__ __forceinline__ void split_value(float x, _Float16& h, _Float16& l) {
     const float r = x - (float)h;
     l = (_Float16)(r - r == 0.f ? r : 0.f); // x not finite: h alone
 }
+// a 1 that the compiler takes for a variable: x * one - h, rounded to fp16, is one mixed-precision instruction, x - h converts twice
+__device__ __forceinline__ float variable_one() {
+    float one = 1.f;
+    asm volatile("" : "+v"(one));
+    return one;
+}
 // ---- the product ----------------------------------------------------------------------------------------------------------------
 
 // C[m, n] = sum over k of A[m, k] B[k, n] for a tile of 256 x 128 and the K steps k_first .., wavefronts 2 x 2, K in steps of 16 through a ring of three stages in LDS
@@ -143,8 +149,28 @@ __device__ __forceinline__ void stage_barrier() {
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-template <bool A_KMAJOR, bool B_KMAJOR>
-__device__ __forceinline__ void split_tile(f32x16 (&acc)[4][2], float* lds, const SplitMatrix& A, int64_t m0, int64_t M, const SplitMatrix& B, int64_t n0, int64_t N, int64_t k_first, int64_t k_steps) {
+// An operand whose rows (of the product's M or N) have scales of their own, and others in every kCodeK of K: a row is worked on at the smallest of its scales, of which the others are multiples
+// by 2^12, 2^24 or more, and what is held at those is brought down as it is read.  Two bits for each kCodeK of K, sixteen of them a word: the power of 2^-12; three stands for nothing.
+constexpr int kCodeK = 64, kCodeBits = 12, kCodesAWord = 16;
+enum { kPlain, kCodedA, kCodedB };
+struct Codes {
+    const uint32_t* p; // [K / (kCodeK * kCodesAWord)][pitch]
+    int64_t pitch;
+};
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ f16x2 code_factor(uint32_t codes, uint32_t at) { // 1, 2^-12, 2^-24 or 0, twice
+    const uint32_t code = (codes >> (2 * at)) & 3u;
+    return __builtin_bit_cast(f16x2, code == 0 ? 0x3c003c00u : code == 1 ? 0x0c000c00u : code == 2 ? 0x00010001u : 0u);
+}
+__device__ __forceinline__ f16x8 times(f16x8 x, f16x2 f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= f[e & 1];
+    return x;
+}
+
+template <bool A_KMAJOR, bool B_KMAJOR, int CODED = kPlain>
+__device__ __forceinline__ void split_tile(f32x16 (&acc)[4][2], float* lds, const SplitMatrix& A, int64_t m0, int64_t M, const SplitMatrix& B, int64_t n0, int64_t N, int64_t k_first, int64_t k_steps,
+                                           const Codes& codes = Codes{}) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TileLoader<kTileM, A_KMAJOR> la;
     TileLoader<kTileN, B_KMAJOR> lb;
@@ -165,20 +191,42 @@ __device__ __forceinline__ void split_tile(f32x16 (&acc)[4][2], float* lds, cons
         la.load(lds, stage * kStageBytes, wave, k_first + t);
         lb.load(lds, stage * kStageBytes + kTileM * kStepK * 4, wave, k_first + t);
     };
+    constexpr int CODES = CODED == kCodedA ? 4 : CODED == kCodedB ? 2 : 1, CODE_STEPS = kCodeK / kStepK;
+    uint32_t code[CODES];
+    f16x2 factor[CODES];
+    auto load_codes = [&](int64_t step) { // waited for here: a wait in every step would be one for the tiles that are on their way
+#pragma unroll
+        for (int i = 0; i < CODES; ++i) {
+            const int64_t row = (CODED == kCodedA ? m0 + (wave & 1) * 128 : n0 + (wave >> 1) * 64) + 32 * i + (lane & 31), last = (CODED == kCodedA ? M : N) - 1;
+            code[i] = codes.p[step / (CODE_STEPS * kCodesAWord) * codes.pitch + (row < last ? row : last)];
+        }
+#pragma unroll
+        for (int i = 0; i < CODES; ++i) asm volatile("" : "+v"(code[i]));
+    };
+    if (CODED != kPlain && k_steps > 0) load_codes(k_first);
     if (k_steps > 0) load(0, 0);
     if (k_steps > 1) load(1, 1);
     uint32_t now = 0;
     for (int64_t t = 0; t < k_steps; ++t) {
         if (t + 1 < k_steps) stage_barrier<LOADS>();
         else stage_barrier<0>();
+        const int64_t step = k_first + t;
+        if (CODED != kPlain && t > 0 && step % (CODE_STEPS * kCodesAWord) == 0) load_codes(step);
         if (t + 2 < k_steps) load(t + 2, now == 0 ? 2 : now - 1);
+        if (CODED != kPlain && (t == 0 || step % CODE_STEPS == 0))
+#pragma unroll
+            for (int i = 0; i < CODES; ++i) factor[i] = code_factor(code[i], (uint32_t)step / CODE_STEPS % kCodesAWord);
         const char* s = (const char*)lds + now * kStageBytes;
         f16x8 b[2][2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) b[j][0] = rb.read(s, j, 0), b[j][1] = rb.read(s, j, 1);
+        for (int j = 0; j < 2; ++j) {
+            b[j][0] = rb.read(s, j, 0), b[j][1] = rb.read(s, j, 1);
+            if (CODED == kCodedB) b[j][0] = times(b[j][0], factor[j % CODES]), b[j][1] = times(b[j][1], factor[j % CODES]);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f16x8 ah = ra.read(s, i, 0), al = ra.read(s, i, 1);
+            f16x8 ah = ra.read(s, i, 0), al = ra.read(s, i, 1);
+            if (CODED == kCodedA) ah = times(ah, factor[i % CODES]), al = times(al, factor[i % CODES]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, b[j][0], acc[i][j], 0, 0, 0);

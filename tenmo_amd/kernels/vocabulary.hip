@@ -8,17 +8,24 @@
 // (split_gemm.hpp); for few tokens or a small W, where reading W or latency is the bound, the kernels of vocabulary_few.hip take their place.
 //   * forward: tiles of 256 words x 128 tokens; the words of a token lie in the registers of two lanes, so that a tile's maximum and sum of a token take
 //     one exchange, and 8 bytes a token and tile leave the chip instead of 1 KiB of logits.  A second launch joins the tiles of a token in a fixed order.
-//   * backward: a piece of the vocabulary at a time; the tiles of the first launch end as G in split form (|G| <= 1, so its scale is known beforehand: 2^14),
-//     which the second launch multiplies with W and with H.  The piece is as large as 1 GiB of G allows.
+//   * backward: a piece of the vocabulary at a time; the tiles of the first launch end as G in split form, which the next one multiplies with W and with H.  The piece is as large as 1 GiB of G allows.
+//     Two forms of G, since its two products sum over different axes:
+//       G W^T    G at 2^14.  A row is a token's, whose target has p - 1, itself right to 2^-24 of 1; the halves hold the others to 2^-40 of 1.
+//       G^T H    scale_m G / (the scale of H's row m), which is what a word's row of dW is summed from: with a scale for each word and 64 tokens, a power of 2^12 that brings their largest into
+//                2^1 .. 2^13 (split_gemm.hpp brings them to the word's smallest).  Words without a target have probabilities alone in their rows, however small, and tokens lie far apart in
+//                their upstream gradients: at 2^14 for all, rows of words whose logits lie 16 below the others' were off by 5e-2 of what enters them, 20 below by 1 (700 tokens,
+//                130 x 9000).  It costs a second G in memory and the scales, 1000 -> 1198 us, and factors as it is read, 1850 -> 1935 us (half of 8192 x 50257, D = 768).
 #include "split_gemm.hpp"
 #include "vocabulary.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tenmo {
 namespace {
 
 constexpr float kGScale = 16384.f;
+constexpr int kWordBits = 13, kMostClass = 9; // a word's scale: 2^(kWordBits + kCodeBits * class)
 constexpr int64_t kPieceValues = 256 << 20; // of G, 4 bytes each
 
 struct Source { // an operand in the order in which it is split: rows x cols
@@ -28,17 +35,20 @@ struct Source { // an operand in the order in which it is split: rows x cols
 
 // ---- amax and split -------------------------------------------------------------------------------------------------------------
 
-// W and, backward, H times its rows' factors have one scale each, since they are summed over along either axis: their largest values first, then the halves.  H itself has a scale of its own in
-// each row (a row is one column of the logits' product), so that no row loses anything to another; its halves come with the first launch.
+// W has one scale, since it is summed over along either axis: its largest value first, then the halves.  H has a scale of its own in each row, so that no row loses anything to another (a row is
+// one column of the logits' product; in G^T H the scales go into G); its halves come with the first launch.
 struct SplitArgs {
     VocabArgs v;
-    Upstream up;
+    Upstream up;      // p NULL: forward
     Source w, h;
-    uint32_t *amax_w, *amax_hs; // kAmaxParts partial maxima
-    SplitMatrix to_w, to_h, to_hs;
+    uint32_t* amax_w; // kAmaxParts partial maxima
+    uint32_t* top_f;  // backward, as many partial maxima: (kNoFactor + log2 of a token's factor over its scale of H) << kFactorShift, 0 without a token that counts
+    SplitMatrix to_w, to_h;
     float* h_inverse; // [M]: 1 / the scale of a row of H
 };
-enum { kSplitW, kSplitH, kSplitHS }; // blockIdx.y
+enum { kSplitW, kSplitH }; // blockIdx.y
+constexpr int kNoFactor = 512, kFactorShift = 21; // (as bits of a normal float: the maxima are taken of those)
+__device__ __forceinline__ int exponent_of(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 127; }
 
 __device__ __forceinline__ void split8(const float* x, float scale, float* to) {
     f16x8 h, l;
@@ -66,9 +76,12 @@ __device__ __forceinline__ void load8(float (&x)[8], const float* p, int64_t cs,
 
 // a wavefront a row
 __device__ __forceinline__ void split_h_rows(const SplitArgs& a) {
+    __shared__ uint32_t tops[4];
     const int lane = threadIdx.x & 63;
+    uint32_t top_f = 0;
     for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < split_pad(a.h.rows); r += 4 * kAmaxParts) {
-        const bool in = r < a.h.rows;
+        const float factor = r >= a.h.rows ? 0.f : a.up.p ? row_factor(a.v, a.up, r) : 1.f;
+        const bool in = factor != 0.f; // rows without a part in the gradient are zeros, whatever they hold
         const float* p = a.h.p + (in ? r : 0) * a.h.rs;
         const int64_t cols = in ? a.h.cols : 0;
         uint32_t top = 0;
@@ -83,27 +96,25 @@ __device__ __forceinline__ void split_h_rows(const SplitArgs& a) {
             load8(x, p, a.h.cs, c, cols);
             split8(x, scale, a.to_h.p + r * a.to_h.pitch + c);
         }
-        if (in && lane == 0) a.h_inverse[r] = 1.f / scale;
+        if (r < a.h.rows && lane == 0) a.h_inverse[r] = 1.f / scale;
+        if (in && finite_magnitude(factor)) top_f = max(top_f, (uint32_t)(kNoFactor + exponent_of(factor) - exponent_of(scale)) << kFactorShift);
     }
+    if (!a.top_f) return;
+    if (lane == 0) tops[threadIdx.x >> 6] = top_f;
+    __syncthreads();
+    if (threadIdx.x == 0) a.top_f[blockIdx.x] = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
 }
 
 // four rows at a time: four loads in flight a thread
 __global__ __launch_bounds__(256) void vocab_amax_kernel(const SplitArgs a) {
     __shared__ uint32_t slots[4];
-    const int job = blockIdx.y;
-    if (job == kSplitH) return split_h_rows(a);
-    const bool hs = job == kSplitHS;
-    const Source s{hs ? a.h.p : a.w.p, hs ? a.h.rows : a.w.rows, hs ? a.h.cols : a.w.cols, hs ? a.h.rs : a.w.rs, hs ? a.h.cs : a.w.cs};
+    if (blockIdx.y == kSplitH) return split_h_rows(a);
+    const Source& s = a.w;
     uint32_t top = 0;
     for (int64_t r0 = blockIdx.x; r0 < s.rows; r0 += 4 * kAmaxParts) {
         const float* p[4];
-        float scale[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) { // (the last row again where there is none)
-            const int64_t r = r0 + u * kAmaxParts < s.rows ? r0 + u * kAmaxParts : s.rows - 1;
-            p[u] = s.p + r * s.rs;
-            scale[u] = hs ? row_factor(a.v, a.up, r) : 1.f;
-        }
+        for (int u = 0; u < 4; ++u) p[u] = s.p + (r0 + u * kAmaxParts < s.rows ? r0 + u * kAmaxParts : s.rows - 1) * s.rs; // (the last row again where there is none)
         int64_t c = threadIdx.x * 4;
         if (s.cs == 1)
             for (; c + 3 < s.cols; c += 1024) {
@@ -113,46 +124,43 @@ __global__ __launch_bounds__(256) void vocab_amax_kernel(const SplitArgs a) {
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top = max(top, finite_magnitude(scale[u] == 0.f ? 0.f : x[u][e] * scale[u]));
+                    for (int e = 0; e < 4; ++e) top = max(top, finite_magnitude(x[u][e]));
             }
         for (; c < s.cols; c += 1024)
             for (int e = 0; e < 4 && c + e < s.cols; ++e)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) top = max(top, finite_magnitude(scale[u] == 0.f ? 0.f : p[u][(c + e) * s.cs] * scale[u]));
+                for (int u = 0; u < 4; ++u) top = max(top, finite_magnitude(p[u][(c + e) * s.cs]));
     }
     top = wave_max_bits(top);
     if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) (hs ? a.amax_hs : a.amax_w)[blockIdx.x] = max(max(slots[0], slots[1]), max(slots[2], slots[3]));
+    if (threadIdx.x == 0) a.amax_w[blockIdx.x] = max(max(slots[0], slots[1]), max(slots[2], slots[3]));
 }
 
-// the scale of a matrix, from its partial maxima, in every thread of a workgroup of 256
-__device__ __forceinline__ float scale_from(const uint32_t* __restrict amax, uint32_t* slots) {
+// the largest of the partial maxima, in every thread of a workgroup of 256
+__device__ __forceinline__ uint32_t top_from(const uint32_t* __restrict amax, uint32_t* slots) {
     uint32_t top = 0;
     for (int i = threadIdx.x; i < kAmaxParts; i += 256) top = max(top, amax[i]);
     top = wave_max_bits(top);
     if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = top;
     __syncthreads();
-    return split_scale(max(max(slots[0], slots[1]), max(slots[2], slots[3])));
+    return max(max(slots[0], slots[1]), max(slots[2], slots[3]));
 }
+__device__ __forceinline__ float scale_from(const uint32_t* __restrict amax, uint32_t* slots) { return split_scale(top_from(amax, slots)); }
+// log2 of the largest of the tokens' factors over their scales of H, rounded down
+__device__ __forceinline__ int factor_from(const uint32_t* __restrict top_f, uint32_t* slots) { return (int)(top_from(top_f, slots) >> kFactorShift) - kNoFactor; }
 
 __global__ __launch_bounds__(256) void vocab_split_kernel(const SplitArgs a) {
     __shared__ uint32_t slots[4];
-    const bool hs = blockIdx.y != 0;
-    const Source s{hs ? a.h.p : a.w.p, hs ? a.h.rows : a.w.rows, hs ? a.h.cols : a.w.cols, hs ? a.h.rs : a.w.rs, hs ? a.h.cs : a.w.cs};
-    float* const to = hs ? a.to_hs.p : a.to_w.p;
-    const int64_t pitch = hs ? a.to_hs.pitch : a.to_w.pitch;
-    const float scale = scale_from(hs ? a.amax_hs : a.amax_w, slots);
+    const Source& s = a.w;
+    const int64_t pitch = a.to_w.pitch;
+    const float scale = scale_from(a.amax_w, slots);
     const int64_t groups = pitch / 8, all = split_pad(s.rows) * groups;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / groups, c = (i - r * groups) * 8;
-        const float factor = r >= s.rows ? 0.f : hs ? row_factor(a.v, a.up, r) : 1.f;
         float x[8];
-        load8(x, s.p + (r < s.rows ? r : 0) * s.rs, s.cs, c, factor == 0.f ? 0 : s.cols); // rows without a part in the gradient are zeros, whatever they hold
-        if (hs)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= factor;
-        split8(x, scale, to + r * pitch + c);
+        load8(x, s.p + (r < s.rows ? r : 0) * s.rs, s.cs, c, r < s.rows ? s.cols : 0);
+        split8(x, scale, a.to_w.p + r * pitch + c);
     }
 }
 
@@ -164,6 +172,10 @@ struct ProductArgs {
     int64_t M, N, k_steps;
     int64_t tiles_m, tiles_n;
     int64_t run_steps, run_stride; // K steps of a run, and floats from one run's result to the next
+    // G with a scale for each word
+    Codes codes;
+    const int* unit;       // [words]: log2 of the scale that the codes bring it to
+    const uint32_t* top_f; // SplitArgs
 };
 
 struct LogitArgs {
@@ -178,9 +190,58 @@ struct LogitArgs {
     // backward
     const float* lse;
     Upstream up;
-    SplitMatrix g;
+    SplitMatrix g, gw; // for dH, and for dW; p NULL: not wanted
+    uint8_t* word_class; // [blocks of 64 tokens][gw.pitch]
+    const uint32_t* top_f; // SplitArgs
     float* part_db; // [2 * token tiles][V], with a wanted bias gradient
 };
+
+// A token's 4 words in this lane, and 4 in the lane 32 further, in split form: the two lanes hold half each of a group of eight; the lower one stores the eight h, the upper one the eight l
+__device__ __forceinline__ f32x4 split_words(f32x4 x, float one) {
+    union { f16x4 v[2]; uint32_t u[4]; f32x4 f; } y;
+    asm("" : "+v"(x)); // (a product: one rounding of it for both halves)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y.v[0][e] = (_Float16)x[e];
+    asm("" : "+v"(y.v[0]));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y.v[1][e] = (_Float16)__builtin_fmaf(x[e], one, -(float)y.v[0][e]);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const auto z = __builtin_amdgcn_permlane32_swap(y.u[w], y.u[2 + w], false, false);
+        y.u[w] = z[0];
+        y.u[2 + w] = z[1];
+    }
+    return y.f;
+}
+
+// The scales of a wavefront's 16 words from their magnitudes in this lane, the same in the 32 lanes of a half, and their classes to memory (four words of the half at `classes` + 8 q)
+template <int CTRL>
+__device__ __forceinline__ uint32_t lane_move_bits(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+__device__ __forceinline__ void word_scales(float (&x)[16], uint8_t* classes, int lane, int words) {
+    uint32_t cls[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { // the lower 16 lanes of a half go on with words 0 .. 7, the upper with 8 .. 15
+        const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[e]), __float_as_uint(x[e + 8]), false, false);
+        uint32_t top = max(y[0], y[1]); // (magnitudes: ordered as their bits are)
+        top = max(top, (uint32_t)lane_move_bits<0xB1>(top));
+        top = max(top, (uint32_t)lane_move_bits<0x4E>(top));
+        top = max(top, (uint32_t)lane_move_bits<0x141>(top));
+        top = max(top, (uint32_t)lane_move_bits<0x140>(top));
+        const int below = 127 - (int)(top >> 23); // top in [2^-below, 2^(1 - below))
+        const uint32_t c = (uint32_t)(fmaxf((float)below, 0.f) * (171.f / 2048.f)); // / kCodeBits, exactly so
+        cls[e] = c < kMostClass ? c : kMostClass;
+        const uint32_t scale = (127 + kWordBits + __umul24(cls[e], kCodeBits)) << 23;
+        const auto z = __builtin_amdgcn_permlane16_swap(scale, scale, false, false);
+        x[e] = __uint_as_float(z[0]);
+        x[e + 8] = __uint_as_float(z[1]);
+    }
+    if ((lane & 15) == 0) {
+        const int q = (lane >> 4) & 1; // groups 2 q and 2 q + 1
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (8 * (2 * q + u) < words) *(uint32_t*)(classes + 8 * (2 * q + u)) = cls[4 * u] | cls[4 * u + 1] << 8 | cls[4 * u + 2] << 16 | cls[4 * u + 3] << 24;
+    }
+}
 
 template <bool A_KMAJOR, bool GRAD>
 __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs p, const LogitArgs a) {
@@ -272,51 +333,86 @@ __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs 
             if (a.part_x) a.part_x[tm * a.v.M + n0 + threadIdx.x] = x[2] + y[2];
         }
     } else {
-        const float smooth = a.v.ls / (float)a.v.V;
-        float db[64];
-        if (a.part_db)
-#pragma unroll
-            for (int x = 0; x < 64; ++x) db[x] = 0.f;
+        const float smooth = a.v.ls / (float)a.v.V, one = variable_one();
+        __shared__ uint32_t slots_f[4];
+        const int top_f = a.gw.p ? factor_from(a.top_f, slots_f) : 0;
+        bool valid[2], store[2];
+        float lse[2], row_scale[2], factor[2];
+        int at[2]; // the target's place in this lane's words
+        float *to_g[2], *to_gw[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int64_t token = n0 + (wave >> 1) * 64 + 32 * j + (lane & 31);
-            const int64_t t = token < a.v.M ? target_of(a.v, token) : a.v.ignore;
-            const bool valid = token < a.v.M && t != a.v.ignore;
-            const float lse = valid ? a.lse[token] : 0.f, row_scale = valid && a.part_db ? row_factor(a.v, a.up, token) : 0.f;
-            const int64_t at = t - a.first - v0;
-            const bool here = __any(at >= 0 && at < 128); // a target among this wavefront's words: one in six at 50257 words
-            const bool store = token < split_pad(a.v.M);
-            float* to = a.g.p + (store ? token : 0) * a.g.pitch;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int64_t v = v0 + 32 * i + 8 * q;
-                    f16x4 h, l;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float g = __expf(acc[i][j][4 * q + e] - lse) - smooth;
-                        if (here && at == 32 * i + 8 * q + e) g -= 1.f - a.v.ls;
-                        g = valid && v + e < a.words ? g : 0.f;
-                        if (a.part_db) db[16 * i + 4 * q + e] += g * row_scale;
-                        _Float16 hi, lo;
-                        split_value(g * kGScale, hi, lo);
-                        h[e] = hi;
-                        l[e] = lo;
-                    }
-                    // The two lanes of a token hold four words each of a group of eight: the lower one takes the eight h, the upper one the eight l
-                    union { f16x4 v[2]; uint32_t u[4]; f32x4 f; } x;
-                    x.v[0] = h;
-                    x.v[1] = l;
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const auto y = __builtin_amdgcn_permlane32_swap(x.u[w], x.u[2 + w], false, false);
-                        x.u[w] = y[0];
-                        x.u[2 + w] = y[1];
-                    }
-                    if (store && v < a.g.pitch) *(f32x4*)(to + v) = x.f;
-                }
+            row_scale[j] = token < a.v.M ? row_factor(a.v, a.up, token) : 0.f;
+            valid[j] = row_scale[j] != 0.f;
+            lse[j] = valid[j] ? a.lse[token] : 0.f;
+            factor[j] = __builtin_amdgcn_ldexpf(row_scale[j], exponent_of(inv[j]) - top_f); // below 2
+            const int64_t place = valid[j] ? target_of(a.v, token) - a.first - v0 : -1;
+            at[j] = place >= 0 && place < 128 ? (int)place : -1;
+            store[j] = token < split_pad(a.v.M);
+            to_g[j] = a.g.p + (store[j] ? token : 0) * a.g.pitch + v0;
+            to_gw[j] = a.gw.p + (store[j] ? token : 0) * a.gw.pitch + v0;
         }
+        const bool here = __any(at[0] >= 0 || at[1] >= 0); // a target among this wavefront's words: one in three at 50257 words
+        const int words = (int)(a.words - v0 < 256 ? a.words - v0 : 256), pitch = (int)((a.g.p ? a.g.pitch : a.gw.pitch) - v0 < 256 ? (a.g.p ? a.g.pitch : a.gw.pitch) - v0 : 256);
+        float db[64];
+        uint8_t* const classes = a.word_class + ((n0 >> 6) + (wave >> 1)) * a.gw.pitch + v0;
+        // WHOLE: every word and token of the tile is there
+        auto end = [&](auto whole) {
+            constexpr bool WHOLE = decltype(whole)::value;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int w = 32 * i + 8 * (e >> 2) + (e & 3);
+                        const float g = __expf(acc[i][j][e] - lse[j]) - smooth;
+                        acc[i][j][e] = valid[j] && (WHOLE || w < words) ? g : 0.f;
+                    }
+                if (here)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            acc[i][j][e] -= at[j] == 32 * i + 8 * (e >> 2) + (e & 3) ? 1.f - a.v.ls : 0.f;
+                if (a.part_db)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) db[16 * i + e] = acc[i][0][e] * row_scale[0] + acc[i][1][e] * row_scale[1];
+                if (a.g.p)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            f32x4 x;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] = acc[i][j][4 * q + e] * kGScale;
+                            x = split_words(x, one);
+                            if (WHOLE || (store[j] && 32 * i + 8 * q < pitch)) *(f32x4*)(to_g[j] + 32 * i + 8 * q) = x;
+                        }
+                if (!a.gw.p) continue;
+                float scale[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    acc[i][0][e] *= factor[0];
+                    acc[i][1][e] *= factor[1];
+                    scale[e] = fmaxf(fabsf(acc[i][0][e]), fabsf(acc[i][1][e]));
+                }
+                word_scales(scale, classes + 32 * i, lane, pitch - 32 * i);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        f32x4 x;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = acc[i][j][4 * q + e] * scale[4 * q + e];
+                        x = split_words(x, one);
+                        if (WHOLE || (store[j] && 32 * i + 8 * q < pitch)) *(f32x4*)(to_gw[j] + 32 * i + 8 * q) = x;
+                    }
+            }
+        };
+        if (!edge && n0 + kTileN <= a.v.M) end(std::true_type{});
+        else end(std::false_type{});
         if (a.part_db) { // 64 values in each of 32 lanes, summed over the lanes: lane x keeps the sums of values 2 x and 2 x + 1 in bit-reversed order
 #pragma unroll
             for (int step = 16, n = 32; step > 0; step >>= 1, n >>= 1) {
@@ -345,7 +441,7 @@ struct StoreArgs {
     int accumulate;
 };
 
-template <bool A_KMAJOR, bool B_KMAJOR>
+template <bool A_KMAJOR, bool B_KMAJOR, int CODED>
 __device__ __forceinline__ void product_tile(const ProductArgs& p, const StoreArgs& s, uint32_t id, float* lds, uint32_t (*slots)[4]) {
     int64_t tm, tn;
     const uint32_t tiles = (uint32_t)(p.tiles_m * p.tiles_n), run = id / tiles;
@@ -354,10 +450,36 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p, const StoreAr
     const int64_t k0 = __builtin_amdgcn_readfirstlane((uint32_t)(run * p.run_steps));
     const int64_t steps = p.k_steps - k0 < p.run_steps ? p.k_steps - k0 : p.run_steps;
     f32x16 acc[4][2];
-    split_tile<A_KMAJOR, B_KMAJOR>(acc, lds, p.a, m0, p.M, p.b, n0, p.N, k0, steps);
-    float inv = 1.f / (p.amax_a ? scale_from(p.amax_a, slots[0]) : kGScale);
-    inv /= p.amax_b ? scale_from(p.amax_b, slots[1]) : kGScale;
+    split_tile<A_KMAJOR, B_KMAJOR, CODED>(acc, lds, p.a, m0, p.M, p.b, n0, p.N, k0, steps, p.codes);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if constexpr (CODED == kPlain) {
+        const float inv = 1.f / kGScale / scale_from(p.amax_b, slots[1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[i][j] *= inv;
+    } else { // each word's scale, and the tokens' largest factor
+        const int top_f = factor_from(p.top_f, slots[0]);
+        if constexpr (CODED == kCodedA) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int up = top_f - p.unit[m0 + (wave & 1) * 128 + 32 * i + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[i][j][e] = __builtin_amdgcn_ldexpf(acc[i][j][e], up);
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int up = top_f - p.unit[n0 + (wave >> 1) * 64 + 32 * j + (lane & 31)];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_ldexpf(acc[i][j][e], up);
+            }
+        }
+    }
     float* c = s.c + (int64_t)run * p.run_stride;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -370,19 +492,35 @@ __device__ __forceinline__ void product_tile(const ProductArgs& p, const StoreAr
                 const int64_t n = n0 + (wave >> 1) * 64 + 32 * j + (lane & 31);
                 if (n >= p.N) continue;
                 float* to = c + m * s.rs + n * s.cs;
-                *to = s.accumulate ? *to + acc[i][j][e] * inv : acc[i][j][e] * inv;
+                *to = s.accumulate ? *to + acc[i][j][e] : acc[i][j][e];
             }
         }
 }
 
 // Both products of a piece in one launch, since neither fills the chip evenly by itself: the first `h_tiles` workgroups are G W^T (its reduction over the words cut into runs of about the
-// length of the other's, each into a sum of its own), the others (scale H)^T G, or its transpose.
-template <bool W_KMAJOR>
+// length of the other's, each into a sum of its own), the others G^T H (words in the rows), or its transpose.
+template <bool W_KMAJOR, bool WORD_ROWS>
 __global__ __launch_bounds__(256, 2) void vocab_products_kernel(const ProductArgs h, const StoreArgs sh, uint32_t h_tiles, const ProductArgs w, const StoreArgs sw) {
     __shared__ __align__(1024) float lds[kStages * kStageBytes / 4];
     __shared__ uint32_t slots[2][4];
-    if (blockIdx.x < h_tiles) product_tile<true, W_KMAJOR>(h, sh, blockIdx.x, lds, slots);
-    else product_tile<false, false>(w, sw, blockIdx.x - h_tiles, lds, slots);
+    if (blockIdx.x < h_tiles) product_tile<true, W_KMAJOR, kPlain>(h, sh, blockIdx.x, lds, slots);
+    else product_tile<false, false, WORD_ROWS ? kCodedA : kCodedB>(w, sw, blockIdx.x - h_tiles, lds, slots);
+}
+
+// Each word's scale in G^T H, the smallest of those of its blocks of 64 tokens, and what brings the others to it
+__global__ __launch_bounds__(256) void vocab_unit_kernel(const uint8_t* __restrict classes, int64_t pitch, int64_t blocks, uint32_t* __restrict codes, int* __restrict unit) {
+    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (v >= pitch) return;
+    uint32_t least = kMostClass;
+#pragma unroll 16
+    for (int64_t t = 0; t < blocks; ++t) least = min(least, (uint32_t)classes[t * pitch + v]);
+    unit[v] = kWordBits + kCodeBits * (int)least;
+    for (int64_t t = 0; t < blocks; t += kCodesAWord) {
+        uint32_t word = 0;
+#pragma unroll
+        for (int u = 0; u < kCodesAWord; ++u) word |= min((t + u < blocks ? classes[(t + u) * pitch + v] : least) - least, 3u) << (2 * u);
+        codes[t / kCodesAWord * pitch + v] = word;
+    }
 }
 
 // ---- rows ------------------------------------------------------------------------------------------------------------------------------
@@ -526,14 +664,16 @@ __global__ __launch_bounds__(256) void vocab_db_kernel(const float* __restrict p
 // ---- host -----------------------------------------------------------------------------------------------------------------------------------
 
 struct Plan {
-    SplitMatrix h, w, hs, g;
-    uint32_t *amax_w, *amax_hs;
+    SplitMatrix h, w, g, gw;
+    uint32_t *amax_w, *top_f, *codes;
+    uint8_t* word_class;
+    int* unit;
     float* h_inverse;
     float2* part;
     float *part_x, *target_logit, *part_db, *part_h, *part_w;
     int64_t piece;  // words
     int64_t runs;   // of the words of a piece, in G W^T
-    int64_t w_runs; // of the tokens, in (scale H)^T G
+    int64_t w_runs; // of the tokens, in G^T H
 };
 
 int64_t tiles_of(int64_t n, int64_t t) { return (n + t - 1) / t; }
@@ -559,13 +699,16 @@ void plan_forward(Workspace& ws, Plan& p, int64_t M, int64_t D, int64_t V, bool 
 }
 void plan_backward(Workspace& ws, Plan& p, int64_t M, int64_t D, int64_t V, bool word_rows) {
     plan_operands(ws, p, M, D, V, word_rows);
-    p.hs = take_split(ws, M, D);
-    p.amax_hs = ws.take<uint32_t>(kAmaxParts);
+    p.top_f = ws.take<uint32_t>(kAmaxParts);
     p.part_db = ws.take<float>(2 * tiles_of(M, kTileN) * V);
     const int64_t most = std::max<int64_t>(kTileM, kPieceValues / split_pad(M) / kTileM * kTileM);
     p.piece = tiles_of(tiles_of(V, tiles_of(V, most)), kTileM) * kTileM; // pieces of equal size
     p.piece = std::min(p.piece, split_pad(V));
     p.g = take_split(ws, M, p.piece);
+    p.gw = take_split(ws, M, p.piece);
+    p.word_class = ws.take<uint8_t>(2 * tiles_of(M, kTileN) * p.gw.pitch);
+    p.codes = ws.take<uint32_t>(tiles_of(tiles_of(M, kCodeK), kCodesAWord) * p.gw.pitch);
+    p.unit = ws.take<int>(tiles_of(p.piece, kTileM) * kTileM); // (a tile reads those of all its rows)
     // As many runs as bring their length near the other product's (but not below 2048), or as fill two workgroups a CU where there are fewer
     // tiles than that, none shorter than 128 words.
     const int64_t tiles = tiles_of(M, kTileM) * tiles_of(D, kTileN);
@@ -602,16 +745,16 @@ Source source_w(const tenmo_view* W) {
     return Source{W->data + W->offset, W->shape[0], W->shape[1], W->strides[0], W->strides[1]};
 }
 
-// W and H, and H times its rows' factors where `hs` is wanted
-void launch_split(const Plan& p, const tenmo_view* H, const tenmo_view* W, const VocabArgs& v, const Upstream& up, bool hs, const LibraryState& lib) {
-    const SplitArgs a{v, up, source_w(W), source_h(H), p.amax_w, p.amax_hs, p.w, p.h, p.hs, p.h_inverse};
-    const int64_t groups = std::max(split_pad(a.w.rows) * p.w.pitch, split_pad(v.M) * p.h.pitch) / 8;
-    hipLaunchKernelGGL(vocab_amax_kernel, dim3(kAmaxParts, hs ? 3 : 2), dim3(256), 0, lib.stream, a);
-    hipLaunchKernelGGL(vocab_split_kernel, dim3((unsigned)std::min<int64_t>(tiles_of(groups, 256), 16 * lib.cus), hs ? 2 : 1), dim3(256), 0, lib.stream, a);
+// W and H
+void launch_split(const Plan& p, const tenmo_view* H, const tenmo_view* W, const VocabArgs& v, const Upstream& up, const LibraryState& lib) {
+    const SplitArgs a{v, up, source_w(W), source_h(H), p.amax_w, p.top_f, p.w, p.h, p.h_inverse};
+    const int64_t groups = split_pad(a.w.rows) * p.w.pitch / 8;
+    hipLaunchKernelGGL(vocab_amax_kernel, dim3(kAmaxParts, 2), dim3(256), 0, lib.stream, a);
+    hipLaunchKernelGGL(vocab_split_kernel, dim3((unsigned)std::min<int64_t>(tiles_of(groups, 256), 16 * lib.cus)), dim3(256), 0, lib.stream, a);
 }
 
 ProductArgs product(const SplitMatrix& a, const uint32_t* amax_a, const SplitMatrix& b, const uint32_t* amax_b, int64_t M, int64_t N, int64_t K) {
-    return ProductArgs{a, b, amax_a, amax_b, M, N, split_pad(K) / kStepK, tiles_of(M, kTileM), tiles_of(N, kTileN), split_pad(K) / kStepK, 0};
+    return ProductArgs{a, b, amax_a, amax_b, M, N, split_pad(K) / kStepK, tiles_of(M, kTileM), tiles_of(N, kTileN), split_pad(K) / kStepK, 0, Codes{}, nullptr, nullptr};
 }
 dim3 grid_of_dh(const VocabArgs& v, const LibraryState& lib) { return dim3((unsigned)std::min<int64_t>(tiles_of(v.M * v.D, 1024), 8 * lib.cus)); }
 dim3 grid_of(const ProductArgs& p) { return dim3((unsigned)(p.tiles_m * p.tiles_n)); }
@@ -661,7 +804,7 @@ int tenmo_hip_vocabulary_loss_forward_f32(const tenmo_view* H, const tenmo_view*
         Plan p{};
         plan_forward(ws, p, v.M, v.D, v.V, word_rows);
         if (int rc = ws.check(who)) return rc;
-        launch_split(p, H, W, v, Upstream{}, false, call.state);
+        launch_split(p, H, W, v, Upstream{}, call.state);
         const ProductArgs g = product(p.w, p.amax_w, p.h, nullptr, v.V, v.M, v.D);
         LogitArgs a{};
         a.v = v; a.words = v.V; a.h_inverse = p.h_inverse; a.part = p.part; a.part_x = label_smoothing > 0.f ? p.part_x : nullptr; a.target_logit = p.target_logit;
@@ -711,7 +854,7 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
     const int add = accumulate ? 1 : 0;
     float* gw = grad_W ? const_cast<float*>(grad_W->data) + grad_W->offset : nullptr;
     const int64_t gw_d = grad_W ? grad_W->strides[0] : 0, gw_v = grad_W ? grad_W->strides[1] : 0;
-    const bool word_rows = rows_of_words(W);
+    const bool word_rows = rows_of_words(W), dw_by_words = gw_d == 1 || gw_v != 1;
     Workspace ws(workspace, workspace_bytes);
     const Upstream up{upstream, (int)reduction, valid_count};
     if (v.M > 0 && few_for_backward(v.M, v.D, v.V)) {
@@ -725,20 +868,24 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
     Plan p{};
     if (v.M > 0) plan_backward(ws, p, v.M, v.D, v.V, word_rows);
     if (int rc = ws.check(who)) return rc;
-    if (v.M > 0) launch_split(p, H, W, v, up, grad_W != nullptr, call.state);
+    if (v.M > 0) launch_split(p, H, W, v, up, call.state);
     const int64_t piece = v.M > 0 ? p.piece : v.V;
     int64_t runs = 0;
     for (int64_t first = 0; first < v.V; first += piece) {
         const int64_t words = std::min(piece, v.V - first);
-        SplitMatrix G = p.g;
-        G.pitch = split_pad(words);
+        SplitMatrix G = p.g, GW = p.gw;
+        G.pitch = GW.pitch = split_pad(words);
         if (v.M > 0) {
             const SplitMatrix w = words_of(p.w, first, word_rows);
             const ProductArgs g = product(w, p.amax_w, p.h, nullptr, words, v.M, v.D);
             LogitArgs a{};
-            a.v = v; a.first = first; a.words = words; a.h_inverse = p.h_inverse; a.lse = lse; a.up = up; a.g = G; a.part_db = grad_bias ? p.part_db : nullptr;
+            a.v = v; a.first = first; a.words = words; a.h_inverse = p.h_inverse; a.lse = lse; a.up = up; a.part_db = grad_bias ? p.part_db : nullptr;
+            if (grad_H) a.g = G;
+            if (grad_W) a.gw = GW, a.word_class = p.word_class, a.top_f = p.top_f;
             if (word_rows) hipLaunchKernelGGL((vocab_logits_kernel<true, true>), grid_of(g), dim3(256), 0, stream, g, a);
             else hipLaunchKernelGGL((vocab_logits_kernel<false, true>), grid_of(g), dim3(256), 0, stream, g, a);
+            if (grad_W)
+                hipLaunchKernelGGL(vocab_unit_kernel, dim3((unsigned)tiles_of(GW.pitch, 256)), dim3(256), 0, stream, p.word_class, GW.pitch, tiles_of(v.M, kCodeK), p.codes, p.unit);
         }
         ProductArgs dh{}, dw{};
         StoreArgs sh{}, sw{};
@@ -753,13 +900,16 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
         }
         if (grad_W) { // as [words][D] or [D][words], whichever puts the axis with unit stride across the lanes
             float* to = gw + first * gw_v;
-            if (gw_d == 1 || gw_v != 1) {
-                dw = product(G, nullptr, p.hs, p.amax_hs, words, v.D, v.M);
+            if (dw_by_words) {
+                dw = product(GW, nullptr, p.h, nullptr, words, v.D, v.M);
                 sw = StoreArgs{to, gw_v, gw_d, add};
             } else {
-                dw = product(p.hs, p.amax_hs, G, nullptr, v.D, words, v.M);
+                dw = product(p.h, nullptr, GW, nullptr, v.D, words, v.M);
                 sw = StoreArgs{to, gw_d, gw_v, add};
             }
+            dw.codes = Codes{p.codes, GW.pitch};
+            dw.unit = p.unit;
+            dw.top_f = p.top_f;
             w_tiles = dw.tiles_m * dw.tiles_n;
         }
         const StoreArgs to_w = sw;
@@ -773,8 +923,10 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
         }
         if (h_tiles + w_tiles == 0) continue;
         const dim3 grid((unsigned)(h_tiles + w_tiles));
-        if (word_rows) hipLaunchKernelGGL(vocab_products_kernel<false>, grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
-        else hipLaunchKernelGGL(vocab_products_kernel<true>, grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
+        if (word_rows && dw_by_words) hipLaunchKernelGGL((vocab_products_kernel<false, true>), grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
+        else if (word_rows) hipLaunchKernelGGL((vocab_products_kernel<false, false>), grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
+        else if (dw_by_words) hipLaunchKernelGGL((vocab_products_kernel<true, true>), grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
+        else hipLaunchKernelGGL((vocab_products_kernel<true, false>), grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
         if (grad_W && p.w_runs > 1)
             hipLaunchKernelGGL(vocab_dw_kernel, dim3((unsigned)std::min<int64_t>(tiles_of(dw.run_stride, 256), 8 * call.state.cus)), dim3(256), 0, stream, p.part_w, w_runs, dw.M, dw.N, to_w);
     }

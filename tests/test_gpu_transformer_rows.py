@@ -1,4 +1,4 @@
-"""Each row of a result of attention on its own, where sizes within a call lie far apart.
+"""Each row of a result on its own: attention's and the vocabulary loss's, where sizes within a call lie far apart.
 
 A row is a sum of products.  Its error is measured against what enters it, the square root of the sum of the squares of its terms, so that neither the largest row of the call nor
 terms that cancel count.  Tolerances are those of whole results in test_gpu_transformer.py, 1e-5 and 2e-5 for gradients: a term is off by the roundings of its factors (2^-22 as two halves,
@@ -107,3 +107,73 @@ def test_attention_values_far_out_of_little_weight(ops, size, seed):  # noqa: F8
     k[:, 1::9, :, 0] = -22.0 / (3.0 * scale)
     check_attention(ops, q, k, v, dout, scale, causal)
 
+
+# ---- vocabulary loss ------------------------------------------------------------------------------------------------------------------
+
+
+def vocabulary_rows(h, w, bias, target, upstream, reduction, smoothing):
+    """Gradients in 64 bits with the sizes of their rows: of dH a token's, of dW a word's, of db a word's value."""
+    h, w, bias = h.double(), w.double(), bias.double()
+    x = h @ w + bias
+    valid = target >= 0
+    g = torch.softmax(x, -1) - smoothing / w.shape[1]
+    g[torch.arange(len(target)), target.clamp(min=0)] -= 1.0 - smoothing
+    s = upstream.double() / (valid.sum() if reduction == "mean" else 1)
+    g = g * torch.where(valid, s, 0.0).expand(len(target))[:, None]
+    square = lambda t, d: (t ** 2).sum(d)  # noqa: E731
+    return [g @ w.t(), (h.t() @ g).t(), g.sum(0)[:, None]], [((g ** 2) @ square(w, 0)).sqrt(), ((g ** 2).t() @ square(h, 1)).sqrt(), g.abs().sum(0)]
+
+
+def check_vocabulary(ops, h, w, bias, target, upstream, reduction, smoothing, tied):
+    want, size = vocabulary_rows(h, w, bias, target, upstream, reduction, smoothing)
+    H, B, W = up(ops, h), up(ops, bias), up(ops, w.t().contiguous()).transpose() if tied else up(ops, w)
+    kind = dict(ignore_index=-100, label_smoothing=smoothing)
+    t = target.cuda()
+    loss = ops.V.vocabulary_loss(H, W, B, t, **kind)
+    gh, gw, gb = ops.V.vocabulary_loss_backward(H, W, B, t, loss, upstream.cuda(), reduction=reduction, **kind)
+    # db sums probabilities of one sign, whose errors have one sign too where they are the exponent's: log2(e) as a float is off by 1.3e-8 of itself, so that every exp(-t) is by t 1.3e-8, 7e-7 at
+    # t = 53, all in one direction.  Over 1500 tokens that alone is sqrt(1500) * 7e-7 = 2.7e-5 of the square root of the sum of squares: it is measured against the sum of magnitudes.
+    for g, want_g, s, what in zip((down(gh), down(gw).t(), down(gb)[:, None]), want, size, ("grad_h", "grad_w", "grad_bias")):
+        rows_close(g, want_g, s, 2 * RTOL_FRO, what)
+
+
+VOCABULARY = [(300, 96, 20000), (700, 130, 9000), (1500, 64, 4100), (40, 96, 3000)]  # tokens, dim, words; the last by the kernels for few tokens
+
+
+@pytest.mark.parametrize("size", VOCABULARY, ids=str)
+@pytest.mark.parametrize("tied", [True, False], ids=["tied", "plain"])
+@pytest.mark.parametrize("far", [8.0, 16.0, 20.0, 25.0, 40.0])
+def test_vocabulary_words_of_little_weight(ops, size, tied, far):  # noqa: F811
+    """A confident head: words whose logits lie `far` below the others' and that no target names.  Their rows of dW are sums of such probabilities alone."""
+    m, d, v = size
+    h, w, bias = randn(50, m, d), randn(51, d, v) * (1.3 / math.sqrt(d)), randn(52, v) * 0.1
+    rare = torch.rand(v, generator=torch.Generator().manual_seed(53)) < 0.5
+    rare[300:700] = True  # (and whole tiles of them)
+    bias[rare] -= far
+    common = torch.nonzero(~rare)[:, 0]
+    target = common[torch.randint(0, len(common), (m,), generator=torch.Generator().manual_seed(54))]
+    target[::17] = -100
+    check_vocabulary(ops, h, w, bias, target, torch.ones(1), "mean", 0.0, tied)
+
+
+@pytest.mark.parametrize("size", VOCABULARY, ids=str)
+@pytest.mark.parametrize("tied", [True, False], ids=["tied", "plain"])
+@pytest.mark.parametrize("what", ["upstream", "hidden", "both", "large"])
+def test_vocabulary_tokens_of_different_sizes(ops, size, tied, what):  # noqa: F811
+    """Tokens whose upstream gradients or hidden states lie up to 10^8 apart: a word that matters to small ones alone keeps its row of dW."""
+    m, d, v = size
+    h, w, bias = randn(60, m, d), randn(61, d, v) * (1.3 / math.sqrt(d)), randn(62, v) * 0.1
+    target = torch.randint(0, v, (m,), generator=torch.Generator().manual_seed(63))
+    target[::19] = -100
+    upstream = randn(64, m)
+    spread = 10.0 ** (-8.0 * torch.rand(m, generator=torch.Generator().manual_seed(65)))
+    if what in ("upstream", "both"):
+        upstream *= spread
+    if what in ("hidden", "both"):
+        h *= spread[:, None]
+    if what == "large":
+        upstream *= 1e25
+        h *= 1e-25
+    upstream[5] = 0.0
+    bias[target.clamp(min=0)] -= 25.0  # (so that its tokens' G is nearly all that there is of a word)
+    check_vocabulary(ops, h, w, bias, target, upstream, "none", 0.0, tied)

@@ -25,12 +25,12 @@ extern "C" {
 
 /* out[r, :] = (x[r, :] - mean[r]) * rstd[r] * weight + bias over the last axis of X (any strides, rank 1 to 8, N = its last extent >= 1),
  * mean and biased variance of each row, rstd = 1 / sqrt(variance + eps), eps >= 0, N up to 2^27.  weight, bias: N floats or NULL (1 and 0).
- * out: dense, X's shape.  mean, rstd: one float a row, or NULL (both) when no gradient is wanted. */
+ * out: dense, X's shape; it may be X's own place where X is dense.  mean, rstd: one float a row, or NULL (both) when no gradient is wanted. */
 int tenmo_hip_layer_norm_forward_f32(const tenmo_view* X, const float* weight, const float* bias, float eps,
                                      float* out, float* mean, float* rstd, int32_t sync);
 /* For the upstream gradient dY (dense, X's shape), with xhat = (x - mean) * rstd and g = dY * weight:
  * grad_X = rstd * (g - mean_row(g) - xhat * mean_row(g * xhat)) (dense, X's shape), grad_weight = sum over rows of dY * xhat,
- * grad_bias = sum over rows of dY. */
+ * grad_bias = sum over rows of dY.  grad_X may be dY's own place, or X's where X is dense, and shares none with them otherwise; grad_weight and grad_bias share none with anything. */
 int64_t tenmo_hip_layer_norm_backward_workspace_bytes(int64_t rows, int64_t n);
 int tenmo_hip_layer_norm_backward_f32(const tenmo_view* X, const float* weight, const float* mean, const float* rstd, const float* dY,
                                       float* grad_X, float* grad_weight, float* grad_bias, int32_t accumulate,

@@ -10,7 +10,8 @@
 //   * loads and stores are 16 bytes whatever the row's alignment (global memory needs 4): rows of odd length cost split cache lines,
 //     not instructions.
 //   * backward: each wavefront (or workgroup) takes every G-th row and keeps the sums of its columns for dw and db in registers; a row of partial sums a workgroup
-//     goes to the workspace, and a second launch adds them in a fixed order.  For few rows workgroups of columns in the one launch take their place.
+//     goes to the workspace, and a second launch adds them in a fixed order.  For few rows workgroups of columns in the one launch take their place, unless grad_X is
+//     written where they read.
 #include "entry.hpp"
 
 #include <algorithm>
@@ -339,6 +340,13 @@ int norm_rows(const tenmo_view* X, const char* who, NormRows* r) {
     return 0;
 }
 
+// Whether the n floats at p may share a place with the view
+bool may_share(const float* p, int64_t n, const tenmo_view* X) {
+    int64_t low = X->offset, high = X->offset;
+    for (int d = 0; d < X->rank; ++d) (X->strides[d] < 0 ? low : high) += (X->shape[d] - 1) * X->strides[d];
+    return p && (uintptr_t)p <= (uintptr_t)(X->data + high) && (uintptr_t)(X->data + low) < (uintptr_t)(p + n);
+}
+
 // Rows of partial sums, which is workgroups: enough to fill the chip two or three times over
 constexpr int64_t kNormWorkgroups = 768;
 int64_t norm_rows_at_a_time(int64_t n) { return n <= 1024 ? 4 : 1; }
@@ -420,7 +428,10 @@ int tenmo_hip_layer_norm_backward_f32(const tenmo_view* X, const float* weight, 
     a.grad_x = grad_X; a.grad_weight = grad_weight; a.grad_bias = grad_bias; a.accumulate = accumulate ? 1 : 0;
     const hipStream_t stream = call.state.stream;
     const int64_t n = a.in.n;
-    const bool by_rows = n <= 8192 && (a.in.col_stride == 1 || n == 1), columns_too = by_rows && a.in.rows > 0 && norm_columns_in_launch(a.in.rows, n) && (grad_weight || grad_bias);
+    const int64_t all = a.in.rows * n;
+    const bool in_place = all > 0 && (may_share(grad_X, all, X) || (grad_X && (uintptr_t)grad_X < (uintptr_t)(dY + all) && (uintptr_t)dY < (uintptr_t)(grad_X + all)));
+    const bool by_rows = n <= 8192 && (a.in.col_stride == 1 || n == 1);
+    const bool columns_too = by_rows && all > 0 && !in_place && norm_columns_in_launch(a.in.rows, n) && (grad_weight || grad_bias);
     if ((grad_weight || grad_bias) && !columns_too) {
         Workspace ws(workspace, workspace_bytes);
         a.parts = a.in.rows ? norm_parts(a.in.rows, n) : 0;
@@ -432,8 +443,9 @@ int tenmo_hip_layer_norm_backward_f32(const tenmo_view* X, const float* weight, 
             a.row_groups = grad_X || !columns_too ? norm_parts(a.in.rows, n) : 0;
             hipLaunchKernelGGL(norm_backward_for(n), dim3((unsigned)(a.row_groups + (columns_too ? (n + 15) / 16 : 0))), dim3(256), 0, stream, a);
         } else {
-            if (grad_X) hipLaunchKernelGGL(norm_backward_any_kernel, dim3(norm_grid(a.in.rows)), dim3(256), 0, stream, a);
+            // (the sums first: grad_X may be written where they read)
             if (a.partial) hipLaunchKernelGGL(norm_columns_any_kernel, dim3((unsigned)((n + 255) / 256), (unsigned)a.parts), dim3(256), 0, stream, a);
+            if (grad_X) hipLaunchKernelGGL(norm_backward_any_kernel, dim3(norm_grid(a.in.rows)), dim3(256), 0, stream, a);
         }
     }
     if ((grad_weight || grad_bias) && !columns_too) hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)((n + 63) / 64), 2), dim3(1024), 0, stream, a);

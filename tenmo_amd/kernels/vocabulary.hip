@@ -12,7 +12,7 @@
 //     Two forms of G, since its two products sum over different axes:
 //       G W^T    G at 2^14.  A row is a token's, whose target has p - 1, itself right to 2^-24 of 1; the halves hold the others to 2^-40 of 1.
 //       G^T H    scale_m G / (the scale of H's row m), which is what a word's row of dW is summed from: with a scale for each word and 64 tokens, a power of 2^12 that brings their largest into
-//                2^1 .. 2^13 (split_gemm.hpp brings them to the word's smallest).  Words without a target have probabilities alone in their rows, however small, and tokens lie far apart in
+//                2^2 .. 2^14 (split_gemm.hpp brings them to the word's smallest).  Words without a target have probabilities alone in their rows, however small, and tokens lie far apart in
 //                their upstream gradients: at 2^14 for all, rows of words whose logits lie 16 below the others' were off by 5e-2 of what enters them, 20 below by 1 (700 tokens,
 //                130 x 9000).  It costs a second G in memory and the scales, 1000 -> 1198 us, and factors as it is read, 1850 -> 1935 us (half of 8192 x 50257, D = 768).
 #include "split_gemm.hpp"

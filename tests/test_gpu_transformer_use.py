@@ -1,0 +1,52 @@
+"""The transformer's operators as a program puts them together: gradients in place of what they are made from, one tensor in several roles, refusals inside a capture, and all of
+them in one graph of tensors."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from helpers import RTOL_FRO
+from test_gpu_transformer import close, down, ops, randn, up  # noqa: F401  (ops is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("shape", [(1, 768), (7, 64), (300, 768), (1024, 1024), (1030, 2049), (3, 8192), (3, 8193), (20, 20001)], ids=str)
+@pytest.mark.parametrize("where", ["dy", "x"])
+@pytest.mark.parametrize("accumulate", [0, 1])
+def test_layer_norm_gradient_in_place(ops, shape, where, accumulate):  # noqa: F811
+    """grad_X written over dY, or over X: the same bits as beside them."""
+    from tenmo_amd import _transformer as T
+
+    rows, n = shape
+    x, w, b, dy = up(ops, randn(1, rows, n)), up(ops, randn(2, n)), up(ops, randn(3, n)), up(ops, randn(4, rows, n))
+    y, mean, rstd = ops.N.layer_norm(x, w, b)
+    L = T.load()
+    size = L.tenmo_hip_layer_norm_backward_workspace_bytes(rows, n)
+    workspace = torch.empty((size + 3) // 4, device="cuda")
+    got = []
+    for aside in (True, False):
+        xs, dys = x.storage.clone(), dy.storage.clone()
+        place = dys if where == "dy" else xs
+        gx = place.clone() if aside else place
+        gw, gb = torch.ones(n, device="cuda"), torch.ones(n, device="cuda")
+        torch.cuda.synchronize()
+        X = ops.NDBuffer(xs, shape)
+        ops.lib.check(L.tenmo_hip_layer_norm_backward_f32(T.view(X), T.address(w), T.address(mean), T.address(rstd), dys.data_ptr(), gx.data_ptr(), gw.data_ptr(), gb.data_ptr(),
+                                                          accumulate, workspace.data_ptr(), size, 1))
+        got.append((gx, gw, gb))
+    # few rows: dw and db are summed in another order beside them than in place, 16 rows against 4 a workgroup
+    assert torch.equal(got[0][0], got[1][0])
+    for a, c in zip(got[0][1:], got[1][1:]):
+        close(a.cpu(), c.cpu(), RTOL_FRO)
+
+
+@pytest.mark.parametrize("shape", [(5, 64), (300, 768), (9, 2049), (3, 20001)], ids=str)
+def test_layer_norm_in_place(ops, shape):  # noqa: F811
+    from tenmo_amd import _transformer as T
+
+    x, w = up(ops, randn(5, *shape)), up(ops, randn(6, shape[1]))
+    want = down(ops.N.layer_norm(x, w, None)[0])
+    ops.lib.check(T.load().tenmo_hip_layer_norm_forward_f32(T.view(x), T.address(w), None, 1e-5, x.data_ptr(), None, None, 1))
+    assert torch.equal(down(x), want)

@@ -52,7 +52,7 @@ def load() -> C.CDLL:
 
 def enter(*operands: Optional[NDBuffer]):
     """(library, token): the library initialised, every operand on its device, its stream behind the current one.  ``leave(token)`` puts the
-    current stream behind the library's."""
+    current stream behind the library's, and has to follow also where the call between them raises: a capture cannot end while the library's stream is forked from it."""
     _lib.init()
     for b in operands:
         if b is not None and b.storage.get_device() != 0:  # _lib.init's device

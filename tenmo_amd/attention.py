@@ -34,12 +34,14 @@ def attention(q: NDBuffer, k: NDBuffer, v: NDBuffer, scale: Optional[float] = No
     lengths = _t.device_ints(key_lengths, batch, "attention: key_lengths")
     starts = _t.device_ints(query_starts, batch, "attention: query_starts")
     L, joined = _t.enter(q, k, v)
-    out = _t.empty(q, batch, queries, heads, dim)
-    lse = _t.empty(q, batch, heads, queries) if statistics else None
-    _, ws, size = _keep = _t.workspace(q, L.tenmo_hip_attention_forward_workspace_bytes(*sizes))
-    check(L.tenmo_hip_attention_forward_f32(_t.view(q), _t.view(k), _t.view(v), 1.0 / math.sqrt(dim) if scale is None else scale,
-                                            1 if causal else 0, lengths, starts, out.data_ptr(), _t.address(lse), ws, size, 1 if sync else 0))
-    _t.leave(joined)
+    try:
+        out = _t.empty(q, batch, queries, heads, dim)
+        lse = _t.empty(q, batch, heads, queries) if statistics else None
+        _, ws, size = _keep = _t.workspace(q, L.tenmo_hip_attention_forward_workspace_bytes(*sizes))
+        check(L.tenmo_hip_attention_forward_f32(_t.view(q), _t.view(k), _t.view(v), 1.0 / math.sqrt(dim) if scale is None else scale,
+                                                1 if causal else 0, lengths, starts, out.data_ptr(), _t.address(lse), ws, size, 1 if sync else 0))
+    finally:
+        _t.leave(joined)
     return out, lse
 
 
@@ -57,13 +59,15 @@ def attention_backward(q: NDBuffer, k: NDBuffer, v: NDBuffer, out: NDBuffer, lse
     _t.dense(dout, q.shape, "attention_backward: dout")
     _t.dense(lse, (batch, heads, queries), "attention_backward: lse")
     L, joined = _t.enter(q, k, v, out, lse, dout, *(into or ()))
-    grads = tuple(into) if into is not None else tuple(_t.empty(b, *b.shape) if n else None for b, n in zip((q, k, v), need))
-    _, ws, size = _keep = _t.workspace(q, L.tenmo_hip_attention_backward_workspace_bytes(*sizes))
-    views = [_t.view(g) for g in grads]
-    check(L.tenmo_hip_attention_backward_f32(_t.view(q), _t.view(k), _t.view(v), 1.0 / math.sqrt(dim) if scale is None else scale,
-                                             1 if causal else 0, lengths, starts, _t.address(out), _t.address(lse), _t.address(dout), *views,
-                                             0 if into is None else 1, ws, size, 1 if sync else 0))
-    _t.leave(joined)
+    try:
+        grads = tuple(into) if into is not None else tuple(_t.empty(b, *b.shape) if n else None for b, n in zip((q, k, v), need))
+        _, ws, size = _keep = _t.workspace(q, L.tenmo_hip_attention_backward_workspace_bytes(*sizes))
+        views = [_t.view(g) for g in grads]
+        check(L.tenmo_hip_attention_backward_f32(_t.view(q), _t.view(k), _t.view(v), 1.0 / math.sqrt(dim) if scale is None else scale,
+                                                 1 if causal else 0, lengths, starts, _t.address(out), _t.address(lse), _t.address(dout), *views,
+                                                 0 if into is None else 1, ws, size, 1 if sync else 0))
+    finally:
+        _t.leave(joined)
     return grads
 
 

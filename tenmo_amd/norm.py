@@ -25,11 +25,13 @@ def layer_norm(x: NDBuffer, weight: Optional[NDBuffer] = None, bias: Optional[ND
     _t.dense(weight, (n,), "layer_norm: weight")
     _t.dense(bias, (n,), "layer_norm: bias")
     L, joined = _t.enter(x, weight, bias)
-    out = _t.empty(x, *x.shape)
-    mean, rstd = (_t.empty(x, rows), _t.empty(x, rows)) if statistics else (None, None)
-    check(L.tenmo_hip_layer_norm_forward_f32(_t.view(x), _t.address(weight), _t.address(bias), eps, out.data_ptr(),
-                                             _t.address(mean), _t.address(rstd), 1 if sync else 0))
-    _t.leave(joined)
+    try:
+        out = _t.empty(x, *x.shape)
+        mean, rstd = (_t.empty(x, rows), _t.empty(x, rows)) if statistics else (None, None)
+        check(L.tenmo_hip_layer_norm_forward_f32(_t.view(x), _t.address(weight), _t.address(bias), eps, out.data_ptr(),
+                                                 _t.address(mean), _t.address(rstd), 1 if sync else 0))
+    finally:
+        _t.leave(joined)
     return out, mean, rstd
 
 
@@ -49,12 +51,14 @@ def layer_norm_backward(x: NDBuffer, weight: Optional[NDBuffer], mean: NDBuffer,
         for g, shape, what in zip(into, (x.shape, (n,), (n,)), ("grad_x", "grad_weight", "grad_bias")):
             _t.dense(g, shape, "layer_norm_backward: " + what)
     L, joined = _t.enter(x, weight, mean, rstd, dy, *(into or ()))
-    gx, gw, gb = into if into is not None else (_t.empty(x, *x.shape) if need_x else None, _t.empty(x, n) if need_weight else None,
-                                                _t.empty(x, n) if need_bias else None)
-    _, ws, size = _keep = _t.workspace(x, L.tenmo_hip_layer_norm_backward_workspace_bytes(rows, n) if gw is not None or gb is not None else 0)
-    check(L.tenmo_hip_layer_norm_backward_f32(_t.view(x), _t.address(weight), _t.address(mean), _t.address(rstd), _t.address(dy),
-                                              _t.address(gx), _t.address(gw), _t.address(gb), 0 if into is None else 1, ws, size, 1 if sync else 0))
-    _t.leave(joined)
+    try:
+        gx, gw, gb = into if into is not None else (_t.empty(x, *x.shape) if need_x else None, _t.empty(x, n) if need_weight else None,
+                                                    _t.empty(x, n) if need_bias else None)
+        _, ws, size = _keep = _t.workspace(x, L.tenmo_hip_layer_norm_backward_workspace_bytes(rows, n) if gw is not None or gb is not None else 0)
+        check(L.tenmo_hip_layer_norm_backward_f32(_t.view(x), _t.address(weight), _t.address(mean), _t.address(rstd), _t.address(dy),
+                                                  _t.address(gx), _t.address(gw), _t.address(gb), 0 if into is None else 1, ws, size, 1 if sync else 0))
+    finally:
+        _t.leave(joined)
     return gx, gw, gb
 
 

@@ -37,12 +37,14 @@ def vocabulary_loss(h: NDBuffer, w: NDBuffer, bias: Optional[NDBuffer], target: 
     sizes = m, _, _ = _sizes(h, w, bias)
     t = _t.device_ints(target, m, "vocabulary_loss: target", (torch.int64, torch.int32))
     L, joined = _t.enter(h, w, bias)
-    loss = Loss(_t.empty(h, m), _t.empty(h, m), _t.empty(h, 1), torch.empty(1, dtype=torch.int32, device=h.storage.device))
-    _, ws, size = _keep = _t.workspace(h, L.tenmo_hip_vocabulary_loss_forward_workspace_bytes(*sizes))
-    check(L.tenmo_hip_vocabulary_loss_forward_f32(_t.view(h), _t.view(w), _t.address(bias), t, 1 if target.dtype == torch.int64 else 0,
-                                                  ignore_index, label_smoothing, loss.per_sample.data_ptr(), loss.lse.data_ptr(), loss.loss_sum.data_ptr(),
-                                                  loss.valid_count.data_ptr(), ws, size, 1 if sync else 0))
-    _t.leave(joined)
+    try:
+        loss = Loss(_t.empty(h, m), _t.empty(h, m), _t.empty(h, 1), torch.empty(1, dtype=torch.int32, device=h.storage.device))
+        _, ws, size = _keep = _t.workspace(h, L.tenmo_hip_vocabulary_loss_forward_workspace_bytes(*sizes))
+        check(L.tenmo_hip_vocabulary_loss_forward_f32(_t.view(h), _t.view(w), _t.address(bias), t, 1 if target.dtype == torch.int64 else 0,
+                                                      ignore_index, label_smoothing, loss.per_sample.data_ptr(), loss.lse.data_ptr(), loss.loss_sum.data_ptr(),
+                                                      loss.valid_count.data_ptr(), ws, size, 1 if sync else 0))
+    finally:
+        _t.leave(joined)
     return loss
 
 
@@ -62,20 +64,22 @@ def vocabulary_loss_backward(h: NDBuffer, w: NDBuffer, bias: Optional[NDBuffer],
         _t.dense(into[0], (m, d), "vocabulary_loss_backward: grad_h")
         _t.dense(into[2], (v,), "vocabulary_loss_backward: grad_bias")
     L, joined = _t.enter(h, w, bias, *(into or ()))
-    if into is not None:
-        gh, gw, gb = into
-    else:
-        gh = _t.empty(h, m, d) if need[0] else None
-        gb = _t.empty(h, v) if need[2] and bias is not None else None
-        gw = None
-        if need[1]:
-            gw = _t.empty(w, v, d).transpose() if w.strides[0] == 1 and d > 1 else _t.empty(w, d, v)
-    _, ws, size = _keep = _t.workspace(h, L.tenmo_hip_vocabulary_loss_backward_workspace_bytes(*sizes))
-    check(L.tenmo_hip_vocabulary_loss_backward_f32(_t.view(h), _t.view(w), _t.address(bias), t, 1 if target.dtype == torch.int64 else 0,
-                                                   ignore_index, label_smoothing, loss.lse.data_ptr(), up, REDUCTIONS[reduction], loss.valid_count.data_ptr(),
-                                                   _t.address(gh), _t.view(gw), _t.address(gb), 0 if into is None else 1,
-                                                   ws, size, 1 if sync else 0))
-    _t.leave(joined)
+    try:
+        if into is not None:
+            gh, gw, gb = into
+        else:
+            gh = _t.empty(h, m, d) if need[0] else None
+            gb = _t.empty(h, v) if need[2] and bias is not None else None
+            gw = None
+            if need[1]:
+                gw = _t.empty(w, v, d).transpose() if w.strides[0] == 1 and d > 1 else _t.empty(w, d, v)
+        _, ws, size = _keep = _t.workspace(h, L.tenmo_hip_vocabulary_loss_backward_workspace_bytes(*sizes))
+        check(L.tenmo_hip_vocabulary_loss_backward_f32(_t.view(h), _t.view(w), _t.address(bias), t, 1 if target.dtype == torch.int64 else 0,
+                                                       ignore_index, label_smoothing, loss.lse.data_ptr(), up, REDUCTIONS[reduction], loss.valid_count.data_ptr(),
+                                                       _t.address(gh), _t.view(gw), _t.address(gb), 0 if into is None else 1,
+                                                       ws, size, 1 if sync else 0))
+    finally:
+        _t.leave(joined)
     return gh, gw, gb
 
 

@@ -50,3 +50,32 @@ def test_layer_norm_in_place(ops, shape):  # noqa: F811
     want = down(ops.N.layer_norm(x, w, None)[0])
     ops.lib.check(T.load().tenmo_hip_layer_norm_forward_f32(T.view(x), T.address(w), None, 1e-5, x.data_ptr(), None, None, 1))
     assert torch.equal(down(x), want)
+
+
+def test_refusals_inside_a_capture(ops):  # noqa: F811
+    """A program that catches a refusal while it captures goes on with its graph."""
+    N = ops.NDBuffer
+    q, wide, x, h, w = up(ops, randn(1, 1, 40, 2, 32)), N.empty((1, 8, 2, 129)), up(ops, randn(2, 6, 64)), up(ops, randn(3, 5, 32)), up(ops, randn(4, 32, 50))
+    target, lse, many = torch.arange(5, device="cuda"), N.empty((1, 2, 8)), N.empty((1 << 23, 1))
+    words = N(torch.zeros(1, device="cuda"), (32, (1 << 22) + 1), (0, 0))
+    calls = [lambda: ops.A.attention(wide, wide, wide), lambda: ops.A.attention_backward(wide, wide, wide, wide, lse, wide),
+             lambda: ops.N.layer_norm(x, eps=-1.0), lambda: ops.N.layer_norm_backward(N(x.storage, (2, 0)), None, N.empty((0,)), N.empty((0,)), N.empty((2, 0))),
+             lambda: ops.V.vocabulary_loss(many, N.empty((1, 4)), None, torch.zeros(1 << 23, dtype=torch.int64, device="cuda")),
+             lambda: ops.V.vocabulary_loss(h, words, None, target),
+             lambda: ops.V.vocabulary_loss_backward(h, w, None, target, loss, torch.ones(1, device="cuda"), label_smoothing=2.0)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss = ops.V.vocabulary_loss(h, w, None, target)
+        want = down(ops.A.attention(q, q, q, causal=True)[0])
+    for call in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(ops.lib.TenmoHipError):
+                call()
+            o, _ = ops.A.attention(q, q, q, causal=True)
+        for _ in range(3):
+            o.storage.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(down(o), want)

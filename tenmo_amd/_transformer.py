@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
-from typing import Optional
+from typing import Callable, Optional, Sequence
 
 import torch
 
@@ -123,6 +123,20 @@ def address(b: Optional[NDBuffer]) -> Optional[int]:
 def dense(b: Optional[NDBuffer], shape: tuple, what: str) -> None:
     if b is not None and (b.shape != shape or not (b.strides == (1,) or b.is_contiguous())):
         raise TenmoHipError(-2, f"{what} must be dense with shape {shape}, got shape {b.shape} with strides {b.strides}")
+
+
+def into_gradients(tensors: Sequence, call: Callable) -> list:
+    """For the tensors of a node (None where it has none): ``call(into)`` with the gradients that are to be added to, None where there is none; once for each role where a tensor has
+    several, since two gradients of one call may not share a place.  The tensors that got one."""
+    wanted = [t is not None and t.requires_grad for t in tensors]
+    given = [id(t) for t in tensors if t is not None]
+    if len(set(given)) == len(given):
+        call([t.ensure_gradbox() if w else None for t, w in zip(tensors, wanted)])
+    else:
+        for role, w in enumerate(wanted):
+            if w:
+                call([t.ensure_gradbox() if i == role else None for i, t in enumerate(tensors)])
+    return [t for t, w in zip(tensors, wanted) if w]
 
 
 def device_ints(t: Optional[torch.Tensor], n: int, what: str, dtypes=(torch.int32,)) -> Optional[int]:

@@ -94,16 +94,10 @@ class Attention:
         out = Tensor(o)
         if track:
             def backward(output: Tensor, retain_graph: bool = False) -> List[Tensor]:
-                if q is k or q is v or k is v:  # one tensor in two roles: its gradients are added one after the other
-                    for role in range(3):
-                        into = [t.ensure_gradbox() if t.requires_grad and i == role else None for i, t in enumerate((q, k, v))]
-                        attention_backward(q.buffer, k.buffer, v.buffer, o, lse, output.gradbox, into=into, **mask)
-                else:
-                    into = [t.ensure_gradbox() if t.requires_grad else None for t in (q, k, v)]
-                    attention_backward(q.buffer, k.buffer, v.buffer, o, lse, output.gradbox, into=into, **mask)
+                got = _t.into_gradients((q, k, v), lambda into: attention_backward(q.buffer, k.buffer, v.buffer, o, lse, output.gradbox, into=into, **mask))
                 if not retain_graph:
                     output.zero_grad()
-                return [t for t in (q, k, v) if t.requires_grad]
+                return got
 
             out.requires_grad = True
             out.add_ancestry(backward, q, k, v)

@@ -81,11 +81,10 @@ class LayerNorm:
             w, b = self.weight, self.bias
 
             def backward(output: Tensor, retain_graph: bool = False) -> List[Tensor]:
-                into = [p.ensure_gradbox() if p.requires_grad else None for p in (xs, w, b)]
-                layer_norm_backward(xs.buffer, w.buffer, mean, rstd, output.gradbox, into=into)
+                got = _t.into_gradients((xs, w, b), lambda into: layer_norm_backward(xs.buffer, w.buffer, mean, rstd, output.gradbox, into=into))
                 if not retain_graph:
                     output.zero_grad()
-                return [p for p in (xs, w, b) if p.requires_grad]
+                return got
 
             out.requires_grad = True
             out.add_ancestry(backward, xs, w, b)

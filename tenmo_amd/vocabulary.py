@@ -103,11 +103,11 @@ class VocabularyLoss:
             out = Tensor(NDBuffer(loss.loss_sum.storage / loss.valid_count.clamp(min=1), (1,)))
         if track_grad and any(p.requires_grad for p in parents):
             def backward(output: Tensor, retain_graph: bool = False) -> List[Tensor]:
-                grads = [p.ensure_gradbox() if p.requires_grad else None for p in parents] + [None] * (3 - len(parents))
-                vocabulary_loss_backward(h.buffer, w.buffer, b, target, loss, output.gradbox.storage[:output.numels()], reduction=reduction, into=grads, **kind)
+                upstream = output.gradbox.storage[:output.numels()]
+                got = _t.into_gradients((h, w, bias), lambda into: vocabulary_loss_backward(h.buffer, w.buffer, b, target, loss, upstream, reduction=reduction, into=into, **kind))
                 if not retain_graph:
                     output.zero_grad()
-                return [p for p in parents if p.requires_grad]
+                return got
 
             out.requires_grad = True
             out.add_ancestry(backward, *parents)

@@ -79,3 +79,40 @@ def test_refusals_inside_a_capture(ops):  # noqa: F811
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(down(o), want)
+
+
+def grad(t):
+    return t.grad().reshape(-1)
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+def test_one_tensor_in_several_roles(ops, rows):  # noqa: F811
+    """The gradient of a tensor with several roles in a node is the sum of those it would have in each."""
+    T, n = ops.Tensor, 320
+    x, w, b = (randn(i, *s).numpy() for i, s in enumerate(((rows, n), (n,), (n,))))
+    new = lambda a: T.from_numpy(a, requires_grad=True)  # noqa: E731
+
+    def norm(X, W, B):
+        layer = ops.N.LayerNorm(n)
+        layer.weight, layer.bias = W, B
+        layer(X).backward()
+
+    X, W, B = new(x), new(w), new(w)
+    norm(X, W, B)
+    X2, W2 = new(x), new(w)
+    norm(X2, W2, W2)
+    assert np.array_equal(grad(X), grad(X2))
+    close(grad(W2), grad(W).astype(np.float64) + grad(B), RTOL_FRO, "weight and bias")
+    A, W, B = new(w), new(w), new(b)
+    norm(A, W, B)
+    A2, B2 = new(w), new(b)
+    norm(A2, A2, B2)
+    close(grad(A2), grad(A).astype(np.float64) + grad(W), RTOL_FRO, "input and weight")
+
+    h = randn(7, n, n).numpy() * 0.05
+    target = (torch.arange(n, device="cuda") * 7) % n
+    H, V = new(h), new(h)
+    ops.V.VocabularyLoss.forward(H, V, None, target).backward()
+    H2 = new(h)
+    ops.V.VocabularyLoss.forward(H2, H2, None, target).backward()
+    close(grad(H2), grad(H).astype(np.float64) + grad(V), RTOL_FRO, "hidden states and weight")

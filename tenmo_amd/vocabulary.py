@@ -5,6 +5,7 @@ h is [tokens, dim], w [dim, vocabulary] (a ``Linear``'s weight, or the transpose
 """
 from __future__ import annotations
 
+import math
 from typing import List, NamedTuple, Optional, Tuple
 
 import torch
@@ -83,20 +84,34 @@ def vocabulary_loss_backward(h: NDBuffer, w: NDBuffer, bias: Optional[NDBuffer],
     return gh, gw, gb
 
 
+def _rows(h: NDBuffer) -> NDBuffer:
+    """[..., dim] as [tokens, dim]."""
+    if h.rank() < 3:
+        return h
+    if not h.is_contiguous():
+        raise TenmoHipError(-5, f"VocabularyLoss: hidden states {h.shape} with strides {h.strides}: more than two axes need to be dense")
+    return h.view((math.prod(h.shape[:-1]), h.shape[-1]), (h.shape[-1], 1), h.offset)
+
+
 class VocabularyLoss:
     """The loss at a language model's head in the autograd graph."""
 
     @staticmethod
     def forward(h: Tensor, w: Tensor, bias: Optional[Tensor], target: torch.Tensor, reduction: str = "mean", ignore_index: int = -100,
-                label_smoothing: float = 0.0, track_grad: bool = True, sync: bool = False) -> Tensor:
+                label_smoothing: float = 0.0, track_grad: bool = True, sync: bool = False, tied: bool = False) -> Tensor:
+        """h: [..., dim], as the layers before it return it, and target as many values.  w: [dim, vocabulary], or, ``tied``, an embedding [vocabulary, dim], whose gradient it is then that
+        is added to (a ``Tensor.transpose`` is a leaf of its own).  The loss is [1], or of h's leading axes for "none"."""
         if reduction not in REDUCTIONS:
             raise TenmoHipError(-3, f"VocabularyLoss: reduction must be one of {sorted(REDUCTIONS)}, got {reduction!r}")
         parents = (h, w) + ((bias,) if bias is not None else ())
         kind = dict(ignore_index=ignore_index, label_smoothing=label_smoothing)
         b = bias.buffer if bias is not None else None
-        loss = vocabulary_loss(h.buffer, w.buffer, b, target, sync=sync, **kind)
+        if tied and w.rank() != 2:
+            raise TenmoHipError(-2, f"VocabularyLoss: an embedding is [vocabulary, dim], got {w.shape()}")
+        rows, weight = _rows(h.buffer), w.buffer.transpose() if tied else w.buffer
+        loss = vocabulary_loss(rows, weight, b, target, sync=sync, **kind)
         if reduction == "none":
-            out = Tensor(loss.per_sample)
+            out = Tensor(NDBuffer(loss.per_sample.storage, h.shape()[:-1]))
         elif reduction == "sum":
             out = Tensor(loss.loss_sum)
         else:
@@ -104,7 +119,14 @@ class VocabularyLoss:
         if track_grad and any(p.requires_grad for p in parents):
             def backward(output: Tensor, retain_graph: bool = False) -> List[Tensor]:
                 upstream = output.gradbox.storage[:output.numels()]
-                got = _t.into_gradients((h, w, bias), lambda into: vocabulary_loss_backward(h.buffer, w.buffer, b, target, loss, upstream, reduction=reduction, into=into, **kind))
+
+                def add(into):
+                    gh, gw, gb = into
+                    gh = None if gh is None else NDBuffer(gh.storage, rows.shape)
+                    gw = gw.transpose() if tied and gw is not None else gw
+                    vocabulary_loss_backward(rows, weight, b, target, loss, upstream, reduction=reduction, into=(gh, gw, gb), **kind)
+
+                got = _t.into_gradients((h, w, bias), add)
                 if not retain_graph:
                     output.zero_grad()
                 return got

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from helpers import RTOL_FRO
-from test_gpu_transformer import close, down, ops, randn, up  # noqa: F401  (ops is a fixture)
+from test_gpu_transformer import block_tensors, close, down, ops, randn, up  # noqa: F401  (ops is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +116,56 @@ def test_one_tensor_in_several_roles(ops, rows):  # noqa: F811
     H2 = new(h)
     ops.V.VocabularyLoss.forward(H2, H2, None, target).backward()
     close(grad(H2), grad(H).astype(np.float64) + grad(V), RTOL_FRO, "hidden states and weight")
+
+
+def test_a_block_and_its_head_in_one_graph(ops):  # noqa: F811
+    """norm -> joint projection -> attention -> norm -> loss over a tied embedding: one backward call from the loss to every leaf, against 64-bit autograd."""
+    h, norm, qkv, head_norm, emb, target, H = block_tensors(ops)
+    B, S, E = h.shape()
+    target[5::11] = -100
+    y = head_norm(ops.A.Attention.packed(qkv(norm(h)), heads=H, causal=True))
+    loss = ops.V.VocabularyLoss.forward(y, emb, None, target.reshape(B, S), tied=True)
+    loss.backward()
+    tensors = [h, norm.weight, norm.bias, qkv.weight, qkv.bias, head_norm.weight, head_norm.bias, emb]
+    x, nw, nb, w, b, hw, hb, e = leaves = [torch.from_numpy(t.to_numpy()).double().requires_grad_(True) for t in tensors]
+    q, k, v = (torch.nn.functional.layer_norm(x, (E,), nw, nb, 1e-5) @ w + b).reshape(B, S, 3, H, E // H).permute(2, 0, 3, 1, 4)
+    s = (q @ k.transpose(2, 3) / math.sqrt(E // H)).masked_fill(torch.ones(S, S).triu(1).bool(), -math.inf)
+    o = torch.nn.functional.layer_norm((torch.softmax(s, -1) @ v).transpose(1, 2).reshape(B * S, E), (E,), hw, hb, 1e-5)
+    want = torch.nn.functional.cross_entropy(o @ e.t(), target.cpu())
+    want.backward()
+    close(loss.to_numpy(), want.detach().reshape(1), RTOL_FRO, "loss")
+    names = ("h", "norm.weight", "norm.bias", "qkv.weight", "qkv.bias", "head_norm.weight", "head_norm.bias", "embedding")
+    for t, ref, what in zip(tensors, leaves, names):  # four operators in a row, each with a gradient's tolerance of its own
+        close(t.grad(), ref.grad.numpy(), 8 * RTOL_FRO, what)
+
+
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("bias", [False, True])
+def test_vocabulary_loss_of_a_batch(ops, reduction, tied, bias):  # noqa: F811
+    """Hidden states [batch, length, dim] and an embedding give what [tokens, dim] and its transposed view do, the gradient in the embedding's own place."""
+    T, B, S, d, v = ops.Tensor, 3, 30, 48, 700
+    h, e, b = randn(1, B, S, d).numpy(), randn(2, v, d).numpy(), randn(3, v).numpy()
+    target = torch.randint(0, v, (B, S), generator=torch.Generator().manual_seed(4)).cuda()
+    target[1, 3:9] = -100
+    new = lambda a: T.from_numpy(np.ascontiguousarray(a), requires_grad=True)  # noqa: E731
+    H, W, C = new(h), new(e if tied else e.T), new(b) if bias else None
+    got = ops.V.VocabularyLoss.forward(H, W, C, target, reduction=reduction, tied=tied)
+    got.backward()
+    H2, W2, C2 = new(h.reshape(B * S, d)), new(e).transpose() if tied else new(e.T), new(b) if bias else None
+    want = ops.V.VocabularyLoss.forward(H2, W2, C2, target.reshape(-1), reduction=reduction)
+    want.backward()
+    assert got.shape() == ((B, S) if reduction == "none" else (1,)) and H.grad().shape == (B, S, d)
+    assert np.array_equal(got.to_numpy().reshape(-1), want.to_numpy().reshape(-1)) and np.array_equal(grad(H), grad(H2))
+    assert not bias or np.array_equal(C.grad(), C2.grad())
+    # (the gradient of the view lies along the other axis: the same sums by other tiles)
+    close(W.grad().T if tied else W.grad(), W2.grad(), RTOL_FRO, "grad_w")
+
+
+def test_vocabulary_loss_of_a_batch_refusals(ops):  # noqa: F811
+    T, N = ops.Tensor, ops.NDBuffer
+    w, t = T.zeros(48, 700), torch.zeros(60, dtype=torch.int64, device="cuda")
+    cases = [(T(N.zeros((2, 48, 30)).transpose()), w, False, "dense"), (T.zeros(2, 31, 48), w, False, "60"), (T.zeros(2, 30, 48), w, True, "inner|needed"), (T.zeros(2, 30, 48), T.zeros(48), True, "embedding")]
+    for h, weight, tied, text in cases:
+        with pytest.raises(ops.lib.TenmoHipError, match=text if text != "60" else "needs 62"):
+            ops.V.VocabularyLoss.forward(h, weight, None, t, tied=tied)

@@ -91,7 +91,8 @@ __device__ __forceinline__ void split_h_rows(const SplitArgs& a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = max(top, finite_magnitude(x[e]));
         }
-        const float scale = split_scale(wave_max_bits(top));
+        top = wave_max_bits(top);
+        const float scale = top ? split_scale(top) : 0x1p126f; // (a row of zeros has the smallest part in G^T H: it leaves the scales of the tokens beside it as they are)
         for (int64_t c = lane * 8; c < a.to_h.pitch; c += 512) {
             load8(x, p, a.h.cs, c, cols);
             split8(x, scale, a.to_h.p + r * a.to_h.pitch + c);

@@ -177,3 +177,16 @@ def test_vocabulary_tokens_of_different_sizes(ops, size, tied, what):  # noqa: F
     upstream[5] = 0.0
     bias[target.clamp(min=0)] -= 25.0  # (so that its tokens' G is nearly all that there is of a word)
     check_vocabulary(ops, h, w, bias, target, upstream, "none", 0.0, tied)
+
+
+@pytest.mark.parametrize("size", VOCABULARY, ids=str)
+@pytest.mark.parametrize("tied", [True, False], ids=["tied", "plain"])
+@pytest.mark.parametrize("hidden", [1e-5, 1.0, 300.0])
+def test_vocabulary_hidden_states_of_zeros(ops, size, tied, hidden):  # noqa: F811
+    """Tokens that count, with hidden states of zeros: the weight's gradient is that of the tokens beside them."""
+    m, d, v = size
+    h, w, bias = randn(70, m, d) * hidden, randn(71, d, v) * (1.3 / math.sqrt(d) / hidden), randn(72, v) * 0.1
+    h[::3] = 0.0
+    target = torch.randint(0, v, (m,), generator=torch.Generator().manual_seed(73))
+    target[::19] = -100
+    check_vocabulary(ops, h, w, bias, target, torch.ones(1), "mean", 0.0, tied)

@@ -150,18 +150,26 @@ __device__ __forceinline__ void stage_barrier() {
 }
 
 // An operand whose rows (of the product's M or N) have scales of their own, and others in every kCodeK of K: a row is worked on at the smallest of its scales, of which the others are multiples
-// by 2^12, 2^24 or more, and what is held at those is brought down as it is read.  Two bits for each kCodeK of K, sixteen of them a word: the power of 2^-12; three stands for nothing.
-constexpr int kCodeK = 64, kCodeBits = 12, kCodesAWord = 16;
+// by powers of 2^6, and what is held at those is brought down as it is read.  Four bits for each kCodeK of K, eight of them a word: the power of 2^-6.
+// With the largest at 2^8 .. 2^14, what lies below it by more than 2^-33 is lost (l, by itself, from 2^-30 on).  Powers of 2^12 in two bits, and nothing left from the third on, take
+// as long (2010 us for both products of half of 8192 x 50257, D = 768), but lose values from 2^-24 of the largest on: 1.5e-4 of a sum over 4100 tokens, one of which is the largest.
+constexpr int kCodeK = 64, kCodeBits = 6, kCodesAWord = 8, kMostCode = 7; // (7: h ends below 2^-28, as nothing)
 enum { kPlain, kCodedA, kCodedB };
 struct Codes {
     const uint32_t* p; // [K / (kCodeK * kCodesAWord)][pitch]
     int64_t pitch;
 };
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ f16x2 code_factor(uint32_t codes, uint32_t at) { // 1, 2^-12, 2^-24 or 0, twice
-    const uint32_t code = (codes >> (2 * at)) & 3u;
-    return __builtin_bit_cast(f16x2, code == 0 ? 0x3c003c00u : code == 1 ? 0x0c000c00u : code == 2 ? 0x00010001u : 0u);
-}
+struct CodeFactor { // fp16 ends at 2^-24: h takes two factors, l is nothing where the second counts
+    f16x2 near, far, low;
+    __device__ __forceinline__ void set(uint32_t codes, uint32_t at) {
+        const int code = (int)((codes >> (4 * at)) & 15u);
+        const _Float16 n = (_Float16)__builtin_amdgcn_ldexpf(1.f, -kCodeBits * (code < 4 ? code : 4)), f = (_Float16)__builtin_amdgcn_ldexpf(1.f, -kCodeBits * (code > 4 ? code - 4 : 0));
+        near = f16x2{n, n};
+        far = f16x2{f, f};
+        low = code > 4 ? f16x2{0, 0} : near;
+    }
+};
 __device__ __forceinline__ f16x8 times(f16x8 x, f16x2 f) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= f[e & 1];
@@ -193,7 +201,7 @@ __device__ __forceinline__ void split_tile(f32x16 (&acc)[4][2], float* lds, cons
     };
     constexpr int CODES = CODED == kCodedA ? 4 : CODED == kCodedB ? 2 : 1, CODE_STEPS = kCodeK / kStepK;
     uint32_t code[CODES];
-    f16x2 factor[CODES];
+    CodeFactor factor[CODES];
     auto load_codes = [&](int64_t step) { // waited for here: a wait in every step would be one for the tiles that are on their way
 #pragma unroll
         for (int i = 0; i < CODES; ++i) {
@@ -215,18 +223,18 @@ __device__ __forceinline__ void split_tile(f32x16 (&acc)[4][2], float* lds, cons
         if (t + 2 < k_steps) load(t + 2, now == 0 ? 2 : now - 1);
         if (CODED != kPlain && (t == 0 || step % CODE_STEPS == 0))
 #pragma unroll
-            for (int i = 0; i < CODES; ++i) factor[i] = code_factor(code[i], (uint32_t)step / CODE_STEPS % kCodesAWord);
+            for (int i = 0; i < CODES; ++i) factor[i].set(code[i], (uint32_t)step / CODE_STEPS % kCodesAWord);
         const char* s = (const char*)lds + now * kStageBytes;
         f16x8 b[2][2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             b[j][0] = rb.read(s, j, 0), b[j][1] = rb.read(s, j, 1);
-            if (CODED == kCodedB) b[j][0] = times(b[j][0], factor[j % CODES]), b[j][1] = times(b[j][1], factor[j % CODES]);
+            if (CODED == kCodedB) b[j][0] = times(times(b[j][0], factor[j % CODES].near), factor[j % CODES].far), b[j][1] = times(b[j][1], factor[j % CODES].low);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             f16x8 ah = ra.read(s, i, 0), al = ra.read(s, i, 1);
-            if (CODED == kCodedA) ah = times(ah, factor[i % CODES]), al = times(al, factor[i % CODES]);
+            if (CODED == kCodedA) ah = times(times(ah, factor[i % CODES].near), factor[i % CODES].far), al = times(al, factor[i % CODES].low);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, b[j][0], acc[i][j], 0, 0, 0);

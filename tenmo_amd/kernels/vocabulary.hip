@@ -11,8 +11,8 @@
 //   * backward: a piece of the vocabulary at a time; the tiles of the first launch end as G in split form, which the next one multiplies with W and with H.  The piece is as large as 1 GiB of G allows.
 //     Two forms of G, since its two products sum over different axes:
 //       G W^T    G at 2^14.  A row is a token's, whose target has p - 1, itself right to 2^-24 of 1; the halves hold the others to 2^-40 of 1.
-//       G^T H    scale_m G / (the scale of H's row m), which is what a word's row of dW is summed from: with a scale for each word and 64 tokens, a power of 2^12 that brings their largest into
-//                2^2 .. 2^14 (split_gemm.hpp brings them to the word's smallest).  Words without a target have probabilities alone in their rows, however small, and tokens lie far apart in
+//       G^T H    scale_m G / (the scale of H's row m), which is what a word's row of dW is summed from: with a scale for each word and 64 tokens, a power of 2^6 that brings their largest into
+//                2^8 .. 2^14 (split_gemm.hpp brings them to the word's smallest).  Words without a target have probabilities alone in their rows, however small, and tokens lie far apart in
 //                their upstream gradients: at 2^14 for all, rows of words whose logits lie 16 below the others' were off by 5e-2 of what enters them, 20 below by 1 (700 tokens,
 //                130 x 9000).  It costs a second G in memory and the scales, 1000 -> 1198 us, and factors as it is read, 1850 -> 1935 us (half of 8192 x 50257, D = 768).
 #include "split_gemm.hpp"
@@ -25,7 +25,7 @@ namespace tenmo {
 namespace {
 
 constexpr float kGScale = 16384.f;
-constexpr int kWordBits = 13, kMostClass = 9; // a word's scale: 2^(kWordBits + kCodeBits * class)
+constexpr int kWordBits = 13, kMostClass = 18; // a word's scale: 2^(kWordBits + kCodeBits * class)
 constexpr int64_t kPieceValues = 256 << 20; // of G, 4 bytes each
 
 struct Source { // an operand in the order in which it is split: rows x cols
@@ -229,7 +229,7 @@ __device__ __forceinline__ void word_scales(float (&x)[16], uint8_t* classes, in
         top = max(top, (uint32_t)lane_move_bits<0x141>(top));
         top = max(top, (uint32_t)lane_move_bits<0x140>(top));
         const int below = 127 - (int)(top >> 23); // top in [2^-below, 2^(1 - below))
-        const uint32_t c = (uint32_t)(fmaxf((float)below, 0.f) * (171.f / 2048.f)); // / kCodeBits, exactly so
+        const uint32_t c = (uint32_t)(fmaxf((float)below, 0.f) * (342.f / 2048.f)); // / kCodeBits, exactly so
         cls[e] = c < kMostClass ? c : kMostClass;
         const uint32_t scale = (127 + kWordBits + __umul24(cls[e], kCodeBits)) << 23;
         const auto z = __builtin_amdgcn_permlane16_swap(scale, scale, false, false);
@@ -519,7 +519,7 @@ __global__ __launch_bounds__(256) void vocab_unit_kernel(const uint8_t* __restri
     for (int64_t t = 0; t < blocks; t += kCodesAWord) {
         uint32_t word = 0;
 #pragma unroll
-        for (int u = 0; u < kCodesAWord; ++u) word |= min((t + u < blocks ? classes[(t + u) * pitch + v] : least) - least, 3u) << (2 * u);
+        for (int u = 0; u < kCodesAWord; ++u) word |= min((t + u < blocks ? classes[(t + u) * pitch + v] : least) - least, (uint32_t)kMostCode) << (4 * u);
         codes[t / kCodesAWord * pitch + v] = word;
     }
 }

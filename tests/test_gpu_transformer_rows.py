@@ -121,11 +121,13 @@ def vocabulary_rows(h, w, bias, target, upstream, reduction, smoothing):
     s = upstream.double() / (valid.sum() if reduction == "mean" else 1)
     g = g * torch.where(valid, s, 0.0).expand(len(target))[:, None]
     square = lambda t, d: (t ** 2).sum(d)  # noqa: E731
-    return [g @ w.t(), (h.t() @ g).t(), g.sum(0)[:, None]], [((g ** 2) @ square(w, 0)).sqrt(), ((g ** 2).t() @ square(h, 1)).sqrt(), g.abs().sum(0)]
+    return [g @ w.t(), (h.t() @ g).t(), g.sum(0)[:, None]], [((g ** 2) @ square(w, 0)).sqrt(), ((g ** 2).t() @ square(h, 1)).sqrt(), g.abs().sum(0)], g.abs().t() @ h.norm(dim=1)
 
 
-def check_vocabulary(ops, h, w, bias, target, upstream, reduction, smoothing, tied):
-    want, size = vocabulary_rows(h, w, bias, target, upstream, reduction, smoothing)
+def check_vocabulary(ops, h, w, bias, target, upstream, reduction, smoothing, tied, one_way=None):
+    want, size, magnitudes = vocabulary_rows(h, w, bias, target, upstream, reduction, smoothing)
+    if one_way is not None:
+        size[1] = magnitudes
     H, B, W = up(ops, h), up(ops, bias), up(ops, w.t().contiguous()).transpose() if tied else up(ops, w)
     kind = dict(ignore_index=-100, label_smoothing=smoothing)
     t = target.cuda()
@@ -134,7 +136,7 @@ def check_vocabulary(ops, h, w, bias, target, upstream, reduction, smoothing, ti
     # db sums probabilities of one sign, whose errors have one sign too where they are the exponent's: log2(e) as a float is off by 1.3e-8 of itself, so that every exp(-t) is by t 1.3e-8, 7e-7 at
     # t = 53, all in one direction.  Over 1500 tokens that alone is sqrt(1500) * 7e-7 = 2.7e-5 of the square root of the sum of squares: it is measured against the sum of magnitudes.
     for g, want_g, s, what in zip((down(gh), down(gw).t(), down(gb)[:, None]), want, size, ("grad_h", "grad_w", "grad_bias")):
-        rows_close(g, want_g, s, 2 * RTOL_FRO, what)
+        rows_close(g, want_g, s, 2 * RTOL_FRO + (one_way or 0.0), what)
 
 
 VOCABULARY = [(300, 96, 20000), (700, 130, 9000), (1500, 64, 4100), (40, 96, 3000)]  # tokens, dim, words; the last by the kernels for few tokens
@@ -190,3 +192,25 @@ def test_vocabulary_hidden_states_of_zeros(ops, size, tied, hidden):  # noqa: F8
     target = torch.randint(0, v, (m,), generator=torch.Generator().manual_seed(73))
     target[::19] = -100
     check_vocabulary(ops, h, w, bias, target, torch.ones(1), "mean", 0.0, tied)
+
+
+@pytest.mark.parametrize("m", [1000, 4100])
+@pytest.mark.parametrize("tied", [True, False], ids=["tied", "plain"])
+@pytest.mark.parametrize("near,far", [(0.0, 15.0), (0.3, 18.0), (2.0, 19.0), (4.5, 22.0), (8.6, 26.4)], ids=str)
+def test_vocabulary_a_word_that_one_token_sees(ops, m, tied, near, far):  # noqa: F811
+    """Words that one token gives a probability e^-near times the others' and all other tokens e^-far, with hidden states that point one way: what thousands of those add up to counts beside it.
+
+    Terms of one sign, so rows of dW are measured against the sum of their magnitudes: a sum of n of them takes 3 n / 16 matrix instructions, each of which rounds it by up to 2^-24 of itself, 1.7e-6 of
+    itself over 4100 tokens were they independent, and the sum is 64 times the square root of the sum of squares.  For the words that one token sees the two measures are the same to 1e-3.
+    Their row is one probability, as good as that token's logit, in which 2 (near - far) meets a bias of as much: two operands held to 2^-22 and the product of their rests left out, 3 * 2^-22 of that, two
+    additions of 2^-24."""
+    d, v = 64, 2100
+    h, w, bias = randn(80, m, d) * 0.3, randn(81, d, v) * 0.05, randn(82, v) * 0.1
+    rare = torch.arange(v) % 3 == 0
+    h[:, 0], h[m // 2, 0] = 3.0, 2.0
+    h[:, 1] = 2.0
+    w[0] = torch.where(rare, near - far, 0.0)
+    w[1] = 0.0
+    bias += torch.where(rare, 2.0 * (far - near) - near, 0.0)  # 3 (near - far) + this: -far; 2 (near - far) + this: -near
+    target = torch.randint(0, v // 3, (m,), generator=torch.Generator().manual_seed(83)) * 3 + 1
+    check_vocabulary(ops, h, w, bias, target, torch.ones(1), "mean", 0.0, tied, one_way=2.0 * (far - near) * (3 * 2.0 ** -22 + 2 * 2.0 ** -24))

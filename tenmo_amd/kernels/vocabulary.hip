@@ -14,7 +14,7 @@
 //       G^T H    scale_m G / (the scale of H's row m), which is what a word's row of dW is summed from: with a scale for each word and 64 tokens, a power of 2^6 that brings their largest into
 //                2^8 .. 2^14 (split_gemm.hpp brings them to the word's smallest).  Words without a target have probabilities alone in their rows, however small, and tokens lie far apart in
 //                their upstream gradients: at 2^14 for all, rows of words whose logits lie 16 below the others' were off by 5e-2 of what enters them, 20 below by 1 (700 tokens,
-//                130 x 9000).  It costs a second G in memory and the scales, 1000 -> 1198 us, and factors as it is read, 1850 -> 1935 us (half of 8192 x 50257, D = 768).
+//                130 x 9000).  It costs a second G in memory and the scales, 1000 -> 1180 us, and factors as it is read, 1850 -> 1940 us (half of 8192 x 50257, D = 768).
 #include "split_gemm.hpp"
 #include "vocabulary.hpp"
 
@@ -356,7 +356,6 @@ __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs 
         }
         const bool here = __any(at[0] >= 0 || at[1] >= 0); // a target among this wavefront's words: one in three at 50257 words
         const int words = (int)(a.words - v0 < 256 ? a.words - v0 : 256), pitch = (int)((a.g.p ? a.g.pitch : a.gw.pitch) - v0 < 256 ? (a.g.p ? a.g.pitch : a.gw.pitch) - v0 : 256);
-        float db[64];
         uint8_t* const classes = a.word_class + ((n0 >> 6) + (wave >> 1)) * a.gw.pitch + v0;
         // WHOLE: every word and token of the tile is there
         auto end = [&](auto whole) {
@@ -377,9 +376,24 @@ __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs 
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
                             acc[i][j][e] -= at[j] == 32 * i + 8 * (e >> 2) + (e & 3) ? 1.f - a.v.ls : 0.f;
-                if (a.part_db)
+                if (a.part_db) { // 16 values in each of 32 lanes, summed over the lanes: lanes 2 x and 2 x + 1 end with the sum of the value whose number has x's bits
+                    float db[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) db[16 * i + e] = acc[i][0][e] * row_scale[0] + acc[i][1][e] * row_scale[1];
+                    for (int e = 0; e < 16; ++e) db[e] = acc[i][0][e] * row_scale[0] + acc[i][1][e] * row_scale[1];
+#pragma unroll
+                    for (int step = 16, n = 8; step > 1; step >>= 1, n >>= 1) {
+                        const bool up = lane & step;
+#pragma unroll
+                        for (int x = 0; x < n; ++x) {
+                            const float give = up ? db[x] : db[x + n], keep = up ? db[x + n] : db[x];
+                            db[x] = keep + __shfl_xor(give, step, 64);
+                        }
+                    }
+                    db[0] += __shfl_xor(db[0], 1, 64);
+                    const int x = (lane & 31) >> 1;
+                    const int64_t v = v0 + 32 * i + 8 * (x >> 2) + (x & 3);
+                    if (!(lane & 1) && v < a.words) a.part_db[(2 * tn + (wave >> 1)) * a.v.V + a.first + v] = db[0];
+                }
                 if (a.g.p)
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
@@ -414,25 +428,6 @@ __global__ __launch_bounds__(256, 2) void vocab_logits_kernel(const ProductArgs 
         };
         if (!edge && n0 + kTileN <= a.v.M) end(std::true_type{});
         else end(std::false_type{});
-        if (a.part_db) { // 64 values in each of 32 lanes, summed over the lanes: lane x keeps the sums of values 2 x and 2 x + 1 in bit-reversed order
-#pragma unroll
-            for (int step = 16, n = 32; step > 0; step >>= 1, n >>= 1) {
-                const bool up = lane & step;
-#pragma unroll
-                for (int x = 0; x < n; ++x) {
-                    const float give = up ? db[x] : db[x + n], keep = up ? db[x + n] : db[x];
-                    db[x] = keep + __shfl_xor(give, step, 64);
-                }
-            }
-            // after the steps this lane holds x = 32 b4 + 16 b3 + 8 b2 + 4 b1 + 2 b0 + {0, 1} with b the bits of its number
-            const int x0 = 2 * (lane & 31);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int x = x0 + e, i = x >> 4, q = (x >> 2) & 3;
-                const int64_t v = v0 + 32 * i + 8 * q + (x & 3);
-                if (v < a.words) a.part_db[(2 * tn + (wave >> 1)) * a.v.V + a.first + v] = db[e];
-            }
-        }
     }
 }
 

@@ -23,7 +23,7 @@
 // What a row of a gradient is summed from is held to the row's own sizes, however small they are against the head's (with one scale a head, keys of a weight of e^-18 got dK to 0.1 of itself,
 // and rows of dQ where dO is 2^-20 of the head's largest to 0.05):
 //   * a row of dO that is small against the head's largest has a scale a_i of its own, and P is taken times A / a_i (A: the head's scale): P dO is the same, and what the row adds is small in P
-//     instead.  The factor goes into the row's lse.
+//     instead (zeros: nothing).  The factor goes into the row's lse.
 //   * P and dS have a scale for each row of the result, which is a lane: a power of two that brings the largest so far into 2^10 .. 2^15, renewed, with the sums, when one passes it.
 //     Since it is known only when a tile is done, it costs a maximum of the tile's 16 values and a branch (the kernel at [8,1024,12,64] 187 us with and without, at [1,8192,16/4,128] 2967 and
 //     2960; with 2^12 in place of 2^10 scales are renewed more often: 194 and 3150, and with sums moved by the compiler, see scale_sums, 200 and 3670).
@@ -212,14 +212,15 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
             for (int u = 0; u < 2; ++u) v[i][u] = attn_load4<kind.value>(p + at * j.src.s, j.src.d, x % GROUPS * 2 + u, a.s.dim);
         }
     });
-    float scales[N];
+    float scales[N], ups[N]; // ups: scales over the head's
 #pragma unroll
-    for (int i = 0; i < N; ++i) scales[i] = scale;
+    for (int i = 0; i < N; ++i) scales[i] = scale, ups[i] = 1.f;
     if (j.job == kDO) { // (in the whole workgroup)
 #pragma unroll
         for (int i = 0; i < N; ++i) { // (at most 2^120 times the head's, so that the quotient of the two is a float; 2^-12 of the largest is held to 2^-28 by the head's)
             const float mine = a.stats[stat_at((int64_t)j.bh * j.pad + block * ROWS + (threadIdx.x + 256 * i) / GROUPS, kDown)];
-            if (mine > 0.f && mine < top * 0x1p-12f) scales[i] = fminf(split_scale(__float_as_uint(mine)), scale * 0x1p120f);
+            if (mine > 0.f && mine < top * 0x1p-12f) scales[i] = fminf(split_scale(__float_as_uint(mine)), scale * 0x1p120f), ups[i] = scales[i] * power_inverse(scale);
+            if (mine == 0.f) ups[i] = 0x1p120f; // a row of zeros takes the smallest P: it leaves the scale that the others' have as it is
         }
         __syncthreads(); // each row's magnitude is read by all of its threads before one of them writes in its place
 #pragma unroll
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(256) void attn_split_kernel(const TileArgs a) {
             const int x = threadIdx.x + 256 * i;
             if (x % GROUPS) continue;
             const int64_t row = (int64_t)j.bh * j.pad + block * ROWS + x / GROUPS;
-            const float up = scales[i] * power_inverse(scale);
+            const float up = ups[i];
             a.stats[stat_at(row, kLseUp)] += (float)((int)(__float_as_uint(up) >> 23) - 127);
             a.stats[stat_at(row, kDeltaUp)] = a.stats[stat_at(row, kDelta)] * up;
             a.stats[stat_at(row, kDown)] = power_inverse(up);

@@ -108,6 +108,19 @@ def test_attention_values_far_out_of_little_weight(ops, size, seed):  # noqa: F8
     check_attention(ops, q, k, v, dout, scale, causal)
 
 
+@pytest.mark.parametrize("size", SIZES, ids=str)
+@pytest.mark.parametrize("small", [1.0, 2.0 ** -12, 2.0 ** -20, 2.0 ** -30], ids=str)
+def test_attention_output_gradients_of_zeros(ops, size, small):  # noqa: F811
+    """Queries without a gradient among others whose gradients are small against the first one's, which sees other keys: keys get theirs from the small ones alone."""
+    n, m, H, Hk, D, causal = size
+    q, k, v, dout = randn(101, 1, n, H, D), randn(102, 1, m, Hk, D), randn(103, 1, m, Hk, D), randn(104, 1, n, H, D)
+    dout[:, 1:] *= small
+    dout[:, 1::2] = 0.0
+    q[:, 0] = 0.0
+    q[:, 0, :, 0], k[:, -m // 3:, :, 0] = 8.0, -32.0  # (without a mask: the first query gives the last keys little)
+    check_attention(ops, q, k, v, dout, 1.0 / math.sqrt(D), causal)
+
+
 # ---- vocabulary loss ------------------------------------------------------------------------------------------------------------------
 
 

@@ -637,11 +637,11 @@ __global__ __launch_bounds__(256) void vocab_dh_kernel(const float* __restrict p
     }
 }
 
-// dW of a piece: the runs' sums [rows][cols] added in order
+// dW of a piece: the runs' sums [rows][cols] added in order (zeros without a run)
 __global__ __launch_bounds__(256) void vocab_dw_kernel(const float* __restrict part, int64_t runs, int64_t rows, int64_t cols, const StoreArgs s) {
     const int64_t all = rows * cols;
     for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < all; x += (int64_t)gridDim.x * 256) {
-        float sum = part[x];
+        float sum = runs > 0 ? part[x] : 0.f;
 #pragma unroll 8
         for (int64_t r = 1; r < runs; ++r) sum += part[r * all + x];
         float* to = s.c + x / cols * s.rs + x % cols * s.cs;
@@ -861,32 +861,35 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
         if (grad_H) hipLaunchKernelGGL(vocab_dh_kernel, grid_of_dh(v, call.state), dim3(256), 0, stream, p.part_h, p.runs, v, up, grad_H, add);
         return call.finish(sync);
     }
+    auto grid_of_dw = [&](int64_t values) { return dim3((unsigned)std::min<int64_t>(tiles_of(values, 256), 8 * call.state.cus)); };
+    if (v.M == 0) { // nothing is added up
+        if (grad_W && !add) hipLaunchKernelGGL(vocab_dw_kernel, grid_of_dw(v.V * v.D), dim3(256), 0, stream, nullptr, 0, v.V, v.D, StoreArgs{gw, gw_v, gw_d, 0});
+        if (grad_bias) hipLaunchKernelGGL(vocab_db_kernel, dim3((unsigned)tiles_of(v.V, 256)), dim3(256), 0, stream, nullptr, 0, v.V, grad_bias, add);
+        return call.finish(sync);
+    }
     Plan p{};
-    if (v.M > 0) plan_backward(ws, p, v.M, v.D, v.V, word_rows);
+    plan_backward(ws, p, v.M, v.D, v.V, word_rows);
     if (int rc = ws.check(who)) return rc;
-    if (v.M > 0) launch_split(p, H, W, v, up, call.state);
-    const int64_t piece = v.M > 0 ? p.piece : v.V;
+    launch_split(p, H, W, v, up, call.state);
     int64_t runs = 0;
-    for (int64_t first = 0; first < v.V; first += piece) {
-        const int64_t words = std::min(piece, v.V - first);
+    for (int64_t first = 0; first < v.V; first += p.piece) {
+        const int64_t words = std::min(p.piece, v.V - first);
         SplitMatrix G = p.g, GW = p.gw;
         G.pitch = GW.pitch = split_pad(words);
-        if (v.M > 0) {
-            const SplitMatrix w = words_of(p.w, first, word_rows);
-            const ProductArgs g = product(w, p.amax_w, p.h, nullptr, words, v.M, v.D);
-            LogitArgs a{};
-            a.v = v; a.first = first; a.words = words; a.h_inverse = p.h_inverse; a.lse = lse; a.up = up; a.part_db = grad_bias ? p.part_db : nullptr;
-            if (grad_H) a.g = G;
-            if (grad_W) a.gw = GW, a.word_class = p.word_class, a.top_f = p.top_f;
-            if (word_rows) hipLaunchKernelGGL((vocab_logits_kernel<true, true>), grid_of(g), dim3(256), 0, stream, g, a);
-            else hipLaunchKernelGGL((vocab_logits_kernel<false, true>), grid_of(g), dim3(256), 0, stream, g, a);
-            if (grad_W)
-                hipLaunchKernelGGL(vocab_unit_kernel, dim3((unsigned)tiles_of(GW.pitch, 256)), dim3(256), 0, stream, p.word_class, GW.pitch, tiles_of(v.M, kCodeK), p.codes, p.unit);
-        }
+        const SplitMatrix w = words_of(p.w, first, word_rows);
+        const ProductArgs g = product(w, p.amax_w, p.h, nullptr, words, v.M, v.D);
+        LogitArgs a{};
+        a.v = v; a.first = first; a.words = words; a.h_inverse = p.h_inverse; a.lse = lse; a.up = up; a.part_db = grad_bias ? p.part_db : nullptr;
+        if (grad_H) a.g = G;
+        if (grad_W) a.gw = GW, a.word_class = p.word_class, a.top_f = p.top_f;
+        if (word_rows) hipLaunchKernelGGL((vocab_logits_kernel<true, true>), grid_of(g), dim3(256), 0, stream, g, a);
+        else hipLaunchKernelGGL((vocab_logits_kernel<false, true>), grid_of(g), dim3(256), 0, stream, g, a);
+        if (grad_W)
+            hipLaunchKernelGGL(vocab_unit_kernel, dim3((unsigned)tiles_of(GW.pitch, 256)), dim3(256), 0, stream, p.word_class, GW.pitch, tiles_of(v.M, kCodeK), p.codes, p.unit);
         ProductArgs dh{}, dw{};
         StoreArgs sh{}, sw{};
         int64_t h_tiles = 0, w_tiles = 0;
-        if (grad_H && v.M > 0) {
+        if (grad_H) {
             dh = product(G, nullptr, words_of(p.w, first, word_rows), p.amax_w, v.M, v.D, words);
             dh.run_steps = tiles_of(tiles_of(p.piece, kStepK), p.runs); // (of the whole piece: a last one that is shorter has as many or fewer runs)
             dh.run_stride = v.M * v.D;
@@ -924,11 +927,11 @@ int tenmo_hip_vocabulary_loss_backward_f32(const tenmo_view* H, const tenmo_view
         else if (dw_by_words) hipLaunchKernelGGL((vocab_products_kernel<true, true>), grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
         else hipLaunchKernelGGL((vocab_products_kernel<true, false>), grid, dim3(256), 0, stream, dh, sh, (uint32_t)h_tiles, dw, sw);
         if (grad_W && p.w_runs > 1)
-            hipLaunchKernelGGL(vocab_dw_kernel, dim3((unsigned)std::min<int64_t>(tiles_of(dw.run_stride, 256), 8 * call.state.cus)), dim3(256), 0, stream, p.part_w, w_runs, dw.M, dw.N, to_w);
+            hipLaunchKernelGGL(vocab_dw_kernel, grid_of_dw(dw.run_stride), dim3(256), 0, stream, p.part_w, w_runs, dw.M, dw.N, to_w);
     }
-    if (grad_H && v.M > 0)
+    if (grad_H)
         hipLaunchKernelGGL(vocab_dh_kernel, grid_of_dh(v, call.state), dim3(256), 0, stream, p.part_h, runs, v, up, grad_H, add);
-    if (grad_bias) hipLaunchKernelGGL(vocab_db_kernel, dim3((unsigned)tiles_of(v.V, 256)), dim3(256), 0, stream, p.part_db, v.M > 0 ? 2 * tiles_of(v.M, kTileN) : 0, v.V, grad_bias, add);
+    if (grad_bias) hipLaunchKernelGGL(vocab_db_kernel, dim3((unsigned)tiles_of(v.V, 256)), dim3(256), 0, stream, p.part_db, 2 * tiles_of(v.M, kTileN), v.V, grad_bias, add);
     return call.finish(sync);
 }
 

@@ -162,6 +162,25 @@ def test_vocabulary_loss_of_a_batch(ops, reduction, tied, bias):  # noqa: F811
     close(W.grad().T if tied else W.grad(), W2.grad(), RTOL_FRO, "grad_w")
 
 
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("v", [7, 3000])
+def test_vocabulary_loss_of_no_tokens(ops, reduction, tied, v):  # noqa: F811
+    """Nothing to learn from: a loss of zero and gradients of zero, which leave what is added to as it is."""
+    N, d = ops.NDBuffer, 40
+    h, b, w = N.empty((0, d)), up(ops, randn(1, v)), up(ops, randn(2, v, d)).transpose() if tied else up(ops, randn(2, d, v))
+    target = torch.zeros(0, dtype=torch.int64, device="cuda")
+    loss = ops.V.vocabulary_loss(h, w, b, target)
+    assert down(loss.loss_sum) == 0.0 and int(loss.valid_count) == 0
+    upstream = torch.ones(0 if reduction == "none" else 1, device="cuda")
+    gh, gw, gb = ops.V.vocabulary_loss_backward(h, w, b, target, loss, upstream, reduction=reduction)
+    assert gh.shape == (0, d) and gw.shape == (d, v) and not down(gw).any() and not down(gb).any()
+    want = randn(3, d, v)
+    gw, gb = up(ops, want.t().contiguous()).transpose() if tied else up(ops, want), up(ops, randn(4, v))
+    ops.V.vocabulary_loss_backward(h, w, b, target, loss, upstream, reduction=reduction, into=(None, gw, gb))
+    assert torch.equal(down(gw), want) and torch.equal(down(gb), randn(4, v))
+
+
 def test_vocabulary_loss_of_a_batch_refusals(ops):  # noqa: F811
     T, N = ops.Tensor, ops.NDBuffer
     w, t = T.zeros(48, 700), torch.zeros(60, dtype=torch.int64, device="cuda")

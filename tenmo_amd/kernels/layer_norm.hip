@@ -318,6 +318,8 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const NormBackward a) {
     }
 }
 
+constexpr int64_t kMostColumns = 1 << 27;
+
 int norm_rows(const tenmo_view* X, const char* who, NormRows* r) {
     if (int rc = check_operand(X, 1, TENMO_MAX_RANK, who, "X")) return rc;
     r->n = X->shape[X->rank - 1];
@@ -336,7 +338,7 @@ int norm_rows(const tenmo_view* X, const char* who, NormRows* r) {
             r->stride[r->rank++] = X->strides[d];
         }
     }
-    if (r->n > 1 << 27) return refuse(TENMO_ERR_UNSUPPORTED, "%s: more than 2^27 columns", who);
+    if (r->n > kMostColumns) return refuse(TENMO_ERR_UNSUPPORTED, "%s: more than 2^27 columns", who);
     return 0;
 }
 
@@ -408,7 +410,10 @@ int tenmo_hip_layer_norm_forward_f32(const tenmo_view* X, const float* weight, c
 }
 
 int64_t tenmo_hip_layer_norm_backward_workspace_bytes(int64_t rows, int64_t n) {
-    if (rows <= 0 || n <= 0) return 0;
+    const char* who = "tenmo_hip_layer_norm_backward_workspace_bytes";
+    if (rows < 0 || n < 1) return refuse(TENMO_ERR_INVALID_SHAPE, "%s: needs rows >= 0 and columns >= 1", who);
+    if (n > kMostColumns) return refuse(TENMO_ERR_UNSUPPORTED, "%s: more than 2^27 columns", who);
+    if (rows == 0) return 0;
     Workspace ws(nullptr, 0);
     ws.take<float>(2 * norm_parts(rows, n) * n);
     return ws.used();

@@ -125,3 +125,11 @@ def test_calls_without_initialisation_fail_cleanly():
     refused(UNINITIALISED, "not initialised", attn_forward())
     refused(UNINITIALISED, "not initialised", L.tenmo_hip_vocabulary_loss_forward_f32(view((4, 8)), view((8, 10)), None, P, 1, -100, 0.0, P, P, P, P, P, 0, 0))
     refused(UNINITIALISED, "not initialised", L.tenmo_hip_attention_forward_workspace_bytes(1, 1, 1, 1, 1, 16))
+
+
+def test_layer_norm_workspace_refusals():
+    bytes_of = _transformer.load().tenmo_hip_layer_norm_backward_workspace_bytes
+    refused(SHAPE, "columns >= 1", bytes_of(4, 0))
+    refused(SHAPE, "rows >= 0", bytes_of(-1, 8))
+    refused(UNSUPPORTED, "2^27", bytes_of(2, (1 << 27) + 1))
+    assert bytes_of(0, 8) == 0 and bytes_of(4, 8) > 0

@@ -1,7 +1,8 @@
 /*
  * Operators of a transformer's training step, beside the products and losses of tenmo_hip.h and with its conventions: device
  * pointers, sizes and strides in elements, views over strided storage, one stream, 0 or a negative tenmo_status, the message of a
- * failure in tenmo_hip_last_error().  No counterpart in the reference, which has none of these operators.
+ * failure in tenmo_hip_last_error().  Of these the reference has a layer norm (tenmo/layernorm.mojo, tenmo/kernels/layernorm.mojo); attention and the loss from the hidden states have no
+ * counterpart there.
  *
  * Workspace: an entry that needs scratch memory takes it from the caller (device memory, 256-byte aligned), of at least the bytes that
  * its ..._workspace_bytes function returns for the same sizes.  Nothing is kept in it from one call to the next, and no call
@@ -11,7 +12,19 @@
  * Sizes beyond what a launch holds are refused with TENMO_ERR_UNSUPPORTED: each entry says which.
  *
  * Gradients: with accumulate = 0 they are written, with accumulate != 0 added to what is there.  A NULL gradient is not computed.
- * Results do not depend on scheduling: the same inputs give the same bits.
+ * Results do not depend on scheduling: the same inputs give the same bits.  They share no place with operands or with each other where an entry does not say so.
+ *
+ * Precision: operands, results and sums are fp32.  Large attention calls, and those of the vocabulary loss on many tokens, multiply on the fp16 matrix units, each fp32 value as a sum of two
+ * halves: to 2^-22 of itself, and to 2^-40 of the largest value that has the same scale.  Scales are chosen so that each row of a result is right by itself, however small it is against the others of
+ * its call.  Three things remain:
+ *   - A probability exp(-t) is off by up to (t + 2) 2^-24 of itself, and by the error of its score or logit, about 2^-22 |q| |k| scale or 2^-22 |h| |w| on the matrix units and 2^-24 of them elsewhere.
+ *     The target's p - 1 in the loss's gradient is right to that, not to its own size.
+ *   - What a probability is multiplied by does not count in how it is held: attention forward to 2^-28 of the row's largest, backward (and dS) to 2^-35 of the largest that enters the same row of
+ *     the result; the loss to 2^-33 of the largest that enters the same row of grad_W, and 2^-40 of 1 for grad_H.  A row that only smaller ones make, because the vectors of the others are zeros,
+ *     loses them (output gradients and hidden states of zeros do not count among the others).
+ *   - Heads with values that are not finite, with rows of K or V (backward: or Q) whose largest magnitudes lie more than 2^16 apart, rows of zeros aside, or, backward, with scores above 2^16 are
+ *     worked on in fp32, value by value: right, but 40 to 140 times as slow as others of their length.
+ * Small calls are in fp32 throughout.
  */
 #ifndef TENMO_HIP_TRANSFORMER_H
 #define TENMO_HIP_TRANSFORMER_H

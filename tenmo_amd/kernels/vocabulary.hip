@@ -14,7 +14,7 @@
 //       G^T H    scale_m G / (the scale of H's row m), which is what a word's row of dW is summed from: with a scale for each word and 64 tokens, a power of 2^6 that brings their largest into
 //                2^8 .. 2^14 (split_gemm.hpp brings them to the word's smallest).  Words without a target have probabilities alone in their rows, however small, and tokens lie far apart in
 //                their upstream gradients: at 2^14 for all, rows of words whose logits lie 16 below the others' were off by 5e-2 of what enters them, 20 below by 1 (700 tokens,
-//                130 x 9000).  It costs a second G in memory and the scales, 1000 -> 1180 us, and factors as it is read, 1850 -> 1940 us (half of 8192 x 50257, D = 768).
+//                130 x 9000).  It costs a second G in memory and the scales, 1032 -> 1200 us, and factors as it is read, 1892 -> 1990 us (half of 8192 x 50257, D = 768).
 #include "split_gemm.hpp"
 #include "vocabulary.hpp"
 

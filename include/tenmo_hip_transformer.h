@@ -23,7 +23,7 @@
  *     the result; the loss to 2^-33 of the largest that enters the same row of grad_W, and 2^-40 of 1 for grad_H.  A row that only smaller ones make, because the vectors of the others are zeros,
  *     loses them (output gradients and hidden states of zeros do not count among the others).
  *   - Heads with values that are not finite, with rows of K or V (backward: or Q) whose largest magnitudes lie more than 2^16 apart, rows of zeros aside, or, backward, with scores above 2^16 are
- *     worked on in fp32, value by value: right, but 40 to 140 times as slow as others of their length.
+ *     worked on in fp32, value by value: right, but 20 to 140 times as slow as others of their length.
  * Small calls are in fp32 throughout.
  */
 #ifndef TENMO_HIP_TRANSFORMER_H

@@ -16,7 +16,7 @@
  *
  * Precision: operands, results and sums are fp32.  Large attention calls, and those of the vocabulary loss on many tokens, multiply on the fp16 matrix units, each fp32 value as a sum of two
  * halves: to 2^-22 of itself, and to 2^-40 of the largest value that has the same scale.  Scales are chosen so that each row of a result is right by itself, however small it is against the others of
- * its call.  Three things remain:
+ * its call.  Four things remain:
  *   - A probability exp(-t) is off by up to (t + 2) 2^-24 of itself, and by the error of its score or logit, about 2^-22 |q| |k| scale or 2^-22 |h| |w| on the matrix units and 2^-24 of them elsewhere.
  *     The target's p - 1 in the loss's gradient is right to that, not to its own size.
  *   - What a probability is multiplied by does not count in how it is held: attention forward to 2^-28 of the row's largest, backward (and dS) to 2^-35 of the largest that enters the same row of
@@ -24,6 +24,8 @@
  *     loses them (output gradients and hidden states of zeros do not count among the others).
  *   - Heads with values that are not finite, with rows of K or V (backward: or Q) whose largest magnitudes lie more than 2^16 apart, rows of zeros aside, or, backward, with scores above 2^16 are
  *     worked on in fp32, value by value: right, but 20 to 140 times as slow as others of their length.
+ *   - W of the loss has one scale: each of its values is held to 2^-40 of its largest magnitude at the best, so that the logits of words 2^16 smaller than the largest are as good as fp32 ones and those of
+ *     words 2^30 smaller are not.
  * Small calls are in fp32 throughout.
  */
 #ifndef TENMO_HIP_TRANSFORMER_H
